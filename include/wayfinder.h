@@ -374,6 +374,91 @@ WF_API int wf_gather_rows_bulk_bench(const void* k, const void* v, int64_t row_s
  */
 WF_API int wf_testing_withhold_pair_arrive(int32_t round, uint64_t wait_limit_ns);
 
+/*
+ * Linear layer with its epilogue: y = act(x W^T + b) + residual, products and sums in
+ * fp32, y rounded once.  It has no counterpart in the reference, which runs the same
+ * arithmetic as separate PyTorch layers (models/transformer.py:26-72 FFN and residual).
+ *
+ *   x        : (M, K) rows x_row_stride apart;  w : (N, K) rows w_row_stride apart
+ *   bias     : (N) or NULL;  residual : (M, N) rows r_row_stride apart, or NULL
+ *   dtype    : WF_DTYPE_* of all of them, of z and of y
+ *   z        : (M, N) contiguous, gets x W^T + b for the backward (rounded to dtype); may
+ *              be NULL
+ *   y        : (M, N) contiguous
+ *   workspace: wf_linear_workspace_bytes() bytes, 256-byte aligned (NULL if that is 0)
+ *   status   : optional device int32; bit 1 is OR-ed in if a bounded wait timed out
+ * K = 0 is refused; M = 0 or N = 0 does nothing.
+ */
+#define WF_ACT_NONE 0
+#define WF_ACT_GELU 1 /* z Phi(z), the erf form */
+#define WF_ACT_RELU 2
+#define WF_ACT_SILU 3
+WF_API size_t wf_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype);
+WF_API int wf_linear(const void* x, const void* w, const void* bias, const void* residual, int32_t dtype, int64_t M,
+                     int64_t N, int64_t K, int64_t x_row_stride, int64_t w_row_stride, int64_t r_row_stride,
+                     int32_t activation, void* z, void* y, void* workspace, size_t workspace_bytes, int32_t* status,
+                     void* stream);
+/*
+ * Its backward: dz = dy act'(z), dx = dz W, dw = dz^T x, dbias = the column sums of dz;
+ * the residual's gradient is dy itself.  z is what the forward wrote (may be NULL for
+ * WF_ACT_NONE).  dx (M, K), dw (N, K) and dbias (N) are contiguous, of dtype, and each
+ * may be NULL.  The result does not depend on scheduling (no atomics on sums).
+ */
+WF_API size_t wf_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation);
+WF_API int wf_linear_backward(const void* x, const void* w, const void* z, const void* dy, int32_t dtype, int64_t M,
+                              int64_t N, int64_t K, int64_t x_row_stride, int64_t w_row_stride, int64_t dy_row_stride,
+                              int32_t activation, void* dx, void* dw, void* dbias, void* workspace,
+                              size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias, var
+ * the mean squared deviation; statistics in fp32, y rounded once.  No counterpart in the
+ * reference (nn.LayerNorm in models/transformer.py:26-72).
+ *
+ *   x            : (rows, d) rows x_row_stride apart;  y : rows y_row_stride apart
+ *   weight, bias : (d) of param_dtype (dtype or WF_DTYPE_F32), or NULL
+ *   mean, rstd   : (rows) fp32 for the backward, or both NULL
+ */
+WF_API int wf_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t d, int64_t x_row_stride,
+                         const void* weight, const void* bias, int32_t param_dtype, float eps, void* y,
+                         int64_t y_row_stride, float* mean, float* rstd, void* stream);
+/* Its backward: dx (rows, d) contiguous of dtype; dweight and dbias (d) of param_dtype;
+ * each may be NULL.  Column sums are fp32 and added in a fixed order. */
+WF_API size_t wf_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d, int32_t dtype);
+WF_API int wf_layer_norm_backward(const void* x, const void* dy, int32_t dtype, int64_t rows, int64_t d,
+                                  int64_t x_row_stride, int64_t dy_row_stride, const void* weight,
+                                  int32_t param_dtype, const float* mean, const float* rstd, void* dx, void* dweight,
+                                  void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of given tokens under rows of logits, with each row's entropy and
+ * its top alternatives.  No counterpart in the reference (its evaluation applies
+ * log_softmax, gather and topk to the logits).
+ *
+ *   logits       : (rows, vocab) rows row_stride apart; -inf bans a token
+ *   tokens       : (rows) int64; a row whose token is ignore_index gets logprob 0; any
+ *                  other token outside [0, vocab) gets NaN and sets bit 0 of status
+ *   logprob, entropy : (rows) fp32
+ *   stats        : (2, rows) fp32 for the backward, or NULL: each row's maximum m, then log
+ *                  sum exp(x - m)
+ *   top_n        : 0..32, at most vocab; top_logprobs (rows, top_n) fp32 in descending
+ *                  order and top_tokens (rows, top_n) int64, equal logits by lower index,
+ *                  NaN first
+ * A row of nothing but -inf has logprob -inf, entropy 0 and alternatives of -inf with
+ * the lowest indices.
+ */
+WF_API int wf_max_top_tokens(void);
+WF_API int wf_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                             const int64_t* tokens, int64_t ignore_index, int32_t top_n, float* logprob,
+                             float* entropy, float* stats, float* top_logprobs, int64_t* top_tokens, int32_t* status,
+                             void* stream);
+/* Its backward: dlogits (rows, vocab) contiguous of dtype, from the gradients of logprob
+ * and entropy (rows) fp32 (either may be NULL) and the forward's stats and entropy. */
+WF_API int wf_token_logprobs_backward(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
+                                      int64_t row_stride, const int64_t* tokens, int64_t ignore_index,
+                                      const float* stats, const float* entropy, const float* dlogprob,
+                                      const float* dentropy, void* dlogits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

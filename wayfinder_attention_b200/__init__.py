@@ -6,6 +6,10 @@ Public API (names and arguments of the reference's ``routing_attention``):
   TransformerLM (the decoder harness); HostFusedSparseAttention runs the fused
   op on pinned host tensors with upload, compute and download overlapped.
 
+The decoder's other operators, each with its backward: fused_linear (bias,
+activation and residual in the product's epilogue), layer_norm and token_logprobs
+(log probability, entropy and top alternatives of given tokens).
+
 The compute runs in ``libwayfinder_sm100.so`` (C ABI: ``include/wayfinder.h``);
 there is no CPU path.  Kernel faults that do not stop a kernel (an out-of-range
 index, a bounded wait that timed out) raise ``RuntimeError`` at the next call on
@@ -25,6 +29,9 @@ from .router import MultiScaleRouter, PerLayerRouter, RouterMLP
 from .causal_topk import causal_topk, causal_topk_available, promote_compute_dtype
 from .decoder import DenseSDPAAttention, TransformerBlock, TransformerLM
 from .graphs import CapturedForward
+from .layer_norm import layer_norm
+from .linear import fused_linear
+from .token_logprobs import TokenLogprobs, token_logprobs
 from .host_pipeline import HostFusedSparseAttention, host_fused_sparse_attention
 from .fused_sparse import (
     SparseMeatConfig,
@@ -46,6 +53,10 @@ __all__ = [
     "CapturedForward",
     "host_fused_sparse_attention",
     "SparseMeatConfig",
+    "fused_linear",
+    "layer_norm",
+    "token_logprobs",
+    "TokenLogprobs",
     "LearnedAddressModule",
     "LearnedAddressSparseAttention",
     "KeyVectorSparseAttention",

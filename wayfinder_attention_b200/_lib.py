@@ -7,6 +7,7 @@ is no fallback implementation, so a missing library raises immediately.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -58,6 +59,16 @@ EXPORTED_SYMBOLS = (
     "wf_peer_buffer_close",
     "wf_pack_row_blocks",
     "wf_peer_pull_blocks",
+    "wf_linear",
+    "wf_linear_workspace_bytes",
+    "wf_linear_backward",
+    "wf_linear_backward_workspace_bytes",
+    "wf_layer_norm",
+    "wf_layer_norm_backward",
+    "wf_layer_norm_backward_workspace_bytes",
+    "wf_max_top_tokens",
+    "wf_token_logprobs",
+    "wf_token_logprobs_backward",
 )
 
 _DTYPE_CODES = {
@@ -160,6 +171,26 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.wf_causal_topk_key_mask.argtypes = [
         _vp, _vp, _i32, _i64, _i64, _i32, _i64p, _i64p, _vp, _i64p, _i32, _vp, _vp, ctypes.c_size_t, _vp, _vp,
     ]
+    sz = ctypes.c_size_t
+    for name, restype, argtypes in (
+        ("wf_linear_workspace_bytes", sz, [_i64, _i64, _i64, _i32]),
+        ("wf_linear_backward_workspace_bytes", sz, [_i64, _i64, _i64, _i32, _i32]),
+        ("wf_linear", ctypes.c_int, [_vp] * 4 + [_i32] + [_i64] * 6 + [_i32, _vp, _vp, _vp, sz, _vp, _vp]),
+        ("wf_linear_backward", ctypes.c_int,
+         [_vp] * 4 + [_i32] + [_i64] * 6 + [_i32, _vp, _vp, _vp, _vp, sz, _vp, _vp]),
+        ("wf_layer_norm", ctypes.c_int,
+         [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i32, _f32, _vp, _i64, _vp, _vp, _vp]),
+        ("wf_layer_norm_backward_workspace_bytes", sz, [_i64, _i64, _i32]),
+        ("wf_layer_norm_backward", ctypes.c_int,
+         [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, sz, _vp]),
+        ("wf_max_top_tokens", ctypes.c_int, []),
+        ("wf_token_logprobs", ctypes.c_int,
+         [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+        ("wf_token_logprobs_backward", ctypes.c_int,
+         [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    ):
+        f = getattr(lib, name)
+        f.restype, f.argtypes = restype, argtypes
 
 
 def load_library() -> ctypes.CDLL:
@@ -212,6 +243,22 @@ def workspace(B: int, Tq: int, Tk: int, R: int, top_k: int, dtype: torch.dtype, 
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """Context that makes ``dev`` current; nothing is entered when it already is."""
+    return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as (rows, last axis) with unit-strided, non-overlapping rows (copied only if it has to be)."""
+    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if (r.stride(1) != 1 and r.shape[1] > 1) or (r.stride(0) < r.shape[1] and r.shape[0] > 1):
+        r = r.contiguous()
+    return r
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

@@ -126,6 +126,49 @@ int check_attn(const void* q, const void* k, const void* v, int32_t dtype, const
   return WF_OK;
 }
 
+int check_workspace(const char* what, const void* ws, size_t bytes, size_t need) {
+  if (need && (!ws || bytes < need || reinterpret_cast<uintptr_t>(ws) % 256))
+    return fail(WF_ERR_INVALID_ARGUMENT, "%s: workspace missing, not 256-byte aligned or smaller than %zu bytes "
+                "(%s_workspace_bytes)", what, need, what);
+  return WF_OK;
+}
+
+int check_linear(const char* what, int32_t dtype, int64_t M, int64_t N, int64_t K, int64_t x_stride, int64_t w_stride,
+                 int32_t act) {
+  if (!valid_dtype(dtype)) return fail(WF_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (M < 0 || N < 0 || K < 1)
+    return fail(WF_ERR_INVALID_ARGUMENT, "%s: bad sizes (M=%lld, N=%lld, K=%lld)", what, (long long)M, (long long)N,
+                (long long)K);
+  // sizes stay below 2^30 so that tile arithmetic in 32 bits has room
+  if (M >= (1 << 30) || N >= (1 << 30) || K >= (1 << 30))
+    return fail(WF_ERR_UNSUPPORTED, "%s: sizes must be below 2^30", what);
+  if (act < WF_ACT_NONE || act > WF_ACT_SILU) return fail(WF_ERR_INVALID_ARGUMENT, "unknown activation %d", act);
+  if (x_stride < K || w_stride < K) return fail(WF_ERR_INVALID_ARGUMENT, "row strides must cover the rows");
+  return WF_OK;
+}
+
+int check_norm(int32_t dtype, int64_t rows, int64_t d, int32_t param_dtype, int64_t x_stride) {
+  if (!valid_dtype(dtype)) return fail(WF_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (param_dtype != dtype && param_dtype != WF_DTYPE_F32)
+    return fail(WF_ERR_INVALID_ARGUMENT, "weight and bias must be fp32 or of the input's type");
+  if (rows < 0 || d < 1) return fail(WF_ERR_INVALID_ARGUMENT, "bad sizes (rows=%lld, d=%lld)", (long long)rows,
+                                     (long long)d);
+  if (rows > kI32Max || d >= (1 << 30)) return fail(WF_ERR_UNSUPPORTED, "sizes too large (rows < 2^31, d < 2^30)");
+  if (x_stride < 0) return fail(WF_ERR_INVALID_ARGUMENT, "negative row stride");
+  return WF_OK;
+}
+
+int check_logits(int32_t dtype, int64_t rows, int64_t vocab, int64_t stride) {
+  if (!valid_dtype(dtype)) return fail(WF_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (rows < 0 || vocab < 1) return fail(WF_ERR_INVALID_ARGUMENT, "bad sizes (rows=%lld, vocab=%lld)", (long long)rows,
+                                         (long long)vocab);
+  if (stride < 0) return fail(WF_ERR_INVALID_ARGUMENT, "negative row stride");
+  // a block takes a row, or 4096 elements of one in the backward
+  if (vocab >= (1 << 30) || rows > kI32Max / ((vocab + 4095) / 4096))
+    return fail(WF_ERR_UNSUPPORTED, "sizes too large (vocab < 2^30, rows * vocab / 4096 < 2^31)");
+  return WF_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -740,6 +783,161 @@ int wf_causal_topk_key_mask(const void* q_addr, const void* k_addr, int32_t dtyp
                                 static_cast<cudaStream_t>(stream));
   if (rc) return cuda_fail(rc, "wf_causal_topk_key_mask");
   return ok();
+}
+
+
+size_t wf_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+  if (M <= 0 || N <= 0 || K <= 0 || !valid_dtype(dtype)) return 0;
+  return wf::linear_workspace_bytes(M, N, K, dtype);
+}
+
+size_t wf_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation) {
+  if (M <= 0 || N <= 0 || K <= 0 || !valid_dtype(dtype)) return 0;
+  return wf::linear_backward_workspace_bytes(M, N, K, dtype, activation);
+}
+
+int wf_linear(const void* x, const void* w, const void* bias, const void* residual, int32_t dtype, int64_t M,
+              int64_t N, int64_t K, int64_t x_row_stride, int64_t w_row_stride, int64_t r_row_stride,
+              int32_t activation, void* z, void* y, void* workspace, size_t workspace_bytes, int32_t* status,
+              void* stream) {
+  int rc = check_linear("wf_linear", dtype, M, N, K, x_row_stride, w_row_stride, activation);
+  if (rc) return rc;
+  if (M == 0 || N == 0) return ok();
+  if (!x || !w || !y) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (residual && r_row_stride < 0) return fail(WF_ERR_INVALID_ARGUMENT, "negative residual stride");
+  if ((rc = check_workspace("wf_linear", workspace, workspace_bytes, wf::linear_workspace_bytes(M, N, K, dtype))))
+    return rc;
+  wf::LinearParams p{};
+  p.x = x; p.w = w; p.bias = bias; p.residual = residual; p.z = z; p.y = y;
+  p.M = M; p.N = N; p.K = K;
+  p.x_stride = x_row_stride; p.w_stride = w_row_stride; p.r_stride = r_row_stride;
+  p.act = activation;
+  p.ws = workspace;
+  p.status = status;
+  rc = wf::launch_linear(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_linear") : ok();
+}
+
+int wf_linear_backward(const void* x, const void* w, const void* z, const void* dy, int32_t dtype, int64_t M,
+                       int64_t N, int64_t K, int64_t x_row_stride, int64_t w_row_stride, int64_t dy_row_stride,
+                       int32_t activation, void* dx, void* dw, void* dbias, void* workspace, size_t workspace_bytes,
+                       int32_t* status, void* stream) {
+  int rc = check_linear("wf_linear_backward", dtype, M, N, K, x_row_stride, w_row_stride, activation);
+  if (rc) return rc;
+  if (N == 0) return ok();
+  if (M > 0) {
+    if (!x || !w || !dy) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+    if (dy_row_stride < N) return fail(WF_ERR_INVALID_ARGUMENT, "row strides must cover the rows");
+    if (activation != WF_ACT_NONE && !z)
+      return fail(WF_ERR_INVALID_ARGUMENT, "z: the forward's pre-activations are needed with an activation");
+    if ((rc = check_workspace("wf_linear_backward", workspace, workspace_bytes,
+                              wf::linear_backward_workspace_bytes(M, N, K, dtype, activation))))
+      return rc;
+  }
+  wf::LinearBwdParams p{};
+  p.x = x; p.w = w; p.z = z; p.dy = dy; p.dx = dx; p.dw = dw; p.db = dbias;
+  p.M = M; p.N = N; p.K = K;
+  p.x_stride = x_row_stride; p.w_stride = w_row_stride; p.dy_stride = dy_row_stride;
+  p.act = activation;
+  p.ws = workspace;
+  p.status = status;
+  rc = wf::launch_linear_backward(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_linear_backward") : ok();
+}
+
+int wf_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t d, int64_t x_row_stride, const void* weight,
+                  const void* bias, int32_t param_dtype, float eps, void* y, int64_t y_row_stride, float* mean,
+                  float* rstd, void* stream) {
+  int rc = check_norm(dtype, rows, d, param_dtype, x_row_stride);
+  if (rc) return rc;
+  if (!(eps >= 0.f)) return fail(WF_ERR_INVALID_ARGUMENT, "eps must be >= 0, got %g", (double)eps);
+  if (rows == 0) return ok();
+  if (!x || !y || !mean != !rstd) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (y_row_stride < d) return fail(WF_ERR_INVALID_ARGUMENT, "row strides must cover the rows");
+  wf::LayerNormParams p{};
+  p.x = x; p.y = y; p.weight = weight; p.bias = bias; p.mean = mean; p.rstd = rstd;
+  p.rows = rows; p.x_stride = x_row_stride; p.y_stride = y_row_stride;
+  p.d = (int)d;
+  p.param_f32 = param_dtype == WF_DTYPE_F32;
+  p.eps = eps;
+  rc = wf::launch_layer_norm(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_layer_norm") : ok();
+}
+
+size_t wf_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d, int32_t dtype) {
+  if (rows <= 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  return wf::layer_norm_backward_workspace_bytes(rows, d, dtype);
+}
+
+int wf_layer_norm_backward(const void* x, const void* dy, int32_t dtype, int64_t rows, int64_t d, int64_t x_row_stride,
+                           int64_t dy_row_stride, const void* weight, int32_t param_dtype, const float* mean,
+                           const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  int rc = check_norm(dtype, rows, d, param_dtype, x_row_stride);
+  if (rc) return rc;
+  const bool params = dweight || dbias;
+  if (rows == 0) {
+    const size_t n = (size_t)d * dtype_size(param_dtype);
+    for (void* q : {dweight, dbias})
+      if (q)
+        if (cudaError_t e = cudaMemsetAsync(q, 0, n, static_cast<cudaStream_t>(stream)))
+          return cuda_fail((int)e, "wf_layer_norm_backward");
+    return ok();
+  }
+  if (!x || !dy || !mean || !rstd) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (dy_row_stride < d) return fail(WF_ERR_INVALID_ARGUMENT, "row strides must cover the rows");
+  if (!dx && !params) return ok();
+  if (params && (rc = check_workspace("wf_layer_norm_backward", workspace, workspace_bytes,
+                                      wf::layer_norm_backward_workspace_bytes(rows, d, dtype))))
+    return rc;
+  wf::LayerNormBwdParams p{};
+  p.x = x; p.dy = dy; p.weight = weight; p.mean = mean; p.rstd = rstd;
+  p.dx = dx; p.dweight = dweight; p.dbias = dbias;
+  p.partials = params ? static_cast<float*>(workspace) : nullptr;
+  p.rows = rows; p.x_stride = x_row_stride; p.dy_stride = dy_row_stride;
+  p.d = (int)d;
+  p.param_f32 = param_dtype == WF_DTYPE_F32;
+  rc = wf::launch_layer_norm_backward(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_layer_norm_backward") : ok();
+}
+
+int wf_max_top_tokens(void) { return wf::kMaxTopTokens; }
+
+int wf_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                      const int64_t* tokens, int64_t ignore_index, int32_t top_n, float* logprob, float* entropy,
+                      float* stats, float* top_logprobs, int64_t* top_tokens, int32_t* status, void* stream) {
+  int rc = check_logits(dtype, rows, vocab, row_stride);
+  if (rc) return rc;
+  if (top_n < 0 || top_n > vocab) return fail(WF_ERR_INVALID_ARGUMENT, "top_n must be in [0, vocab], got %d", top_n);
+  if (top_n > wf::kMaxTopTokens)
+    return fail(WF_ERR_UNSUPPORTED, "top_n=%d exceeds this build's maximum of %d", top_n, wf::kMaxTopTokens);
+  if (rows == 0) return ok();
+  if (!logits || !tokens || !logprob || !entropy || (top_n && (!top_logprobs || !top_tokens)))
+    return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  wf::LogprobParams p{};
+  p.x = logits; p.tokens = tokens; p.logprob = logprob; p.entropy = entropy; p.stats = stats;
+  p.top_logprobs = top_logprobs; p.top_tokens = top_tokens;
+  p.rows = rows; p.x_stride = row_stride; p.vocab = vocab; p.ignore_index = ignore_index;
+  p.top_n = top_n;
+  p.status = status;
+  rc = wf::launch_token_logprobs(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_token_logprobs") : ok();
+}
+
+int wf_token_logprobs_backward(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                               const int64_t* tokens, int64_t ignore_index, const float* stats, const float* entropy,
+                               const float* dlogprob, const float* dentropy, void* dlogits, void* stream) {
+  int rc = check_logits(dtype, rows, vocab, row_stride);
+  if (rc) return rc;
+  if (rows == 0) return ok();
+  if (!logits || !tokens || !stats || !entropy || !dlogits)
+    return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  wf::LogprobBwdParams p{};
+  p.x = logits; p.tokens = tokens; p.stats = stats; p.entropy = entropy; p.dlogprob = dlogprob; p.dentropy = dentropy;
+  p.dx = dlogits;
+  p.rows = rows; p.x_stride = row_stride; p.vocab = vocab; p.ignore_index = ignore_index;
+  rc = wf::launch_token_logprobs_backward(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_token_logprobs_backward") : ok();
 }
 
 }  // extern "C"

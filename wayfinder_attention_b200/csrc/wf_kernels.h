@@ -138,4 +138,97 @@ int launch_gather_rows_bulk_bench(const void* k, const void* v, int64_t stride_b
                                   int64_t n_query, int K, int64_t n_rows, int read_back, uint32_t* sink,
                                   cudaStream_t stream);
 
+// Layer norm over the last axis (wf_layer_norm.cu).  Rows are unit-strided; weight and
+// bias may be null.
+struct LayerNormParams {
+  const void* x;
+  void* y;
+  const void* weight;
+  const void* bias;
+  float* mean;   // [rows], with rstd; both null when the backward will not run
+  float* rstd;
+  int64_t rows, x_stride, y_stride;
+  int d;
+  bool param_f32;  // weight and bias are fp32 (otherwise of x's type)
+  float eps;
+};
+struct LayerNormBwdParams {
+  const void* x;
+  const void* dy;
+  const void* weight;
+  const float* mean;
+  const float* rstd;
+  void* dx;         // [rows][d] or null
+  void* dweight;    // [d], null with dbias when neither is wanted
+  void* dbias;
+  float* partials;  // workspace; null when no parameter gradient is wanted
+  int64_t rows, x_stride, dy_stride;
+  int d;
+  bool param_f32;
+};
+int launch_layer_norm(const LayerNormParams& p, int dtype, cudaStream_t stream);
+size_t layer_norm_backward_workspace_bytes(int64_t rows, int64_t d, int dtype);
+int launch_layer_norm_backward(const LayerNormBwdParams& p, int dtype, cudaStream_t stream);
+
+// Log probabilities of given tokens (wf_logprobs.cu).
+constexpr int kMaxTopTokens = 32;
+struct LogprobParams {
+  const void* x;          // [rows][vocab], unit stride on the vocabulary
+  const int64_t* tokens;  // [rows]
+  float* logprob;
+  float* entropy;
+  float* stats;           // [2][rows] for the backward, or null: the maximum m, and log sum exp(x - m)
+  float* top_logprobs;    // [rows][top_n]
+  int64_t* top_tokens;
+  int64_t rows, x_stride, vocab, ignore_index;
+  int top_n;
+  int cluster;            // blocks a row (set by the launch)
+  int32_t* status;        // nullable; bit 0 set on a token outside the vocabulary
+};
+struct LogprobBwdParams {
+  const void* x;
+  const int64_t* tokens;
+  const float* stats;
+  const float* entropy;
+  const float* dlogprob;  // [rows] or null
+  const float* dentropy;  // [rows] or null
+  void* dx;               // [rows][vocab]
+  int64_t rows, x_stride, vocab, ignore_index;
+};
+int launch_token_logprobs(const LogprobParams& p, int dtype, cudaStream_t stream);
+int launch_token_logprobs_backward(const LogprobBwdParams& p, int dtype, cudaStream_t stream);
+
+// Linear layer with bias, activation and residual (wf_linear.cu).  x (M, K) and
+// w (N, K) are unit-strided on K; y, z and the gradients are contiguous.
+enum Activation : int { kActNone = 0, kActGelu = 1, kActRelu = 2, kActSilu = 3 };
+struct LinearParams {
+  const void* x;
+  const void* w;
+  const void* bias;      // [N] or null
+  const void* residual;  // (M, N) or null
+  void* z;               // (M, N) pre-activations for the backward, or null
+  void* y;
+  int64_t M, N, K, x_stride, w_stride, r_stride;
+  int act;
+  void* ws;
+  int32_t* status;
+};
+struct LinearBwdParams {
+  const void* x;
+  const void* w;
+  const void* z;
+  const void* dy;
+  void* dx;  // each of the three may be null
+  void* dw;
+  void* db;
+  int64_t M, N, K, x_stride, w_stride, dy_stride;
+  int act;
+  void* ws;
+  int32_t* status;
+};
+size_t linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act);
+int launch_linear(const LinearParams& p, int dtype, cudaStream_t stream);
+int launch_linear_backward(const LinearBwdParams& p, int dtype, cudaStream_t stream);
+
 }  // namespace wf

@@ -1,0 +1,52 @@
+// Row access shared by the row-wise kernels (layer norm, token log probabilities):
+// 16-byte vectors where rows allow them, single elements otherwise, always widened
+// to fp32 for arithmetic.
+#pragma once
+
+#include "wf_common.cuh"
+
+namespace wf {
+
+// VEC consecutive elements as loaded (VEC = 1 or 16 / sizeof(T)).
+template <typename T, int VEC> struct RawVec;
+template <typename T> struct RawVec<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void clear() { v = from_f32<T>(0.f); }
+  __device__ __forceinline__ void unpack(float* f) const { f[0] = to_f32(v); }
+};
+template <typename T, int VEC> struct RawVec {
+  static_assert(VEC == Vec16<T>::N, "vectors are 16 bytes");
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void clear() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void unpack(float* f) const { Vec16<T>::unpack(v, f); }
+};
+
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(__half, float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Rounds VEC fp32 values once to T and stores them.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float* f) {
+  if constexpr (VEC == 1) {
+    *p = from_f32<T>(f[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  } else {
+    uint4 r;
+    r.x = pack2(T(), f[0], f[1]);
+    r.y = pack2(T(), f[2], f[3]);
+    r.z = pack2(T(), f[4], f[5]);
+    r.w = pack2(T(), f[6], f[7]);
+    *reinterpret_cast<uint4*>(p) = r;
+  }
+}
+
+}  // namespace wf
