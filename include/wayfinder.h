@@ -385,7 +385,10 @@ WF_API int wf_testing_withhold_pair_arrive(int32_t round, uint64_t wait_limit_ns
  *   z        : (M, N) contiguous, gets x W^T + b for the backward (rounded to dtype); may
  *              be NULL
  *   y        : (M, N) contiguous
- *   workspace: wf_linear_workspace_bytes() bytes, 256-byte aligned (NULL if that is 0)
+ *   workspace: wf_linear_workspace_bytes() bytes, 256-byte aligned (NULL if that is 0); its
+ *              x_direct / w_direct (dy_direct in the backward) say whether that matrix
+ *              starts on a 16-byte boundary and each of its rows does: others are laid
+ *              out in the workspace, and so are fp32 ones
  *   status   : optional device int32; bit 1 is OR-ed in if a bounded wait timed out
  * K = 0 is refused; M = 0 or N = 0 does nothing.
  */
@@ -393,7 +396,8 @@ WF_API int wf_testing_withhold_pair_arrive(int32_t round, uint64_t wait_limit_ns
 #define WF_ACT_GELU 1 /* z Phi(z), the erf form */
 #define WF_ACT_RELU 2
 #define WF_ACT_SILU 3
-WF_API size_t wf_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype);
+WF_API size_t wf_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t x_direct,
+                                        int32_t w_direct);
 WF_API int wf_linear(const void* x, const void* w, const void* bias, const void* residual, int32_t dtype, int64_t M,
                      int64_t N, int64_t K, int64_t x_row_stride, int64_t w_row_stride, int64_t r_row_stride,
                      int32_t activation, void* z, void* y, void* workspace, size_t workspace_bytes, int32_t* status,
@@ -404,7 +408,8 @@ WF_API int wf_linear(const void* x, const void* w, const void* bias, const void*
  * WF_ACT_NONE).  dx (M, K), dw (N, K) and dbias (N) are contiguous, of dtype, and each
  * may be NULL.  The result does not depend on scheduling (no atomics on sums).
  */
-WF_API size_t wf_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation);
+WF_API size_t wf_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation,
+                                                 int32_t x_direct, int32_t w_direct, int32_t dy_direct);
 WF_API int wf_linear_backward(const void* x, const void* w, const void* z, const void* dy, int32_t dtype, int64_t M,
                               int64_t N, int64_t K, int64_t x_row_stride, int64_t w_row_stride, int64_t dy_row_stride,
                               int32_t activation, void* dx, void* dw, void* dbias, void* workspace,

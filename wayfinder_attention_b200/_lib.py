@@ -173,8 +173,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     ]
     sz = ctypes.c_size_t
     for name, restype, argtypes in (
-        ("wf_linear_workspace_bytes", sz, [_i64, _i64, _i64, _i32]),
-        ("wf_linear_backward_workspace_bytes", sz, [_i64, _i64, _i64, _i32, _i32]),
+        ("wf_linear_workspace_bytes", sz, [_i64] * 3 + [_i32] * 3),
+        ("wf_linear_backward_workspace_bytes", sz, [_i64] * 3 + [_i32] * 5),
         ("wf_linear", ctypes.c_int, [_vp] * 4 + [_i32] + [_i64] * 6 + [_i32, _vp, _vp, _vp, sz, _vp, _vp]),
         ("wf_linear_backward", ctypes.c_int,
          [_vp] * 4 + [_i32] + [_i64] * 6 + [_i32, _vp, _vp, _vp, _vp, sz, _vp, _vp]),
@@ -243,6 +243,11 @@ def workspace(B: int, Tq: int, Tk: int, R: int, top_k: int, dtype: torch.dtype, 
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_16_bytes(t: torch.Tensor) -> bool:
+    """Whether every row of a (rows, columns) tensor starts on a 16-byte boundary."""
+    return t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0
 
 
 _here = contextlib.nullcontext()

@@ -133,6 +133,10 @@ int check_workspace(const char* what, const void* ws, size_t bytes, size_t need)
   return WF_OK;
 }
 
+bool on_16_bytes(const void* p, int64_t row_stride, int32_t dtype) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (row_stride * dtype_size(dtype)) % 16 == 0;
+}
+
 int check_linear(const char* what, int32_t dtype, int64_t M, int64_t N, int64_t K, int64_t x_stride, int64_t w_stride,
                  int32_t act) {
   if (!valid_dtype(dtype)) return fail(WF_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
@@ -786,14 +790,15 @@ int wf_causal_topk_key_mask(const void* q_addr, const void* k_addr, int32_t dtyp
 }
 
 
-size_t wf_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype) {
+size_t wf_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t x_direct, int32_t w_direct) {
   if (M <= 0 || N <= 0 || K <= 0 || !valid_dtype(dtype)) return 0;
-  return wf::linear_workspace_bytes(M, N, K, dtype);
+  return wf::linear_workspace_bytes(M, N, K, dtype, x_direct, w_direct);
 }
 
-size_t wf_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation) {
+size_t wf_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t activation,
+                                          int32_t x_direct, int32_t w_direct, int32_t dy_direct) {
   if (M <= 0 || N <= 0 || K <= 0 || !valid_dtype(dtype)) return 0;
-  return wf::linear_backward_workspace_bytes(M, N, K, dtype, activation);
+  return wf::linear_backward_workspace_bytes(M, N, K, dtype, activation, x_direct, w_direct, dy_direct);
 }
 
 int wf_linear(const void* x, const void* w, const void* bias, const void* residual, int32_t dtype, int64_t M,
@@ -805,7 +810,9 @@ int wf_linear(const void* x, const void* w, const void* bias, const void* residu
   if (M == 0 || N == 0) return ok();
   if (!x || !w || !y) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
   if (residual && r_row_stride < 0) return fail(WF_ERR_INVALID_ARGUMENT, "negative residual stride");
-  if ((rc = check_workspace("wf_linear", workspace, workspace_bytes, wf::linear_workspace_bytes(M, N, K, dtype))))
+  if ((rc = check_workspace("wf_linear", workspace, workspace_bytes, wf::linear_workspace_bytes(
+                                            M, N, K, dtype, on_16_bytes(x, x_row_stride, dtype),
+                                            on_16_bytes(w, w_row_stride, dtype)))))
     return rc;
   wf::LinearParams p{};
   p.x = x; p.w = w; p.bias = bias; p.residual = residual; p.z = z; p.y = y;
@@ -831,7 +838,9 @@ int wf_linear_backward(const void* x, const void* w, const void* z, const void* 
     if (activation != WF_ACT_NONE && !z)
       return fail(WF_ERR_INVALID_ARGUMENT, "z: the forward's pre-activations are needed with an activation");
     if ((rc = check_workspace("wf_linear_backward", workspace, workspace_bytes,
-                              wf::linear_backward_workspace_bytes(M, N, K, dtype, activation))))
+                              wf::linear_backward_workspace_bytes(
+                                  M, N, K, dtype, activation, on_16_bytes(x, x_row_stride, dtype),
+                                  on_16_bytes(w, w_row_stride, dtype), on_16_bytes(dy, dy_row_stride, dtype)))))
       return rc;
   }
   wf::LinearBwdParams p{};

@@ -7,6 +7,8 @@
 
 namespace wf {
 
+constexpr int kSms = 148;  // of a B200
+
 // Causal top-K over address vectors.
 //   query rows:  q[b, l, :]  for local row l in [0, Tq); its sequence position
 //                g(l) = ((l / rt) * rs + r0) * rt + l % rt   (identity when rs=1, r0=0, rt>=Tq)
@@ -226,8 +228,10 @@ struct LinearBwdParams {
   void* ws;
   int32_t* status;
 };
-size_t linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
-size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act);
+// *_direct: the matrix starts on 16 bytes and so does each of its rows.
+size_t linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct, bool w_direct);
+size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act, bool x_direct,
+                                       bool w_direct, bool dy_direct);
 int launch_linear(const LinearParams& p, int dtype, cudaStream_t stream);
 int launch_linear_backward(const LinearBwdParams& p, int dtype, cudaStream_t stream);
 

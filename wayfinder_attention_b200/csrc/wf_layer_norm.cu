@@ -337,7 +337,7 @@ int backward_blocks(int64_t rows, const Shape& s) {
   const int64_t groups = s.warps == 1 ? (rows + 7) / 8 : rows;
   // resident blocks an SM: 2048 threads' worth at about 64 registers each is half of that
   const int per_sm = s.warps == 1 ? 4 : s.warps == 4 ? 8 : s.warps == 8 ? 4 : 2;
-  const int64_t most = 148 * per_sm;
+  const int64_t most = kSms * per_sm;
   return (int)(groups < most ? groups : most);
 }
 

@@ -1,4 +1,4 @@
-// Linear layer with its epilogue, forward and backward.
+// Linear layer with its epilogue, forward and backward, on the tensor-core product.
 //
 //   forward   z = x W^T + b,  y = act(z) + residual
 //   backward  dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum_rows dz
@@ -6,214 +6,281 @@
 // act: none, gelu (z Phi(z), Phi by erf), relu, silu (z sigmoid(z)).  Products and sums
 // are fp32; y is rounded once.  The backward reads z as the forward rounded it to the
 // activations' type, and rounds dz to that type before the two products, as operands of
-// that type are what the products take.
+// that type are what the products take; db sums the unrounded values.
+//
+// The product reads 16-bit matrices whose rows start on 16 bytes.  Others are laid out in
+// the workspace first: 16-bit rows of any width or offset are copied to such rows, and an
+// fp32 matrix becomes three bf16 pieces, x = x0 + x1 + x2 to fp32's last bit.
+#include "wf_activation.cuh"
 #include "wf_columns.cuh"
-#include "wf_kernels.h"
+#include "wf_gemm.h"
 #include "wf_rowio.cuh"
+
+#include <type_traits>
 
 namespace wf {
 namespace {
 
-__device__ __forceinline__ float gelu_cdf(float z) { return 0.5f * (1.f + erff(z * 0.70710678118654752f)); }
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
-__device__ __forceinline__ float activate(int act, float z) {
-  switch (act) {
-    case kActGelu: return z * gelu_cdf(z);
-    case kActRelu: return z < 0.f ? 0.f : z;  // NaN stays
-    case kActSilu: return z * sigmoid(z);
-    default: return z;
-  }
-}
-__device__ __forceinline__ float activation_slope(int act, float z) {
-  switch (act) {
-    case kActGelu: return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), gelu_cdf(z));
-    case kActRelu: return z > 0.f ? 1.f : 0.f;
-    case kActSilu: {
-      const float s = sigmoid(z);
-      return s * fmaf(z, 1.f - s, 1.f);
-    }
-    default: return 1.f;
-  }
+// x = p[0] + p[1] + p[2], each a rounding of what the ones before leave.  Infinities and
+// NaN stay in p[0] alone; what would round to infinity is cut instead.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16* p) {
+  p[0] = __float2bfloat16_rn(x);
+  if (isinf(__bfloat162float(p[0])) && !isinf(x)) p[0] = __float2bfloat16_rz(x);
+  float r = isfinite(x) ? x - __bfloat162float(p[0]) : 0.f;
+  p[1] = __float2bfloat16_rn(r);
+  p[2] = __float2bfloat16_rn(r - __bfloat162float(p[1]));
 }
 
-// C[m][n] = sum_k A(m, k) B(n, k) over any element strides, then the epilogue.
-struct GemmParams {
-  const void* a;
-  const void* b;
-  int64_t am, ak, bn, bk;
-  int64_t M, N, K;
-  const void* bias;
-  const void* residual;
-  void* z;
-  void* y;
-  int64_t r_stride, z_stride, y_stride;
-  int act;
-};
-
-constexpr int kTile = 64, kDepth = 16;
+// 8 fp32 values to the operand at column c of a row: one 16-byte store a piece (the
+// operand's rows are padded to whole vectors).
 template <typename T>
-__global__ void __launch_bounds__(256) gemm_kernel(GemmParams p) {
-  __shared__ float as[kDepth][kTile + 4], bs[kDepth][kTile + 4];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
-  const T* a = static_cast<const T*>(p.a);
-  const T* b = static_cast<const T*>(p.b);
-  // two levels of sums: a long one loses bits with its length
-  float acc[4][4] = {}, sum[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.K; k0 += kDepth) {
-    if (k0 % 256 == 0)
+__device__ __forceinline__ void store_operand(void* out, int64_t at, int64_t piece, const float* f) {
+  if constexpr (std::is_same<T, float>::value) {
+    __nv_bfloat16 p[8][3];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 8; ++j) split3(f[j], p[j]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          sum[i][j] += acc[i][j];
-          acc[i][j] = 0.f;
-        }
-    for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-      // the unit-strided axis runs over the threads
-      const int ka = p.ak == 1 ? i % kDepth : i / kTile, ma = p.ak == 1 ? i / kDepth : i % kTile;
-      const int kb = p.bk == 1 ? i % kDepth : i / kTile, nb = p.bk == 1 ? i / kDepth : i % kTile;
-      as[ka][ma] = m0 + ma < p.M && k0 + ka < p.K ? to_f32(a[(m0 + ma) * p.am + (k0 + ka) * p.ak]) : 0.f;
-      bs[kb][nb] = n0 + nb < p.N && k0 + kb < p.K ? to_f32(b[(n0 + nb) * p.bn + (k0 + kb) * p.bk]) : 0.f;
+    for (int k = 0; k < 3; ++k) {
+      uint4 v;
+      uint32_t* u = &v.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __nv_bfloat162 h;
+        h.x = p[2 * j][k];
+        h.y = p[2 * j + 1][k];
+        u[j] = *reinterpret_cast<uint32_t*>(&h);
+      }
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + k * piece + at) = v;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[k][ty * 4 + i], bs[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+  } else {
+    store_vec<T, 8>(static_cast<T*>(out) + at, f);
   }
+}
+
+// 8 values of a row from column c (zeros past the end), by vectors where the row allows it.
+template <typename T>
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, bool vec, float* f) {
+  if (vec && c + 8 <= cols) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 8; j += Vec16<T>::N) Vec16<T>::unpack(ldg16(row + c + j), f + j);
+  } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m >= p.M || n >= p.N) continue;
-      float v = sum[i][j] + acc[i][j];
-      if (p.bias) v += to_f32(static_cast<const T*>(p.bias)[n]);
-      if (p.z) static_cast<T*>(p.z)[m * p.z_stride + n] = from_f32<T>(v);
-      v = activate(p.act, v);
-      if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[m * p.r_stride + n]);
-      static_cast<T*>(p.y)[m * p.y_stride + n] = from_f32<T>(v);
-    }
+    for (int j = 0; j < 8; ++j) f[j] = c + j < cols ? to_f32(row[c + j]) : 0.f;
+  }
 }
 
 template <typename T>
-int launch_gemm(const GemmParams& p, cudaStream_t stream) {
-  if (p.M == 0 || p.N == 0) return 0;
-  gemm_kernel<T><<<dim3((unsigned)((p.N + kTile - 1) / kTile), (unsigned)((p.M + kTile - 1) / kTile)), 256, 0,
-                   stream>>>(p);
+__global__ void __launch_bounds__(256) lay_out_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, bool vec,
+                                                      void* out, int64_t pitch, int64_t piece) {
+  const int64_t groups = pitch / 8, total = rows * groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups, c = i % groups * 8;
+    float f[8];
+    load8(x + r * stride, c, cols, vec, f);
+    store_operand<T>(out, r * pitch + c, piece, f);
+  }
+}
+
+// dz = dy act'(z) into the operand's layout, and partial column sums: a block takes 256
+// columns (8 a lane) of a share of the rows, its 8 warps a row each.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_stride, bool dy_vec, const T* z,
+                                                        void* out, int64_t pitch, int64_t piece, int64_t M, int64_t N,
+                                                        float* partials) {
+  __shared__ float red[8][32][9];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * 8;
+  float s[8] = {};
+  if (c < N)
+    for (int64_t m = (int64_t)blockIdx.y * 8 + warp; m < M; m += (int64_t)gridDim.y * 8) {
+      float g[8];
+      load8(dy + m * dy_stride, c, N, dy_vec, g);
+      if constexpr (ACT != kActNone) {
+        float f[8];
+        load8(z + m * N, c, N, N % 8 == 0, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] *= activation_slope<ACT>(f[j]);
+      }
+      if (out) store_operand<T>(out, m * pitch + c, piece, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += g[j];
+    }
+  if (!partials) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[warp][lane][j] = s[j];
+  __syncthreads();
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (col < N) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += red[i][threadIdx.x / 8][threadIdx.x % 8];
+    partials[(size_t)blockIdx.y * N + col] = v;
+  }
+}
+
+// Row shares of the column sums: eight blocks an SM over all columns, 32 rows at least.
+int row_shares(int64_t M, int64_t N) {
+  const int64_t by = (N + 255) / 256, want = (8 * kSms + by - 1) / by, most = (M + 31) / 32;
+  return (int)(want < most ? want : most);
+}
+
+template <typename T>
+constexpr int kPieces = std::is_same<T, float>::value ? 3 : 1;
+
+template <typename T>
+bool on_16_bytes(const void* p, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
+}
+
+// A (rows, cols) matrix as the product reads it: itself, or laid out at *ws, which moves on.
+size_t operand_bytes(int64_t rows, int64_t cols, int dtype) {
+  return round256((size_t)rows * round8(cols) * 2 * (dtype == kF32 ? 3 : 1));
+}
+template <typename T>
+GemmOperand blank_operand(int64_t rows, int64_t cols, int dtype, unsigned char** ws) {
+  GemmOperand o{};
+  o.ptr = *ws;
+  o.rows = rows;
+  o.cols = cols;
+  o.pitch = round8(cols);
+  o.piece_stride = rows * o.pitch;
+  *ws += operand_bytes(rows, cols, dtype);
+  return o;
+}
+template <typename T>
+int operand(const void* x, int64_t rows, int64_t cols, int64_t stride, int dtype, unsigned char** ws, GemmOperand* o,
+            cudaStream_t stream) {
+  const bool vec = on_16_bytes<T>(x, stride);
+  if (dtype != kF32 && vec) {
+    *o = GemmOperand{x, rows, cols, stride, 0, false};
+    return 0;
+  }
+  *o = blank_operand<T>(rows, cols, dtype, ws);
+  const int64_t blocks = (rows * (o->pitch / 8) + 255) / 256;
+  lay_out_kernel<T><<<(unsigned)(blocks < 16 * kSms ? blocks : 16 * kSms), 256, 0, stream>>>(
+      static_cast<const T*>(x), rows, cols, stride, vec, const_cast<void*>(o->ptr), o->pitch, o->piece_stride);
   return (int)cudaGetLastError();
 }
 
-// dz = dy act'(z) and the partial column sums of dz (of the unrounded values): a warp
-// owns a column a lane, the block's 8 warps and the grid's y share the rows.
 template <typename T>
-__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_stride, const T* z, T* dz, int64_t M,
-                                                        int64_t N, int act, float* partials) {
-  __shared__ float red[8][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (c < N)
-    for (int64_t m = (int64_t)blockIdx.y * 8 + warp; m < M; m += (int64_t)gridDim.y * 8) {
-      float g = to_f32(dy[m * dy_stride + c]);
-      if (z) {
-        g *= activation_slope(act, to_f32(z[m * N + c]));
-        dz[m * N + c] = from_f32<T>(g);
-      }
-      s += g;
-    }
-  red[warp][lane] = s;
-  __syncthreads();
-  if (warp == 0 && c < N && partials) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][lane];
-    partials[(size_t)blockIdx.y * N + c] = s;
-  }
-}
-
-int row_shares(int64_t M) { return (int)(M <= 64 ? 1 : M / 64 < 64 ? M / 64 : 64); }
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-
-template <typename T>
-int launch_fwd(const LinearParams& p, cudaStream_t stream) {
-  GemmParams g{};
-  g.a = p.x; g.am = p.x_stride; g.ak = 1;
-  g.b = p.w; g.bn = p.w_stride; g.bk = 1;
-  g.M = p.M; g.N = p.N; g.K = p.K;
-  g.bias = p.bias; g.residual = p.residual; g.r_stride = p.r_stride;
-  g.z = p.z; g.z_stride = p.N;
-  g.y = p.y; g.y_stride = p.N;
-  g.act = p.act;
-  return launch_gemm<T>(g, stream);
+GemmProblem problem(const GemmOperand& a, const GemmOperand& b, int64_t M, int64_t N, int64_t K, int dtype, void* ws,
+                    int32_t* status) {
+  GemmProblem g{};
+  g.a = a;
+  g.b = b;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.pieces = kPieces<T>;
+  g.op_dtype = dtype == kF16 ? kF16 : kBF16;
+  g.out_dtype = dtype;
+  g.ws = ws;
+  g.status = status;
+  return g;
 }
 
 template <typename T>
-int launch_bwd(const LinearBwdParams& p, cudaStream_t stream) {
-  const T* dz = static_cast<const T*>(p.dy);
-  int64_t dz_stride = p.dy_stride;
+int launch_fwd(const LinearParams& p, int dtype, cudaStream_t stream) {
   unsigned char* ws = static_cast<unsigned char*>(p.ws);
-  if (p.M > 0 && (p.act != kActNone || p.db)) {
-    T* out = nullptr;
-    if (p.act != kActNone) {
-      out = reinterpret_cast<T*>(ws);
-      ws += round256((size_t)p.M * p.N * sizeof(T));
-      dz = out;
-      dz_stride = p.N;
-    }
-    float* partials = p.db ? reinterpret_cast<float*>(ws) : nullptr;
-    const int shares = row_shares(p.M);
-    linear_dz_kernel<T><<<dim3((unsigned)((p.N + 31) / 32), shares), 256, 0, stream>>>(
-        static_cast<const T*>(p.dy), p.dy_stride, p.act != kActNone ? static_cast<const T*>(p.z) : nullptr, out, p.M,
-        p.N, p.act, partials);
-    if (cudaError_t e = cudaGetLastError()) return (int)e;
-    if (p.db)
-      if (cudaError_t e = join_columns<T>(partials, shares, p.N, p.N, p.db, nullptr, stream)) return (int)e;
-  } else if (p.db) {
-    if (cudaError_t e = cudaMemsetAsync(p.db, 0, (size_t)p.N * sizeof(T), stream)) return (int)e;
+  GemmOperand x, w;
+  if (int rc = operand<T>(p.x, p.M, p.K, p.x_stride, dtype, &ws, &x, stream)) return rc;
+  if (int rc = operand<T>(p.w, p.N, p.K, p.w_stride, dtype, &ws, &w, stream)) return rc;
+  GemmProblem g = problem<T>(x, w, p.M, p.N, p.K, dtype, ws, p.status);
+  g.out = GemmEpilogue{p.bias, p.residual, p.z, p.y, p.r_stride, p.N, p.N, p.act};
+  return launch_gemm(g, stream);
+}
+
+template <typename T, int ACT>
+void launch_dz(const LinearBwdParams& p, const GemmOperand& o, bool write, float* partials, cudaStream_t stream) {
+  linear_dz_kernel<T, ACT><<<dim3((unsigned)((p.N + 255) / 256), row_shares(p.M, p.N)), 256, 0, stream>>>(
+      static_cast<const T*>(p.dy), p.dy_stride, on_16_bytes<T>(p.dy, p.dy_stride), static_cast<const T*>(p.z),
+      write ? const_cast<void*>(o.ptr) : nullptr, o.pitch, o.piece_stride, p.M, p.N, partials);
+}
+
+template <typename T>
+int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
+  if (p.M == 0) {  // sums over no rows
+    for (auto [ptr, n] : {std::pair<void*, size_t>{p.dw, (size_t)p.N * p.K}, {p.db, (size_t)p.N}})
+      if (ptr)
+        if (cudaError_t e = cudaMemsetAsync(ptr, 0, n * sizeof(T), stream)) return (int)e;
+    return 0;
   }
+  unsigned char* ws = static_cast<unsigned char*>(p.ws);
+  const bool products = p.dx || p.dw;
+  const bool direct = p.act == kActNone && dtype != kF32 && on_16_bytes<T>(p.dy, p.dy_stride);
+  GemmOperand dz{p.dy, p.M, p.N, p.dy_stride, 0, false};
+  if (products && !direct) dz = blank_operand<T>(p.M, p.N, dtype, &ws);
+  float* partials = nullptr;
+  if (p.db) {
+    partials = reinterpret_cast<float*>(ws);
+    ws += round256((size_t)row_shares(p.M, p.N) * p.N * sizeof(float));
+  }
+  if (p.db || (products && !direct)) {
+    const bool write = products && !direct;
+    switch (p.act) {
+      case kActGelu: launch_dz<T, kActGelu>(p, dz, write, partials, stream); break;
+      case kActRelu: launch_dz<T, kActRelu>(p, dz, write, partials, stream); break;
+      case kActSilu: launch_dz<T, kActSilu>(p, dz, write, partials, stream); break;
+      default: launch_dz<T, kActNone>(p, dz, write, partials, stream); break;
+    }
+    if (cudaError_t e = cudaGetLastError()) return (int)e;
+  }
+  if (p.db)
+    if (cudaError_t e = join_columns<T>(partials, row_shares(p.M, p.N), p.N, p.N, p.db, nullptr, stream)) return (int)e;
   if (p.dx) {
-    GemmParams g{};
-    g.a = dz; g.am = dz_stride; g.ak = 1;
-    g.b = p.w; g.bn = 1; g.bk = p.w_stride;
-    g.M = p.M; g.N = p.K; g.K = p.N;
-    g.y = p.dx; g.y_stride = p.K;
-    if (int rc = launch_gemm<T>(g, stream)) return rc;
+    GemmOperand w;
+    unsigned char* at = ws;
+    if (int rc = operand<T>(p.w, p.N, p.K, p.w_stride, dtype, &at, &w, stream)) return rc;
+    w.mn_major = true;  // its columns are dx's, its rows the depth
+    GemmProblem g = problem<T>(dz, w, p.M, p.K, p.N, dtype, at, p.status);
+    g.out.y = p.dx;
+    g.out.y_stride = p.K;
+    if (int rc = launch_gemm(g, stream)) return rc;
   }
   if (p.dw) {
-    GemmParams g{};
-    g.a = dz; g.am = 1; g.ak = dz_stride;
-    g.b = p.x; g.bn = 1; g.bk = p.x_stride;
-    g.M = p.N; g.N = p.K; g.K = p.M;
-    g.y = p.dw; g.y_stride = p.K;
-    if (int rc = launch_gemm<T>(g, stream)) return rc;
+    GemmOperand x;
+    unsigned char* at = ws;
+    if (int rc = operand<T>(p.x, p.M, p.K, p.x_stride, dtype, &at, &x, stream)) return rc;
+    dz.mn_major = x.mn_major = true;  // the rows of both are the depth
+    GemmProblem g = problem<T>(dz, x, p.N, p.K, p.M, dtype, at, p.status);
+    g.out.y = p.dw;
+    g.out.y_stride = p.K;
+    if (int rc = launch_gemm(g, stream)) return rc;
   }
   return 0;
 }
 
 }  // namespace
 
-size_t linear_workspace_bytes(int64_t, int64_t, int64_t, int) { return 0; }
+size_t linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct, bool w_direct) {
+  const int pieces = dtype == kF32 ? 3 : 1;
+  return (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype)) +
+         (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) + gemm_workspace_bytes(M, N, K, pieces);
+}
 
-size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t, int dtype, int act) {
-  const size_t dz = act == kActNone ? 0 : round256((size_t)M * N * (dtype == kF32 ? 4 : 2));
-  return dz + (size_t)row_shares(M) * N * sizeof(float);
+size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act, bool x_direct,
+                                       bool w_direct, bool dy_direct) {
+  const int pieces = dtype == kF32 ? 3 : 1;
+  const size_t dz = act == kActNone && pieces == 1 && dy_direct ? 0 : operand_bytes(M, N, dtype);
+  const size_t sums = round256((size_t)row_shares(M, N) * N * sizeof(float));
+  const size_t dx = (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) + gemm_workspace_bytes(M, K, N, pieces);
+  const size_t dw = (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype)) + gemm_workspace_bytes(N, K, M, pieces);
+  return dz + sums + (dx > dw ? dx : dw);
 }
 
 int launch_linear(const LinearParams& p, int dtype, cudaStream_t stream) {
-  if (dtype == kBF16) return launch_fwd<__nv_bfloat16>(p, stream);
-  if (dtype == kF16) return launch_fwd<__half>(p, stream);
-  return launch_fwd<float>(p, stream);
+  if (dtype == kBF16) return launch_fwd<__nv_bfloat16>(p, dtype, stream);
+  if (dtype == kF16) return launch_fwd<__half>(p, dtype, stream);
+  return launch_fwd<float>(p, dtype, stream);
 }
 
 int launch_linear_backward(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
-  if (dtype == kBF16) return launch_bwd<__nv_bfloat16>(p, stream);
-  if (dtype == kF16) return launch_bwd<__half>(p, stream);
-  return launch_bwd<float>(p, stream);
+  if (dtype == kBF16) return launch_bwd<__nv_bfloat16>(p, dtype, stream);
+  if (dtype == kF16) return launch_bwd<__half>(p, dtype, stream);
+  return launch_bwd<float>(p, dtype, stream);
 }
 
 }  // namespace wf

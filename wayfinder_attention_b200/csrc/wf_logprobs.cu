@@ -398,7 +398,7 @@ int launch_fwd(LogprobParams p, cudaStream_t stream) {
     return (int)cudaGetLastError();
   }
   int c = 1;
-  while (c < 8 && p.rows * c * 2 <= 148 * 2 && p.vocab / c > 4 * kWarpRow) c *= 2;
+  while (c < 8 && p.rows * c <= kSms && p.vocab / c > 4 * kWarpRow) c *= 2;
   p.cluster = c;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * c));

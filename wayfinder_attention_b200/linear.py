@@ -18,13 +18,13 @@ ACTIVATIONS = {"none": 0, "gelu": 1, "relu": 2, "silu": 3}
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(M: int, N: int, K: int, dtype: int) -> int:
-    return _lib.load_library().wf_linear_workspace_bytes(M, N, K, dtype)
+def _workspace_bytes(*sizes: int) -> int:
+    return _lib.load_library().wf_linear_workspace_bytes(*sizes)
 
 
 @functools.lru_cache(maxsize=4096)
-def _backward_workspace_bytes(M: int, N: int, K: int, dtype: int, act: int) -> int:
-    return _lib.load_library().wf_linear_backward_workspace_bytes(M, N, K, dtype, act)
+def _backward_workspace_bytes(*sizes: int) -> int:
+    return _lib.load_library().wf_linear_backward_workspace_bytes(*sizes)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -39,7 +39,7 @@ def _launch(x, weight, bias, residual, act, keep_z, status):
     y = torch.empty(M, N, dtype=x.dtype, device=dev)
     z = torch.empty(M, N, dtype=x.dtype, device=dev) if keep_z else None
     code = _lib.dtype_code(x.dtype)
-    n = _workspace_bytes(M, N, K, code)
+    n = _workspace_bytes(M, N, K, code, _lib.on_16_bytes(x), _lib.on_16_bytes(weight))
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     st = _lib.status_arg(dev, status)
     with _lib.on_device(dev):
@@ -76,7 +76,8 @@ class _LinearFunction(torch.autograd.Function):
         db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
         if need_x or need_w or need_b:
             code = _lib.dtype_code(x.dtype)
-            n = _backward_workspace_bytes(M, N, K, code, ctx.act)
+            n = _backward_workspace_bytes(M, N, K, code, ctx.act, _lib.on_16_bytes(x), _lib.on_16_bytes(weight),
+                                          _lib.on_16_bytes(g))
             ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
             st = _lib.status_arg(dev, None)
             with _lib.on_device(dev):
