@@ -1,8 +1,12 @@
 // Tensor-core product with an epilogue: C = act(A B^T + bias) + residual.
 //
-// A persistent kernel, one block an SM, each block walking 128 x BN tiles of C.  Warp 8
-// streams 64-deep slices of A and B into a ring of shared-memory stages with TMA; warp 9
-// issues tcgen05.mma (128 x BN x 16, fp32 accumulators in TMEM) on them; warps 0-7 read a
+// A persistent kernel, one block an SM.  CG = 2: two blocks of a cluster work on a
+// 256 x BN tile together, each loading its 128 rows of A and its half of B's rows and
+// keeping its 128 rows of the accumulator; the leader issues tcgen05.mma.cta_group::2 for
+// both, so each B element is read from L2 once for 256 rows.  CG = 1: 128 x BN tiles.
+//
+// Warp 8 streams 64-deep slices of A and B into a ring of shared-memory stages with TMA;
+// warp 9 issues the products (fp32 accumulators in TMEM) on them; warps 0-7 read a
 // finished accumulator back, apply the epilogue and store.  Two accumulators alternate, so
 // the epilogue of one tile runs under the products of the next.
 //
@@ -16,6 +20,11 @@
 // length of a sum than fp32 rounding would, so every kChunk of depth the accumulator is
 // added to fp32 registers and begun anew.
 //
+// Epilogue: a warp owns 32 rows (its TMEM lanes, a row a lane) and walks them 128 bytes of
+// output at a time through a swizzled shared-memory buffer, which TMA stores write out in
+// whole lines (and a TMA load fills with the residual first).  Outputs whose rows do not
+// start on 16 bytes go from the buffer with coalesced element stores instead.
+//
 // Few tiles with a deep sum (a weight's gradient over many rows) are split along the
 // depth: each part writes fp32 partials, and a second kernel adds them in order and
 // applies the epilogue.
@@ -24,6 +33,7 @@
 #include "wf_rowio.cuh"
 #include "wf_sm100.cuh"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace wf {
@@ -31,31 +41,41 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kBM = 128;
+constexpr int kBM = 128;                // rows of a block
 constexpr int kBK = 64;                 // depth of a stage: 128 bytes
 constexpr int kChunk = 4;               // stages between additions to fp32 registers (three-piece form)
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
+constexpr uint32_t kBuffer = 32 * 128;  // staging: 32 rows of 128 bytes, two a warp
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int kMaxSplits = 32;
 
 struct GemmParams {
-  int M, N, tiles_n, units, splits, k_blocks, pieces;
-  bool a_mn, b_mn, vec;
+  int M, N, tiles_n, units, splits, k_blocks;
+  bool a_mn, b_mn;
+  bool store_tma;     // y (and z) can be TMA's
+  bool residual_tma;
   GemmEpilogue out;
-  float* partial;  // [splits][M][N] when splits > 1
   int32_t* status;
   uint32_t idesc;
 };
 
-template <int BN>
+template <typename T, int BN, int CG>
 struct Layout {
-  static constexpr uint32_t A_BYTES = kBM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  static constexpr size_t off_bar = (size_t)STAGES * STAGE;
-  static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5);
+  static constexpr uint32_t A_BYTES = kBM * 128, B_BYTES = BN / CG * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr uint32_t STAGING = kEpilogueWarps * 2 * kBuffer;
+  static constexpr int FIT = (227 * 1024 - 2048 - (int)STAGING) / (int)STAGE;
+  static constexpr int STAGES = FIT < 8 ? FIT : 8;
+  static constexpr size_t off_staging = (size_t)STAGES * STAGE;
+  static constexpr size_t off_bar = off_staging + STAGING;
+  static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5 + kEpilogueWarps);
   static constexpr size_t smem = off_misc + 16 + 1024;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
+  // columns of a staging buffer, and of an epilogue warp (a half of the tile, unless that is
+  // less than a buffer: then four of the warps take it all)
+  static constexpr int CC = 128 / (int)sizeof(T);
+  static constexpr int COLS = BN / 2 < CC ? BN : BN / 2;
+  static constexpr int WARPS = 4 * (BN / COLS);
 };
 
 // Pieces of a and b multiplied in this order: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0).
@@ -88,83 +108,74 @@ struct Ring {
 // Units of work: a tile and a share of the depth.
 struct Unit {
   int m0, n0, kb0, kb1, split;
-  __device__ __forceinline__ Unit(const GemmParams& p, int u, int BN) {
+  __device__ __forceinline__ Unit(const GemmParams& p, int u, int BM, int BN) {
     split = u % p.splits;
     const int tile = u / p.splits;
-    m0 = tile / p.tiles_n * kBM;
+    m0 = tile / p.tiles_n * BM;
     n0 = tile % p.tiles_n * BN;
     kb0 = (int)((int64_t)p.k_blocks * split / p.splits);
     kb1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
   }
 };
 
-// 32 columns of one row: bias, activation, residual, stores.
+// Byte of a staging buffer that holds byte `at` of row r's 128: the 128-byte swizzle.
+__device__ __forceinline__ uint32_t staged(int r, int at) { return r * 128 + ((at ^ (r << 4)) & 0x70) + (at & 15); }
+
+// Between a staging buffer and rows that start anywhere: a row at a time, a lane an element.
+template <typename T, int CC>
+__device__ __forceinline__ void copy_rows_out(const unsigned char* buf, T* y, int64_t stride, int64_t m, int64_t M,
+                                              int n, int N, int lane) {
+  const int rows = (int)min((int64_t)32, M - m);
+  for (int r = 0; r < rows; ++r)
+#pragma unroll
+    for (int c = lane; c < CC; c += 32)
+      if (n + c < N)
+        y[(m + r) * stride + n + c] = *reinterpret_cast<const T*>(buf + staged(r, c * (int)sizeof(T)));
+}
+template <typename T, int CC>
+__device__ __forceinline__ void copy_rows_in(unsigned char* buf, const T* x, int64_t stride, int64_t m, int64_t M,
+                                             int n, int N, int lane) {
+  const int rows = (int)min((int64_t)32, M - m);
+  for (int r = 0; r < rows; ++r)
+#pragma unroll
+    for (int c = lane; c < CC; c += 32)
+      if (n + c < N) *reinterpret_cast<T*>(buf + staged(r, c * (int)sizeof(T))) = x[(m + r) * stride + n + c];
+}
+
+// y += bias over 32 columns from n.
 template <typename T>
-__device__ __forceinline__ void finish_row(const GemmEpilogue& o, int64_t m, int n, int N, bool vec, float* v) {
+__device__ __forceinline__ void add_bias(const void* bias, int n, int N, float* v) {
   constexpr int V = Vec16<T>::N;
-  if (vec && n + 32 <= N) {
-    if (o.bias) {
-      const T* b = static_cast<const T*>(o.bias) + n;
+  const T* b = static_cast<const T*>(bias) + n;
+  if (n + 32 <= N && reinterpret_cast<uintptr_t>(b) % 16 == 0) {
 #pragma unroll
-      for (int j = 0; j < 32; j += V) {
-        float f[V];
-        Vec16<T>::unpack(ldg16(b + j), f);
+    for (int j = 0; j < 32; j += V) {
+      float f[V];
+      Vec16<T>::unpack(ldg16(b + j), f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[j + i] += f[i];
-      }
+      for (int i = 0; i < V; ++i) v[j + i] += f[i];
     }
-    if (o.z) {
-      T* z = static_cast<T*>(o.z) + m * o.z_stride + n;
-#pragma unroll
-      for (int j = 0; j < 32; j += V) store_vec<T, V>(z + j, v + j);
-    }
-    activate_all<32>(o.act, v);
-    if (o.residual) {
-      const T* r = static_cast<const T*>(o.residual) + m * o.r_stride + n;
-#pragma unroll
-      for (int j = 0; j < 32; j += V) {
-        float f[V];
-        Vec16<T>::unpack(ldg16(r + j), f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j + i] += f[i];
-      }
-    }
-    T* y = static_cast<T*>(o.y) + m * o.y_stride + n;
-#pragma unroll
-    for (int j = 0; j < 32; j += V) store_vec<T, V>(y + j, v + j);
-    return;
-  }
-  if (o.bias) {
-    const T* b = static_cast<const T*>(o.bias) + n;
+  } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
       if (n + j < N) v[j] += to_f32(b[j]);
   }
-  if (o.z) {
-    T* z = static_cast<T*>(o.z) + m * o.z_stride + n;
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n + j < N) z[j] = from_f32<T>(v[j]);
-  }
-  activate_all<32>(o.act, v);
-  if (o.residual) {
-    const T* r = static_cast<const T*>(o.residual) + m * o.r_stride + n;
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n + j < N) v[j] += to_f32(r[j]);
-  }
-  T* y = static_cast<T*>(o.y) + m * o.y_stride + n;
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (n + j < N) y[j] = from_f32<T>(v[j]);
 }
 
-template <typename T, int BN>
+template <typename T>
+__device__ __forceinline__ void stage32(unsigned char* buf, int lane, int at, const float* v) {
+  constexpr int V = Vec16<T>::N;
+#pragma unroll
+  for (int j = 0; j < 32; j += V)
+    store_vec<T, V>(reinterpret_cast<T*>(buf + staged(lane, at + j * (int)sizeof(T))), v + j);
+}
+
+template <typename T, int BN, int CG, bool PIECES>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
-                const GemmParams p) {
-  using L = Layout<BN>;
-  constexpr bool PIECES = std::is_same<T, float>::value;
+                const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap zmap,
+                const __grid_constant__ CUtensorMap rmap, const GemmParams p) {
+  using L = Layout<T, BN, CG>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -173,9 +184,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_full = empty + L::STAGES;  // [2]
   uint64_t* acc_empty = acc_full + 2;      // [2]
   uint64_t* drained = acc_empty + 2;
+  uint64_t* res_full = drained + 1;        // [kEpilogueWarps]
   uint32_t* tmem_s = reinterpret_cast<uint32_t*>(base + L::off_misc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+  constexpr int BM = kBM * CG;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
 
+  // Pair: `full` and `acc_empty` are the leader's alone; the leader's products arrive on
+  // `empty`, `acc_full` and `drained` of both.
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -183,20 +200,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpilogueWarps);
+      mbar_init(&acc_empty[i], CG * L::WARPS);
     }
     mbar_init(drained, 1);
+    for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(&res_full[i], 1);
     fence_mbarrier_init();
   }
   if (warp == 0) {
-    tmem_alloc(tmem_s, L::TMEM_COLS);
-    tmem_relinquish();
+    if constexpr (CG == 2) {
+      tmem_alloc_pair(tmem_s, L::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_s, L::TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CG == 2) {
+    __syncthreads();
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
   tc_fence_after();
   const uint32_t tmem = *tmem_s;
-  const int pairs = PIECES ? 6 : 1;
+  constexpr int pairs = PIECES ? 6 : 1;
   uint32_t why = 0;
 
   if (warp == kEpilogueWarps) {
@@ -206,8 +234,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       prefetch_tmap(&bmap);
       Ring r;
       uint32_t issued = 0;
-      for (int u = blockIdx.x; u < p.units && !why; u += gridDim.x) {
-        const Unit w(p, u, BN);
+      for (int u = first; u < p.units && !why; u += step) {
+        const Unit w(p, u, BM, BN);
+        const int am = w.m0 + (int)rank * kBM, bn = w.n0 + (int)rank * (BN / CG);
         for (int c0 = w.kb0; c0 < w.kb1 && !why; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
           const int c1 = PIECES ? min(c0 + kChunk, w.kb1) : w.kb1;
           for (int pair = 0; pair < pairs && !why; ++pair) {
@@ -216,21 +245,24 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!mbar_wait(&empty[r.stage], r.phase ^ 1, kWaitNs)) { why = 4; break; }
               unsigned char* st = base + (size_t)r.stage * L::STAGE;
               uint64_t* bar = &full[r.stage];
-              mbar_arrive_expect_tx(bar, L::STAGE);
+              if (rank == 0) mbar_arrive_expect_tx(bar, CG * L::STAGE);
+              const uint32_t on = CG == 2 ? map_peer(bar, 0) : 0;
+              auto load = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
+                if constexpr (CG == 2) tma_load_3d_pair(dst, map, on, x, y, z);
+                else tma_load_3d(dst, map, bar, x, y, z);
+              };
               if (p.a_mn) {
 #pragma unroll
-                for (int i = 0; i < kBM / 64; ++i)
-                  tma_load_3d(st + i * kBK * 128, &amap, bar, w.m0 + 64 * i, kb * kBK, pa);
+                for (int i = 0; i < kBM / 64; ++i) load(st + i * kBK * 128, &amap, am + 64 * i, kb * kBK, pa);
               } else {
-                tma_load_3d(st, &amap, bar, kb * kBK, w.m0, pa);
+                load(st, &amap, kb * kBK, am, pa);
               }
               st += L::A_BYTES;
               if (p.b_mn) {
 #pragma unroll
-                for (int i = 0; i < BN / 64; ++i)
-                  tma_load_3d(st + i * kBK * 128, &bmap, bar, w.n0 + 64 * i, kb * kBK, pb);
+                for (int i = 0; i < BN / CG / 64; ++i) load(st + i * kBK * 128, &bmap, bn + 64 * i, kb * kBK, pb);
               } else {
-                tma_load_3d(st, &bmap, bar, kb * kBK, w.n0, pb);
+                load(st, &bmap, kb * kBK, bn, pb);
               }
               ++issued;
               r.next<L::STAGES>();
@@ -239,23 +271,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // after a wait that gave up, loads may be in flight that no product will wait for
-      if (why)
+      if (why && rank == 0)
         for (uint32_t s = 0; s < (uint32_t)L::STAGES && s < issued; ++s) {
-          const uint32_t last = (issued - 1 - s) / L::STAGES * L::STAGES + s;  // newest load of stage s
-          mbar_wait(&full[s], (last / L::STAGES) & 1, kWaitNs);
+          const uint32_t last = (issued - 1 - s) / L::STAGES;  // round of the newest load of stage s
+          mbar_wait(&full[s], last & 1, kWaitNs);
         }
     }
   } else if (warp == kEpilogueWarps + 1) {
     // ------------------------------------------------------------ products
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       Ring r;
       uint32_t acc = 0, acc_phase = 0;
       const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
-      for (int u = blockIdx.x; u < p.units && !why; u += gridDim.x) {
-        const Unit w(p, u, BN);
+      auto commit = [&](uint64_t* bar) {
+        if constexpr (CG == 2) mma_commit_pair(bar);
+        else mma_commit(bar);
+      };
+      for (int u = first; u < p.units && !why; u += step) {
+        const Unit w(p, u, BM, BN);
         for (int c0 = w.kb0; c0 < w.kb1 && !why; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
           const int c1 = PIECES ? min(c0 + kChunk, w.kb1) : w.kb1;
-          if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, kWaitNs)) { why = 8; break; }
+          if (!mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1, kWaitNs)) { why = 8; break; }
           tc_fence_after();
           const uint32_t d = tmem + acc * BN;
           const int n = (c1 - c0) * pairs;
@@ -266,131 +302,183 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k) {
               const uint32_t aa = as + k * a_step, bb = bs + k * b_step;
-              mma_f16(d, p.a_mn ? smem_desc_mnmajor(aa) : smem_desc_kmajor(aa, 128),
-                      p.b_mn ? smem_desc_mnmajor(bb) : smem_desc_kmajor(bb, 128), p.idesc, i > 0 || k > 0);
+              const uint64_t da = p.a_mn ? smem_desc_mnmajor(aa) : smem_desc_kmajor(aa, 128);
+              const uint64_t db = p.b_mn ? smem_desc_mnmajor(bb) : smem_desc_kmajor(bb, 128);
+              if constexpr (CG == 2) mma_f16_pair(d, da, db, p.idesc, i > 0 || k > 0);
+              else mma_f16(d, da, db, p.idesc, i > 0 || k > 0);
             }
-            mma_commit(&empty[r.stage]);
+            commit(&empty[r.stage]);
             r.next<L::STAGES>();
           }
-          mma_commit(&acc_full[acc]);
+          commit(&acc_full[acc]);
           acc ^= 1;
           acc_phase ^= acc == 0;
         }
       }
-      mma_commit(drained);
+      commit(drained);
     }
-  } else {
+  } else if (warp < L::WARPS) {
     // ------------------------------------------------------------ epilogue
-    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (a row a lane) and half w / 4 of the columns
-    constexpr int COLS = BN / 2;
+    constexpr int COLS = L::COLS, CC = L::CC;
+    constexpr int SUB = CC < 32 ? CC : 32;  // columns of a TMEM load
+    static_assert(CC % SUB == 0 && SUB == 32, "a staging buffer holds whole TMEM loads");
     const uint32_t lbase = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * COLS;
-    uint32_t acc = 0, acc_phase = 0;
-    for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
-      const Unit w(p, u, BN);
-      const int64_t m = w.m0 + 32 * (warp & 3) + lane;
+    unsigned char* buf = base + L::off_staging + (size_t)warp * 2 * kBuffer;
+    uint32_t acc = 0, acc_phase = 0, turn = 0, res_phase = 0;
+    auto release = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(&acc_empty[acc]);
+        else mbar_arrive_peer(map_peer(&acc_empty[acc], 0));
+      }
+      acc ^= 1;
+      acc_phase ^= acc == 0;
+    };
+    for (int u = first; u < p.units && !why; u += step) {
+      const Unit w(p, u, BM, BN);
+      const int m = w.m0 + (int)rank * kBM + 32 * (warp & 3);
       const int n0 = w.n0 + (warp >> 2) * COLS;
+      // buffers to use: what is not there to store is skipped, for whole warps
+      const int chunks = m < p.M && n0 < p.N ? (min(COLS, p.N - n0) + CC - 1) / CC : 0;
       float sum[PIECES ? COLS : 1];
       if constexpr (PIECES) {
 #pragma unroll
         for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
       }
       for (int c0 = w.kb0; c0 < w.kb1; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
-        const bool there = __all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_phase, kWaitNs));
-        if (!there) { why = 32; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_phase, kWaitNs))) { why = 32; break; }
         tc_fence_after();
-        const uint32_t src = lbase + acc * BN;
         if constexpr (PIECES) {
 #pragma unroll
           for (int c = 0; c < COLS; c += 32) {
             uint32_t r[32];
-            tmem_ld_32x32b_x32(src + c, r);
+            tmem_ld_32x32b_x32(lbase + acc * BN + c, r);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
           }
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < COLS; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(src + c, r);
-            tmem_ld_wait();
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-            const int n = n0 + c;
-            if (m < p.M && n < p.N) {
-              if (p.splits > 1) {
-                GemmEpilogue o{};
-                o.y = p.partial;
-                o.y_stride = p.N;
-                finish_row<float>(o, (int64_t)w.split * p.M + m, n, p.N, p.N % 4 == 0, v);
-              } else {
-                finish_row<T>(p.out, m, n, p.N, p.vec, v);
-              }
-            }
-          }
+          release();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[acc]);
-        acc ^= 1;
-        acc_phase ^= acc == 0;
       }
       if (why) break;
-      if constexpr (PIECES) {
-#pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-          const int n = n0 + c;
-          if (m < p.M && n < p.N) {
-            if (p.splits > 1) {
-              GemmEpilogue o{};
-              o.y = p.partial;
-              o.y_stride = p.N;
-              finish_row<float>(o, (int64_t)w.split * p.M + m, n, p.N, p.N % 4 == 0, sum + c);
-            } else {
-              finish_row<float>(p.out, m, n, p.N, p.vec, sum + c);
+      const uint32_t src = lbase + acc * BN;
+      auto chunk = [&](int ch) {
+        const int n = n0 + ch * CC;
+        // the buffers' last stores have been read out: both with z, else the older of two in turn
+        unsigned char* zb = buf;
+        unsigned char* yb = p.out.z ? buf + kBuffer : buf + (turn++ & 1) * kBuffer;
+        if (lane == 0) {
+          if (p.out.z) bulk_wait_read<0>();
+          else bulk_wait_read<1>();
+        }
+        __syncwarp();
+        if (p.out.residual) {
+          if (p.residual_tma) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&res_full[warp], kBuffer);
+              tma_load_3d(yb, &rmap, &res_full[warp], n, m, 0);
             }
+          } else {
+            copy_rows_in<T, CC>(yb, static_cast<const T*>(p.out.residual), p.out.r_stride, m, p.M, n, p.N, lane);
+            __syncwarp();
           }
         }
+        float v[CC];
+        if constexpr (PIECES) {
+#pragma unroll
+          for (int j = 0; j < CC; ++j) v[j] = sum[ch * CC + j];
+        } else {
+          uint32_t r[CC / 32][32];
+#pragma unroll
+          for (int c = 0; c < CC / 32; ++c) tmem_ld_32x32b_x32(src + ch * CC + 32 * c, r[c]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < CC; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]);
+          if (ch == chunks - 1) release();
+        }
+        if (p.out.residual && p.residual_tma) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&res_full[warp], res_phase, kWaitNs))) { why = 128; return; }
+          res_phase ^= 1;
+        }
+#pragma unroll
+        for (int c = 0; c < CC; c += 32) {
+          if (p.out.bias) add_bias<T>(p.out.bias, n + c, p.N, v + c);
+          if (p.out.z) stage32<T>(zb, lane, c * (int)sizeof(T), v + c);
+          activate_all<T, 32>(p.out.act, v + c);
+          if (p.out.residual) {
+            constexpr int V = Vec16<T>::N;
+#pragma unroll
+            for (int j = 0; j < 32; j += V) {
+              float f[V];
+              Vec16<T>::unpack(*reinterpret_cast<const uint4*>(yb + staged(lane, (c + j) * (int)sizeof(T))), f);
+#pragma unroll
+              for (int i = 0; i < V; ++i) v[c + j + i] += f[i];
+            }
+          }
+          stage32<T>(yb, lane, c * (int)sizeof(T), v + c);
+        }
+        if (p.store_tma) {
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            if (p.out.z) tma_store_3d(&zmap, zb, n, m, 0);
+            tma_store_3d(&ymap, yb, n, m, w.split);
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
+          if (p.out.z) copy_rows_out<T, CC>(zb, static_cast<T*>(p.out.z), p.out.z_stride, m, p.M, n, p.N, lane);
+          copy_rows_out<T, CC>(yb, static_cast<T*>(p.out.y), p.out.y_stride, m, p.M, n, p.N, lane);
+          fence_async_shared();  // a residual's load may fill the buffer next
+          __syncwarp();
+        }
+      };
+      if constexpr (PIECES) {
+#pragma unroll
+        for (int ch = 0; ch < COLS / CC; ++ch)
+          if (ch < chunks && !why) chunk(ch);
+      } else {
+#pragma unroll 1
+        for (int ch = 0; ch < chunks && !why; ++ch) chunk(ch);
       }
+      if (!PIECES && chunks == 0) release();
     }
+    if (lane == 0) bulk_wait_all();
   }
   __syncwarp();
   if (why && p.status && lane == 0) atomicOr(p.status, 2 | (int)why);
-  // TMEM is given back once no product writes to it
-  const bool done = mbar_wait(drained, 0, kWaitNs);
-  if (!done && p.status && threadIdx.x == 0) atomicOr(p.status, 2 | 64);
+  // TMEM is given back, and a pair parts, once no product writes to it
+  if (warp == 0 && !__all_sync(0xffffffffu, mbar_wait(drained, 0, kWaitNs)) && p.status && lane == 0)
+    atomicOr(p.status, 2 | 64);
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, L::TMEM_COLS);
+    if constexpr (CG == 2) tmem_dealloc_pair(tmem, L::TMEM_COLS);
+    else tmem_dealloc(tmem, L::TMEM_COLS);
   }
 }
 
 // Adds the parts of a split depth and applies the epilogue: a thread takes 4 columns of a row.
 template <typename T>
-__global__ void __launch_bounds__(256) gemm_join_kernel(const float* partial, int splits, int64_t M, int64_t N,
-                                                        GemmEpilogue o) {
-  const int64_t groups = (N + 3) / 4, total = M * groups;
+__global__ void __launch_bounds__(256) gemm_join_kernel(const float* partial, int splits, int64_t pitch, int64_t M,
+                                                        int64_t N, GemmEpilogue o) {
+  const int64_t groups = pitch / 4, total = M * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / groups, n = i % groups * 4;
     const int live = (int)min((int64_t)4, N - n);
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < splits; ++s) {
-      const float* q = partial + ((int64_t)s * M + m) * N + n;
-      if (N % 4 == 0) {
-        const float4 f = *reinterpret_cast<const float4*>(q);
-        v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
-      } else {
-        for (int j = 0; j < live; ++j) v[j] += q[j];
-      }
+      const float4 f = *reinterpret_cast<const float4*>(partial + ((int64_t)s * M + m) * pitch + n);
+      v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
     }
     if (o.bias)
       for (int j = 0; j < live; ++j) v[j] += to_f32(static_cast<const T*>(o.bias)[n + j]);
     if (o.z)
       for (int j = 0; j < live; ++j) static_cast<T*>(o.z)[m * o.z_stride + n + j] = from_f32<T>(v[j]);
-    activate_all<4>(o.act, v);
+    activate_all<T, 4>(o.act, v);
     if (o.residual)
       for (int j = 0; j < live; ++j) v[j] += to_f32(static_cast<const T*>(o.residual)[m * o.r_stride + n + j]);
     for (int j = 0; j < live; ++j) static_cast<T*>(o.y)[m * o.y_stride + n + j] = from_f32<T>(v[j]);
@@ -412,48 +500,78 @@ EncodeTiledFnG encode_fn() {
   return fn;
 }
 
-bool make_map(CUtensorMap* map, const GemmOperand& o, int pieces, int op_dtype, int box_rows) {
-  const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)pieces};
-  const int64_t piece = pieces > 1 ? o.piece_stride : o.pitch * o.rows;
-  const cuuint64_t strides[2] = {(cuuint64_t)(o.pitch * 2), (cuuint64_t)(piece * 2)};
-  const cuuint32_t box[3] = {64, (cuuint32_t)(o.mn_major ? kBK : box_rows), 1};
+// A (layers, rows, cols) tensor in boxes of box_rows x 128 bytes, 128-byte swizzle; pitches in elements.
+bool make_map(CUtensorMap* map, int dtype, const void* ptr, int64_t cols, int64_t rows, int64_t layers, int64_t pitch,
+              int64_t layer_pitch, int box_rows) {
+  const int size = dtype == kF32 ? 4 : 2;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
+  const cuuint64_t strides[2] = {(cuuint64_t)(pitch * size), (cuuint64_t)(layer_pitch * size)};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   EncodeTiledFnG fn = encode_fn();
-  return fn && fn(map, op_dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                  const_cast<void*>(o.ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  return fn && fn(map,
+                  dtype == kBF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                  : dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                  3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-
-// Tile width and depth shares.  The widest tile that still gives every SM one (wider tiles
-// read A less often); below that, narrower tiles and then shares of at least kMinShare
-// stages of depth until the SMs are busy.
-struct Plan {
-  int bn, tiles_n, tiles, splits, k_blocks;
-};
-constexpr int kMinShare = 4;
-Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
-  Plan p{};
-  p.k_blocks = (int)((K + kBK - 1) / kBK);
-  auto tiles = [&](int bn) { return (M + kBM - 1) / kBM * ((N + bn - 1) / bn); };
-  p.bn = pieces == 1 && N > 128 && tiles(256) >= kSms ? 256 : N > 64 && tiles(128) * 2 >= kSms ? 128 : 64;
-  p.tiles_n = (int)((N + p.bn - 1) / p.bn);
-  const int64_t t = tiles(p.bn);
-  p.tiles = (int)t;
-  p.splits = 1;
-  if (t * 2 <= kSms) {
-    const int64_t most = p.k_blocks / kMinShare, fill = kSms / t;
-    const int64_t s = most < fill ? most : fill;
-    p.splits = (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
-  }
-  return p;
+bool make_operand_map(CUtensorMap* map, const GemmOperand& o, int pieces, int op_dtype, int box_rows) {
+  return make_map(map, op_dtype, o.ptr, o.cols, o.rows, pieces, o.pitch, pieces > 1 ? o.piece_stride : o.pitch * o.rows,
+                  o.mn_major ? kBK : box_rows);
 }
 
-template <typename T, int BN>
-int launch_tile(const GemmProblem& g, const Plan& plan, cudaStream_t stream) {
-  using L = Layout<BN>;
-  CUtensorMap amap, bmap;
-  if (!make_map(&amap, g.a, g.pieces, g.op_dtype, kBM) || !make_map(&bmap, g.b, g.pieces, g.op_dtype, BN)) return -1;
+// Tile shape and depth shares: the least of an estimate over the shapes there are.  A
+// unit's time is its stages of depth at the rate the shape can take them plus its
+// accumulator's way out; units run in waves.
+struct Shape {
+  int bn, cg;
+  int cycles;  // a stage: the products' time, or the loads' at about 64 bytes a cycle an SM
+};
+constexpr Shape kShapes[] = {{256, 2, 560}, {128, 2, 400}, {128, 1, 540}, {64, 1, 400}};
+constexpr int kMinShare = 4;  // stages of depth a share has at least
+struct Plan {
+  Shape shape;
+  int tiles_n, tiles, splits, k_blocks;
+};
+Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
+  Plan best{};
+  double least = 0;
+  for (const Shape& s : kShapes) {
+    if (pieces > 1 && s.bn == 256) continue;  // the sums of a 128 x 256 tile do not fit the registers
+    Plan p{};
+    p.shape = s;
+    p.k_blocks = (int)((K + kBK - 1) / kBK);
+    const int64_t tn = (N + s.bn - 1) / s.bn, tm = (M + kBM * s.cg - 1) / (kBM * s.cg);
+    p.tiles_n = (int)tn;
+    p.tiles = (int)(tn * tm);
+    const int slots = kSms / s.cg;
+    for (int splits = 1; splits <= kMaxSplits && (splits == 1 || p.k_blocks / splits >= kMinShare); ++splits) {
+      if (splits > 1 && (int64_t)p.tiles * splits > 2 * slots) break;
+      const int64_t waves = ((int64_t)p.tiles * splits + slots - 1) / slots;
+      const int64_t deep = (p.k_blocks + splits - 1) / splits * (pieces > 1 ? 6 : 1);
+      // partials go through L2 twice, and joining them is a launch
+      const double join = splits > 1 ? 4000 + 8.0 * splits * M * N / 4000 : 0;
+      const double t = (double)waves * (deep * s.cycles + 4 * s.bn) + join;
+      if (best.splits == 0 || t < least) {
+        least = t;
+        best = p;
+        best.splits = splits;
+      }
+    }
+  }
+  return best;
+}
+int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
+
+template <typename T, int BN, int CG, bool PIECES>
+int launch_tile(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, const Plan& plan, cudaStream_t stream) {
+  using L = Layout<T, BN, CG>;
+  CUtensorMap amap, bmap, ymap{}, zmap{}, rmap{};
+  if (!make_operand_map(&amap, g.a, g.pieces, g.op_dtype, kBM) ||
+      !make_operand_map(&bmap, g.b, g.pieces, g.op_dtype, BN / CG))
+    return -1;
   GemmParams p{};
   p.M = (int)g.M;
   p.N = (int)g.N;
@@ -461,40 +579,64 @@ int launch_tile(const GemmProblem& g, const Plan& plan, cudaStream_t stream) {
   p.splits = plan.splits;
   p.units = plan.tiles * plan.splits;
   p.k_blocks = plan.k_blocks;
-  p.pieces = g.pieces;
   p.a_mn = g.a.mn_major;
   p.b_mn = g.b.mn_major;
-  p.out = g.out;
-  p.partial = static_cast<float*>(g.ws);
+  p.out = out;
   p.status = g.status;
-  p.idesc = idesc_f16(g.op_dtype == kBF16, kBM, BN) | (g.a.mn_major ? 1u << 15 : 0u) | (g.b.mn_major ? 1u << 16 : 0u);
+  p.idesc = idesc_f16(g.op_dtype == kBF16, kBM * CG, BN) | (g.a.mn_major ? 1u << 15 : 0u) |
+            (g.b.mn_major ? 1u << 16 : 0u);
   auto on16 = [](const void* q, int64_t stride) {
     return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
   };
-  p.vec = on16(g.out.y, g.out.y_stride) && on16(g.out.z, g.out.z_stride) && on16(g.out.residual, g.out.r_stride) &&
-          on16(g.out.bias, 0);
-  auto kern = gemm_kernel<T, BN>;
+  p.store_tma = on16(out.y, out.y_stride) && on16(out.z, out.z_stride);
+  // rows that overlap (a broadcast residual) are not a tensor map's
+  p.residual_tma = out.residual && on16(out.residual, out.r_stride) && out.r_stride >= g.N;
+  if (p.store_tma &&
+      (!make_map(&ymap, out_dtype, out.y, g.N, g.M, plan.splits, out.y_stride, out.y_stride * g.M, 32) ||
+       (out.z && !make_map(&zmap, out_dtype, out.z, g.N, g.M, 1, out.z_stride, out.z_stride * g.M, 32))))
+    return -1;
+  if (p.residual_tma && !make_map(&rmap, out_dtype, out.residual, g.N, g.M, 1, out.r_stride, out.r_stride * g.M, 32))
+    return -1;
+  auto kern = gemm_kernel<T, BN, CG, PIECES>;
   if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem))
     return (int)e;
-  const int grid = p.units < kSms ? p.units : kSms;
-  kern<<<grid, kThreads, L::smem, stream>>>(amap, bmap, p);
-  if (cudaError_t e = cudaGetLastError()) return (int)e;
-  if (plan.splits > 1) {
-    const int64_t work = (g.M * ((g.N + 3) / 4) + 255) / 256;
-    gemm_join_kernel<T><<<(unsigned)(work < 8 * kSms ? work : 8 * kSms), 256, 0, stream>>>(p.partial, plan.splits, g.M,
-                                                                                        g.N, g.out);
-    return (int)cudaGetLastError();
-  }
-  return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(CG * std::min(p.units, kSms / CG)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = L::smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kern, amap, bmap, ymap, zmap, rmap, p);
+}
+
+template <typename T, bool PIECES>
+int launch_shape(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, const Plan& plan, cudaStream_t stream) {
+  const Shape& s = plan.shape;
+  if constexpr (!PIECES)
+    if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, out_dtype, plan, stream);
+  if (s.cg == 2) return launch_tile<T, 128, 2, PIECES>(g, out, out_dtype, plan, stream);
+  if (s.bn == 128) return launch_tile<T, 128, 1, PIECES>(g, out, out_dtype, plan, stream);
+  return launch_tile<T, 64, 1, PIECES>(g, out, out_dtype, plan, stream);
 }
 
 template <typename T>
 int launch_type(const GemmProblem& g, cudaStream_t stream) {
+  constexpr bool PIECES = std::is_same<T, float>::value;
   const Plan plan = plan_of(g.M, g.N, g.K, g.pieces);
-  if (plan.bn == 64) return launch_tile<T, 64>(g, plan, stream);
-  if (plan.bn == 128) return launch_tile<T, 128>(g, plan, stream);
-  if constexpr (!std::is_same<T, float>::value) return launch_tile<T, 256>(g, plan, stream);
-  return -1;
+  if (plan.splits == 1) return launch_shape<T, PIECES>(g, g.out, g.out_dtype, plan, stream);
+  GemmEpilogue parts{};
+  parts.y = g.ws;
+  parts.y_stride = round4(g.N);
+  if (int rc = launch_shape<float, PIECES>(g, parts, kF32, plan, stream)) return rc;
+  const int64_t work = (g.M * (parts.y_stride / 4) + 255) / 256;
+  gemm_join_kernel<T><<<(unsigned)std::min<int64_t>(work, 8 * kSms), 256, 0, stream>>>(
+      static_cast<const float*>(g.ws), plan.splits, parts.y_stride, g.M, g.N, g.out);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace
@@ -502,7 +644,7 @@ int launch_type(const GemmProblem& g, cudaStream_t stream) {
 size_t gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int pieces) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const Plan p = plan_of(M, N, K, pieces);
-  return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
+  return p.splits > 1 ? (size_t)p.splits * M * round4(N) * sizeof(float) : 0;
 }
 
 int launch_gemm(const GemmProblem& g, cudaStream_t stream) {

@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
         float f[8];
         load8(z + m * N, c, N, N % 8 == 0, f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= activation_slope<ACT>(f[j]);
+        for (int j = 0; j < 8; ++j) g[j] *= activation_slope<ACT, T>(f[j]);
       }
       if (out) store_operand<T>(out, m * pitch + c, piece, g);
 #pragma unroll

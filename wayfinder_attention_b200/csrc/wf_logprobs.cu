@@ -32,12 +32,7 @@ using namespace sm100;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr unsigned kAll = 0xffffffffu;
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// the same with results below 2^-126 kept: a gradient multiplies them by what it likes
+// exp2_approx with results below 2^-126 kept: a gradient multiplies them by what it likes
 __device__ __forceinline__ float exp2_small(float x) {
   float y;
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -56,7 +51,7 @@ struct Sums {
   __device__ __forceinline__ void rebase(float M) {
     if (m != M && m != -INFINITY) {
       // a is 0 long before d = -200; the bound keeps 0 * inf out when m is the type's lowest value
-      const float d = max_nan(m - M, -200.f), a = exp2_fast(d * kLog2e);
+      const float d = max_nan(m - M, -200.f), a = exp2_approx(d * kLog2e);
       u = a * fmaf(d, s, u);
       s *= a;
     }
@@ -75,7 +70,7 @@ struct Sums {
     const float base = m == -INFINITY ? 0.f : m;  // -inf - -inf would be NaN
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float d = x[j] - base, e = exp2_fast(d * kLog2e);
+      const float d = x[j] - base, e = exp2_approx(d * kLog2e);
       s += e;
       u = fmaf(e, fmaxf(d, -1e30f), u);  // e = 0 where d = -inf
     }

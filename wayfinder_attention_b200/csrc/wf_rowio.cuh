@@ -7,6 +7,13 @@
 
 namespace wf {
 
+// 2^x by the hardware's approximation (2 units in the last place; results below 2^-126 are 0)
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // VEC consecutive elements as loaded (VEC = 1 or 16 / sizeof(T)).
 template <typename T, int VEC> struct RawVec;
 template <typename T> struct RawVec<T, 1> {
