@@ -5,8 +5,8 @@
 // keeping its 128 rows of the accumulator; the leader issues tcgen05.mma.cta_group::2 for
 // both, so each B element is read from L2 once for 256 rows.  CG = 1: 128 x BN tiles.
 //
-// Warp 8 streams 64-deep slices of A and B into a ring of shared-memory stages with TMA;
-// warp 9 issues the products (fp32 accumulators in TMEM) on them; warps 0-7 read a
+// Warp 16 streams 64-deep slices of A and B into a ring of shared-memory stages with TMA;
+// warp 17 issues the products (fp32 accumulators in TMEM) on them; warps 0-15 read a
 // finished accumulator back, apply the epilogue and store.  Two accumulators alternate, so
 // the epilogue of one tile runs under the products of the next.
 //
@@ -44,9 +44,9 @@ using namespace sm100;
 constexpr int kBM = 128;                // rows of a block
 constexpr int kBK = 64;                 // depth of a stage: 128 bytes
 constexpr int kChunk = 4;               // stages between additions to fp32 registers (three-piece form)
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 16;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
-constexpr uint32_t kBuffer = 32 * 128;  // staging: 32 rows of 128 bytes, two a warp
+constexpr uint32_t kBuffer = 32 * 128;  // staging: 32 rows of 128 bytes a warp
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int kMaxSplits = 32;
 
@@ -63,7 +63,7 @@ struct GemmParams {
 template <typename T, int BN, int CG>
 struct Layout {
   static constexpr uint32_t A_BYTES = kBM * 128, B_BYTES = BN / CG * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr uint32_t STAGING = kEpilogueWarps * 2 * kBuffer;
+  static constexpr uint32_t STAGING = kEpilogueWarps * kBuffer;
   static constexpr int FIT = (227 * 1024 - 2048 - (int)STAGING) / (int)STAGE;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static constexpr size_t off_staging = (size_t)STAGES * STAGE;
@@ -71,10 +71,10 @@ struct Layout {
   static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5 + kEpilogueWarps);
   static constexpr size_t smem = off_misc + 16 + 1024;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
-  // columns of a staging buffer, and of an epilogue warp (a half of the tile, unless that is
-  // less than a buffer: then four of the warps take it all)
+  // columns of a staging buffer, and of an epilogue warp (a quarter of the tile, or a
+  // buffer's where that is more: then fewer warps work)
   static constexpr int CC = 128 / (int)sizeof(T);
-  static constexpr int COLS = BN / 2 < CC ? BN : BN / 2;
+  static constexpr int COLS = BN / 4 < CC ? CC : BN / 4;
   static constexpr int WARPS = 4 * (BN / COLS);
 };
 
@@ -319,12 +319,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < L::WARPS) {
     // ------------------------------------------------------------ epilogue
+    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (a row a lane) and column share w / 4
     constexpr int COLS = L::COLS, CC = L::CC;
-    constexpr int SUB = CC < 32 ? CC : 32;  // columns of a TMEM load
-    static_assert(CC % SUB == 0 && SUB == 32, "a staging buffer holds whole TMEM loads");
     const uint32_t lbase = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * COLS;
-    unsigned char* buf = base + L::off_staging + (size_t)warp * 2 * kBuffer;
-    uint32_t acc = 0, acc_phase = 0, turn = 0, res_phase = 0;
+    unsigned char* buf = base + L::off_staging + (size_t)warp * kBuffer;
+    const GemmEpilogue& o = p.out;
+    uint32_t acc = 0, acc_phase = 0, res_phase = 0;
     auto release = [&] {
       tc_fence_before();
       __syncwarp();
@@ -335,16 +335,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       acc ^= 1;
       acc_phase ^= acc == 0;
     };
+    // the buffer's last store has been read out
+    auto reuse = [&] {
+      if (lane == 0) bulk_wait_read<0>();
+      __syncwarp();
+    };
+    auto load_residual = [&](int m, int n) {
+      if (p.residual_tma) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&res_full[warp], kBuffer);
+          tma_load_3d(buf, &rmap, &res_full[warp], n, m, 0);
+        }
+      } else {
+        copy_rows_in<T, CC>(buf, static_cast<const T*>(o.residual), o.r_stride, m, p.M, n, p.N, lane);
+        __syncwarp();
+      }
+    };
+    auto store = [&](const CUtensorMap* map, void* to, int64_t stride, int m, int n, int layer) {
+      if (p.store_tma) {
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(map, buf, n, m, layer);
+          bulk_commit();
+        }
+      } else {
+        __syncwarp();
+        copy_rows_out<T, CC>(buf, static_cast<T*>(to), stride, m, p.M, n, p.N, lane);
+        fence_async_shared();  // a residual's load may fill the buffer next
+        __syncwarp();
+      }
+    };
     for (int u = first; u < p.units && !why; u += step) {
       const Unit w(p, u, BM, BN);
       const int m = w.m0 + (int)rank * kBM + 32 * (warp & 3);
       const int n0 = w.n0 + (warp >> 2) * COLS;
-      // buffers to use: what is not there to store is skipped, for whole warps
+      // buffers to fill: what is not there to store is skipped, by whole warps
       const int chunks = m < p.M && n0 < p.N ? (min(COLS, p.N - n0) + CC - 1) / CC : 0;
       float sum[PIECES ? COLS : 1];
       if constexpr (PIECES) {
 #pragma unroll
         for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
+      }
+      // the residual comes while the products run (z needs the buffer first where it is kept)
+      if (o.residual && !o.z && chunks > 0) {
+        reuse();
+        load_residual(m, n0);
       }
       for (int c0 = w.kb0; c0 < w.kb1; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
         if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_phase, kWaitNs))) { why = 32; break; }
@@ -363,84 +399,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (why) break;
       const uint32_t src = lbase + acc * BN;
-      auto chunk = [&](int ch) {
-        const int n = n0 + ch * CC;
-        // the buffers' last stores have been read out: both with z, else the older of two in turn
-        unsigned char* zb = buf;
-        unsigned char* yb = p.out.z ? buf + kBuffer : buf + (turn++ & 1) * kBuffer;
-        if (lane == 0) {
-          if (p.out.z) bulk_wait_read<0>();
-          else bulk_wait_read<1>();
-        }
-        __syncwarp();
-        if (p.out.residual) {
-          if (p.residual_tma) {
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&res_full[warp], kBuffer);
-              tma_load_3d(yb, &rmap, &res_full[warp], n, m, 0);
-            }
-          } else {
-            copy_rows_in<T, CC>(yb, static_cast<const T*>(p.out.residual), p.out.r_stride, m, p.M, n, p.N, lane);
-            __syncwarp();
-          }
-        }
-        float v[CC];
+      // z = A B^T + bias, 32 columns from c of the warp's share
+      auto pre = [&](int c, float* v) {
         if constexpr (PIECES) {
 #pragma unroll
-          for (int j = 0; j < CC; ++j) v[j] = sum[ch * CC + j];
-        } else {
-          uint32_t r[CC / 32][32];
+          for (int k = 0; k < COLS; k += 32)  // c is one of these; registers have no other index
+            if (k == c)
 #pragma unroll
-          for (int c = 0; c < CC / 32; ++c) tmem_ld_32x32b_x32(src + ch * CC + 32 * c, r[c]);
+              for (int j = 0; j < 32; ++j) v[j] = sum[k + j];
+        } else {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(src + c, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < CC; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]);
-          if (ch == chunks - 1) release();
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
         }
-        if (p.out.residual && p.residual_tma) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&res_full[warp], res_phase, kWaitNs))) { why = 128; return; }
-          res_phase ^= 1;
+        if (o.bias) add_bias<T>(o.bias, n0 + c, p.N, v);
+      };
+#pragma unroll 1
+      for (int ch = 0; ch < chunks; ++ch) {
+        const int n = n0 + ch * CC;
+        if (o.z) {
+          reuse();
+#pragma unroll 1
+          for (int c = 0; c < CC; c += 32) {
+            float v[32];
+            pre(ch * CC + c, v);
+            stage32<T>(buf, lane, c * (int)sizeof(T), v);
+          }
+          store(&zmap, o.z, o.z_stride, m, n, 0);
         }
-#pragma unroll
+        if (o.residual) {
+          if (o.z || ch > 0) {
+            reuse();
+            load_residual(m, n);
+          }
+          if (p.residual_tma) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&res_full[warp], res_phase, kWaitNs))) { why = 128; break; }
+            res_phase ^= 1;
+          }
+        } else {
+          reuse();
+        }
+#pragma unroll 1
         for (int c = 0; c < CC; c += 32) {
-          if (p.out.bias) add_bias<T>(p.out.bias, n + c, p.N, v + c);
-          if (p.out.z) stage32<T>(zb, lane, c * (int)sizeof(T), v + c);
-          activate_all<T, 32>(p.out.act, v + c);
-          if (p.out.residual) {
+          float v[32];
+          pre(ch * CC + c, v);
+          if (!PIECES && ch == chunks - 1 && c + 32 >= CC) release();
+          activate_all<T, 32>(o.act, v);
+          if (o.residual) {
             constexpr int V = Vec16<T>::N;
 #pragma unroll
             for (int j = 0; j < 32; j += V) {
               float f[V];
-              Vec16<T>::unpack(*reinterpret_cast<const uint4*>(yb + staged(lane, (c + j) * (int)sizeof(T))), f);
+              Vec16<T>::unpack(*reinterpret_cast<const uint4*>(buf + staged(lane, (c + j) * (int)sizeof(T))), f);
 #pragma unroll
-              for (int i = 0; i < V; ++i) v[c + j + i] += f[i];
+              for (int i = 0; i < V; ++i) v[j + i] += f[i];
             }
           }
-          stage32<T>(yb, lane, c * (int)sizeof(T), v + c);
+          stage32<T>(buf, lane, c * (int)sizeof(T), v);
         }
-        if (p.store_tma) {
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) {
-            if (p.out.z) tma_store_3d(&zmap, zb, n, m, 0);
-            tma_store_3d(&ymap, yb, n, m, w.split);
-            bulk_commit();
-          }
-        } else {
-          __syncwarp();
-          if (p.out.z) copy_rows_out<T, CC>(zb, static_cast<T*>(p.out.z), p.out.z_stride, m, p.M, n, p.N, lane);
-          copy_rows_out<T, CC>(yb, static_cast<T*>(p.out.y), p.out.y_stride, m, p.M, n, p.N, lane);
-          fence_async_shared();  // a residual's load may fill the buffer next
-          __syncwarp();
-        }
-      };
-      if constexpr (PIECES) {
-#pragma unroll
-        for (int ch = 0; ch < COLS / CC; ++ch)
-          if (ch < chunks && !why) chunk(ch);
-      } else {
-#pragma unroll 1
-        for (int ch = 0; ch < chunks && !why; ++ch) chunk(ch);
+        store(&ymap, o.y, o.y_stride, m, n, w.split);
       }
       if (!PIECES && chunks == 0) release();
     }
@@ -539,7 +558,6 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
   Plan best{};
   double least = 0;
   for (const Shape& s : kShapes) {
-    if (pieces > 1 && s.bn == 256) continue;  // the sums of a 128 x 256 tile do not fit the registers
     Plan p{};
     p.shape = s;
     p.k_blocks = (int)((K + kBK - 1) / kBK);
@@ -617,8 +635,7 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, co
 template <typename T, bool PIECES>
 int launch_shape(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, const Plan& plan, cudaStream_t stream) {
   const Shape& s = plan.shape;
-  if constexpr (!PIECES)
-    if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, out_dtype, plan, stream);
+  if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, out_dtype, plan, stream);
   if (s.cg == 2) return launch_tile<T, 128, 2, PIECES>(g, out, out_dtype, plan, stream);
   if (s.bn == 128) return launch_tile<T, 128, 1, PIECES>(g, out, out_dtype, plan, stream);
   return launch_tile<T, 64, 1, PIECES>(g, out, out_dtype, plan, stream);
