@@ -60,7 +60,7 @@ struct GemmParams {
   uint32_t idesc;
 };
 
-template <typename T, int BN, int CG>
+template <typename T, int BN, int CG, bool PIECES>
 struct Layout {
   static constexpr uint32_t A_BYTES = kBM * 128, B_BYTES = BN / CG * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr uint32_t STAGING = kEpilogueWarps * kBuffer;
@@ -71,11 +71,15 @@ struct Layout {
   static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5 + kEpilogueWarps);
   static constexpr size_t smem = off_misc + 16 + 1024;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
-  // columns of a staging buffer, and of an epilogue warp (a quarter of the tile, or a
-  // buffer's where that is more: then fewer warps work)
+  // Epilogue groups: two of 8 warps take tiles in turn, each with an accumulator of its own,
+  // so that one waits while the other computes.  (Three pieces: all 16 warps, as a tile's
+  // sums pass through both accumulators.)
+  static constexpr int GROUPS = PIECES ? 1 : 2;
+  static constexpr int SHARES = kEpilogueWarps / GROUPS / 4;  // of a tile's columns
+  // columns of a staging buffer, and of a warp (a buffer's at least: then fewer warps work)
   static constexpr int CC = 128 / (int)sizeof(T);
-  static constexpr int COLS = BN / 4 < CC ? CC : BN / 4;
-  static constexpr int WARPS = 4 * (BN / COLS);
+  static constexpr int COLS = BN / SHARES < CC ? CC : BN / SHARES;
+  static constexpr int WARPS = 4 * (BN / COLS);  // of a group that have columns
 };
 
 // Pieces of a and b multiplied in this order: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0).
@@ -109,12 +113,21 @@ struct Ring {
 struct Unit {
   int m0, n0, kb0, kb1, split;
   __device__ __forceinline__ Unit(const GemmParams& p, int u, int BM, int BN) {
-    split = u % p.splits;
-    const int tile = u / p.splits;
-    m0 = tile / p.tiles_n * BM;
-    n0 = tile % p.tiles_n * BN;
-    kb0 = (int)((int64_t)p.k_blocks * split / p.splits);
-    kb1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
+    // shares of the depth differ by one stage at most; products stay below 2^30 * 32 / 64
+    const uint32_t splits = p.splits, kb = p.k_blocks;
+    uint32_t tile = u;
+    split = 0;
+    kb0 = 0;
+    kb1 = kb;
+    if (splits > 1) {
+      tile = (uint32_t)u / splits;
+      split = u - tile * splits;
+      kb0 = kb * split / splits;
+      kb1 = kb * (split + 1) / splits;
+    }
+    const uint32_t tm = tile / (uint32_t)p.tiles_n;
+    m0 = tm * BM;
+    n0 = (tile - tm * p.tiles_n) * BN;
   }
 };
 
@@ -142,32 +155,65 @@ __device__ __forceinline__ void copy_rows_in(unsigned char* buf, const T* x, int
       if (n + c < N) *reinterpret_cast<T*>(buf + staged(r, c * (int)sizeof(T))) = x[(m + r) * stride + n + c];
 }
 
-// y += bias over 32 columns from n.
+// bias over 32 columns from n, raw where whole vectors can be loaded
 template <typename T>
-__device__ __forceinline__ void add_bias(const void* bias, int n, int N, float* v) {
-  constexpr int V = Vec16<T>::N;
-  const T* b = static_cast<const T*>(bias) + n;
-  if (n + 32 <= N && reinterpret_cast<uintptr_t>(b) % 16 == 0) {
+struct Bias32 {
+  static constexpr int V = Vec16<T>::N;
+  uint4 raw[32 / V];
+  bool vec;
+  __device__ __forceinline__ void load(const void* bias, int n, int N) {
+    const T* b = static_cast<const T*>(bias) + n;
+    vec = n + 32 <= N && reinterpret_cast<uintptr_t>(b) % 16 == 0;
+    if (vec) {
 #pragma unroll
-    for (int j = 0; j < 32; j += V) {
-      float f[V];
-      Vec16<T>::unpack(ldg16(b + j), f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[j + i] += f[i];
+      for (int j = 0; j < 32 / V; ++j) raw[j] = ldg16(b + j * V);
     }
-  } else {
+  }
+  __device__ __forceinline__ void add(const void* bias, int n, int N, float* v) const {
+    if (vec) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n + j < N) v[j] += to_f32(b[j]);
+      for (int j = 0; j < 32 / V; ++j) {
+        float f[V];
+        Vec16<T>::unpack(raw[j], f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j * V + i] += f[i];
+      }
+    } else {
+      const T* b = static_cast<const T*>(bias) + n;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (n + j < N) v[j] += to_f32(b[j]);
+    }
+  }
+};
+
+// 32 columns of a lane's row to bytes `at` on of its staging row, and back.
+template <typename T>
+__device__ __forceinline__ void stage32(uint32_t buf, int lane, int at, const float* v) {
+  constexpr int V = Vec16<T>::N;
+#pragma unroll
+  for (int j = 0; j < 32; j += V) {
+    uint4 q;
+    if constexpr (sizeof(T) == 4) {
+      q = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]),
+                     __float_as_uint(v[j + 3]));
+    } else {
+      q = make_uint4(pack2(T(), v[j], v[j + 1]), pack2(T(), v[j + 2], v[j + 3]), pack2(T(), v[j + 4], v[j + 5]),
+                     pack2(T(), v[j + 6], v[j + 7]));
+    }
+    st_shared_16(buf + staged(lane, at + j * (int)sizeof(T)), q);
   }
 }
-
 template <typename T>
-__device__ __forceinline__ void stage32(unsigned char* buf, int lane, int at, const float* v) {
+__device__ __forceinline__ void add_staged32(uint32_t buf, int lane, int at, float* v) {
   constexpr int V = Vec16<T>::N;
 #pragma unroll
-  for (int j = 0; j < 32; j += V)
-    store_vec<T, V>(reinterpret_cast<T*>(buf + staged(lane, at + j * (int)sizeof(T))), v + j);
+  for (int j = 0; j < 32; j += V) {
+    float f[V];
+    Vec16<T>::unpack(ld_shared_16(buf + staged(lane, at + j * (int)sizeof(T))), f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[j + i] += f[i];
+  }
 }
 
 template <typename T, int BN, int CG, bool PIECES>
@@ -175,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                 const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap zmap,
                 const __grid_constant__ CUtensorMap rmap, const GemmParams p) {
-  using L = Layout<T, BN, CG>;
+  using L = Layout<T, BN, CG, PIECES>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -291,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Unit w(p, u, BM, BN);
         for (int c0 = w.kb0; c0 < w.kb1 && !why; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
           const int c1 = PIECES ? min(c0 + kChunk, w.kb1) : w.kb1;
-          if (!mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1, kWaitNs)) { why = 8; break; }
+          if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, kWaitNs)) { why = 8; break; }
           tc_fence_after();
           const uint32_t d = tmem + acc * BN;
           const int n = (c1 - c0) * pairs;
@@ -317,23 +363,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       commit(drained);
     }
-  } else if (warp < L::WARPS) {
+  } else if (warp % (kEpilogueWarps / L::GROUPS) < L::WARPS) {
     // ------------------------------------------------------------ epilogue
-    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (a row a lane) and column share w / 4
+    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (a row a lane) and one share of the columns
     constexpr int COLS = L::COLS, CC = L::CC;
-    const uint32_t lbase = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * COLS;
+    const int group = warp / (kEpilogueWarps / L::GROUPS), share = warp / 4 % L::SHARES;
+    const uint32_t lbase = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + share * COLS;
     unsigned char* buf = base + L::off_staging + (size_t)warp * kBuffer;
+    const uint32_t sbuf = smem_u32(buf);
     const GemmEpilogue& o = p.out;
-    uint32_t acc = 0, acc_phase = 0, res_phase = 0;
+    uint32_t acc = group, acc_phase = 0, res_phase = 0;
     auto release = [&] {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         if (rank == 0) mbar_arrive(&acc_empty[acc]);
-        else mbar_arrive_peer(map_peer(&acc_empty[acc], 0));
+        else mbar_arrive_peer_relaxed(map_peer(&acc_empty[acc], 0));
       }
-      acc ^= 1;
-      acc_phase ^= acc == 0;
+      if constexpr (L::GROUPS == 2) {
+        acc_phase ^= 1;
+      } else {
+        acc ^= 1;
+        acc_phase ^= acc == 0;
+      }
     };
     // the buffer's last store has been read out
     auto reuse = [&] {
@@ -366,10 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     };
-    for (int u = first; u < p.units && !why; u += step) {
+    for (int u = first + group * step; u < p.units && !why; u += L::GROUPS * step) {
       const Unit w(p, u, BM, BN);
       const int m = w.m0 + (int)rank * kBM + 32 * (warp & 3);
-      const int n0 = w.n0 + (warp >> 2) * COLS;
+      const int n0 = w.n0 + share * COLS;
       // buffers to fill: what is not there to store is skipped, by whole warps
       const int chunks = m < p.M && n0 < p.N ? (min(COLS, p.N - n0) + CC - 1) / CC : 0;
       float sum[PIECES ? COLS : 1];
@@ -378,10 +430,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
       }
       // the residual comes while the products run (z needs the buffer first where it is kept)
-      if (o.residual && !o.z && chunks > 0) {
-        reuse();
-        load_residual(m, n0);
-      }
+      reuse();
+      if (o.residual && !o.z && chunks > 0) load_residual(m, n0);
       for (int c0 = w.kb0; c0 < w.kb1; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
         if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_phase, kWaitNs))) { why = 32; break; }
         tc_fence_after();
@@ -401,12 +451,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t src = lbase + acc * BN;
       // z = A B^T + bias, 32 columns from c of the warp's share
       auto pre = [&](int c, float* v) {
+        Bias32<T> bias;
+        if (o.bias) bias.load(o.bias, n0 + c, p.N);
         if constexpr (PIECES) {
 #pragma unroll
-          for (int k = 0; k < COLS; k += 32)  // c is one of these; registers have no other index
-            if (k == c)
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = sum[k + j];
+          for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
         } else {
           uint32_t r[32];
           tmem_ld_32x32b_x32(src + c, r);
@@ -414,18 +463,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
         }
-        if (o.bias) add_bias<T>(o.bias, n0 + c, p.N, v);
+        if (o.bias) bias.add(o.bias, n0 + c, p.N, v);
       };
-#pragma unroll 1
-      for (int ch = 0; ch < chunks; ++ch) {
+#pragma unroll(PIECES ? COLS / CC : 1)
+      for (int ch = 0; ch < COLS / CC; ++ch) {
+        if (ch >= chunks || why) break;
         const int n = n0 + ch * CC;
         if (o.z) {
-          reuse();
-#pragma unroll 1
+          if (ch > 0) reuse();
+#pragma unroll(PIECES ? CC / 32 : 1)
           for (int c = 0; c < CC; c += 32) {
             float v[32];
             pre(ch * CC + c, v);
-            stage32<T>(buf, lane, c * (int)sizeof(T), v);
+            stage32<T>(sbuf, lane, c * (int)sizeof(T), v);
           }
           store(&zmap, o.z, o.z_stride, m, n, 0);
         }
@@ -438,26 +488,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!__all_sync(0xffffffffu, mbar_wait(&res_full[warp], res_phase, kWaitNs))) { why = 128; break; }
             res_phase ^= 1;
           }
-        } else {
+        } else if (o.z || ch > 0) {
           reuse();
         }
-#pragma unroll 1
+#pragma unroll(PIECES ? CC / 32 : 1)
         for (int c = 0; c < CC; c += 32) {
           float v[32];
           pre(ch * CC + c, v);
           if (!PIECES && ch == chunks - 1 && c + 32 >= CC) release();
           activate_all<T, 32>(o.act, v);
-          if (o.residual) {
-            constexpr int V = Vec16<T>::N;
-#pragma unroll
-            for (int j = 0; j < 32; j += V) {
-              float f[V];
-              Vec16<T>::unpack(*reinterpret_cast<const uint4*>(buf + staged(lane, (c + j) * (int)sizeof(T))), f);
-#pragma unroll
-              for (int i = 0; i < V; ++i) v[j + i] += f[i];
-            }
-          }
-          stage32<T>(buf, lane, c * (int)sizeof(T), v);
+          if (o.residual) add_staged32<T>(sbuf, lane, c * (int)sizeof(T), v);
+          stage32<T>(sbuf, lane, c * (int)sizeof(T), v);
         }
         store(&ymap, o.y, o.y_stride, m, n, w.split);
       }
@@ -585,7 +626,7 @@ int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 
 template <typename T, int BN, int CG, bool PIECES>
 int launch_tile(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, const Plan& plan, cudaStream_t stream) {
-  using L = Layout<T, BN, CG>;
+  using L = Layout<T, BN, CG, PIECES>;
   CUtensorMap amap, bmap, ymap{}, zmap{}, rmap{};
   if (!make_operand_map(&amap, g.a, g.pieces, g.op_dtype, kBM) ||
       !make_operand_map(&bmap, g.b, g.pieces, g.op_dtype, BN / CG))
