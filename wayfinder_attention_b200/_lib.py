@@ -241,7 +241,13 @@ def workspace(B: int, Tq: int, Tk: int, R: int, top_k: int, dtype: torch.dtype, 
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
+# The current stream's handle without building a torch.cuda.Stream (2 us a call less).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -260,6 +266,8 @@ def on_device(dev: torch.device):
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """``t`` as (rows, last axis) with unit-strided, non-overlapping rows (copied only if it has to be)."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if (r.stride(1) != 1 and r.shape[1] > 1) or (r.stride(0) < r.shape[1] and r.shape[0] > 1):
         r = r.contiguous()

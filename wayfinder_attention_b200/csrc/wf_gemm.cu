@@ -34,6 +34,7 @@
 #include "wf_sm100.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace wf {
@@ -607,7 +608,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
     p.tiles = (int)(tn * tm);
     const int slots = kSms / s.cg;
     for (int splits = 1; splits <= kMaxSplits && (splits == 1 || p.k_blocks / splits >= kMinShare); ++splits) {
-      if (splits > 1 && (int64_t)p.tiles * splits > 2 * slots) break;
+      if (splits > 1 && (int64_t)p.tiles * splits > 2 * slots) break;  // most shapes look at one split
       const int64_t waves = ((int64_t)p.tiles * splits + slots - 1) / slots;
       const int64_t deep = (p.k_blocks + splits - 1) / splits * (pieces > 1 ? 6 : 1);
       // partials go through L2 twice, and joining them is a launch
@@ -657,8 +658,14 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, co
   if (p.residual_tma && !make_map(&rmap, out_dtype, out.residual, g.N, g.M, 1, out.r_stride, out.r_stride * g.M, 32))
     return -1;
   auto kern = gemm_kernel<T, BN, CG, PIECES>;
-  if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem))
-    return (int)e;
+  static std::atomic<uint64_t> allowed{0};  // devices whose limit has been raised for this kernel
+  int device = 0;
+  if (cudaError_t e = cudaGetDevice(&device)) return (int)e;
+  if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
+    if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem))
+      return (int)e;
+    if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(CG * std::min(p.units, kSms / CG)));
   cfg.blockDim = dim3(kThreads);

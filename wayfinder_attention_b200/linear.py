@@ -31,23 +31,26 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _launch(x, weight, bias, residual, act, keep_z, status):
-    """y (and the pre-activations z when the backward will want them); x and residual as rows."""
+def _launch(x, weight, bias, residual, act, keep_z, shape, status):
+    """y of the given shape (and the pre-activations z when the backward will want them); x and residual as rows."""
     dev = x.device
     M, K = x.shape
     N = weight.shape[0]
-    y = torch.empty(M, N, dtype=x.dtype, device=dev)
-    z = torch.empty(M, N, dtype=x.dtype, device=dev) if keep_z else None
+    y = x.new_empty(shape)
+    z = x.new_empty((M, N)) if keep_z else None
     code = _lib.dtype_code(x.dtype)
-    n = _workspace_bytes(M, N, K, code, _lib.on_16_bytes(x), _lib.on_16_bytes(weight))
+    xp, xs, wp, w_stride = x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0)
+    size = 4 if code == _lib.WF_DTYPE_F32 else 2
+    n = _workspace_bytes(M, N, K, code, (xp | xs * size) & 15 == 0, (wp | w_stride * size) & 15 == 0)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     st = _lib.status_arg(dev, status)
     with _lib.on_device(dev):
         rc = _lib.load_library().wf_linear(
-            x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), code, M, N, K, x.stride(0), weight.stride(0),
+            xp, wp, _ptr(bias), _ptr(residual), code, M, N, K, xs, w_stride,
             0 if residual is None else residual.stride(0), act, _ptr(z), y.data_ptr(), _ptr(ws), n, st,
             _lib.stream_ptr(dev))
-    _lib.check(rc)
+    if rc:
+        _lib.check(rc)
     _lib.status_after(dev, status)
     return y, z
 
@@ -55,12 +58,12 @@ def _launch(x, weight, bias, residual, act, keep_z, status):
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        x2, w2 = _lib.rows_of(x), _lib.rows_of(weight)
-        r2 = None if residual is None else _lib.rows_of(residual)
-        y, z = _launch(x2, w2, bias, r2, act, act != 0, None)
+        x2, w2 = _lib.row_strideof(x), _lib.row_strideof(weight)
+        r2 = None if residual is None else _lib.row_strideof(residual)
+        y, z = _launch(x2, w2, bias, r2, act, act != 0, (*x.shape[:-1], w2.shape[0]), None)
         ctx.save_for_backward(x2, w2, z)
         ctx.act, ctx.x_shape = act, x.shape
-        return y.view(*x.shape[:-1], y.shape[1])
+        return y
 
     @staticmethod
     @once_differentiable
@@ -70,10 +73,10 @@ class _LinearFunction(torch.autograd.Function):
         M, K = x.shape
         N = weight.shape[0]
         dev = x.device
-        g = _lib.rows_of(dy)
-        dx = torch.empty(M, K, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty(N, K, dtype=x.dtype, device=dev) if need_w else None
-        db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
+        g = _lib.row_strideof(dy)
+        dx = x.new_empty(ctx.x_shape) if need_x else None
+        dw = x.new_empty((N, K)) if need_w else None
+        db = x.new_empty(N) if need_b else None
         if need_x or need_w or need_b:
             code = _lib.dtype_code(x.dtype)
             n = _backward_workspace_bytes(M, N, K, code, ctx.act, _lib.on_16_bytes(x), _lib.on_16_bytes(weight),
@@ -85,9 +88,10 @@ class _LinearFunction(torch.autograd.Function):
                     x.data_ptr(), weight.data_ptr(), _ptr(z), g.data_ptr(), code, M, N, K, x.stride(0),
                     weight.stride(0), g.stride(0), ctx.act, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), n, st,
                     _lib.stream_ptr(dev))
-            _lib.check(rc)
+            if rc:
+                _lib.check(rc)
             _lib.status_after(dev, None)
-        return (dx.view(ctx.x_shape) if need_x else None), dw, db, (dy if need_r else None), None
+        return dx, dw, db, (dy if need_r else None), None
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, activation: str = "none",
@@ -100,28 +104,32 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     Differentiable in x, weight, bias and residual; the backward reads the
     pre-activations as rounded to x's type and gives every gradient in it.
     """
-    tensors = [t for t in (x, weight, bias, residual) if t is not None]
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}; expected one of {', '.join(ACTIVATIONS)}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError(f"expected x (..., d_in) and weight (d_out, d_in) with widths >= 1, got {tuple(x.shape)} "
                          f"and {tuple(weight.shape)}")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError(f"bias {tuple(bias.shape)} does not match d_out={weight.shape[0]}")
-    if residual is not None and residual.shape != x.shape[:-1] + weight.shape[:1]:
-        raise ValueError(f"residual {tuple(residual.shape)} does not have the output's shape "
-                         f"{(*x.shape[:-1], weight.shape[0])}")
+    shape = (*x.shape[:-1], weight.shape[0])
+    tensors = [x, weight]
+    if bias is not None:
+        if bias.shape != weight.shape[:1]:
+            raise ValueError(f"bias {tuple(bias.shape)} does not match d_out={weight.shape[0]}")
+        bias = bias.contiguous()
+        tensors.append(bias)
+    if residual is not None:
+        if residual.shape != shape:
+            raise ValueError(f"residual {tuple(residual.shape)} does not have the output's shape {shape}")
+        tensors.append(residual)
+    dtype, need_grad = x.dtype, False
     for t in tensors:
-        if t.dtype != x.dtype:
-            raise ValueError(f"x, weight, bias and residual must have one type, got {x.dtype} and {t.dtype}")
+        if t.dtype != dtype:
+            raise ValueError(f"x, weight, bias and residual must have one type, got {dtype} and {t.dtype}")
+        need_grad = need_grad or t.requires_grad
     _lib.require_cuda(*tensors)
-    _lib.dtype_code(x.dtype)
-    bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if need_grad and torch.is_grad_enabled():
         if status is not None:
             raise ValueError("status is not supported on the differentiable path")
         return _LinearFunction.apply(x, weight, bias, residual, ACTIVATIONS[activation])
-    x2 = _lib.rows_of(x)
-    y, _ = _launch(x2, _lib.rows_of(weight), bias, None if residual is None else _lib.rows_of(residual),
-                   ACTIVATIONS[activation], False, status)
-    return y.view(*x.shape[:-1], weight.shape[0])
+    y, _ = _launch(_lib.row_strideof(x), _lib.row_strideof(weight), bias, None if residual is None else _lib.row_strideof(residual),
+                   ACTIVATIONS[activation], False, shape, status)
+    return y

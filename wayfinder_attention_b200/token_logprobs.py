@@ -15,6 +15,9 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 
+MAX_TOP_TOKENS = 32  # wf_max_top_tokens()
+
+
 class TokenLogprobs(NamedTuple):
     logprob: torch.Tensor  # (...) float32
     entropy: torch.Tensor  # (...) float32
@@ -22,30 +25,31 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor  # (..., top_n) int64
 
 
-def _launch(logits, tokens, top_n, ignore_index, keep_stats, status):
+def _launch(logits, tokens, top_n, ignore_index, lead, keep_stats, status):
     dev = logits.device
     rows, vocab = logits.shape
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
     stats = torch.empty(2, rows, dtype=torch.float32, device=dev) if keep_stats else None
-    top_logprobs = torch.empty(rows, top_n, dtype=torch.float32, device=dev)
-    top_tokens = torch.empty(rows, top_n, dtype=torch.int64, device=dev)
+    top_logprobs = torch.empty((*lead, top_n), dtype=torch.float32, device=dev)
+    top_tokens = torch.empty((*lead, top_n), dtype=torch.int64, device=dev)
     st = _lib.status_arg(dev, status)
     with _lib.on_device(dev):
         rc = _lib.load_library().wf_token_logprobs(
             logits.data_ptr(), _lib.dtype_code(logits.dtype), rows, vocab, logits.stride(0), tokens.data_ptr(),
             ignore_index, top_n, logprob.data_ptr(), entropy.data_ptr(), None if stats is None else stats.data_ptr(),
             top_logprobs.data_ptr(), top_tokens.data_ptr(), st, _lib.stream_ptr(dev))
-    _lib.check(rc)
+    if rc:
+        _lib.check(rc)
     _lib.status_after(dev, status)
     return logprob, entropy, stats, top_logprobs, top_tokens
 
 
 class _TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, top_n, ignore_index):
+    def forward(ctx, logits, tokens, top_n, ignore_index, lead):
         x = _lib.rows_of(logits)
-        logprob, entropy, stats, top_logprobs, top_tokens = _launch(x, tokens, top_n, ignore_index, True, None)
+        logprob, entropy, stats, top_logprobs, top_tokens = _launch(x, tokens, top_n, ignore_index, lead, True, None)
         ctx.save_for_backward(x, tokens, stats, entropy)
         ctx.ignore_index, ctx.shape = ignore_index, logits.shape
         ctx.mark_non_differentiable(top_logprobs, top_tokens)
@@ -56,20 +60,21 @@ class _TokenLogprobsFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dlogprob, dentropy, _top_logprobs, _top_tokens):
         if dlogprob is None and dentropy is None:
-            return None, None, None, None
+            return None, None, None, None, None
         x, tokens, stats, entropy = ctx.saved_tensors
         rows, vocab = x.shape
         dev = x.device
         dlogprob = None if dlogprob is None else dlogprob.contiguous()
         dentropy = None if dentropy is None else dentropy.contiguous()
-        dx = torch.empty(rows, vocab, dtype=x.dtype, device=dev)
+        dx = x.new_empty(ctx.shape)
         with _lib.on_device(dev):
             rc = _lib.load_library().wf_token_logprobs_backward(
                 x.data_ptr(), _lib.dtype_code(x.dtype), rows, vocab, x.stride(0), tokens.data_ptr(), ctx.ignore_index,
                 stats.data_ptr(), entropy.data_ptr(), None if dlogprob is None else dlogprob.data_ptr(),
                 None if dentropy is None else dentropy.data_ptr(), dx.data_ptr(), _lib.stream_ptr(dev))
-        _lib.check(rc)
-        return dx.view(ctx.shape), None, None, None
+        if rc:
+            _lib.check(rc)
+        return dx, None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0, ignore_index: int = -100,
@@ -89,20 +94,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0, i
         raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
     if tokens.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"tokens must be int64 or int32, got {tokens.dtype}")
-    most = min(logits.shape[-1], _lib.load_library().wf_max_top_tokens())
+    most = min(logits.shape[-1], MAX_TOP_TOKENS)
     if not 0 <= top_n <= most:
         raise ValueError(f"top_n must be in [0, {most}] here, got {top_n}")
     _lib.require_cuda(logits, tokens)
-    _lib.dtype_code(logits.dtype)
     lead = tokens.shape
-    flat = tokens.reshape(-1).to(torch.int64).contiguous()
+    flat = tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)
+    flat = flat if flat.is_contiguous() else flat.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         if status is not None:
             raise ValueError("status is not supported on the differentiable path")
-        logprob, entropy, top_logprobs, top_tokens = _TokenLogprobsFunction.apply(logits, flat, int(top_n),
-                                                                                  int(ignore_index))
-    else:
-        logprob, entropy, _, top_logprobs, top_tokens = _launch(_lib.rows_of(logits), flat, int(top_n),
-                                                                int(ignore_index), False, status)
-    return TokenLogprobs(logprob.view(lead), entropy.view(lead), top_logprobs.view(*lead, top_n),
-                         top_tokens.view(*lead, top_n))
+        return TokenLogprobs(*_TokenLogprobsFunction.apply(logits, flat, top_n, ignore_index, lead))
+    logprob, entropy, _, top_logprobs, top_tokens = _launch(_lib.rows_of(logits), flat, top_n, ignore_index, lead,
+                                                            False, status)
+    return TokenLogprobs(logprob, entropy, top_logprobs, top_tokens)
