@@ -58,28 +58,65 @@ __device__ __forceinline__ float max_keep_nan(float a, float b) {
   return y;
 }
 
-// gelu(z) = max(z, 0) - |z| Phi(-|z|), two at a time with the polynomial in paired
-// arithmetic.  Past 100 the tail is 0, and inf * 0 is kept out.
-__device__ __forceinline__ void gelu2(float& a, float& b) {
-  const Pair az(fminf(fabsf(a), 100.f), fminf(fabsf(b), 100.f));
-  float d0, d1, x0, x1;
-  fma2(az, Pair(kErfcP), Pair(1.f)).get(d0, d1);
-  mul2(mul2(az, Pair(kGaussExp2)), az).get(x0, x1);
-  const Pair t(rcp_approx(d0), rcp_approx(d1)), e(exp2_approx(x0), exp2_approx(x1));
-  Pair q = fma2(t, Pair(-kErfc4), Pair(-kErfc3));
-  q = fma2(t, q, Pair(-kErfc2));
-  q = fma2(t, q, Pair(-kErfc1));
-  q = fma2(t, q, Pair(-kErfc0));
-  q = mul2(mul2(q, t), e);
-  fma2(az, q, Pair(max_keep_nan(a, 0.f), max_keep_nan(b, 0.f))).get(a, b);
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
 }
+
+// gelu(z) = max(z, 0) - |z| Phi(-|z|), two at a time with the polynomial in paired
+// arithmetic.  Past 100 the tail is 0, and inf * 0 is kept out.  Paired instructions take
+// no immediates: the constants are made once, and hidden from the compiler so that it keeps
+// them in registers instead of moving them there again for each pair.
+struct Gelu2 {
+  Pair p, g, c4, c3, c2, c1, c0, one;
+  __device__ __forceinline__ static Pair kept(float x) {
+    Pair q(x);
+    asm volatile("" : "+l"(q.v));
+    return q;
+  }
+  __device__ __forceinline__ Gelu2()
+      : p(kept(kErfcP)), g(kept(kGaussExp2)), c4(kept(-kErfc4)), c3(kept(-kErfc3)), c2(kept(-kErfc2)),
+        c1(kept(-kErfc1)), c0(kept(-kErfc0)), one(kept(1.f)) {}
+  // B pairs side by side: a pair alone is a chain of some hundred cycles.
+  template <int B>
+  __device__ __forceinline__ void apply(float* v) const {
+    Pair az[B], q[B], t[B], e[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      az[i] = Pair(fminf(fabsf(v[2 * i]), 100.f), fminf(fabsf(v[2 * i + 1]), 100.f));
+      float d0, d1;
+      fma2(az[i], p, one).get(d0, d1);
+      t[i] = Pair(rcp_approx(d0), rcp_approx(d1));
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      float x0, x1;
+      mul2(mul2(az[i], g), az[i]).get(x0, x1);
+      e[i] = Pair(exp2_approx(x0), exp2_approx(x1));
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], c4, c3);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c2);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c1);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c0);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = mul2(mul2(q[i], t[i]), e[i]);
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+      fma2(az[i], q[i], Pair(max_keep_nan(v[2 * i], 0.f), max_keep_nan(v[2 * i + 1], 0.f))).get(v[2 * i], v[2 * i + 1]);
+  }
+};
 
 // T: the type of the result.  fp32 takes CUDA's erff and expf and a true division.
 template <int ACT, typename T>
 __device__ __forceinline__ float activate(float z) {
   constexpr bool FAST = sizeof(T) == 2;
   if constexpr (ACT == kActGelu) {
-    static_assert(!FAST, "gelu2 is the 16-bit form");
+    static_assert(!FAST, "Gelu2 is the 16-bit form");
     return z * 0.5f * (1.f + erff(z * 0.70710678118654752f));
   } else if constexpr (ACT == kActRelu) {
     return z < 0.f ? 0.f : z;  // NaN stays
@@ -121,8 +158,10 @@ __device__ __forceinline__ void activate_all(int act, float* v) {
   switch (act) {
     case kActGelu:
       if constexpr (sizeof(T) == 2) {
+        const Gelu2 gelu;
+        constexpr int BATCH = N < 8 ? N / 2 : 4;
 #pragma unroll
-        for (int j = 0; j < N; j += 2) gelu2(v[j], v[j + 1]);
+        for (int j = 0; j < N; j += 2 * BATCH) gelu.apply<BATCH>(v + j);
       } else {
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = activate<kActGelu, T>(v[j]);

@@ -20,10 +20,12 @@
 // length of a sum than fp32 rounding would, so every kChunk of depth the accumulator is
 // added to fp32 registers and begun anew.
 //
-// Epilogue: a warp owns 32 rows (its TMEM lanes, a row a lane) and walks them 128 bytes of
-// output at a time through a swizzled shared-memory buffer, which TMA stores write out in
-// whole lines (and a TMA load fills with the residual first).  Outputs whose rows do not
-// start on 16 bytes go from the buffer with coalesced element stores instead.
+// Epilogue: a warp owns 32 rows (its TMEM lanes, a row a lane) and walks them in slices of
+// 64 bytes of output, through two swizzled shared-memory buffers in turn that TMA stores
+// write out (and TMA loads fill with the residual first).  The next slice's accumulator,
+// the next tile's too, is on its way while one is computed.  (Stores from registers, 32
+// bytes a lane and row, took half as long again: 32 lines an instruction.)  Outputs whose
+// rows do not start on 16 bytes go from the buffers with coalesced element stores instead.
 //
 // Few tiles with a deep sum (a weight's gradient over many rows) are split along the
 // depth: each part writes fp32 partials, and a second kernel adds them in order and
@@ -36,6 +38,7 @@
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
+#include <utility>
 
 namespace wf {
 namespace {
@@ -47,15 +50,16 @@ constexpr int kBK = 64;                 // depth of a stage: 128 bytes
 constexpr int kChunk = 4;               // stages between additions to fp32 registers (three-piece form)
 constexpr int kEpilogueWarps = 16;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
-constexpr uint32_t kBuffer = 32 * 128;  // staging: 32 rows of 128 bytes a warp
+constexpr int kSliceBytes = 64;         // of a row of output
+constexpr uint32_t kBuffer = 32 * kSliceBytes;  // staging: two a warp
 constexpr uint64_t kWaitNs = 1000000000ull;
 constexpr int kMaxSplits = 32;
 
 struct GemmParams {
   int M, N, tiles_n, units, splits, k_blocks;
   bool a_mn, b_mn;
-  bool store_tma;     // y (and z) can be TMA's
-  bool residual_tma;
+  bool store_tma, residual_tma;  // y and z, the residual start and step on 16 bytes
+  bool bias_vec;                 // so does the bias
   GemmEpilogue out;
   int32_t* status;
   uint32_t idesc;
@@ -64,23 +68,19 @@ struct GemmParams {
 template <typename T, int BN, int CG, bool PIECES>
 struct Layout {
   static constexpr uint32_t A_BYTES = kBM * 128, B_BYTES = BN / CG * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr uint32_t STAGING = kEpilogueWarps * kBuffer;
+  static constexpr uint32_t STAGING = kEpilogueWarps * 2 * kBuffer;
   static constexpr int FIT = (227 * 1024 - 2048 - (int)STAGING) / (int)STAGE;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   static constexpr size_t off_staging = (size_t)STAGES * STAGE;
   static constexpr size_t off_bar = off_staging + STAGING;
-  static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5 + kEpilogueWarps);
+  static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5 + 2 * kEpilogueWarps);
   static constexpr size_t smem = off_misc + 16 + 1024;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
-  // Epilogue groups: two of 8 warps take tiles in turn, each with an accumulator of its own,
-  // so that one waits while the other computes.  (Three pieces: all 16 warps, as a tile's
-  // sums pass through both accumulators.)
-  static constexpr int GROUPS = PIECES ? 1 : 2;
-  static constexpr int SHARES = kEpilogueWarps / GROUPS / 4;  // of a tile's columns
-  // columns of a staging buffer, and of a warp (a buffer's at least: then fewer warps work)
-  static constexpr int CC = 128 / (int)sizeof(T);
-  static constexpr int COLS = BN / SHARES < CC ? CC : BN / SHARES;
-  static constexpr int WARPS = 4 * (BN / COLS);  // of a group that have columns
+  // columns of a slice, and of an epilogue warp (a quarter of the tile, or a slice's where
+  // that is more: then fewer warps work)
+  static constexpr int SC = kSliceBytes / (int)sizeof(T);
+  static constexpr int COLS = BN / 4 < SC ? SC : BN / 4;
+  static constexpr int WARPS = 4 * (BN / COLS);
 };
 
 // Pieces of a and b multiplied in this order: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0).
@@ -113,107 +113,97 @@ struct Ring {
 // Units of work: a tile and a share of the depth.
 struct Unit {
   int m0, n0, kb0, kb1, split;
-  __device__ __forceinline__ Unit(const GemmParams& p, int u, int BM, int BN) {
+  __device__ __forceinline__ Unit(const GemmParams& p, uint32_t u, int BM, int BN) {
     // shares of the depth differ by one stage at most; products stay below 2^30 * 32 / 64
-    const uint32_t splits = p.splits, kb = p.k_blocks;
-    uint32_t tile = u;
+    const uint32_t kb = p.k_blocks;
     split = 0;
     kb0 = 0;
     kb1 = kb;
-    if (splits > 1) {
-      tile = (uint32_t)u / splits;
+    if (p.splits > 1) {
+      const uint32_t splits = p.splits, tile = u / splits;
       split = u - tile * splits;
       kb0 = kb * split / splits;
       kb1 = kb * (split + 1) / splits;
+      u = tile;
     }
-    const uint32_t tm = tile / (uint32_t)p.tiles_n;
+    const uint32_t tm = u / (uint32_t)p.tiles_n;
     m0 = tm * BM;
-    n0 = (tile - tm * p.tiles_n) * BN;
+    n0 = (u - tm * p.tiles_n) * BN;
   }
 };
 
-// Byte of a staging buffer that holds byte `at` of row r's 128: the 128-byte swizzle.
-__device__ __forceinline__ uint32_t staged(int r, int at) { return r * 128 + ((at ^ (r << 4)) & 0x70) + (at & 15); }
+// Byte of a staging buffer that holds byte `at` of row r's 64: the 64-byte swizzle.
+__device__ __forceinline__ uint32_t staged(int r, int at) {
+  return r * kSliceBytes + ((at ^ (r << 3)) & 0x30) + (at & 15);
+}
 
-// Between a staging buffer and rows that start anywhere: a row at a time, a lane an element.
-template <typename T, int CC>
+// Between a staging buffer and rows that start anywhere: 32 lanes take consecutive elements
+// of a row, or of two rows of 16.
+template <typename T>
 __device__ __forceinline__ void copy_rows_out(const unsigned char* buf, T* y, int64_t stride, int64_t m, int64_t M,
                                               int n, int N, int lane) {
-  const int rows = (int)min((int64_t)32, M - m);
-  for (int r = 0; r < rows; ++r)
-#pragma unroll
-    for (int c = lane; c < CC; c += 32)
-      if (n + c < N)
-        y[(m + r) * stride + n + c] = *reinterpret_cast<const T*>(buf + staged(r, c * (int)sizeof(T)));
+  constexpr int SC = kSliceBytes / (int)sizeof(T);
+  const int c = lane % SC;
+#pragma unroll 4
+  for (int r = lane / SC; r < 32; r += 32 / SC)
+    if (m + r < M && n + c < N)
+      y[(m + r) * stride + n + c] = *reinterpret_cast<const T*>(buf + staged(r, c * (int)sizeof(T)));
 }
-template <typename T, int CC>
+template <typename T>
 __device__ __forceinline__ void copy_rows_in(unsigned char* buf, const T* x, int64_t stride, int64_t m, int64_t M,
                                              int n, int N, int lane) {
-  const int rows = (int)min((int64_t)32, M - m);
-  for (int r = 0; r < rows; ++r)
-#pragma unroll
-    for (int c = lane; c < CC; c += 32)
-      if (n + c < N) *reinterpret_cast<T*>(buf + staged(r, c * (int)sizeof(T))) = x[(m + r) * stride + n + c];
+  constexpr int SC = kSliceBytes / (int)sizeof(T);
+  const int c = lane % SC;
+#pragma unroll 4
+  for (int r = lane / SC; r < 32; r += 32 / SC)
+    if (m + r < M && n + c < N)
+      *reinterpret_cast<T*>(buf + staged(r, c * (int)sizeof(T))) = x[(m + r) * stride + n + c];
 }
 
-// bias over 32 columns from n, raw where whole vectors can be loaded
 template <typename T>
-struct Bias32 {
-  static constexpr int V = Vec16<T>::N;
-  uint4 raw[32 / V];
-  bool vec;
-  __device__ __forceinline__ void load(const void* bias, int n, int N) {
-    const T* b = static_cast<const T*>(bias) + n;
-    vec = n + 32 <= N && reinterpret_cast<uintptr_t>(b) % 16 == 0;
-    if (vec) {
-#pragma unroll
-      for (int j = 0; j < 32 / V; ++j) raw[j] = ldg16(b + j * V);
-    }
-  }
-  __device__ __forceinline__ void add(const void* bias, int n, int N, float* v) const {
-    if (vec) {
-#pragma unroll
-      for (int j = 0; j < 32 / V; ++j) {
-        float f[V];
-        Vec16<T>::unpack(raw[j], f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[j * V + i] += f[i];
-      }
-    } else {
-      const T* b = static_cast<const T*>(bias) + n;
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (n + j < N) v[j] += to_f32(b[j]);
-    }
-  }
-};
-
-// 32 columns of a lane's row to bytes `at` on of its staging row, and back.
+__device__ __forceinline__ uint4 pack16(const float* v) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  else
+    return make_uint4(pack2(T(), v[0], v[1]), pack2(T(), v[2], v[3]), pack2(T(), v[4], v[5]), pack2(T(), v[6], v[7]));
+}
+// A lane's slice to its staging row.
 template <typename T>
-__device__ __forceinline__ void stage32(uint32_t buf, int lane, int at, const float* v) {
-  constexpr int V = Vec16<T>::N;
+__device__ __forceinline__ void stage_slice(uint32_t buf, int lane, const float* v) {
 #pragma unroll
-  for (int j = 0; j < 32; j += V) {
-    uint4 q;
-    if constexpr (sizeof(T) == 4) {
-      q = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]),
-                     __float_as_uint(v[j + 3]));
-    } else {
-      q = make_uint4(pack2(T(), v[j], v[j + 1]), pack2(T(), v[j + 2], v[j + 3]), pack2(T(), v[j + 4], v[j + 5]),
-                     pack2(T(), v[j + 6], v[j + 7]));
-    }
-    st_shared_16(buf + staged(lane, at + j * (int)sizeof(T)), q);
-  }
+  for (int j = 0; j < 4; ++j) st_shared_16(buf + staged(lane, 16 * j), pack16<T>(v + j * Vec16<T>::N));
+}
+__device__ __forceinline__ void add_pairs(const float* f, int n, float* v) {
+#pragma unroll
+  for (int i = 0; i < n; i += 2) add2(Pair(v[i], v[i + 1]), Pair(f[i], f[i + 1])).get(v[i], v[i + 1]);
 }
 template <typename T>
-__device__ __forceinline__ void add_staged32(uint32_t buf, int lane, int at, float* v) {
+__device__ __forceinline__ void add_staged_slice(uint32_t buf, int lane, float* v) {
   constexpr int V = Vec16<T>::N;
 #pragma unroll
-  for (int j = 0; j < 32; j += V) {
+  for (int j = 0; j < 4; ++j) {
     float f[V];
-    Vec16<T>::unpack(ld_shared_16(buf + staged(lane, at + j * (int)sizeof(T))), f);
+    Vec16<T>::unpack(ld_shared_16(buf + staged(lane, 16 * j)), f);
+    add_pairs(f, V, v + j * V);
+  }
+}
+// The bias of a slice's columns, from column n on.
+template <typename T>
+__device__ __forceinline__ void add_bias(const GemmParams& p, int n, float* v) {
+  constexpr int V = Vec16<T>::N, SC = kSliceBytes / (int)sizeof(T);
+  if (!p.out.bias) return;
+  const T* b = static_cast<const T*>(p.out.bias) + n;
+  if (p.bias_vec && n + SC <= p.N) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[j + i] += f[i];
+    for (int j = 0; j < 4; ++j) {
+      float f[V];
+      Vec16<T>::unpack(ldg16(b + j * V), f);
+      add_pairs(f, V, v + j * V);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < SC; ++j)
+      if (n + j < p.N) v[j] += to_f32(b[j]);
   }
 }
 
@@ -231,12 +221,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* acc_full = empty + L::STAGES;  // [2]
   uint64_t* acc_empty = acc_full + 2;      // [2]
   uint64_t* drained = acc_empty + 2;
-  uint64_t* res_full = drained + 1;        // [kEpilogueWarps]
+  uint64_t* res_full = drained + 1;        // [kEpilogueWarps][2]
   uint32_t* tmem_s = reinterpret_cast<uint32_t*>(base + L::off_misc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
   constexpr int BM = kBM * CG;
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
 
   // Pair: `full` and `acc_empty` are the leader's alone; the leader's products arrive on
   // `empty`, `acc_full` and `drained` of both.
@@ -250,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&acc_empty[i], CG * L::WARPS);
     }
     mbar_init(drained, 1);
-    for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(&res_full[i], 1);
+    for (int i = 0; i < 2 * kEpilogueWarps; ++i) mbar_init(&res_full[i], 1);
     fence_mbarrier_init();
   }
   if (warp == 0) {
@@ -281,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       prefetch_tmap(&bmap);
       Ring r;
       uint32_t issued = 0;
-      for (int u = first; u < p.units && !why; u += step) {
+      for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step) {
         const Unit w(p, u, BM, BN);
         const int am = w.m0 + (int)rank * kBM, bn = w.n0 + (int)rank * (BN / CG);
         for (int c0 = w.kb0; c0 < w.kb1 && !why; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
@@ -289,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int pair = 0; pair < pairs && !why; ++pair) {
             const int pa = PIECES ? piece_a(pair) : 0, pb = PIECES ? piece_b(pair) : 0;
             for (int kb = c0; kb < c1; ++kb) {
-              if (!mbar_wait(&empty[r.stage], r.phase ^ 1, kWaitNs)) { why = 4; break; }
+              if (!mbar_wait_asleep(&empty[r.stage], r.phase ^ 1, kWaitNs)) { why = 4; break; }
               unsigned char* st = base + (size_t)r.stage * L::STAGE;
               uint64_t* bar = &full[r.stage];
               if (rank == 0) mbar_arrive_expect_tx(bar, CG * L::STAGE);
@@ -321,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (why && rank == 0)
         for (uint32_t s = 0; s < (uint32_t)L::STAGES && s < issued; ++s) {
           const uint32_t last = (issued - 1 - s) / L::STAGES;  // round of the newest load of stage s
-          mbar_wait(&full[s], last & 1, kWaitNs);
+          mbar_wait_asleep(&full[s], last & 1, kWaitNs);
         }
     }
   } else if (warp == kEpilogueWarps + 1) {
@@ -334,16 +324,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (CG == 2) mma_commit_pair(bar);
         else mma_commit(bar);
       };
-      for (int u = first; u < p.units && !why; u += step) {
+      for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step) {
         const Unit w(p, u, BM, BN);
         for (int c0 = w.kb0; c0 < w.kb1 && !why; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
           const int c1 = PIECES ? min(c0 + kChunk, w.kb1) : w.kb1;
-          if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1, kWaitNs)) { why = 8; break; }
+          if (!mbar_wait_asleep(&acc_empty[acc], acc_phase ^ 1, kWaitNs)) { why = 8; break; }
           tc_fence_after();
           const uint32_t d = tmem + acc * BN;
           const int n = (c1 - c0) * pairs;
           for (int i = 0; i < n; ++i) {
-            if (!mbar_wait(&full[r.stage], r.phase, kWaitNs)) { why = 16; break; }
+            if (!mbar_wait_asleep(&full[r.stage], r.phase, kWaitNs)) { why = 16; break; }
             tc_fence_after();
             const uint32_t as = smem_u32(base + (size_t)r.stage * L::STAGE), bs = as + L::A_BYTES;
 #pragma unroll
@@ -364,16 +354,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       commit(drained);
     }
-  } else if (warp % (kEpilogueWarps / L::GROUPS) < L::WARPS) {
+  } else if (warp < L::WARPS) {
     // ------------------------------------------------------------ epilogue
-    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (a row a lane) and one share of the columns
-    constexpr int COLS = L::COLS, CC = L::CC;
-    const int group = warp / (kEpilogueWarps / L::GROUPS), share = warp / 4 % L::SHARES;
-    const uint32_t lbase = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + share * COLS;
-    unsigned char* buf = base + L::off_staging + (size_t)warp * kBuffer;
-    const uint32_t sbuf = smem_u32(buf);
+    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (a row a lane) and share w / 4 of the columns
+    constexpr int COLS = L::COLS, SC = L::SC;
+    const uint32_t lbase = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * COLS;
+    unsigned char* bufs = base + L::off_staging + (size_t)warp * 2 * kBuffer;
     const GemmEpilogue& o = p.out;
-    uint32_t acc = group, acc_phase = 0, res_phase = 0;
+    uint32_t acc = 0, acc_phase = 0, turn = 0, res_phase = 0;
+    auto buffer = [&](uint32_t i) { return bufs + (i & 1) * kBuffer; };
     auto release = [&] {
       tc_fence_before();
       __syncwarp();
@@ -381,30 +370,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (rank == 0) mbar_arrive(&acc_empty[acc]);
         else mbar_arrive_peer_relaxed(map_peer(&acc_empty[acc], 0));
       }
-      if constexpr (L::GROUPS == 2) {
-        acc_phase ^= 1;
-      } else {
-        acc ^= 1;
-        acc_phase ^= acc == 0;
-      }
-    };
-    // the buffer's last store has been read out
-    auto reuse = [&] {
-      if (lane == 0) bulk_wait_read<0>();
-      __syncwarp();
-    };
-    auto load_residual = [&](int m, int n) {
-      if (p.residual_tma) {
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&res_full[warp], kBuffer);
-          tma_load_3d(buf, &rmap, &res_full[warp], n, m, 0);
-        }
-      } else {
-        copy_rows_in<T, CC>(buf, static_cast<const T*>(o.residual), o.r_stride, m, p.M, n, p.N, lane);
-        __syncwarp();
-      }
+      acc ^= 1;
+      acc_phase ^= acc == 0;
     };
     auto store = [&](const CUtensorMap* map, void* to, int64_t stride, int m, int n, int layer) {
+      unsigned char* buf = buffer(turn++);
       if (p.store_tma) {
         fence_async_shared();
         __syncwarp();
@@ -414,103 +384,117 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         __syncwarp();
-        copy_rows_out<T, CC>(buf, static_cast<T*>(to), stride, m, p.M, n, p.N, lane);
+        copy_rows_out<T>(buf, static_cast<T*>(to) + (int64_t)layer * p.M * stride, stride, m, p.M, n, p.N, lane);
         fence_async_shared();  // a residual's load may fill the buffer next
         __syncwarp();
       }
     };
-    for (int u = first + group * step; u < p.units && !why; u += L::GROUPS * step) {
-      const Unit w(p, u, BM, BN);
-      const int m = w.m0 + (int)rank * kBM + 32 * (warp & 3);
-      const int n0 = w.n0 + share * COLS;
-      // buffers to fill: what is not there to store is skipped, by whole warps
-      const int chunks = m < p.M && n0 < p.N ? (min(COLS, p.N - n0) + CC - 1) / CC : 0;
-      float sum[PIECES ? COLS : 1];
-      if constexpr (PIECES) {
+    // z, activation, residual and y of one slice; the buffers take turns
+    auto out = [&](float* v, int m, int n, int layer) {
+      if (o.z) {
+        if (lane == 0) bulk_wait_read<1>();
+        __syncwarp();
+        stage_slice<T>(smem_u32(buffer(turn)), lane, v);
+        store(&zmap, o.z, o.z_stride, m, n, 0);
+      }
+      if (lane == 0) bulk_wait_read<1>();
+      __syncwarp();
+      const uint32_t i = turn & 1;
+      if (o.residual) {
+        if (p.residual_tma) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&res_full[2 * warp + i], kBuffer);
+            tma_load_3d(buffer(turn), &rmap, &res_full[2 * warp + i], n, m, 0);
+          }
+        } else {
+          copy_rows_in<T>(buffer(turn), static_cast<const T*>(o.residual), o.r_stride, m, p.M, n, p.N, lane);
+          __syncwarp();
+        }
+      }
+      activate_all<T, SC>(o.act, v);
+      if (o.residual) {
+        if (p.residual_tma) {
+          if (!__all_sync(0xffffffffu, mbar_wait_asleep(&res_full[2 * warp + i], res_phase >> i & 1, kWaitNs)))
+            why = 128;
+          res_phase ^= 1u << i;
+        }
+        add_staged_slice<T>(smem_u32(buffer(turn)), lane, v);
+      }
+      stage_slice<T>(smem_u32(buffer(turn)), lane, v);
+      store(&ymap, o.y, o.y_stride, m, n, layer);
+    };
+    auto ready = [&] {
+      if (!__all_sync(0xffffffffu, mbar_wait_asleep(&acc_full[acc], acc_phase, kWaitNs))) why = 32;
+      tc_fence_after();
+      return why == 0;
+    };
+    if constexpr (PIECES) {
+      for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step) {
+        const Unit w(p, u, BM, BN);
+        const int m = w.m0 + (int)rank * kBM + 32 * (warp & 3), n0 = w.n0 + (warp >> 2) * COLS;
+        float sum[COLS];
 #pragma unroll
         for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
-      }
-      // the residual comes while the products run (z needs the buffer first where it is kept)
-      reuse();
-      if (o.residual && !o.z && chunks > 0) load_residual(m, n0);
-      for (int c0 = w.kb0; c0 < w.kb1; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], acc_phase, kWaitNs))) { why = 32; break; }
-        tc_fence_after();
-        if constexpr (PIECES) {
+        for (int c0 = w.kb0; c0 < w.kb1; c0 += kChunk) {
+          if (!ready()) break;
 #pragma unroll
-          for (int c = 0; c < COLS; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(lbase + acc * BN + c, r);
+          for (int c = 0; c < COLS; c += SC) {
+            uint32_t r[SC];
+            tmem_ld(lbase + acc * BN + c, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < SC; ++j) sum[c + j] += __uint_as_float(r[j]);
           }
           release();
         }
-      }
-      if (why) break;
-      const uint32_t src = lbase + acc * BN;
-      // z = A B^T + bias, 32 columns from c of the warp's share
-      auto pre = [&](int c, float* v) {
-        Bias32<T> bias;
-        if (o.bias) bias.load(o.bias, n0 + c, p.N);
-        if constexpr (PIECES) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
-        } else {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(src + c, r);
+        for (int c = 0; c < COLS; c += SC)
+          if (m < p.M && n0 + c < p.N && !why) {
+            add_bias<T>(p, n0 + c, sum + c);
+            out(sum + c, m, n0 + c, w.split);
+          }
+      }
+    } else {
+      // slices come in order over the units; the one after the current is asked for before
+      // the current is computed, across units where its accumulator is finished by then
+      uint32_t r[SC];
+      bool asked = false;
+      for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step) {
+        const Unit w(p, u, BM, BN);
+        const int m = w.m0 + (int)rank * kBM + 32 * (warp & 3), n0 = w.n0 + (warp >> 2) * COLS;
+        if (!asked) {
+          if (!ready()) break;
+          tmem_ld(lbase + acc * BN, r);
+        }
+        asked = false;
+#pragma unroll 1
+        for (int c = 0; c < COLS && !why; c += SC) {
+          float v[SC];
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-        }
-        if (o.bias) bias.add(o.bias, n0 + c, p.N, v);
-      };
-#pragma unroll(PIECES ? COLS / CC : 1)
-      for (int ch = 0; ch < COLS / CC; ++ch) {
-        if (ch >= chunks || why) break;
-        const int n = n0 + ch * CC;
-        if (o.z) {
-          if (ch > 0) reuse();
-#pragma unroll(PIECES ? CC / 32 : 1)
-          for (int c = 0; c < CC; c += 32) {
-            float v[32];
-            pre(ch * CC + c, v);
-            stage32<T>(sbuf, lane, c * (int)sizeof(T), v);
+          for (int j = 0; j < SC; ++j) v[j] = __uint_as_float(r[j]);
+          add_bias<T>(p, n0 + c, v);
+          if (c + SC < COLS) {
+            tmem_ld(lbase + acc * BN + c + SC, r);
+          } else {
+            release();
+            if (u + step < (uint32_t)p.units && __all_sync(0xffffffffu, mbar_try_wait(&acc_full[acc], acc_phase))) {
+              tc_fence_after();
+              tmem_ld(lbase + acc * BN, r);
+              asked = true;
+            }
           }
-          store(&zmap, o.z, o.z_stride, m, n, 0);
+          if (m < p.M && n0 + c < p.N) out(v, m, n0 + c, w.split);
         }
-        if (o.residual) {
-          if (o.z || ch > 0) {
-            reuse();
-            load_residual(m, n);
-          }
-          if (p.residual_tma) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&res_full[warp], res_phase, kWaitNs))) { why = 128; break; }
-            res_phase ^= 1;
-          }
-        } else if (o.z || ch > 0) {
-          reuse();
-        }
-#pragma unroll(PIECES ? CC / 32 : 1)
-        for (int c = 0; c < CC; c += 32) {
-          float v[32];
-          pre(ch * CC + c, v);
-          if (!PIECES && ch == chunks - 1 && c + 32 >= CC) release();
-          activate_all<T, 32>(o.act, v);
-          if (o.residual) add_staged32<T>(sbuf, lane, c * (int)sizeof(T), v);
-          stage32<T>(sbuf, lane, c * (int)sizeof(T), v);
-        }
-        store(&ymap, o.y, o.y_stride, m, n, w.split);
       }
-      if (!PIECES && chunks == 0) release();
+      if (asked) tmem_ld_wait();
     }
     if (lane == 0) bulk_wait_all();
   }
   __syncwarp();
   if (why && p.status && lane == 0) atomicOr(p.status, 2 | (int)why);
   // TMEM is given back, and a pair parts, once no product writes to it
-  if (warp == 0 && !__all_sync(0xffffffffu, mbar_wait(drained, 0, kWaitNs)) && p.status && lane == 0)
+  if (warp == 0 && !__all_sync(0xffffffffu, mbar_wait_asleep(drained, 0, kWaitNs)) && p.status && lane == 0)
     atomicOr(p.status, 2 | 64);
   tc_fence_before();
   __syncthreads();
@@ -561,26 +545,33 @@ EncodeTiledFnG encode_fn() {
   return fn;
 }
 
-// A (layers, rows, cols) tensor in boxes of box_rows x 128 bytes, 128-byte swizzle; pitches in elements.
-bool make_map(CUtensorMap* map, int dtype, const void* ptr, int64_t cols, int64_t rows, int64_t layers, int64_t pitch,
-              int64_t layer_pitch, int box_rows) {
-  const int size = dtype == kF32 ? 4 : 2;
-  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
+bool encode(CUtensorMap* map, int dtype, const void* ptr, const int64_t (&dims)[3], int64_t pitch, int64_t layer_pitch,
+            int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
+  const int64_t size = dtype == kF32 ? 4 : 2;
+  const cuuint64_t d[3] = {(cuuint64_t)dims[0], (cuuint64_t)dims[1], (cuuint64_t)dims[2]};
   const cuuint64_t strides[2] = {(cuuint64_t)(pitch * size), (cuuint64_t)(layer_pitch * size)};
-  const cuuint32_t box[3] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows, 1};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   EncodeTiledFnG fn = encode_fn();
   return fn && fn(map,
                   dtype == kBF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                   : dtype == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
-                  3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                  3, const_cast<void*>(ptr), d, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-bool make_operand_map(CUtensorMap* map, const GemmOperand& o, int pieces, int op_dtype, int box_rows) {
-  return make_map(map, op_dtype, o.ptr, o.cols, o.rows, pieces, o.pitch, pieces > 1 ? o.piece_stride : o.pitch * o.rows,
-                  o.mn_major ? kBK : box_rows);
+// An operand in boxes of 64 columns (128 bytes); its pieces are the third axis.
+bool make_map(CUtensorMap* map, const GemmOperand& o, int pieces, int op_dtype, int box_rows) {
+  return encode(map, op_dtype, o.ptr, {o.cols, o.rows, pieces}, o.pitch,
+                pieces > 1 ? o.piece_stride : o.pitch * o.rows, 64, o.mn_major ? kBK : box_rows,
+                CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// An epilogue's matrix in slices of 32 rows; the parts of a split depth are the third axis.
+template <typename T>
+bool make_out_map(CUtensorMap* map, const void* ptr, int64_t cols, int64_t rows, int64_t layers, int64_t pitch) {
+  constexpr int dtype = std::is_same<T, float>::value ? kF32 : std::is_same<T, __half>::value ? kF16 : kBF16;
+  return encode(map, dtype, ptr, {cols, rows, layers}, pitch, pitch * rows, kSliceBytes / (int)sizeof(T), 32,
+                CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Tile shape and depth shares: the least of an estimate over the shapes there are.  A
@@ -600,6 +591,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
   Plan best{};
   double least = 0;
   for (const Shape& s : kShapes) {
+    if (pieces > 1 && s.bn == 256) continue;  // a warp's fp32 sums would not fit its registers
     Plan p{};
     p.shape = s;
     p.k_blocks = (int)((K + kBK - 1) / kBK);
@@ -623,14 +615,14 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
   }
   return best;
 }
-int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
 template <typename T, int BN, int CG, bool PIECES>
-int launch_tile(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, const Plan& plan, cudaStream_t stream) {
+int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, cudaStream_t stream) {
   using L = Layout<T, BN, CG, PIECES>;
   CUtensorMap amap, bmap, ymap{}, zmap{}, rmap{};
-  if (!make_operand_map(&amap, g.a, g.pieces, g.op_dtype, kBM) ||
-      !make_operand_map(&bmap, g.b, g.pieces, g.op_dtype, BN / CG))
+  if (!make_map(&amap, g.a, g.pieces, g.op_dtype, kBM) ||
+      !make_map(&bmap, g.b, g.pieces, g.op_dtype, BN / CG))
     return -1;
   GemmParams p{};
   p.M = (int)g.M;
@@ -651,12 +643,11 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, co
   p.store_tma = on16(out.y, out.y_stride) && on16(out.z, out.z_stride);
   // rows that overlap (a broadcast residual) are not a tensor map's
   p.residual_tma = out.residual && on16(out.residual, out.r_stride) && out.r_stride >= g.N;
-  if (p.store_tma &&
-      (!make_map(&ymap, out_dtype, out.y, g.N, g.M, plan.splits, out.y_stride, out.y_stride * g.M, 32) ||
-       (out.z && !make_map(&zmap, out_dtype, out.z, g.N, g.M, 1, out.z_stride, out.z_stride * g.M, 32))))
+  if (p.store_tma && (!make_out_map<T>(&ymap, out.y, g.N, g.M, plan.splits, out.y_stride) ||
+                      (out.z && !make_out_map<T>(&zmap, out.z, g.N, g.M, 1, out.z_stride))))
     return -1;
-  if (p.residual_tma && !make_map(&rmap, out_dtype, out.residual, g.N, g.M, 1, out.r_stride, out.r_stride * g.M, 32))
-    return -1;
+  if (p.residual_tma && !make_out_map<T>(&rmap, out.residual, g.N, g.M, 1, out.r_stride)) return -1;
+  p.bias_vec = reinterpret_cast<uintptr_t>(out.bias) % 16 == 0;
   auto kern = gemm_kernel<T, BN, CG, PIECES>;
   static std::atomic<uint64_t> allowed{0};  // devices whose limit has been raised for this kernel
   int device = 0;
@@ -681,23 +672,24 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, co
 }
 
 template <typename T, bool PIECES>
-int launch_shape(const GemmProblem& g, const GemmEpilogue& out, int out_dtype, const Plan& plan, cudaStream_t stream) {
+int launch_shape(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, cudaStream_t stream) {
   const Shape& s = plan.shape;
-  if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, out_dtype, plan, stream);
-  if (s.cg == 2) return launch_tile<T, 128, 2, PIECES>(g, out, out_dtype, plan, stream);
-  if (s.bn == 128) return launch_tile<T, 128, 1, PIECES>(g, out, out_dtype, plan, stream);
-  return launch_tile<T, 64, 1, PIECES>(g, out, out_dtype, plan, stream);
+  if constexpr (!PIECES)
+    if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, plan, stream);
+  if (s.cg == 2) return launch_tile<T, 128, 2, PIECES>(g, out, plan, stream);
+  if (s.bn == 128) return launch_tile<T, 128, 1, PIECES>(g, out, plan, stream);
+  return launch_tile<T, 64, 1, PIECES>(g, out, plan, stream);
 }
 
 template <typename T>
 int launch_type(const GemmProblem& g, cudaStream_t stream) {
   constexpr bool PIECES = std::is_same<T, float>::value;
   const Plan plan = plan_of(g.M, g.N, g.K, g.pieces);
-  if (plan.splits == 1) return launch_shape<T, PIECES>(g, g.out, g.out_dtype, plan, stream);
+  if (plan.splits == 1) return launch_shape<T, PIECES>(g, g.out, plan, stream);
   GemmEpilogue parts{};
   parts.y = g.ws;
-  parts.y_stride = round4(g.N);
-  if (int rc = launch_shape<float, PIECES>(g, parts, kF32, plan, stream)) return rc;
+  parts.y_stride = round8(g.N);
+  if (int rc = launch_shape<float, PIECES>(g, parts, plan, stream)) return rc;
   const int64_t work = (g.M * (parts.y_stride / 4) + 255) / 256;
   gemm_join_kernel<T><<<(unsigned)std::min<int64_t>(work, 8 * kSms), 256, 0, stream>>>(
       static_cast<const float*>(g.ws), plan.splits, parts.y_stride, g.M, g.N, g.out);
@@ -709,7 +701,7 @@ int launch_type(const GemmProblem& g, cudaStream_t stream) {
 size_t gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int pieces) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const Plan p = plan_of(M, N, K, pieces);
-  return p.splits > 1 ? (size_t)p.splits * M * round4(N) * sizeof(float) : 0;
+  return p.splits > 1 ? (size_t)p.splits * M * round8(N) * sizeof(float) : 0;
 }
 
 int launch_gemm(const GemmProblem& g, cudaStream_t stream) {

@@ -58,8 +58,8 @@ def _launch(x, weight, bias, residual, act, keep_z, shape, status):
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        x2, w2 = _lib.row_strideof(x), _lib.row_strideof(weight)
-        r2 = None if residual is None else _lib.row_strideof(residual)
+        x2, w2 = _lib.rows_of(x), _lib.rows_of(weight)
+        r2 = None if residual is None else _lib.rows_of(residual)
         y, z = _launch(x2, w2, bias, r2, act, act != 0, (*x.shape[:-1], w2.shape[0]), None)
         ctx.save_for_backward(x2, w2, z)
         ctx.act, ctx.x_shape = act, x.shape
@@ -73,7 +73,7 @@ class _LinearFunction(torch.autograd.Function):
         M, K = x.shape
         N = weight.shape[0]
         dev = x.device
-        g = _lib.row_strideof(dy)
+        g = _lib.rows_of(dy)
         dx = x.new_empty(ctx.x_shape) if need_x else None
         dw = x.new_empty((N, K)) if need_w else None
         db = x.new_empty(N) if need_b else None
@@ -130,6 +130,6 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         if status is not None:
             raise ValueError("status is not supported on the differentiable path")
         return _LinearFunction.apply(x, weight, bias, residual, ACTIVATIONS[activation])
-    y, _ = _launch(_lib.row_strideof(x), _lib.row_strideof(weight), bias, None if residual is None else _lib.row_strideof(residual),
+    y, _ = _launch(_lib.rows_of(x), _lib.rows_of(weight), bias, None if residual is None else _lib.rows_of(residual),
                    ACTIVATIONS[activation], False, shape, status)
     return y
