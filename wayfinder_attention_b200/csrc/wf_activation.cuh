@@ -3,6 +3,7 @@
 
 #include "wf_rowio.cuh"
 #include "wf_kernels.h"
+#include "wf_pair.cuh"
 
 namespace wf {
 
@@ -30,38 +31,10 @@ __device__ __forceinline__ float upper_tail(float az, float& e) {
   return q * t * e;
 }
 
-// Two fp32 values an instruction.
-struct Pair {
-  uint64_t v;
-  __device__ __forceinline__ Pair() {}
-  __device__ __forceinline__ Pair(float a, float b) {
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  }
-  __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
-  __device__ __forceinline__ void get(float& a, float& b) const {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  }
-};
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
 __device__ __forceinline__ float max_keep_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
-}
-
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
 }
 
 // gelu(z) = max(z, 0) - |z| Phi(-|z|), two at a time with the polynomial in paired

@@ -16,7 +16,9 @@
 #include "wf_gemm.h"
 #include "wf_rowio.cuh"
 
+#include <cstring>
 #include <type_traits>
+#include <utility>
 
 namespace wf {
 namespace {
@@ -62,15 +64,25 @@ __device__ __forceinline__ void store_operand(void* out, int64_t at, int64_t pie
 
 // 8 values of a row from column c (zeros past the end), by vectors where the row allows it.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, bool vec, float* f) {
-  if (vec && c + 8 <= cols) {
+struct Raw8 {
+  static constexpr int V = Vec16<T>::N;
+  uint4 raw[8 / V];
+  __device__ __forceinline__ void load(const T* row, int64_t c, int64_t cols, bool vec) {
+    if (vec && c + 8 <= cols) {
 #pragma unroll
-    for (int j = 0; j < 8; j += Vec16<T>::N) Vec16<T>::unpack(ldg16(row + c + j), f + j);
-  } else {
+      for (int j = 0; j < 8 / V; ++j) raw[j] = ldg16(row + c + j * V);
+    } else {
+      T e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = c + j < cols ? to_f32(row[c + j]) : 0.f;
+      for (int j = 0; j < 8; ++j) e[j] = c + j < cols ? row[c + j] : from_f32<T>(0.f);
+      memcpy(raw, e, sizeof(e));
+    }
   }
-}
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int j = 0; j < 8 / V; ++j) Vec16<T>::unpack(raw[j], f + j * V);
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(256) lay_out_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, bool vec,
@@ -78,8 +90,10 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const T* x, int64_t rows, 
   const int64_t groups = pitch / 8, total = rows * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / groups, c = i % groups * 8;
+    Raw8<T> raw;
+    raw.load(x + r * stride, c, cols, vec);
     float f[8];
-    load8(x + r * stride, c, cols, vec, f);
+    raw.unpack(f);
     store_operand<T>(out, r * pitch + c, piece, f);
   }
 }
@@ -94,19 +108,36 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * 8;
   float s[8] = {};
+  const bool z_vec = N % 8 == 0;
+  constexpr int U = std::is_same<T, float>::value ? 2 : 4;  // rows asked for at once
   if (c < N)
-    for (int64_t m = (int64_t)blockIdx.y * 8 + warp; m < M; m += (int64_t)gridDim.y * 8) {
-      float g[8];
-      load8(dy + m * dy_stride, c, N, dy_vec, g);
-      if constexpr (ACT != kActNone) {
-        float f[8];
-        load8(z + m * N, c, N, N % 8 == 0, f);
+    for (int64_t m0 = (int64_t)blockIdx.y * 8 + warp; m0 < M; m0 += (int64_t)gridDim.y * 8 * U) {
+      Raw8<T> rg[U], rz[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] *= activation_slope<ACT, T>(f[j]);
+      for (int i = 0; i < U; ++i) {
+        const int64_t m = m0 + (int64_t)i * gridDim.y * 8;
+        if (m < M) {
+          rg[i].load(dy + m * dy_stride, c, N, dy_vec);
+          if constexpr (ACT != kActNone) rz[i].load(z + m * N, c, N, z_vec);
+        }
       }
-      if (out) store_operand<T>(out, m * pitch + c, piece, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] += g[j];
+      for (int i = 0; i < U; ++i) {
+        const int64_t m = m0 + (int64_t)i * gridDim.y * 8;
+        if (m < M) {
+          float g[8];
+          rg[i].unpack(g);
+          if constexpr (ACT != kActNone) {
+            float f[8];
+            rz[i].unpack(f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] *= activation_slope<ACT, T>(f[j]);
+          }
+          if (out) store_operand<T>(out, m * pitch + c, piece, g);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[j] += g[j];
+        }
+      }
     }
   if (!partials) return;
 #pragma unroll

@@ -10,10 +10,13 @@
 // blocks of a cluster combine by the same rule, and L = m + log s, H = log s - u / s.
 // Everything is fp32 (logits are widened exactly).
 //
-// The top n are kept while the logits stream by: a warp holds its n best as sorted
-// 64-bit keys, one a lane (the logit's bits in an order-preserving form above the
-// inverted index, so equal logits rank by the lower index), and a vector is looked at
-// only if its maximum reaches the warp's n-th.  Lists merge like the sums do.
+// Alternatives are ranked by 64-bit keys: the logit's bits in an order-preserving form above
+// the inverted index, so that equal logits rank by the lower index and no two keys are
+// equal.  Long rows: the n-th largest of the threads' maxima bounds the n-th logit from
+// below; a second look at the row (in L2 by then) collects the few logits that reach it,
+// and each finds its rank by counting the keys above its own.  Where too many reach it
+// (ties, orders), and for short rows, each warp keeps its n best as it goes, one key a
+// lane, and the lists are merged.
 //
 // -inf is a token that cannot be said: p = 0, nothing added to H.  A row of nothing
 // else has no distribution: logprob -inf, H 0, gradient 0.  A NaN (or +inf) makes its
@@ -21,6 +24,7 @@
 //
 // Bound by bytes: one read of the logits; the backward reads them again and writes dx.
 #include "wf_kernels.h"
+#include "wf_pair.cuh"
 #include "wf_rowio.cuh"
 #include "wf_sm100.cuh"
 
@@ -32,16 +36,16 @@ using namespace sm100;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr unsigned kAll = 0xffffffffu;
 
-// exp2_approx with results below 2^-126 kept: a gradient multiplies them by what it likes
-__device__ __forceinline__ float exp2_small(float x) {
-  float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // NaN if either is
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 
@@ -64,22 +68,50 @@ struct Sums {
     s += o.s;
     u += o.u;
   }
+  // N values (even, or 1) of which `most` is the largest.
   template <int N>
   __device__ __forceinline__ void add(const float* x, float most) {
     if (!(most <= m)) rebase(max_nan(m, most));
     const float base = m == -INFINITY ? 0.f : m;  // -inf - -inf would be NaN
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float d = x[j] - base, e = exp2_approx(d * kLog2e);
+    // e^d is 0 long before d = -200: the bound keeps 0 * inf out of u
+    if constexpr (N == 1) {
+      const float d = max_nan(x[0] - base, -200.f), e = exp2_approx(d * kLog2e);
       s += e;
-      u = fmaf(e, fmaxf(d, -1e30f), u);  // e = 0 where d = -inf
+      u = fmaf(e, d, u);
+    } else {
+      Pair ps(0.f), pu(0.f);
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        float d0, d1, y0, y1;
+        add2(Pair(x[j], x[j + 1]), Pair(-base)).get(d0, d1);
+        const Pair d(max_nan(d0, -200.f), max_nan(d1, -200.f));
+        mul2(d, Pair(kLog2e)).get(y0, y1);
+        const Pair e(exp2_approx(y0), exp2_approx(y1));
+        ps = add2(ps, e);
+        pu = fma2(e, d, pu);
+      }
+      float a, b;
+      ps.get(a, b);
+      s += a + b;
+      pu.get(a, b);
+      u += a + b;
     }
   }
 };
 
+template <int N>
+__device__ __forceinline__ float max_of(const float* x) {
+  float m = x[0];
+#pragma unroll
+  for (int j = 1; j + 1 < N; j += 2) m = max3_nan(m, x[j], x[j + 1]);
+  if constexpr (N % 2 == 0) m = max_nan(m, x[N - 1]);
+  return m;
+}
+
+template <int LANES = 32>
 __device__ __forceinline__ Sums warp_join(Sums a) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = LANES / 2; o > 0; o >>= 1) {
     Sums b;
     b.m = __shfl_xor_sync(kAll, a.m, o);
     b.s = __shfl_xor_sync(kAll, a.s, o);
@@ -89,9 +121,9 @@ __device__ __forceinline__ Sums warp_join(Sums a) {
   return a;
 }
 
+__device__ __forceinline__ uint32_t value_key(float x) { return x != x ? 0xffffffffu : ordered_key(x); }
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
-  const uint32_t k = x != x ? 0xffffffffu : ordered_key(x);
-  return (uint64_t)k << 32 | (uint32_t)~index;
+  return (uint64_t)value_key(x) << 32 | (uint32_t)~index;
 }
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) { return __shfl_xor_sync(kAll, v, o); }
 
@@ -167,160 +199,409 @@ struct Span {
 };
 
 constexpr int kWarps = 8;     // of a block
+constexpr int kThreads = 32 * kWarps;
 constexpr int kUnroll = 4;    // vectors a thread requests at once
 
-// One row a warp (WIDE = false), or one row a cluster of 1 to 8 blocks (WIDE = true).
-template <typename T, bool WIDE, bool TOP>
-__global__ void __launch_bounds__(kWarps * 32) token_logprobs_kernel(LogprobParams p) {
-  constexpr int V = Vec16<T>::N;
-  constexpr int G = WIDE ? kWarps * 32 : 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t parts = WIDE ? p.cluster : 1, part = WIDE ? blockIdx.x % parts : 0;
-  const int64_t row = WIDE ? blockIdx.x / parts : (int64_t)blockIdx.x * kWarps + warp;
-  if (!WIDE && row >= p.rows) return;
-  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
-  int64_t lo = 0, hi = p.vocab;
-  if (WIDE) {
-    const int64_t share = ((p.vocab + parts - 1) / parts + V - 1) / V * V;
-    lo = min((int64_t)part * share, p.vocab);
-    hi = min(lo + share, p.vocab);
+// What a row's sums say, written by one thread; `log_s` is -inf for a row without a
+// distribution.
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobParams& p, int64_t row, const T* x, const Sums& a, float log_s) {
+  const bool none = a.s == 0.f;
+  const int64_t tok = p.tokens[row];
+  float lp;
+  if (tok == p.ignore_index) {
+    lp = 0.f;
+  } else if (tok < 0 || tok >= p.vocab) {
+    lp = NAN;
+    if (p.status) atomicOr(p.status, 1);
+  } else {
+    lp = none ? -INFINITY : to_f32(x[tok]) - a.m - log_s;
   }
-  const Span<T> span(x, lo, hi);
+  p.logprob[row] = lp;
+  p.entropy[row] = none ? 0.f : log_s - a.u / a.s;
+  if (p.stats) {  // apart, so that p = exp((x - m) - log s) keeps its bits however large the logits are
+    p.stats[row] = a.m;
+    p.stats[p.rows + row] = log_s;
+  }
+}
+__device__ __forceinline__ void write_top(const LogprobParams& p, int64_t row, int rank, uint64_t key, const Sums& a,
+                                          float log_s) {
+  const uint32_t hi = (uint32_t)(key >> 32);
+  const float v = hi == 0xffffffffu ? NAN : key_to_float(hi);
+  p.top_logprobs[row * p.top_n + rank] = a.s == 0.f ? -INFINITY : v - a.m - log_s;
+  p.top_tokens[row * p.top_n + rank] = (uint32_t)~(uint32_t)key;
+}
 
+// Short rows that start on 16 bytes, without alternatives: LANES lanes a row, which they hold
+// in registers, so the maximum is known before the first exponential.
+template <typename T, int LANES, int NV>
+__global__ void __launch_bounds__(kThreads) token_logprobs_short_kernel(LogprobParams p) {
+  constexpr int V = Vec16<T>::N;
+  const int t = threadIdx.x % LANES;
+  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
+  const bool live = row < p.rows;
+  const T* x = static_cast<const T*>(p.x) + (live ? row : 0) * p.x_stride;
+  RawVec<T, V> raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + t) * V;
+    if (c < p.vocab) raw[i].load(x + c);
+  }
+  float f[NV][V];
   Sums a{-INFINITY, 0.f, 0.f};
-  TopList top;
-  if (TOP) top.clear();
-  // A warp's lanes stay together (the list is the warp's): bounds are tested a vector.
-  const int64_t first = span.head + (int64_t)(WIDE ? warp * 32 : 0) * V;
-  for (int64_t c0 = first; c0 < span.tail; c0 += (int64_t)G * V * kUnroll) {
-    RawVec<T, V> raw[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int64_t c = c0 + ((int64_t)i * G + lane) * V;
-      if (c < span.tail) raw[i].load(x + c);
-    }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int64_t c = c0 + ((int64_t)i * G + lane) * V;
-      const bool live = c < span.tail;
-      float f[V];
-      float most = -INFINITY;
-      if (live) {
-        raw[i].unpack(f);
-        most = f[0];
-#pragma unroll
-        for (int j = 1; j < V; ++j) most = max_nan(most, f[j]);
-        a.template add<V>(f, most);
-      }
-      if constexpr (TOP) {
-        if (__any_sync(kAll, live && !(most < top.bar))) {
-          if (top.bar == -INFINITY && c0 == first && i == 0) {
-            // the n-th largest of the lanes' maxima is a first bar: n elements reach it
-            TopList firsts;
-            firsts.clear();
-            firsts.merge(live ? rank_key(most, lane) : 0, lane);
-            firsts.set_bar(p.top_n);
-            top.bar = firsts.bar;
-          }
-#pragma unroll
-          for (int j = 0; j < V; ++j) top.offer(live ? f[j] : 0.f, (uint32_t)(c + j), live, p.top_n, lane);
-        }
-      }
+  for (int i = 0; i < NV; ++i) {
+    if ((i * LANES + t) * V < p.vocab) {
+      raw[i].unpack(f[i]);
+      a.m = max_nan(a.m, max_of<V>(f[i]));
     }
   }
-  // the ends: fewer than V elements each, offered by the first warp of the row
-  if (!WIDE || warp == 0) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) a.m = max_nan(a.m, __shfl_xor_sync(kAll, a.m, o));
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i * LANES + t) * V < p.vocab) a.template add<V>(f[i], a.m);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(kAll, a.s, o);
+    a.u += __shfl_xor_sync(kAll, a.u, o);
+  }
+  if (t == 0 && live) write_row(p, row, x, a, logf(a.s));
+}
+
+// The streaming list of a warp over elements [lo, hi) of a row: `warp` of `warps` take vectors
+// in turn, the first one the ends.
+template <typename T>
+__device__ void stream_top(TopList& top, const T* x, int64_t lo, int64_t hi, int warp, int warps, int lane, int n) {
+  constexpr int V = Vec16<T>::N;
+  const Span<T> span(x, lo, hi);
+  bool first = true;
+  for (int64_t c0 = span.head + (int64_t)warp * 32 * V; c0 < span.tail; c0 += (int64_t)warps * 32 * V) {
+    const int64_t c = c0 + (int64_t)lane * V;
+    const bool live = c < span.tail;
+    float f[V], most = -INFINITY;
+    if (live) {
+      RawVec<T, V> raw;
+      raw.load(x + c);
+      raw.unpack(f);
+      most = max_of<V>(f);
+    }
+    if (first) {
+      // the n-th largest of the lanes' maxima is a first bar: n elements reach it
+      TopList firsts;
+      firsts.clear();
+      firsts.merge(live ? rank_key(most, lane) : 0, lane);
+      firsts.set_bar(n);
+      top.bar = firsts.bar;
+      first = false;
+    }
+    if (__any_sync(kAll, live && !(most < top.bar)))
+#pragma unroll
+      for (int j = 0; j < V; ++j) top.offer(live ? f[j] : 0.f, (uint32_t)(c + j), live, n, lane);
+  }
+  if (warp == 0) {
     const int64_t n_head = span.head - lo, n_tail = hi - span.tail;
     const int64_t c = lane < n_head ? lo + lane : span.tail + (lane - n_head);
     const bool live = lane < n_head + n_tail;
-    float f = 0.f;
-    if (live) {
-      f = to_f32(x[c]);
-      a.template add<1>(&f, f);
+    top.offer(live ? to_f32(x[c]) : 0.f, (uint32_t)c, live, n, lane);
+  }
+}
+
+// The sums of a thread over its share of [lo, hi): vectors t, t + threads, ... and, for the
+// first threads, the ends.
+template <typename T>
+__device__ __forceinline__ Sums thread_sums(const T* x, int64_t lo, int64_t hi, int t, int threads) {
+  constexpr int V = Vec16<T>::N;
+  const Span<T> span(x, lo, hi);
+  Sums a{-INFINITY, 0.f, 0.f};
+  const int64_t stride = (int64_t)threads * V;
+  int64_t c = span.head + (int64_t)t * V;
+  for (; c + (kUnroll - 1) * stride < span.tail; c += kUnroll * stride) {
+    RawVec<T, V> raw[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) raw[i].load(x + c + i * stride);
+    float f[kUnroll * V];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) raw[i].unpack(f + i * V);
+    a.template add<kUnroll * V>(f, max_of<kUnroll * V>(f));
+  }
+  for (; c < span.tail; c += stride) {
+    RawVec<T, V> raw;
+    raw.load(x + c);
+    float f[V];
+    raw.unpack(f);
+    a.template add<V>(f, max_of<V>(f));
+  }
+  const int64_t n_head = span.head - lo, n_tail = hi - span.tail;
+  if (t < n_head + n_tail) {
+    const float f = to_f32(x[t < n_head ? lo + t : span.tail + (t - n_head)]);
+    a.template add<1>(&f, f);
+  }
+  return a;
+}
+
+// Up to 32 N logits, with alternatives: a warp holds the row, an element a lane and turn, and
+// sorts 32 keys a turn into its list.
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) token_logprobs_sort_kernel(LogprobParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  float f[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = lane + 32 * i < p.vocab ? to_f32(x[lane + 32 * i]) : -INFINITY;
+  Sums a{-INFINITY, 0.f, 0.f};
+  a.template add<N>(f, max_of<N>(f));
+  a = warp_join(a);
+  TopList top;
+  top.clear();
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (32 * i < p.vocab) top.merge(lane + 32 * i < p.vocab ? rank_key(f[i], lane + 32 * i) : 0, lane);
+  const float log_s = logf(a.s);
+  if (lane == 0) write_row(p, row, x, a, log_s);
+  if (lane < p.top_n) write_top(p, row, lane, top.mine, a, log_s);
+}
+
+// Short rows of any start, or longer ones with alternatives: a warp a row.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_warp_kernel(LogprobParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  const Sums a = warp_join(thread_sums(x, 0, p.vocab, lane, 32));
+  const float log_s = logf(a.s);
+  if (lane == 0) write_row(p, row, x, a, log_s);
+  if constexpr (TOP) {
+    TopList top;
+    top.clear();
+    stream_top(top, x, 0, p.vocab, 0, 1, lane, p.top_n);
+    if (lane < p.top_n) write_top(p, row, lane, top.mine, a, log_s);
+  }
+}
+
+constexpr int kCandidates = 256;  // keys that a block ranks at once
+
+// Each thread's key finds its place among `count` of them in shared memory.
+__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int count) {
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) above += keys[i] > key;
+  return above;
+}
+
+// Long rows: one row a cluster of 1 to 8 blocks.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams p) {
+  constexpr int V = Vec16<T>::N;
+  __shared__ Sums warp_sums[kWarps];
+  __shared__ Sums sums[8];  // of the cluster's blocks, in its first block
+  __shared__ uint64_t found[kCandidates];             // keys of this block that reach its bar
+  __shared__ uint64_t best[8][kMaxTopTokens];         // of the cluster's blocks, in its first block
+  __shared__ uint64_t lists[kWarps][kMaxTopTokens];   // of the warps, and the block's own best
+  __shared__ uint32_t maxima[kThreads];
+  __shared__ uint32_t bar_key;
+  __shared__ int n_found;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t parts = p.cluster, part = blockIdx.x % parts;
+  const int64_t row = blockIdx.x / parts;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  const int64_t share = ((p.vocab + parts - 1) / parts + V - 1) / V * V;
+  const int64_t lo = min((int64_t)part * share, p.vocab), hi = min(lo + share, p.vocab);
+
+  Sums a = thread_sums(x, lo, hi, threadIdx.x, kThreads);
+  if constexpr (TOP) {
+    maxima[threadIdx.x] = value_key(a.m);
+    if (threadIdx.x == 0) {
+      n_found = 0;
+      bar_key = 0;
     }
-    if constexpr (TOP) top.offer(f, (uint32_t)c, live, p.top_n, lane);
   }
   a = warp_join(a);
-
-  if constexpr (WIDE) {
-    __shared__ Sums sums[8];  // of the cluster's blocks, in its first block
-    __shared__ uint64_t keys[8][kMaxTopTokens];
-    __shared__ uint64_t own[kWarps][kMaxTopTokens];
-    __shared__ Sums own_sums[kWarps];
-    if (lane == 0) own_sums[warp] = a;
-    if (TOP) own[warp][lane] = top.mine;
-    __syncthreads();
-    if (warp == 0) {
-      a = lane < kWarps ? own_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
-      a = warp_join(a);
-      if constexpr (TOP)
-        for (int w = 1; w < kWarps; ++w) top.merge_sorted(own[w][lane], lane);
-    }
-    if (parts > 1) {
-      if (warp == 0 && part > 0) {
-        if (lane == 0) {
-          const uint32_t d = map_peer(&sums[part], 0);
-          st_peer_u32(d, __float_as_uint(a.m));
-          st_peer_u32(d + 4, __float_as_uint(a.s));
-          st_peer_u32(d + 8, __float_as_uint(a.u));
-        }
-        if (TOP) {
-          const uint32_t d = map_peer(&keys[part][lane], 0);
-          st_peer_u32(d, (uint32_t)top.mine);
-          st_peer_u32(d + 4, (uint32_t)(top.mine >> 32));
-        }
-      }
-      __syncwarp();
-      cluster_sync();
-      if (part > 0) return;
-      if (warp == 0) {
-        Sums b{-INFINITY, 0.f, 0.f};
-        if (lane == 0) b = a;
-        else if (lane < (int)parts) b = sums[lane];
-        a = warp_join(b);
-        if constexpr (TOP)
-          for (uint32_t r = 1; r < parts; ++r) top.merge_sorted(keys[r][lane], lane);
-      }
-    }
-    if (warp != 0) return;
-  }
-
-  const float log_s = logf(a.s);  // -inf for a row without a distribution
-  const bool none = a.s == 0.f;
-  if (lane == 0) {
-    const int64_t tok = p.tokens[row];
-    float lp;
-    if (tok == p.ignore_index) {
-      lp = 0.f;
-    } else if (tok < 0 || tok >= p.vocab) {
-      lp = NAN;
-      if (p.status) atomicOr(p.status, 1);
-    } else {
-      lp = none ? -INFINITY : to_f32(x[tok]) - a.m - log_s;
-    }
-    p.logprob[row] = lp;
-    p.entropy[row] = none ? 0.f : log_s - a.u / a.s;
-    if (p.stats) {  // apart, so that p = exp((x - m) - log s) keeps its bits however large the logits are
-      p.stats[row] = a.m;
-      p.stats[p.rows + row] = log_s;
-    }
-  }
+  if (lane == 0) warp_sums[warp] = a;
+  __syncthreads();
   if constexpr (TOP) {
-    if (lane < p.top_n) {
-      const uint32_t hi32 = (uint32_t)(top.mine >> 32), index = ~(uint32_t)top.mine;
-      const float v = hi32 == 0xffffffffu ? NAN : key_to_float(hi32);
-      p.top_logprobs[row * p.top_n + lane] = none ? -INFINITY : v - a.m - log_s;
-      p.top_tokens[row * p.top_n + lane] = index;
+    // the n-th largest of the maxima, equal ones by thread
+    const uint32_t mine = maxima[threadIdx.x];
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < kThreads; ++i) {
+      const uint32_t k = maxima[i];
+      above += k > mine || (k == mine && i < (int)threadIdx.x);
+    }
+    if (above == p.top_n - 1) bar_key = mine;
+    __syncthreads();
+    const uint32_t bar = bar_key;
+    // elements that reach it; beyond kCandidates only their number is kept
+    auto look = [&](float f, int64_t c) {
+      if (value_key(f) >= bar) {
+        const int at = atomicAdd(&n_found, 1);
+        if (at < kCandidates) found[at] = rank_key(f, (uint32_t)c);
+      }
+    };
+    const Span<T> span(x, lo, hi);
+    const float bar_value = bar == 0xffffffffu ? INFINITY : key_to_float(bar);
+#pragma unroll 4
+    for (int64_t c = span.head + (int64_t)threadIdx.x * V; c < span.tail; c += kThreads * V) {
+      RawVec<T, V> raw;
+      raw.load(x + c);
+      float f[V];
+      raw.unpack(f);
+      if (!(max_of<V>(f) < bar_value))
+#pragma unroll
+        for (int j = 0; j < V; ++j) look(f[j], c + j);
+    }
+    const int64_t n_head = span.head - lo, n_tail = hi - span.tail;
+    if ((int64_t)threadIdx.x < n_head + n_tail) {
+      const int64_t c = threadIdx.x < n_head ? lo + threadIdx.x : span.tail + ((int64_t)threadIdx.x - n_head);
+      look(to_f32(x[c]), c);
+    }
+    __syncthreads();
+    const int count = n_found;
+    if (count <= kCandidates) {
+      if ((int)threadIdx.x < count) {
+        const uint64_t key = found[threadIdx.x];
+        const int rank = rank_of(key, found, count);
+        if (rank < kMaxTopTokens) lists[0][rank] = key;
+      }
+      if ((int)threadIdx.x >= count && threadIdx.x < kMaxTopTokens) lists[0][threadIdx.x] = 0;
+    } else {
+      TopList top;
+      top.clear();
+      stream_top(top, x, lo, hi, warp, kWarps, lane, p.top_n);
+      lists[warp][lane] = top.mine;
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < kWarps; ++w) top.merge_sorted(lists[w][lane], lane);
+        lists[0][lane] = top.mine;
+      }
+    }
+    __syncthreads();
+  }
+  if (warp == 0) a = warp_join(lane < kWarps ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f});
+  if (parts > 1) {
+    if (warp == 0 && part > 0) {
+      if (lane == 0) {
+        const uint32_t d = map_peer(&sums[part], 0);
+        st_peer_u32(d, __float_as_uint(a.m));
+        st_peer_u32(d + 4, __float_as_uint(a.s));
+        st_peer_u32(d + 8, __float_as_uint(a.u));
+      }
+      if (TOP) {
+        const uint64_t key = lists[0][lane];
+        const uint32_t d = map_peer(&best[part][lane], 0);
+        st_peer_u32(d, (uint32_t)key);
+        st_peer_u32(d + 4, (uint32_t)(key >> 32));
+      }
+    }
+    if (warp == 0 && part == 0) {
+      if (lane == 0) sums[0] = a;
+      if (TOP) best[0][lane] = lists[0][lane];
+    }
+    __syncwarp();
+    cluster_sync();
+    if (part > 0) return;
+    a = warp_join(lane < (int)parts ? sums[lane] : Sums{-INFINITY, 0.f, 0.f});  // every warp the same
+    const float log_s = logf(a.s);
+    if (threadIdx.x == 0) write_row(p, row, x, a, log_s);
+    if constexpr (TOP) {
+      // 32 keys a block at most 8 blocks: a thread each
+      const int count = (int)parts * kMaxTopTokens;
+      if ((int)threadIdx.x < count) {
+        const uint64_t key = (&best[0][0])[threadIdx.x];
+        const int rank = key ? rank_of(key, &best[0][0], count) : p.top_n;
+        if (rank < p.top_n) write_top(p, row, rank, key, a, log_s);
+      }
+    }
+    return;
+  }
+  if (warp != 0) return;
+  const float log_s = logf(a.s);
+  if (lane == 0) write_row(p, row, x, a, log_s);
+  if constexpr (TOP)
+    if (lane < p.top_n) write_top(p, row, lane, lists[0][lane], a, log_s);
+}
+
+// The gradient of a row's elements.
+struct RowGrad {
+  float m, log_s, gh, gl, base;
+  bool none;
+  int64_t tok;
+  __device__ __forceinline__ RowGrad(const LogprobBwdParams& p, int64_t row)
+      : m(p.stats[row]), log_s(p.stats[p.rows + row]), gh(p.dentropy ? p.dentropy[row] : 0.f),
+        gl(p.dlogprob ? p.dlogprob[row] : 0.f), tok(p.tokens[row]) {
+    if (tok == p.ignore_index) gl = 0.f;
+    else if (tok < 0 || tok >= p.vocab) gl = NAN;
+    none = m == -INFINITY;
+    base = fmaf(gh, p.entropy[row], gl);
+  }
+  // f[j] is x[c + j] and becomes dx[c + j].  p is computed 2^64 times too large, so that its
+  // last bits survive where a gradient multiplies them up again; it is 0 long before
+  // lp = -200, which keeps 0 * inf out.
+  template <int N>
+  __device__ __forceinline__ void apply(float* f, int64_t c) const {
+    constexpr float kDown = 5.421010862427522e-20f;  // 2^-64
+    if constexpr (N == 1) {
+      const float lp = max_nan(f[0] - m - log_s, -200.f);
+      f[0] = exp2_approx(fmaf(lp, kLog2e, 64.f)) * -fmaf(gh, lp, base) * kDown;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; j += 2) {
+        float l0, l1, y0, y1;
+        add2(add2(Pair(f[j], f[j + 1]), Pair(-m)), Pair(-log_s)).get(l0, l1);
+        const Pair lp(max_nan(l0, -200.f), max_nan(l1, -200.f));
+        fma2(lp, Pair(kLog2e), Pair(64.f)).get(y0, y1);
+        const Pair q = fma2(lp, Pair(-gh), Pair(-base));
+        mul2(mul2(Pair(exp2_approx(y0), exp2_approx(y1)), q), Pair(kDown)).get(f[j], f[j + 1]);
+      }
+    }
+    if (none) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = 0.f;
+    } else if ((uint64_t)(tok - c) < (uint64_t)N) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (c + j == tok) f[j] += gl;
+    }
+  }
+};
+
+// Short rows that start on 16 bytes, as in the forward.
+template <typename T, int LANES, int NV>
+__global__ void __launch_bounds__(kThreads) token_logprobs_backward_short_kernel(LogprobBwdParams p) {
+  constexpr int V = Vec16<T>::N;
+  const int t = threadIdx.x % LANES;
+  const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
+  if (row >= p.rows) return;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  T* dx = static_cast<T*>(p.dx) + row * p.vocab;
+  RawVec<T, V> raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + t) * V;
+    if (c < p.vocab) raw[i].load(x + c);
+  }
+  const RowGrad g(p, row);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + t) * V;
+    if (c < p.vocab) {
+      float f[V];
+      raw[i].unpack(f);
+      g.template apply<V>(f, c);
+      store_vec<T, V>(dx + c, f);
     }
   }
 }
 
-// One row a warp (WIDE = false) or kSpan elements of a row a block (WIDE = true).
+// Any rows: a warp a row (WIDE = false), or a block a share of one.
 constexpr int64_t kBwdVectors = 4;
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kWarps * 32) token_logprobs_backward_kernel(LogprobBwdParams p, int64_t chunks) {
+__global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(LogprobBwdParams p, int64_t chunks) {
   constexpr int V = Vec16<T>::N;
-  constexpr int G = WIDE ? kWarps * 32 : 32;
+  constexpr int G = WIDE ? kThreads : 32;
   const int t = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 31);
   const int64_t row = WIDE ? blockIdx.x / chunks : (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (!WIDE && row >= p.rows) return;
@@ -332,21 +613,7 @@ __global__ void __launch_bounds__(kWarps * 32) token_logprobs_backward_kernel(Lo
     lo = min(blockIdx.x % chunks * share, p.vocab);
     hi = min(lo + share, p.vocab);
   }
-  const int64_t tok = p.tokens[row];
-  const float m = p.stats[row], log_s = p.stats[p.rows + row], h = p.entropy[row];
-  const float gh = p.dentropy ? p.dentropy[row] : 0.f;
-  float gl = p.dlogprob ? p.dlogprob[row] : 0.f;
-  if (tok == p.ignore_index) gl = 0.f;
-  else if (tok < 0 || tok >= p.vocab) gl = NAN;
-  const bool none = m == -INFINITY;
-  const float base = fmaf(gh, h, gl);
-  auto grad = [&](float v, int64_t c) {
-    const float lp = v - m - log_s, pr = exp2_small(lp * kLog2e);
-    // p is 0 long before lp = -200; the bound keeps 0 * inf out
-    float g = -pr * fmaf(gh, fmaxf(lp, -200.f), base);
-    if (c == tok) g += gl;
-    return none ? 0.f : g;
-  };
+  const RowGrad g(p, row);
   const Span<T> span(x, lo, hi);
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
   for (int64_t c0 = span.head + (int64_t)t * V; c0 < span.tail; c0 += (int64_t)G * V * kBwdVectors) {
@@ -362,8 +629,7 @@ __global__ void __launch_bounds__(kWarps * 32) token_logprobs_backward_kernel(Lo
       if (c < span.tail) {
         float f[V];
         raw[i].unpack(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = grad(f[j], c + j);
+        g.template apply<V>(f, c);
         if (same) {
           store_vec<T, V>(dx + c, f);
         } else {
@@ -376,9 +642,29 @@ __global__ void __launch_bounds__(kWarps * 32) token_logprobs_backward_kernel(Lo
   const int64_t n_head = span.head - lo, n_tail = hi - span.tail;
   if (t < n_head + n_tail) {
     const int64_t c = t < n_head ? lo + t : span.tail + (t - n_head);
-    dx[c] = from_f32<T>(grad(to_f32(x[c]), c));
+    float f = to_f32(x[c]);
+    g.template apply<1>(&f, c);
+    dx[c] = from_f32<T>(f);
   }
 }
+
+// Whether rows of up to 1024 logits can be taken by whole vectors.
+template <typename T>
+bool short_vectors(const void* x, int64_t stride, const void* dx, int64_t vocab) {
+  constexpr int V = Vec16<T>::N;
+  return vocab <= 1024 && vocab % V == 0 && stride % V == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+}
+// LAUNCH(LANES, NV): 8 lanes a row while 16 elements a lane hold it, else a warp.
+#define WF_SHORT_ROWS(T, LAUNCH)                                           \
+  constexpr int V = Vec16<T>::N;                                           \
+  if (p.vocab <= 8 * V) LAUNCH(8, 1);                                      \
+  else if (p.vocab <= 16 * V) LAUNCH(8, 2);                                \
+  else if (V == 4 && p.vocab <= 32 * V) LAUNCH(8, 4);                      \
+  else if (p.vocab <= 32 * V) LAUNCH(32, 1);                               \
+  else if (p.vocab <= 64 * V) LAUNCH(32, 2);                               \
+  else if (p.vocab <= 128 * V) LAUNCH(32, 4);                              \
+  else LAUNCH(32, 8)
 
 // A warp takes a row of up to 1024 logits (4 KB at most); longer rows take a block, and
 // a cluster of up to 8 when there are fewer rows than SMs to give them to.
@@ -386,10 +672,20 @@ constexpr int64_t kWarpRow = 1024;
 
 template <typename T>
 int launch_fwd(LogprobParams p, cudaStream_t stream) {
+  if (p.top_n == 0 && short_vectors<T>(p.x, p.x_stride, nullptr, p.vocab)) {
+#define WF_LAUNCH(LANES, NV) \
+  token_logprobs_short_kernel<T, LANES, NV>  \
+      <<<(unsigned)((p.rows * LANES + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p)
+    WF_SHORT_ROWS(T, WF_LAUNCH);
+#undef WF_LAUNCH
+    return (int)cudaGetLastError();
+  }
   if (p.vocab <= kWarpRow) {
     const unsigned grid = (unsigned)((p.rows + kWarps - 1) / kWarps);
-    if (p.top_n) token_logprobs_kernel<T, false, true><<<grid, kWarps * 32, 0, stream>>>(p);
-    else token_logprobs_kernel<T, false, false><<<grid, kWarps * 32, 0, stream>>>(p);
+    if (p.top_n && p.vocab <= 64) token_logprobs_sort_kernel<T, 2><<<grid, kThreads, 0, stream>>>(p);
+    else if (p.top_n && p.vocab <= 256) token_logprobs_sort_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
+    else if (p.top_n) token_logprobs_warp_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
+    else token_logprobs_warp_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
     return (int)cudaGetLastError();
   }
   int c = 1;
@@ -397,7 +693,7 @@ int launch_fwd(LogprobParams p, cudaStream_t stream) {
   p.cluster = c;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * c));
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -405,19 +701,25 @@ int launch_fwd(LogprobParams p, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return (int)(p.top_n ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true, true>, p)
-                       : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true, false>, p));
+  return (int)(p.top_n ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true>, p)
+                       : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, false>, p));
 }
 
 template <typename T>
 int launch_bwd(const LogprobBwdParams& p, cudaStream_t stream) {
-  if (p.vocab <= kWarpRow) {
+  if (short_vectors<T>(p.x, p.x_stride, p.dx, p.vocab)) {
+#define WF_LAUNCH(LANES, NV) \
+  token_logprobs_backward_short_kernel<T, LANES, NV>  \
+      <<<(unsigned)((p.rows * LANES + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p)
+    WF_SHORT_ROWS(T, WF_LAUNCH);
+#undef WF_LAUNCH
+  } else if (p.vocab <= kWarpRow) {
     token_logprobs_backward_kernel<T, false>
-        <<<(unsigned)((p.rows + kWarps - 1) / kWarps), kWarps * 32, 0, stream>>>(p, 1);
+        <<<(unsigned)((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream>>>(p, 1);
   } else {
-    const int64_t span = (int64_t)kWarps * 32 * Vec16<T>::N * kBwdVectors;
+    const int64_t span = (int64_t)kThreads * Vec16<T>::N * kBwdVectors;
     const int64_t chunks = (p.vocab + span - 1) / span;
-    token_logprobs_backward_kernel<T, true><<<(unsigned)(p.rows * chunks), kWarps * 32, 0, stream>>>(p, chunks);
+    token_logprobs_backward_kernel<T, true><<<(unsigned)(p.rows * chunks), kThreads, 0, stream>>>(p, chunks);
   }
   return (int)cudaGetLastError();
 }
