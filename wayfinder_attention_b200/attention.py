@@ -6,8 +6,8 @@ Drop-in for the reference module of the same name
 signature, same submodule names (``q_proj``, ``k_proj``, ``v_proj``,
 ``out_proj``, ``address.q_addr_proj``, ``address.k_addr_proj``), so reference
 ``state_dict``s load unchanged.  Projections, address normalisation and
-``out_proj`` stay in PyTorch; retrieval + sparse attention run in the CUDA
-library.
+``out_proj`` stay in PyTorch unless ``fused_linear`` is set on the module;
+retrieval + sparse attention run in the CUDA library.
 
 Differences from the reference module, all deliberate:
   * no ``RoutingRetriever`` is built, so no ``max_seq_len**2`` causal mask is
@@ -34,6 +34,7 @@ import torch.nn.functional as F
 
 from .causal_topk import causal_topk
 from .fused_sparse import fused_sparse_attention, sparse_meat_attention
+from .linear import project
 
 
 @dataclass
@@ -155,6 +156,8 @@ class LearnedAddressSparseAttention(nn.Module):
         # reference ignores it there, so the default keeps its behaviour.
         self.mask_padded_keys = mask_padded_keys
         self._retrieval_cfg = _resolve_retrieval_cfg(retrieval_config, top_k)
+        # the four projections through fused_linear (and the block's residual in the last one)
+        self.fused_linear = False
         self.q_proj = nn.Linear(d_model, d_model)
         self.k_proj = nn.Linear(d_model, d_model)
         self.v_proj = nn.Linear(d_model, d_model)
@@ -172,14 +175,15 @@ class LearnedAddressSparseAttention(nn.Module):
         x: torch.Tensor,
         attn_mask: Optional[torch.Tensor] = None,
         return_attention: bool = False,
+        residual: Optional[torch.Tensor] = None,
         **kwargs,
     ):
         # attn_mask is ignored, as on the reference's sparse path (attention.py:456-490), unless the
         # module was built with mask_padded_keys=True (fused path: padded keys are never retrieved).
         B, T, D = x.shape
-        q = self.q_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
-        k = self.k_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
-        v = self.v_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+        q = project(self.q_proj, x, self.fused_linear).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+        k = project(self.k_proj, x, self.fused_linear).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+        v = project(self.v_proj, x, self.fused_linear).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
         q_addr, k_addr = self.address.forward_query_key(x)
         if self._retrieval_cfg.use_fused_sparse:
             key_mask = attn_mask if (self.mask_padded_keys and attn_mask is not None and not bool(attn_mask.all())) else None
@@ -194,7 +198,7 @@ class LearnedAddressSparseAttention(nn.Module):
                 dropout_p=self.dropout.p if self.training else 0.0,
             )
         out = meat.transpose(1, 2).contiguous().view(B, T, D)
-        out = self.out_proj(out)
+        out = project(self.out_proj, out, self.fused_linear, residual=residual)
         if return_attention:
             # Same debug map as attention.py:492-500 (1/K at each retrieved position), built vectorised.
             k_eff = candidate_idx.shape[-1]
@@ -240,6 +244,8 @@ class KeyVectorSparseAttention(nn.Module):
         self.pad_mode = pad_mode
         self._retrieval_cfg = _resolve_retrieval_cfg(retrieval_config, top_k)
         self.use_fast_retrieval = self._retrieval_cfg.apply_to_key_vector
+        # the four projections through fused_linear (and the block's residual in the last one)
+        self.fused_linear = False
         self.q_proj = nn.Linear(d_model, d_model)
         self.k_proj = nn.Linear(d_model, d_model)
         self.v_proj = nn.Linear(d_model, d_model)
@@ -251,11 +257,11 @@ class KeyVectorSparseAttention(nn.Module):
         return k.mean(dim=1).contiguous(), q.mean(dim=1).contiguous()
 
     def forward(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor] = None, return_attention: bool = False,
-                **kwargs):
+                residual: Optional[torch.Tensor] = None, **kwargs):
         B, T, D = x.shape
-        q = self.q_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
-        k = self.k_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
-        v = self.v_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+        q = project(self.q_proj, x, self.fused_linear).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+        k = project(self.k_proj, x, self.fused_linear).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+        v = project(self.v_proj, x, self.fused_linear).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
         qs, ks = self._search_vectors(q, k)
         if self._retrieval_cfg.use_fused_sparse:
             meat, candidate_idx = fused_sparse_attention(qs, ks, q, k, v, self.top_k, self.scale,
@@ -268,7 +274,8 @@ class KeyVectorSparseAttention(nn.Module):
             meat = sparse_meat_attention(q, k, v, candidate_idx, self.scale,
                                          mask_negative=self.pad_mode == "masked",
                                          dropout_p=self.dropout.p if self.training else 0.0)
-        out = self.out_proj(meat.transpose(1, 2).contiguous().view(B, T, D))
+        out = project(self.out_proj, meat.transpose(1, 2).contiguous().view(B, T, D), self.fused_linear,
+                      residual=residual)
         if return_attention:
             k_eff = candidate_idx.shape[-1]
             attn_dense = torch.zeros(B, T, T, device=x.device)

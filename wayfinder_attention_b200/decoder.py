@@ -9,6 +9,16 @@ an LM head tied to the token embedding.  Parameter names match the reference
 ``state_dict`` loads.  Only ``attention_type`` "learned_address" (this build's
 kernels) and "dense_flash" (PyTorch SDPA, the dense baseline of
 ``models/attention.py:130-173``) are provided.
+
+``fused_layers=True`` runs the rest of the blocks on this package's operators too
+(``layer_norm``, and ``fused_linear`` with bias, GELU and residual in its epilogue),
+forward and backward; ``score`` gives the log probability of each next token with
+``token_logprobs``, which is what answers are scored and the model is trained by:
+
+    lm = TransformerLM(vocab, fused_layers=True, dropout=0.0).to("cuda", torch.bfloat16)
+    r = lm.score(input_ids, top_n=5)          # .logprob, .entropy, .top_logprobs, .top_tokens
+    loss = -r.logprob.sum() / (input_ids[:, 1:] != lm.pad_token_id).sum()
+    loss.backward()
 """
 
 from __future__ import annotations
@@ -20,6 +30,9 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .attention import KeyVectorSparseAttention, LearnedAddressSparseAttention
+from .layer_norm import layer_norm
+from .linear import project
+from .token_logprobs import TokenLogprobs, token_logprobs
 
 
 class DenseSDPAAttention(nn.Module):
@@ -35,23 +48,32 @@ class DenseSDPAAttention(nn.Module):
         self.v_proj = nn.Linear(d_model, d_model)
         self.out_proj = nn.Linear(d_model, d_model)
         self.dropout_p = dropout
+        self.fused_linear = False
 
-    def forward(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor] = None, **kwargs) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor] = None,
+                residual: Optional[torch.Tensor] = None, **kwargs) -> torch.Tensor:
         B, T, D = x.shape
-        q = self.q_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
-        k = self.k_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
-        v = self.v_proj(x).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+        q, k, v = (project(layer, x, self.fused_linear).view(B, T, self.n_heads, self.head_dim).transpose(1, 2)
+                   for layer in (self.q_proj, self.k_proj, self.v_proj))
         out = F.scaled_dot_product_attention(
             q, k, v, is_causal=True, scale=self.scale, dropout_p=self.dropout_p if self.training else 0.0
         )
-        return self.out_proj(out.transpose(1, 2).contiguous().view(B, T, D))
+        return project(self.out_proj, out.transpose(1, 2).contiguous().view(B, T, D), self.fused_linear,
+                       residual=residual)
+
+
+def _norm(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
+    return layer_norm(x, ln.weight, ln.bias, ln.eps)
 
 
 class TransformerBlock(nn.Module):
     def __init__(self, d_model: int, n_heads: int, d_ff: int, dropout: float, attention_module: nn.Module,
-                 layer_idx: int = 0):
+                 layer_idx: int = 0, fused_layers: bool = False):
         super().__init__()
         self.attn = attention_module
+        self.fused_layers = fused_layers
+        if fused_layers:
+            self.attn.fused_linear = True
         self.layer_idx = layer_idx
         self.ln1 = nn.LayerNorm(d_model)
         self.ln2 = nn.LayerNorm(d_model)
@@ -60,8 +82,19 @@ class TransformerBlock(nn.Module):
         )
 
     def forward(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.fused_layers:
+            return self._forward_fused(x, attn_mask)
         x = x + self.attn(self.ln1(x), attn_mask=attn_mask)
         return x + self.ff(self.ln2(x))
+
+    def _forward_fused(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor]) -> torch.Tensor:
+        """The same block on ``layer_norm`` and ``fused_linear``; dropout, where it acts, comes between them."""
+        up, _, drop_hidden, down, drop_out = self.ff
+        x = self.attn(_norm(self.ln1, x), attn_mask=attn_mask, residual=x)
+        h = drop_hidden(project(up, _norm(self.ln2, x), True, activation="gelu"))
+        if self.training and drop_out.p > 0.0:
+            return x + drop_out(project(down, h, True))
+        return project(down, h, True, residual=x)
 
 
 class TransformerLM(nn.Module):
@@ -79,6 +112,7 @@ class TransformerLM(nn.Module):
         address_dim: int = 32,
         retrieval_config: Optional[dict] = None,
         pad_token_id: int = 0,
+        fused_layers: bool = False,
     ):
         super().__init__()
         if attention_type not in ("learned_address", "key_vector", "dense_flash", "dense"):
@@ -86,6 +120,7 @@ class TransformerLM(nn.Module):
         self.d_model = d_model
         self.max_seq_len = max_seq_len
         self.pad_token_id = pad_token_id
+        self.fused_layers = fused_layers
         self.token_emb = nn.Embedding(vocab_size, d_model)
         self.pos_emb = nn.Embedding(max_seq_len, d_model)
         self.dropout = nn.Dropout(dropout)
@@ -101,7 +136,8 @@ class TransformerLM(nn.Module):
                                                 retrieval_config=retrieval_config)
             else:
                 attn = DenseSDPAAttention(d_model, n_heads, dropout)
-            self.blocks.append(TransformerBlock(d_model, n_heads, d_ff, dropout, attn, layer_idx=i))
+            self.blocks.append(TransformerBlock(d_model, n_heads, d_ff, dropout, attn, layer_idx=i,
+                                                fused_layers=fused_layers))
         self.ln_f = nn.LayerNorm(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)
         self.lm_head.weight = self.token_emb.weight
@@ -114,4 +150,18 @@ class TransformerLM(nn.Module):
         x = self.dropout(self.token_emb(input_ids) + self.pos_emb(pos))
         for block in self.blocks:
             x = block(x, attn_mask=attn_mask)
+        if self.fused_layers:
+            return {"logits": project(self.lm_head, _norm(self.ln_f, x), True)}
         return {"logits": self.lm_head(self.ln_f(x))}
+
+    def score(self, input_ids: torch.Tensor, attn_mask: Optional[torch.Tensor] = None, top_n: int = 0) -> TokenLogprobs:
+        """How likely each next token is: ``TokenLogprobs`` of shape (B, T - 1) for ``input_ids`` (B, T).
+
+        Entry t is about token t + 1 given the tokens up to t.  Padding (``pad_token_id``) gets
+        log probability 0 and no gradient.
+        """
+        logits = self(input_ids, attn_mask)["logits"]
+        # the last position has no next token; a whole row of logits a token keeps them uncopied
+        following = torch.cat([input_ids[:, 1:], input_ids.new_full((input_ids.shape[0], 1), self.pad_token_id)], 1)
+        r = token_logprobs(logits, following, top_n=top_n, ignore_index=self.pad_token_id)
+        return TokenLogprobs(*(t[:, :-1] for t in r))

@@ -133,3 +133,12 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     y, _ = _launch(_lib.rows_of(x), _lib.rows_of(weight), bias, None if residual is None else _lib.rows_of(residual),
                    ACTIVATIONS[activation], False, shape, status)
     return y
+
+
+def project(layer: torch.nn.Linear, x: torch.Tensor, fused: bool, activation: str = "none",
+            residual: torch.Tensor | None = None) -> torch.Tensor:
+    """An ``nn.Linear`` of a model: through ``fused_linear``, or as PyTorch layers (no activation then)."""
+    if fused:
+        return fused_linear(x, layer.weight, layer.bias, activation=activation, residual=residual)
+    y = layer(x)
+    return y if residual is None else residual + y
