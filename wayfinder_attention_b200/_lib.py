@@ -7,8 +7,8 @@ is no fallback implementation, so a missing library raises immediately.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import importlib.util
 import os
 import threading
 import time
@@ -211,6 +211,26 @@ def load_library() -> ctypes.CDLL:
     return _lib
 
 
+_ops = None
+
+
+def torch_ops():
+    """The package's PyTorch calls (``csrc/wf_torch.cpp``), bound to the CUDA library; raise if not built."""
+    global _ops
+    if _ops is None:
+        load_library()
+        path = Path(__file__).resolve().parent / "_wf_torch.so"
+        if not path.exists():
+            raise RuntimeError(f"wayfinder PyTorch calls not found at {path}; build them with "
+                               "`python -m wayfinder_attention_b200.build`")
+        spec = importlib.util.spec_from_file_location("_wf_torch", path)
+        ops = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ops)
+        ops.bind(str(LIB_PATH))
+        _ops = ops
+    return _ops
+
+
 def dtype_code(dt: torch.dtype) -> int:
     try:
         return _DTYPE_CODES[dt]
@@ -241,37 +261,8 @@ def workspace(B: int, Tq: int, Tk: int, R: int, top_k: int, dtype: torch.dtype, 
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-# The current stream's handle without building a torch.cuda.Stream (2 us a call less).
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
 def stream_ptr(device: torch.device) -> int:
-    if _raw_stream is not None and device.index is not None:
-        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def on_16_bytes(t: torch.Tensor) -> bool:
-    """Whether every row of a (rows, columns) tensor starts on a 16-byte boundary."""
-    return t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0
-
-
-_here = contextlib.nullcontext()
-
-
-def on_device(dev: torch.device):
-    """Context that makes ``dev`` current; nothing is entered when it already is."""
-    return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-
-def rows_of(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as (rows, last axis) with unit-strided, non-overlapping rows (copied only if it has to be)."""
-    if t.dim() == 2 and t.is_contiguous():
-        return t
-    r = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if (r.stride(1) != 1 and r.shape[1] > 1) or (r.stride(0) < r.shape[1] and r.shape[0] > 1):
-        r = r.contiguous()
-    return r
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

@@ -1,10 +1,11 @@
-"""Build libwayfinder_sm100.so in-tree with nvcc (sm_100a only).
+"""Build libwayfinder_sm100.so in-tree with nvcc (sm_100a only), and _wf_torch.so with g++.
 
 Usage: python -m wayfinder_attention_b200.build [--verbose]
 
-The shared library is written next to this file so that it travels with the
-source tree; the Python package loads it from there and refuses to run
-without it.
+The shared libraries are written next to this file so that they travel with the
+source tree; the Python package loads them from there and refuses to run
+without them.  The first holds the kernels behind the C ABI; the second the
+PyTorch calls (argument checks, autograd nodes) of the operators that have them.
 """
 
 from __future__ import annotations
@@ -26,6 +27,8 @@ SOURCES = ["wf_abi.cu", "wf_topk.cu", "wf_topk_tc.cu", "wf_attn.cu", "wf_attn_bf
            "wf_attn_f32.cu", "wf_addr_proj.cu",
            "wf_attn_bwd.cu", "wf_keymask.cu", "wf_bench.cu",
            "wf_gemm.cu", "wf_linear.cu", "wf_layer_norm.cu", "wf_logprobs.cu"]
+TORCH_SOURCE = "wf_torch.cpp"
+TORCH_LIB_PATH = PKG_DIR / "_wf_torch.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -41,14 +44,32 @@ def _sources() -> list[Path]:
 
 
 def _deps() -> list[Path]:
-    return _sources() + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [REPO_DIR / "include" / "wayfinder.h"]
+    return _sources() + [CSRC / TORCH_SOURCE] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [REPO_DIR / "include" / "wayfinder.h"]
 
 
 def up_to_date() -> bool:
-    if not LIB_PATH.exists():
+    if not (LIB_PATH.exists() and TORCH_LIB_PATH.exists()):
         return False
-    t = LIB_PATH.stat().st_mtime
+    t = min(LIB_PATH.stat().st_mtime, TORCH_LIB_PATH.stat().st_mtime)
     return all(p.stat().st_mtime <= t for p in _deps())
+
+
+def torch_command(out: Path) -> list[str]:
+    """g++ on the PyTorch calls, against the headers and libraries of the torch that is installed."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include"]
+    return [
+        os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+        "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        "-I", sysconfig.get_path("include"), *[a for p in include for a in ("-isystem", str(p))],
+        str(CSRC / TORCH_SOURCE), "-o", str(out), "-L", str(root / "lib"),
+        "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ldl",
+    ]
 
 
 def build(verbose: bool = False, force: bool = False) -> Path:
@@ -73,6 +94,8 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         common += ["-Xptxas", "-v"]
     # translation units compile concurrently (the attention instantiations dominate)
     jobs = []
+    torch_tmp = TORCH_LIB_PATH.with_suffix(".so.tmp")
+    torch_job = subprocess.Popen(torch_command(torch_tmp), stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
     for src in _sources():
         obj = obj_dir / (src.stem + ".o")
         cmd = [nvcc, *common, "-c", str(src), "-o", str(obj)]
@@ -86,6 +109,9 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         elif verbose and err:
             sys.stderr.write(err)
         objs.append(str(obj))
+    _, err = torch_job.communicate()
+    if torch_job.returncode != 0:
+        errors.append(f"g++ failed on {TORCH_SOURCE}:\n{err}")
     if errors:
         raise RuntimeError("\n".join(errors))
     tmp = LIB_PATH.with_suffix(".so.tmp")
@@ -94,6 +120,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"nvcc link failed:\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
+    os.replace(torch_tmp, TORCH_LIB_PATH)
     return LIB_PATH
 
 
