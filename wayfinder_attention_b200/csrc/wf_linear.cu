@@ -14,6 +14,7 @@
 #include "wf_activation.cuh"
 #include "wf_columns.cuh"
 #include "wf_gemm.h"
+#include "wf_linear_few.h"
 #include "wf_rowio.cuh"
 
 #include <cstring>
@@ -215,6 +216,7 @@ GemmProblem problem(const GemmOperand& a, const GemmOperand& b, int64_t M, int64
 
 template <typename T>
 int launch_fwd(const LinearParams& p, int dtype, cudaStream_t stream) {
+  if (linear_few_takes(p, dtype)) return launch_linear_few(p, dtype, stream);
   unsigned char* ws = static_cast<unsigned char*>(p.ws);
   GemmOperand x, w;
   if (int rc = operand<T>(p.x, p.M, p.K, p.x_stride, dtype, &ws, &x, stream)) return rc;
