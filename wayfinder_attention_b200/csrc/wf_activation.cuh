@@ -20,17 +20,6 @@ constexpr float kErfcP = 0.3275911f * 0.70710678118654752f;
 constexpr float kErfc0 = 0.5f * 0.254829592f, kErfc1 = 0.5f * -0.284496736f, kErfc2 = 0.5f * 1.421413741f,
                 kErfc3 = 0.5f * -1.453152027f, kErfc4 = 0.5f * 1.061405429f;
 constexpr float kGaussExp2 = -0.5f * 1.4426950408889634f;  // exp(-z^2 / 2) = 2^(this z^2)
-// `e` gets exp(-z^2 / 2).
-__device__ __forceinline__ float upper_tail(float az, float& e) {
-  const float t = rcp_approx(fmaf(kErfcP, az, 1.f));
-  e = exp2_approx(az * az * kGaussExp2);
-  float q = fmaf(t, kErfc4, kErfc3);
-  q = fmaf(t, q, kErfc2);
-  q = fmaf(t, q, kErfc1);
-  q = fmaf(t, q, kErfc0);
-  return q * t * e;
-}
-
 __device__ __forceinline__ float max_keep_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -51,10 +40,11 @@ struct Gelu2 {
   __device__ __forceinline__ Gelu2()
       : p(kept(kErfcP)), g(kept(kGaussExp2)), c4(kept(-kErfc4)), c3(kept(-kErfc3)), c2(kept(-kErfc2)),
         c1(kept(-kErfc1)), c0(kept(-kErfc0)), one(kept(1.f)) {}
-  // B pairs side by side: a pair alone is a chain of some hundred cycles.
+  // -Phi(-|z|) and exp(-z^2 / 2) of B pairs side by side: a pair alone is a chain of some
+  // hundred cycles.
   template <int B>
-  __device__ __forceinline__ void apply(float* v) const {
-    Pair az[B], q[B], t[B], e[B];
+  __device__ __forceinline__ void tail(const float* v, Pair (&az)[B], Pair (&q)[B], Pair (&e)[B]) const {
+    Pair t[B];
 #pragma unroll
     for (int i = 0; i < B; ++i) {
       az[i] = Pair(fminf(fabsf(v[2 * i]), 100.f), fminf(fabsf(v[2 * i + 1]), 100.f));
@@ -78,9 +68,30 @@ struct Gelu2 {
     for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c0);
 #pragma unroll
     for (int i = 0; i < B; ++i) q[i] = mul2(mul2(q[i], t[i]), e[i]);
+  }
+  template <int B>
+  __device__ __forceinline__ void apply(float* v) const {
+    Pair az[B], q[B], e[B];
+    tail(v, az, q, e);
 #pragma unroll
     for (int i = 0; i < B; ++i)
       fma2(az[i], q[i], Pair(max_keep_nan(v[2 * i], 0.f), max_keep_nan(v[2 * i + 1], 0.f))).get(v[2 * i], v[2 * i + 1]);
+  }
+  // Phi(z) + z phi(z)
+  template <int B>
+  __device__ __forceinline__ void slope(float* v) const {
+    Pair az[B], q[B], e[B];
+    tail(v, az, q, e);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      float h0, h1, x0, x1, s0, s1;  // h: -Phi(-|z|);  x: |z| phi(z)
+      q[i].get(h0, h1);
+      mul2(mul2(az[i], e[i]), Pair(0.3989422804014327f)).get(x0, x1);
+      s0 = v[2 * i] < 0.f ? -(h0 + x0) : 1.f + (h0 + x0);
+      s1 = v[2 * i + 1] < 0.f ? -(h1 + x1) : 1.f + (h1 + x1);
+      v[2 * i] = v[2 * i] != v[2 * i] ? v[2 * i] : s0;
+      v[2 * i + 1] = v[2 * i + 1] != v[2 * i + 1] ? v[2 * i + 1] : s1;
+    }
   }
 };
 
@@ -104,15 +115,8 @@ template <int ACT, typename T>
 __device__ __forceinline__ float activation_slope(float z) {
   constexpr bool FAST = sizeof(T) == 2;
   if constexpr (ACT == kActGelu) {
-    if constexpr (FAST) {
-      const float az = fminf(fabsf(z), 100.f);
-      float e;
-      const float h = upper_tail(az, e);
-      const float s = fmaf(z < 0.f ? -az : az, 0.3989422804014327f * e, z < 0.f ? h : 1.f - h);
-      return z != z ? z : s;
-    } else {
-      return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
-    }
+    static_assert(!FAST, "Gelu2 is the 16-bit form");
+    return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
   } else if constexpr (ACT == kActRelu) {
     return z > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == kActSilu) {
@@ -123,6 +127,22 @@ __device__ __forceinline__ float activation_slope(float z) {
   } else {
     return 1.f;
   }
+}
+
+// g[j] *= act'(z[j]), z overwritten.
+template <int ACT, typename T, int N>
+__device__ __forceinline__ void times_slope(float* z, float* g) {
+  if constexpr (ACT == kActNone) {
+    return;
+  } else if constexpr (ACT == kActGelu && sizeof(T) == 2) {
+    const Gelu2 gelu;
+    gelu.slope<N / 2>(z);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = activation_slope<ACT, T>(z[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) g[j] *= z[j];
 }
 
 // One branch for N values instead of one for each.

@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * 8;
   float s[8] = {};
   const bool z_vec = N % 8 == 0;
-  constexpr int U = std::is_same<T, float>::value ? 2 : 4;  // rows asked for at once
+  constexpr int U = 2;  // rows asked for at once
   if (c < N)
     for (int64_t m0 = (int64_t)blockIdx.y * 8 + warp; m0 < M; m0 += (int64_t)gridDim.y * 8 * U) {
       Raw8<T> rg[U], rz[U];
@@ -131,8 +131,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
           if constexpr (ACT != kActNone) {
             float f[8];
             rz[i].unpack(f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] *= activation_slope<ACT, T>(f[j]);
+            times_slope<ACT, T, 8>(f, g);
           }
           if (out) store_operand<T>(out, m * pitch + c, piece, g);
 #pragma unroll
