@@ -12,6 +12,7 @@ template <typename P>
 __global__ void __launch_bounds__(1024) column_join_kernel(const float* partials, int blocks, int64_t width,
                                                            int64_t split, P* a, P* b) {
   __shared__ float red[32][33];
+  pdl_wait();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + tx;
   float s = 0.f;
@@ -35,9 +36,8 @@ __global__ void __launch_bounds__(1024) column_join_kernel(const float* partials
 template <typename P>
 inline cudaError_t join_columns(const float* partials, int blocks, int64_t width, int64_t split, void* a, void* b,
                                 cudaStream_t stream) {
-  column_join_kernel<P><<<(unsigned)((width + 31) / 32), 1024, 0, stream>>>(partials, blocks, width, split,
-                                                                          static_cast<P*>(a), static_cast<P*>(b));
-  return cudaGetLastError();
+  return launch_pdl(column_join_kernel<P>, dim3((unsigned)((width + 31) / 32)), dim3(1024), 0, stream, partials, blocks,
+                    width, split, static_cast<P*>(a), static_cast<P*>(b));
 }
 
 }  // namespace wf

@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   }
   tc_fence_after();
+  pdl_wait();  // what comes before this kernel on its stream is done; nothing above touched global memory
   const uint32_t tmem = *tmem_s;
   constexpr int pairs = PIECES ? 6 : 1;
   uint32_t why = 0;
@@ -510,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T>
 __global__ void __launch_bounds__(256) gemm_join_kernel(const float* partial, int splits, int64_t pitch, int64_t M,
                                                         int64_t N, GemmEpilogue o) {
+  pdl_wait();
   const int64_t groups = pitch / 4, total = M * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / groups, n = i % groups * 4;
@@ -662,12 +664,14 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan,
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = L::smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CG;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return (int)cudaLaunchKernelEx(&cfg, kern, amap, bmap, ymap, zmap, rmap, p);
 }
 
@@ -691,9 +695,8 @@ int launch_type(const GemmProblem& g, cudaStream_t stream) {
   parts.y_stride = round8(g.N);
   if (int rc = launch_shape<float, PIECES>(g, parts, plan, stream)) return rc;
   const int64_t work = (g.M * (parts.y_stride / 4) + 255) / 256;
-  gemm_join_kernel<T><<<(unsigned)std::min<int64_t>(work, 8 * kSms), 256, 0, stream>>>(
-      static_cast<const float*>(g.ws), plan.splits, parts.y_stride, g.M, g.N, g.out);
-  return (int)cudaGetLastError();
+  return (int)launch_pdl(gemm_join_kernel<T>, dim3((unsigned)std::min<int64_t>(work, 8 * kSms)), dim3(256), 0, stream,
+                         static_cast<const float*>(g.ws), plan.splits, parts.y_stride, g.M, g.N, g.out);
 }
 
 }  // namespace

@@ -138,6 +138,7 @@ struct RowRing {
 // of them side by side, so that more is in flight and a parameter is loaded once for R rows).
 template <typename T, int VEC, int W, int NV, int R>
 __global__ void __launch_bounds__(threads_of(W)) layer_norm_kernel(LayerNormParams p) {
+  pdl_wait();
   static_assert(R == 1 || W == 1, "rows of a block share its barriers");
   constexpr int G = 32 * W;
   __shared__ float2 red[2][W];
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(threads_of(W)) layer_norm_kernel(LayerNormPara
 // third find it in L2).
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(LayerNormParams p) {
+  pdl_wait();
   __shared__ float2 red[2][32];
   const int wig = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
@@ -243,6 +245,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(LayerNormParams p
 // Partials of the column sums: [blocks][2][d] fp32, dw first.
 template <typename T, int VEC, int W, int NV>
 __global__ void __launch_bounds__(threads_of(W), W == 1 ? 2 : 16 / W) layer_norm_backward_kernel(LayerNormBwdParams p) {
+  pdl_wait();
   constexpr int G = 32 * W, ROWS = threads_of(W) / G;
   __shared__ float2 red[2][W];
   extern __shared__ uint4 ring_smem[];
@@ -376,6 +379,7 @@ __global__ void __launch_bounds__(threads_of(W), W == 1 ? 2 : 16 / W) layer_norm
 // Rows too long for registers: dx by one block a row in two passes ...
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(LayerNormBwdParams p) {
+  pdl_wait();
   __shared__ float2 red[32];
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
@@ -401,6 +405,7 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(LayerNor
 // ... and the column sums by threads that each walk one column of a share of the rows.
 template <typename T>
 __global__ void __launch_bounds__(256) layer_norm_columns_kernel(LayerNormBwdParams p) {
+  pdl_wait();
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= p.d) return;
   const T* x = static_cast<const T*>(p.x) + c;
@@ -465,8 +470,7 @@ int launch_rows(void (*kern)(P), int blocks, int threads, size_t smem, const P& 
   if (smem > 40 * 1024)  // 48 KB without asking, static shared memory included
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
       return (int)e;
-  kern<<<blocks, threads, smem, stream>>>(p);
-  return (int)cudaGetLastError();
+  return (int)launch_pdl(kern, dim3(blocks), dim3(threads), smem, stream, p);
 }
 template <bool BACKWARD, typename T, int VEC, int W, int NV, typename P>
 int launch_shape(int blocks, const P& p, cudaStream_t stream) {

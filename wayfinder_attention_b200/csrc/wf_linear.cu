@@ -88,6 +88,7 @@ struct Raw8 {
 template <typename T>
 __global__ void __launch_bounds__(256) lay_out_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, bool vec,
                                                       void* out, int64_t pitch, int64_t piece) {
+  pdl_wait();
   const int64_t groups = pitch / 8, total = rows * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / groups, c = i % groups * 8;
@@ -106,6 +107,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
                                                         void* out, int64_t pitch, int64_t piece, int64_t M, int64_t N,
                                                         float* partials) {
   __shared__ float red[8][32][9];
+  pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * 8;
   float s[8] = {};
@@ -191,9 +193,9 @@ int operand(const void* x, int64_t rows, int64_t cols, int64_t stride, int dtype
   }
   *o = blank_operand<T>(rows, cols, dtype, ws);
   const int64_t blocks = (rows * (o->pitch / 8) + 255) / 256;
-  lay_out_kernel<T><<<(unsigned)(blocks < 16 * kSms ? blocks : 16 * kSms), 256, 0, stream>>>(
-      static_cast<const T*>(x), rows, cols, stride, vec, const_cast<void*>(o->ptr), o->pitch, o->piece_stride);
-  return (int)cudaGetLastError();
+  return (int)launch_pdl(lay_out_kernel<T>, dim3((unsigned)(blocks < 16 * kSms ? blocks : 16 * kSms)), dim3(256), 0,
+                         stream, static_cast<const T*>(x), rows, cols, stride, vec, const_cast<void*>(o->ptr), o->pitch,
+                         o->piece_stride);
 }
 
 template <typename T>
@@ -226,10 +228,12 @@ int launch_fwd(const LinearParams& p, int dtype, cudaStream_t stream) {
 }
 
 template <typename T, int ACT>
-void launch_dz(const LinearBwdParams& p, const GemmOperand& o, bool write, float* partials, cudaStream_t stream) {
-  linear_dz_kernel<T, ACT><<<dim3((unsigned)((p.N + 255) / 256), row_shares(p.M, p.N)), 256, 0, stream>>>(
-      static_cast<const T*>(p.dy), p.dy_stride, on_16_bytes<T>(p.dy, p.dy_stride), static_cast<const T*>(p.z),
-      write ? const_cast<void*>(o.ptr) : nullptr, o.pitch, o.piece_stride, p.M, p.N, partials);
+cudaError_t launch_dz(const LinearBwdParams& p, const GemmOperand& o, bool write, float* partials,
+                      cudaStream_t stream) {
+  return launch_pdl(linear_dz_kernel<T, ACT>, dim3((unsigned)((p.N + 255) / 256), row_shares(p.M, p.N)), dim3(256), 0,
+                    stream, static_cast<const T*>(p.dy), p.dy_stride, on_16_bytes<T>(p.dy, p.dy_stride),
+                    static_cast<const T*>(p.z), write ? const_cast<void*>(o.ptr) : nullptr, o.pitch, o.piece_stride,
+                    p.M, p.N, partials);
 }
 
 template <typename T>
@@ -252,13 +256,14 @@ int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
   }
   if (p.db || (products && !direct)) {
     const bool write = products && !direct;
+    cudaError_t e;
     switch (p.act) {
-      case kActGelu: launch_dz<T, kActGelu>(p, dz, write, partials, stream); break;
-      case kActRelu: launch_dz<T, kActRelu>(p, dz, write, partials, stream); break;
-      case kActSilu: launch_dz<T, kActSilu>(p, dz, write, partials, stream); break;
-      default: launch_dz<T, kActNone>(p, dz, write, partials, stream); break;
+      case kActGelu: e = launch_dz<T, kActGelu>(p, dz, write, partials, stream); break;
+      case kActRelu: e = launch_dz<T, kActRelu>(p, dz, write, partials, stream); break;
+      case kActSilu: e = launch_dz<T, kActSilu>(p, dz, write, partials, stream); break;
+      default: e = launch_dz<T, kActNone>(p, dz, write, partials, stream); break;
     }
-    if (cudaError_t e = cudaGetLastError()) return (int)e;
+    if (e) return (int)e;
   }
   if (p.db)
     if (cudaError_t e = join_columns<T>(partials, row_shares(p.M, p.N), p.N, p.N, p.db, nullptr, stream)) return (int)e;

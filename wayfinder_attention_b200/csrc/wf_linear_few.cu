@@ -58,6 +58,7 @@ constexpr int kMmaCols = 16, kAhead = 4;
 template <typename T, int TILES>
 __global__ void __launch_bounds__(32 * kWarps) linear_few_mma_kernel(LinearParams p, int parts) {
   __shared__ float sums[kWarps][kMmaCols][8 * TILES + 1];
+  pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = warp % parts, group = warp / parts, groups = kWarps / parts;
   const int64_t n0 = ((int64_t)blockIdx.x * groups + group) * kMmaCols;
@@ -130,6 +131,7 @@ template <typename T, int VEC, int MB, int kCols>
 __global__ void __launch_bounds__(32 * kWarps) linear_few_kernel(LinearParams p, int parts) {
   constexpr int SUMS = MB * kCols;
   __shared__ float sums[kWarps][SUMS];
+  pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = warp % parts, group = warp / parts, groups = kWarps / parts;
   const int64_t n0 = ((int64_t)blockIdx.x * groups + group) * kCols;
@@ -215,9 +217,8 @@ template <typename T, int VEC, int MB, int COLS>
 int launch_rows(const LinearParams& p, cudaStream_t stream) {
   const int64_t groups = (p.N + COLS - 1) / COLS;
   const int parts = parts_of(groups, p.K, 64 * VEC);
-  linear_few_kernel<T, VEC, MB, COLS>
-      <<<(unsigned)((groups * parts + kWarps - 1) / kWarps), 32 * kWarps, 0, stream>>>(p, parts);
-  return (int)cudaGetLastError();
+  return (int)launch_pdl(linear_few_kernel<T, VEC, MB, COLS>, dim3((unsigned)((groups * parts + kWarps - 1) / kWarps)),
+                         dim3(32 * kWarps), 0, stream, p, parts);
 }
 template <typename T, int VEC>
 int launch_vec(const LinearParams& p, cudaStream_t stream) {
@@ -240,9 +241,8 @@ int launch(const LinearParams& p, int dtype, cudaStream_t stream) {
       const int64_t groups = (p.N + kMmaCols - 1) / kMmaCols;
       const int parts = parts_of(groups, p.K, 32 * kAhead);
       const unsigned grid = (unsigned)((groups * parts + kWarps - 1) / kWarps);
-      if (p.M <= 8) linear_few_mma_kernel<T, 1><<<grid, 32 * kWarps, 0, stream>>>(p, parts);
-      else linear_few_mma_kernel<T, 2><<<grid, 32 * kWarps, 0, stream>>>(p, parts);
-      return (int)cudaGetLastError();
+      return (int)launch_pdl(p.M <= 8 ? linear_few_mma_kernel<T, 1> : linear_few_mma_kernel<T, 2>, dim3(grid),
+                             dim3(32 * kWarps), 0, stream, p, parts);
     }
   }
   return on_16_bytes(p, sizeof(T)) ? launch_vec<T, Vec16<T>::N>(p, stream) : launch_vec<T, 1>(p, stream);

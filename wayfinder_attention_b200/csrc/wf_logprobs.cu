@@ -236,6 +236,7 @@ __device__ __forceinline__ void write_top(const LogprobParams& p, int64_t row, i
 // in registers, so the maximum is known before the first exponential.
 template <typename T, int LANES, int NV>
 __global__ void __launch_bounds__(kThreads) token_logprobs_short_kernel(LogprobParams p) {
+  pdl_wait();
   constexpr int V = Vec16<T>::N;
   const int t = threadIdx.x % LANES;
   const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
@@ -344,6 +345,7 @@ __device__ __forceinline__ Sums thread_sums(const T* x, int64_t lo, int64_t hi, 
 // sorts 32 keys a turn into its list.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) token_logprobs_sort_kernel(LogprobParams p) {
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (row >= p.rows) return;
@@ -367,6 +369,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_sort_kernel(LogprobPa
 // Short rows of any start, or longer ones with alternatives: a warp a row.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_warp_kernel(LogprobParams p) {
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (row >= p.rows) return;
@@ -395,6 +398,7 @@ __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int c
 // Long rows: one row a cluster of 1 to 8 blocks.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams p) {
+  pdl_wait();
   constexpr int V = Vec16<T>::N;
   __shared__ Sums warp_sums[kWarps];
   __shared__ Sums sums[8];  // of the cluster's blocks, in its first block
@@ -571,6 +575,7 @@ struct RowGrad {
 // Short rows that start on 16 bytes, as in the forward.
 template <typename T, int LANES, int NV>
 __global__ void __launch_bounds__(kThreads) token_logprobs_backward_short_kernel(LogprobBwdParams p) {
+  pdl_wait();
   constexpr int V = Vec16<T>::N;
   const int t = threadIdx.x % LANES;
   const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LANES;
@@ -600,6 +605,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_short_kernel
 constexpr int64_t kBwdVectors = 4;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(LogprobBwdParams p, int64_t chunks) {
+  pdl_wait();
   constexpr int V = Vec16<T>::N;
   constexpr int G = WIDE ? kThreads : 32;
   const int t = WIDE ? (int)threadIdx.x : (int)(threadIdx.x & 31);
@@ -672,21 +678,24 @@ constexpr int64_t kWarpRow = 1024;
 
 template <typename T>
 int launch_fwd(LogprobParams p, cudaStream_t stream) {
+  cudaError_t rc;
+  auto launch = [&](void (*kern)(LogprobParams), int64_t blocks) {
+    return launch_pdl(kern, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
+  };
   if (p.top_n == 0 && short_vectors<T>(p.x, p.x_stride, nullptr, p.vocab)) {
 #define WF_LAUNCH(LANES, NV) \
-  token_logprobs_short_kernel<T, LANES, NV>  \
-      <<<(unsigned)((p.rows * LANES + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p)
+  rc = launch(token_logprobs_short_kernel<T, LANES, NV>, (p.rows * LANES + kThreads - 1) / kThreads)
     WF_SHORT_ROWS(T, WF_LAUNCH);
 #undef WF_LAUNCH
-    return (int)cudaGetLastError();
+    return (int)rc;
   }
   if (p.vocab <= kWarpRow) {
-    const unsigned grid = (unsigned)((p.rows + kWarps - 1) / kWarps);
-    if (p.top_n && p.vocab <= 64) token_logprobs_sort_kernel<T, 2><<<grid, kThreads, 0, stream>>>(p);
-    else if (p.top_n && p.vocab <= 256) token_logprobs_sort_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
-    else if (p.top_n) token_logprobs_warp_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
-    else token_logprobs_warp_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
-    return (int)cudaGetLastError();
+    const int64_t grid = (p.rows + kWarps - 1) / kWarps;
+    if (p.top_n && p.vocab <= 64) rc = launch(token_logprobs_sort_kernel<T, 2>, grid);
+    else if (p.top_n && p.vocab <= 256) rc = launch(token_logprobs_sort_kernel<T, 8>, grid);
+    else if (p.top_n) rc = launch(token_logprobs_warp_kernel<T, true>, grid);
+    else rc = launch(token_logprobs_warp_kernel<T, false>, grid);
+    return (int)rc;
   }
   int c = 1;
   while (c < 8 && p.rows * c <= kSms && p.vocab / c > 4 * kWarpRow) c *= 2;
@@ -695,33 +704,39 @@ int launch_fwd(LogprobParams p, cudaStream_t stream) {
   cfg.gridDim = dim3((unsigned)(p.rows * c));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)c;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return (int)(p.top_n ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, true>, p)
                        : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, false>, p));
 }
 
 template <typename T>
 int launch_bwd(const LogprobBwdParams& p, cudaStream_t stream) {
+  cudaError_t rc;
+  auto launch = [&](void (*kern)(LogprobBwdParams), int64_t blocks) {
+    return launch_pdl(kern, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
+  };
   if (short_vectors<T>(p.x, p.x_stride, p.dx, p.vocab)) {
 #define WF_LAUNCH(LANES, NV) \
-  token_logprobs_backward_short_kernel<T, LANES, NV>  \
-      <<<(unsigned)((p.rows * LANES + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p)
+  rc = launch(token_logprobs_backward_short_kernel<T, LANES, NV>, (p.rows * LANES + kThreads - 1) / kThreads)
     WF_SHORT_ROWS(T, WF_LAUNCH);
 #undef WF_LAUNCH
   } else if (p.vocab <= kWarpRow) {
-    token_logprobs_backward_kernel<T, false>
-        <<<(unsigned)((p.rows + kWarps - 1) / kWarps), kThreads, 0, stream>>>(p, 1);
+    rc = launch_pdl(token_logprobs_backward_kernel<T, false>, dim3((unsigned)((p.rows + kWarps - 1) / kWarps)),
+                    dim3(kThreads), 0, stream, p, int64_t(1));
   } else {
     const int64_t span = (int64_t)kThreads * Vec16<T>::N * kBwdVectors;
     const int64_t chunks = (p.vocab + span - 1) / span;
-    token_logprobs_backward_kernel<T, true><<<(unsigned)(p.rows * chunks), kThreads, 0, stream>>>(p, chunks);
+    rc = launch_pdl(token_logprobs_backward_kernel<T, true>, dim3((unsigned)(p.rows * chunks)), dim3(kThreads), 0,
+                    stream, p, chunks);
   }
-  return (int)cudaGetLastError();
+  return (int)rc;
 }
 
 }  // namespace
