@@ -14,11 +14,13 @@
 // box of a K-major operand is 64 of depth by all its rows; of an MN-major one, 64 rows of
 // the product by 64 of depth, side by side.  Both use the 128-byte swizzle.
 //
-// fp32 operands come as three bf16 pieces (8 + 8 + 8 bits of mantissa).  The six products
-// of pieces that reach fp32's last bit go into one accumulator, smallest first; the other
-// three are below 2^-24 of the whole.  The tensor cores' own adds lose more with the
-// length of a sum than fp32 rounding would, so every kChunk of depth the accumulator is
-// added to fp32 registers and begun anew.
+// fp32 operands come as three bf16 pieces (8 + 8 + 8 bits of mantissa).  Six of the nine
+// products of pieces reach fp32's last bit; the others are below 2^-24 of the whole.  A stage
+// holds one piece of A and of B, each is loaded once and the six products of a depth are made
+// from three stages.  The tensor cores' own adds lose more with the length of a sum than fp32
+// rounding would: the product of the first pieces has an accumulator of its own, apart from
+// the five small ones, and every kChunk of depth both are added to fp32 registers and begun
+// anew.
 //
 // Epilogue: a warp owns 32 rows (its TMEM lanes, a row a lane) and walks them in slices of
 // 64 bytes of output, through two swizzled shared-memory buffers in turn that TMA stores
@@ -75,17 +77,15 @@ struct Layout {
   static constexpr size_t off_bar = off_staging + STAGING;
   static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5 + 2 * kEpilogueWarps);
   static constexpr size_t smem = off_misc + 16 + 1024;
-  static constexpr uint32_t TMEM_COLS = 2 * BN;
+  static constexpr int ACC = PIECES ? 2 * BN : BN;  // TMEM columns of an accumulator (main and small products)
+  static constexpr uint32_t TMEM_COLS = 2 * ACC;
+  static_assert(!PIECES || STAGES >= 6, "two depths of three pieces");
   // columns of a slice, and of an epilogue warp (a quarter of the tile, or a slice's where
   // that is more: then fewer warps work)
   static constexpr int SC = kSliceBytes / (int)sizeof(T);
   static constexpr int COLS = BN / 4 < SC ? SC : BN / 4;
   static constexpr int WARPS = 4 * (BN / COLS);
 };
-
-// Pieces of a and b multiplied in this order: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0).
-__device__ __forceinline__ int piece_a(int pair) { return (0x010210 >> (4 * pair)) & 3; }
-__device__ __forceinline__ int piece_b(int pair) { return (0x001012 >> (4 * pair)) & 3; }
 
 // Descriptor of an MN-major operand with the 128-byte swizzle: 64 rows of the product are
 // 128 bytes, 8 of depth 1024 bytes apart, the next 64 rows 64 of depth further.
@@ -262,7 +262,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   pdl_wait();  // what comes before this kernel on its stream is done; nothing above touched global memory
   const uint32_t tmem = *tmem_s;
-  constexpr int pairs = PIECES ? 6 : 1;
   uint32_t why = 0;
 
   if (warp == kEpilogueWarps) {
@@ -275,36 +274,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step) {
         const Unit w(p, u, BM, BN);
         const int am = w.m0 + (int)rank * kBM, bn = w.n0 + (int)rank * (BN / CG);
-        for (int c0 = w.kb0; c0 < w.kb1 && !why; c0 += PIECES ? kChunk : w.kb1 - w.kb0) {
-          const int c1 = PIECES ? min(c0 + kChunk, w.kb1) : w.kb1;
-          for (int pair = 0; pair < pairs && !why; ++pair) {
-            const int pa = PIECES ? piece_a(pair) : 0, pb = PIECES ? piece_b(pair) : 0;
-            for (int kb = c0; kb < c1; ++kb) {
-              if (!mbar_wait_asleep(&empty[r.stage], r.phase ^ 1, kWaitNs)) { why = 4; break; }
-              unsigned char* st = base + (size_t)r.stage * L::STAGE;
-              uint64_t* bar = &full[r.stage];
-              if (rank == 0) mbar_arrive_expect_tx(bar, CG * L::STAGE);
-              const uint32_t on = CG == 2 ? map_peer(bar, 0) : 0;
-              auto load = [&](void* dst, const CUtensorMap* map, int x, int y, int z) {
-                if constexpr (CG == 2) tma_load_3d_pair(dst, map, on, x, y, z);
-                else tma_load_3d(dst, map, bar, x, y, z);
-              };
-              if (p.a_mn) {
+        for (int kb = w.kb0; kb < w.kb1 && !why; ++kb) {
+#pragma unroll 1
+          for (int piece = 0; piece < (PIECES ? 3 : 1); ++piece) {
+            if (!mbar_wait_asleep(&empty[r.stage], r.phase ^ 1, kWaitNs)) { why = 4; break; }
+            unsigned char* st = base + (size_t)r.stage * L::STAGE;
+            uint64_t* bar = &full[r.stage];
+            if (rank == 0) mbar_arrive_expect_tx(bar, CG * L::STAGE);
+            const uint32_t on = CG == 2 ? map_peer(bar, 0) : 0;
+            auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
+              if constexpr (CG == 2) tma_load_3d_pair(dst, map, on, x, y, piece);
+              else tma_load_3d(dst, map, bar, x, y, piece);
+            };
+            if (p.a_mn) {
 #pragma unroll
-                for (int i = 0; i < kBM / 64; ++i) load(st + i * kBK * 128, &amap, am + 64 * i, kb * kBK, pa);
-              } else {
-                load(st, &amap, kb * kBK, am, pa);
-              }
-              st += L::A_BYTES;
-              if (p.b_mn) {
-#pragma unroll
-                for (int i = 0; i < BN / CG / 64; ++i) load(st + i * kBK * 128, &bmap, bn + 64 * i, kb * kBK, pb);
-              } else {
-                load(st, &bmap, kb * kBK, bn, pb);
-              }
-              ++issued;
-              r.next<L::STAGES>();
+              for (int i = 0; i < kBM / 64; ++i) load(st + i * kBK * 128, &amap, am + 64 * i, kb * kBK);
+            } else {
+              load(st, &amap, kb * kBK, am);
             }
+            st += L::A_BYTES;
+            if (p.b_mn) {
+#pragma unroll
+              for (int i = 0; i < BN / CG / 64; ++i) load(st + i * kBK * 128, &bmap, bn + 64 * i, kb * kBK);
+            } else {
+              load(st, &bmap, kb * kBK, bn);
+            }
+            ++issued;
+            r.next<L::STAGES>();
           }
         }
       }
@@ -331,22 +327,51 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int c1 = PIECES ? min(c0 + kChunk, w.kb1) : w.kb1;
           if (!mbar_wait_asleep(&acc_empty[acc], acc_phase ^ 1, kWaitNs)) { why = 8; break; }
           tc_fence_after();
-          const uint32_t d = tmem + acc * BN;
-          const int n = (c1 - c0) * pairs;
-          for (int i = 0; i < n; ++i) {
-            if (!mbar_wait_asleep(&full[r.stage], r.phase, kWaitNs)) { why = 16; break; }
-            tc_fence_after();
-            const uint32_t as = smem_u32(base + (size_t)r.stage * L::STAGE), bs = as + L::A_BYTES;
+          const uint32_t d = tmem + acc * L::ACC;
+          // the products of a stage's A with a stage's B
+          auto multiply = [&](uint32_t to, uint32_t a_stage, uint32_t b_stage, bool onto) {
+            const uint32_t as = smem_u32(base + (size_t)a_stage * L::STAGE);
+            const uint32_t bs = smem_u32(base + (size_t)b_stage * L::STAGE) + L::A_BYTES;
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k) {
               const uint32_t aa = as + k * a_step, bb = bs + k * b_step;
               const uint64_t da = p.a_mn ? smem_desc_mnmajor(aa) : smem_desc_kmajor(aa, 128);
               const uint64_t db = p.b_mn ? smem_desc_mnmajor(bb) : smem_desc_kmajor(bb, 128);
-              if constexpr (CG == 2) mma_f16_pair(d, da, db, p.idesc, i > 0 || k > 0);
-              else mma_f16(d, da, db, p.idesc, i > 0 || k > 0);
+              if constexpr (CG == 2) mma_f16_pair(to, da, db, p.idesc, onto || k > 0);
+              else mma_f16(to, da, db, p.idesc, onto || k > 0);
             }
-            commit(&empty[r.stage]);
+          };
+          auto arrived = [&](const Ring& at) {
+            if (!mbar_wait_asleep(&full[at.stage], at.phase, kWaitNs)) {
+              why = 16;
+              return false;
+            }
+            tc_fence_after();
+            return true;
+          };
+          for (int kb = c0; kb < c1; ++kb) {
+            const bool onto = kb > c0;
+            const Ring r0 = r;
+            if (!arrived(r0)) break;
+            multiply(d, r0.stage, r0.stage, onto);
             r.next<L::STAGES>();
+            if constexpr (PIECES) {
+              const uint32_t small = d + BN;
+              const Ring r1 = r;
+              if (!arrived(r1)) break;
+              multiply(small, r0.stage, r1.stage, onto);
+              multiply(small, r1.stage, r0.stage, true);
+              multiply(small, r1.stage, r1.stage, true);
+              commit(&empty[r1.stage]);
+              r.next<L::STAGES>();
+              const Ring r2 = r;
+              if (!arrived(r2)) break;
+              multiply(small, r0.stage, r2.stage, true);
+              multiply(small, r2.stage, r0.stage, true);
+              commit(&empty[r2.stage]);
+              r.next<L::STAGES>();
+            }
+            commit(&empty[r0.stage]);
           }
           commit(&acc_full[acc]);
           acc ^= 1;
@@ -440,11 +465,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ready()) break;
 #pragma unroll
           for (int c = 0; c < COLS; c += SC) {
-            uint32_t r[SC];
-            tmem_ld(lbase + acc * BN + c, r);
+            uint32_t r[SC], s[SC];
+            tmem_ld(lbase + acc * L::ACC + c, r);
+            tmem_ld(lbase + acc * L::ACC + BN + c, s);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < SC; ++j) sum[c + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < SC; ++j) sum[c + j] += __uint_as_float(r[j]) + __uint_as_float(s[j]);
           }
           release();
         }
@@ -465,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int m = w.m0 + (int)rank * kBM + 32 * (warp & 3), n0 = w.n0 + (warp >> 2) * COLS;
         if (!asked) {
           if (!ready()) break;
-          tmem_ld(lbase + acc * BN, r);
+          tmem_ld(lbase + acc * L::ACC, r);
         }
         asked = false;
 #pragma unroll 1
@@ -476,12 +502,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < SC; ++j) v[j] = __uint_as_float(r[j]);
           add_bias<T>(p, n0 + c, v);
           if (c + SC < COLS) {
-            tmem_ld(lbase + acc * BN + c + SC, r);
+            tmem_ld(lbase + acc * L::ACC + c + SC, r);
           } else {
             release();
             if (u + step < (uint32_t)p.units && __all_sync(0xffffffffu, mbar_try_wait(&acc_full[acc], acc_phase))) {
               tc_fence_after();
-              tmem_ld(lbase + acc * BN, r);
+              tmem_ld(lbase + acc * L::ACC, r);
               asked = true;
             }
           }
@@ -581,9 +607,11 @@ bool make_out_map(CUtensorMap* map, const void* ptr, int64_t cols, int64_t rows,
 // accumulator's way out; units run in waves.
 struct Shape {
   int bn, cg;
-  int cycles;  // a stage: the products' time, or the loads' at about 64 bytes a cycle an SM
+  // 64 of depth: the products' time, or the loads' at about 64 bytes a cycle an SM; of one
+  // piece, and of three with their six products (0: no room for the stages or the sums)
+  int cycles, cycles3;
 };
-constexpr Shape kShapes[] = {{256, 2, 560}, {128, 2, 400}, {128, 1, 540}, {64, 1, 400}};
+constexpr Shape kShapes[] = {{256, 2, 560, 0}, {128, 2, 400, 1700}, {128, 1, 540, 0}, {64, 1, 400, 1300}};
 constexpr int kMinShare = 4;  // stages of depth a share has at least
 struct Plan {
   Shape shape;
@@ -593,7 +621,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
   Plan best{};
   double least = 0;
   for (const Shape& s : kShapes) {
-    if (pieces > 1 && s.bn == 256) continue;  // a warp's fp32 sums would not fit its registers
+    if (pieces > 1 && !s.cycles3) continue;
     Plan p{};
     p.shape = s;
     p.k_blocks = (int)((K + kBK - 1) / kBK);
@@ -604,10 +632,10 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
     for (int splits = 1; splits <= kMaxSplits && (splits == 1 || p.k_blocks / splits >= kMinShare); ++splits) {
       if (splits > 1 && (int64_t)p.tiles * splits > 2 * slots) break;  // most shapes look at one split
       const int64_t waves = ((int64_t)p.tiles * splits + slots - 1) / slots;
-      const int64_t deep = (p.k_blocks + splits - 1) / splits * (pieces > 1 ? 6 : 1);
+      const int64_t deep = (p.k_blocks + splits - 1) / splits;
       // partials go through L2 twice, and joining them is a launch
       const double join = splits > 1 ? 4000 + 8.0 * splits * M * N / 4000 : 0;
-      const double t = (double)waves * (deep * s.cycles + 4 * s.bn) + join;
+      const double t = (double)waves * (deep * (pieces > 1 ? s.cycles3 : s.cycles) + 4 * s.bn) + join;
       if (best.splits == 0 || t < least) {
         least = t;
         best = p;
@@ -678,10 +706,11 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan,
 template <typename T, bool PIECES>
 int launch_shape(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, cudaStream_t stream) {
   const Shape& s = plan.shape;
-  if constexpr (!PIECES)
+  if constexpr (!PIECES) {
     if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, plan, stream);
+    if (s.bn == 128 && s.cg == 1) return launch_tile<T, 128, 1, PIECES>(g, out, plan, stream);
+  }
   if (s.cg == 2) return launch_tile<T, 128, 2, PIECES>(g, out, plan, stream);
-  if (s.bn == 128) return launch_tile<T, 128, 1, PIECES>(g, out, plan, stream);
   return launch_tile<T, 64, 1, PIECES>(g, out, plan, stream);
 }
 
