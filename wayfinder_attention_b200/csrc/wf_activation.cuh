@@ -123,11 +123,20 @@ __device__ __forceinline__ float activation_slope(float z) {
     float s;
     if constexpr (FAST) s = rcp_approx(1.f + exp2_approx(-1.4426950408889634f * z));
     else s = 1.f / (1.f + expf(-z));
-    return s * fmaf(z, 1.f - s, 1.f);
+    // z may have been kept as an infinity: 0 times that is the slope's limit, 0
+    return s * fmaf(fabsf(z) > 200.f ? 0.f : z, 1.f - s, 1.f);
   } else {
     return 1.f;
   }
 }
+
+// How the forward keeps z for the backward: fp16 for both 16-bit types (a slope is flat where
+// fp16 ends, and its eleven bits are worth more than bf16's range: with bf16's eight, the
+// gradients' rounding errors grew by a half instead of by root two over one rounding).
+template <typename T> struct Kept { using type = __half; };
+template <> struct Kept<float> { using type = float; };
+// What is kept of z; relu's slope asks for the sign only, which a rounding to 0 would lose.
+__device__ __forceinline__ float kept_z(int act, float z) { return act == kActRelu && z > 0.f ? fmaxf(z, 6.2e-5f) : z; }
 
 // g[j] *= act'(z[j]), z overwritten.
 template <int ACT, typename T, int N>

@@ -420,7 +420,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (o.z) {
         if (lane == 0) bulk_wait_read<1>();
         __syncwarp();
-        stage_slice<T>(smem_u32(buffer(turn)), lane, v);
+        float kept[SC];
+#pragma unroll
+        for (int j = 0; j < SC; ++j) kept[j] = kept_z(o.act, v[j]);
+        stage_slice<typename Kept<T>::type>(smem_u32(buffer(turn)), lane, kept);
         store(&zmap, o.z, o.z_stride, m, n, 0);
       }
       if (lane == 0) bulk_wait_read<1>();
@@ -537,6 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T>
 __global__ void __launch_bounds__(256) gemm_join_kernel(const float* partial, int splits, int64_t pitch, int64_t M,
                                                         int64_t N, GemmEpilogue o) {
+  using Z = typename Kept<T>::type;
   pdl_wait();
   const int64_t groups = pitch / 4, total = M * groups;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -550,7 +554,8 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const float* partial, in
     if (o.bias)
       for (int j = 0; j < live; ++j) v[j] += to_f32(static_cast<const T*>(o.bias)[n + j]);
     if (o.z)
-      for (int j = 0; j < live; ++j) static_cast<T*>(o.z)[m * o.z_stride + n + j] = from_f32<T>(v[j]);
+      for (int j = 0; j < live; ++j)
+        static_cast<Z*>(o.z)[m * o.z_stride + n + j] = from_f32<Z>(kept_z(o.act, v[j]));
     activate_all<T, 4>(o.act, v);
     if (o.residual)
       for (int j = 0; j < live; ++j) v[j] += to_f32(static_cast<const T*>(o.residual)[m * o.r_stride + n + j]);

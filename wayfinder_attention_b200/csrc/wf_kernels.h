@@ -208,7 +208,7 @@ struct LinearParams {
   const void* w;
   const void* bias;      // [N] or null
   const void* residual;  // (M, N) or null
-  void* z;               // (M, N) pre-activations for the backward, or null
+  void* z;               // (M, N) pre-activations for the backward (fp16, or fp32 for fp32), or null
   void* y;
   int64_t M, N, K, x_stride, w_stride, r_stride;
   int act;

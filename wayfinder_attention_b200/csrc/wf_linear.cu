@@ -4,9 +4,9 @@
 //   backward  dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum_rows dz
 //
 // act: none, gelu (z Phi(z), Phi by erf), relu, silu (z sigmoid(z)).  Products and sums
-// are fp32; y is rounded once.  The backward reads z as the forward rounded it to the
-// activations' type, and rounds dz to that type before the two products, as operands of
-// that type are what the products take; db sums the unrounded values.
+// are fp32; y is rounded once.  The backward reads z as the forward kept it (fp16 for both
+// 16-bit types), and rounds dz to the activations' type before the two products, as
+// operands of that type are what the products take; db sums the unrounded values.
 //
 // The product reads 16-bit matrices whose rows start on 16 bytes.  Others are laid out in
 // the workspace first: 16-bit rows of any width or offset are copied to such rows, and an
@@ -103,9 +103,9 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const T* x, int64_t rows, 
 // dz = dy act'(z) into the operand's layout, and partial column sums: a block takes 256
 // columns (8 a lane) of a share of the rows, its 8 warps a row each.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_stride, bool dy_vec, const T* z,
-                                                        void* out, int64_t pitch, int64_t piece, int64_t M, int64_t N,
-                                                        float* partials) {
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_stride, bool dy_vec,
+                                                        const typename Kept<T>::type* z, void* out, int64_t pitch,
+                                                        int64_t piece, int64_t M, int64_t N, float* partials) {
   __shared__ float red[8][32][9];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
   constexpr int U = 2;  // rows asked for at once
   if (c < N)
     for (int64_t m0 = (int64_t)blockIdx.y * 8 + warp; m0 < M; m0 += (int64_t)gridDim.y * 8 * U) {
-      Raw8<T> rg[U], rz[U];
+      Raw8<T> rg[U];
+      Raw8<typename Kept<T>::type> rz[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int64_t m = m0 + (int64_t)i * gridDim.y * 8;
@@ -232,7 +233,7 @@ cudaError_t launch_dz(const LinearBwdParams& p, const GemmOperand& o, bool write
                       cudaStream_t stream) {
   return launch_pdl(linear_dz_kernel<T, ACT>, dim3((unsigned)((p.N + 255) / 256), row_shares(p.M, p.N)), dim3(256), 0,
                     stream, static_cast<const T*>(p.dy), p.dy_stride, on_16_bytes<T>(p.dy, p.dy_stride),
-                    static_cast<const T*>(p.z), write ? const_cast<void*>(o.ptr) : nullptr, o.pitch, o.piece_stride,
+                    static_cast<const typename Kept<T>::type*>(p.z), write ? const_cast<void*>(o.ptr) : nullptr, o.pitch, o.piece_stride,
                     p.M, p.N, partials);
 }
 

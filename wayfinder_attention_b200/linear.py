@@ -22,7 +22,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     shape (..., d_out) or None; all CUDA tensors of one type (bfloat16, float16 or
     float32).  activation: "none", "gelu" (the erf form), "relu" or "silu".
     Differentiable in x, weight, bias and residual; the backward reads the
-    pre-activations as rounded to x's type and gives every gradient in it.  fp32 inputs
+    pre-activations as kept in fp16 (fp32 for fp32) and gives every gradient in x's type.  fp32 inputs
     are multiplied to fp32 accuracy on the tensor cores, as three bf16 pieces each: an
     infinite or NaN input makes its outputs NaN or infinite, not always the same of the two.
     """
