@@ -17,6 +17,7 @@
 #include "wf_linear_few.h"
 #include "wf_rowio.cuh"
 
+#include <algorithm>
 #include <cstring>
 #include <type_traits>
 #include <utility>
@@ -85,18 +86,29 @@ struct Raw8 {
   }
 };
 
+// Lays matrices out as operands: the blocks are shared between up to two of them.
 template <typename T>
-__global__ void __launch_bounds__(256) lay_out_kernel(const T* x, int64_t rows, int64_t cols, int64_t stride, bool vec,
-                                                      void* out, int64_t pitch, int64_t piece) {
+struct LayOut {
+  const T* x;
+  void* out;
+  int64_t rows, cols, stride, pitch, piece;
+  int blocks;
+  bool vec;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) lay_out_kernel(LayOut<T> first, LayOut<T> second) {
   pdl_wait();
-  const int64_t groups = pitch / 8, total = rows * groups;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+  const bool one = (int)blockIdx.x < first.blocks;
+  const LayOut<T>& j = one ? first : second;
+  const int64_t block = one ? blockIdx.x : blockIdx.x - first.blocks;
+  const int64_t groups = j.pitch / 8, total = j.rows * groups;
+  for (int64_t i = block * 256 + threadIdx.x; i < total; i += (int64_t)j.blocks * 256) {
     const int64_t r = i / groups, c = i % groups * 8;
     Raw8<T> raw;
-    raw.load(x + r * stride, c, cols, vec);
+    raw.load(j.x + r * j.stride, c, j.cols, j.vec);
     float f[8];
     raw.unpack(f);
-    store_operand<T>(out, r * pitch + c, piece, f);
+    store_operand<T>(j.out, r * j.pitch + c, j.piece, f);
   }
 }
 
@@ -155,9 +167,9 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
   }
 }
 
-// Row shares of the column sums: eight blocks an SM over all columns, 32 rows at least.
+// Row shares of the column sums: eight blocks an SM over all columns, 16 rows at least.
 int row_shares(int64_t M, int64_t N) {
-  const int64_t by = (N + 255) / 256, want = (8 * kSms + by - 1) / by, most = (M + 31) / 32;
+  const int64_t by = (N + 255) / 256, want = (8 * kSms + by - 1) / by, most = (M + 15) / 16;
   return (int)(want < most ? want : most);
 }
 
@@ -184,19 +196,29 @@ GemmOperand blank_operand(int64_t rows, int64_t cols, int dtype, unsigned char**
   *ws += operand_bytes(rows, cols, dtype);
   return o;
 }
+// Two matrices as operands, either of which may be missing (no pointer); what has to be laid
+// out goes in one launch.
+struct Matrix {
+  const void* ptr;
+  int64_t rows, cols, stride;
+};
 template <typename T>
-int operand(const void* x, int64_t rows, int64_t cols, int64_t stride, int dtype, unsigned char** ws, GemmOperand* o,
-            cudaStream_t stream) {
-  const bool vec = on_16_bytes<T>(x, stride);
-  if (dtype != kF32 && vec) {
-    *o = GemmOperand{x, rows, cols, stride, 0, false};
-    return 0;
+int operands(const Matrix (&m)[2], int dtype, unsigned char** ws, GemmOperand (&o)[2], cudaStream_t stream) {
+  LayOut<T> jobs[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    if (!m[i].ptr) continue;
+    const bool vec = on_16_bytes<T>(m[i].ptr, m[i].stride);
+    if (dtype != kF32 && vec) {
+      o[i] = GemmOperand{m[i].ptr, m[i].rows, m[i].cols, m[i].stride, 0, false};
+      continue;
+    }
+    o[i] = blank_operand<T>(m[i].rows, m[i].cols, dtype, ws);
+    const int64_t blocks = (m[i].rows * (o[i].pitch / 8) + 255) / 256;
+    jobs[i] = LayOut<T>{static_cast<const T*>(m[i].ptr), const_cast<void*>(o[i].ptr), m[i].rows, m[i].cols,
+                        m[i].stride, o[i].pitch, o[i].piece_stride, (int)std::min<int64_t>(blocks, 16 * kSms), vec};
   }
-  *o = blank_operand<T>(rows, cols, dtype, ws);
-  const int64_t blocks = (rows * (o->pitch / 8) + 255) / 256;
-  return (int)launch_pdl(lay_out_kernel<T>, dim3((unsigned)(blocks < 16 * kSms ? blocks : 16 * kSms)), dim3(256), 0,
-                         stream, static_cast<const T*>(x), rows, cols, stride, vec, const_cast<void*>(o->ptr), o->pitch,
-                         o->piece_stride);
+  const int blocks = jobs[0].blocks + jobs[1].blocks;
+  return blocks ? (int)launch_pdl(lay_out_kernel<T>, dim3(blocks), dim3(256), 0, stream, jobs[0], jobs[1]) : 0;
 }
 
 template <typename T>
@@ -220,10 +242,9 @@ template <typename T>
 int launch_fwd(const LinearParams& p, int dtype, cudaStream_t stream) {
   if (linear_few_takes(p, dtype)) return launch_linear_few(p, dtype, stream);
   unsigned char* ws = static_cast<unsigned char*>(p.ws);
-  GemmOperand x, w;
-  if (int rc = operand<T>(p.x, p.M, p.K, p.x_stride, dtype, &ws, &x, stream)) return rc;
-  if (int rc = operand<T>(p.w, p.N, p.K, p.w_stride, dtype, &ws, &w, stream)) return rc;
-  GemmProblem g = problem<T>(x, w, p.M, p.N, p.K, dtype, ws, p.status);
+  GemmOperand o[2];
+  if (int rc = operands<T>({{p.x, p.M, p.K, p.x_stride}, {p.w, p.N, p.K, p.w_stride}}, dtype, &ws, o, stream)) return rc;
+  GemmProblem g = problem<T>(o[0], o[1], p.M, p.N, p.K, dtype, ws, p.status);
   g.out = GemmEpilogue{p.bias, p.residual, p.z, p.y, p.r_stride, p.N, p.N, p.act};
   return launch_gemm(g, stream);
 }
@@ -268,22 +289,20 @@ int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
   }
   if (p.db)
     if (cudaError_t e = join_columns<T>(partials, row_shares(p.M, p.N), p.N, p.N, p.db, nullptr, stream)) return (int)e;
+  GemmOperand o[2];  // w for dx, x for dw
+  if (int rc = operands<T>({{p.dx ? p.w : nullptr, p.N, p.K, p.w_stride}, {p.dw ? p.x : nullptr, p.M, p.K, p.x_stride}},
+                           dtype, &ws, o, stream))
+    return rc;
   if (p.dx) {
-    GemmOperand w;
-    unsigned char* at = ws;
-    if (int rc = operand<T>(p.w, p.N, p.K, p.w_stride, dtype, &at, &w, stream)) return rc;
-    w.mn_major = true;  // its columns are dx's, its rows the depth
-    GemmProblem g = problem<T>(dz, w, p.M, p.K, p.N, dtype, at, p.status);
+    o[0].mn_major = true;  // its columns are dx's, its rows the depth
+    GemmProblem g = problem<T>(dz, o[0], p.M, p.K, p.N, dtype, ws, p.status);
     g.out.y = p.dx;
     g.out.y_stride = p.K;
     if (int rc = launch_gemm(g, stream)) return rc;
   }
   if (p.dw) {
-    GemmOperand x;
-    unsigned char* at = ws;
-    if (int rc = operand<T>(p.x, p.M, p.K, p.x_stride, dtype, &at, &x, stream)) return rc;
-    dz.mn_major = x.mn_major = true;  // the rows of both are the depth
-    GemmProblem g = problem<T>(dz, x, p.N, p.K, p.M, dtype, at, p.status);
+    dz.mn_major = o[1].mn_major = true;  // the rows of both are the depth
+    GemmProblem g = problem<T>(dz, o[1], p.N, p.K, p.M, dtype, ws, p.status);
     g.out.y = p.dw;
     g.out.y_stride = p.K;
     if (int rc = launch_gemm(g, stream)) return rc;
@@ -304,9 +323,10 @@ size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtyp
   const int pieces = dtype == kF32 ? 3 : 1;
   const size_t dz = act == kActNone && pieces == 1 && dy_direct ? 0 : operand_bytes(M, N, dtype);
   const size_t sums = round256((size_t)row_shares(M, N) * N * sizeof(float));
-  const size_t dx = (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) + gemm_workspace_bytes(M, K, N, pieces);
-  const size_t dw = (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype)) + gemm_workspace_bytes(N, K, M, pieces);
-  return dz + sums + (dx > dw ? dx : dw);
+  const size_t laid_out = (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) +
+                          (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype));
+  const size_t dx = gemm_workspace_bytes(M, K, N, pieces), dw = gemm_workspace_bytes(N, K, M, pieces);
+  return dz + sums + laid_out + std::max(dx, dw);  // the products' parts, one after the other
 }
 
 int launch_linear(const LinearParams& p, int dtype, cudaStream_t stream) {
