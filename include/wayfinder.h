@@ -382,8 +382,9 @@ WF_API int wf_testing_withhold_pair_arrive(int32_t round, uint64_t wait_limit_ns
  *   x        : (M, K) rows x_row_stride apart;  w : (N, K) rows w_row_stride apart
  *   bias     : (N) or NULL;  residual : (M, N) rows r_row_stride apart, or NULL
  *   dtype    : WF_DTYPE_* of all of them and of y
- *   z        : (M, N) contiguous, gets x W^T + b for the backward, as fp16 for both 16-bit
- *              types and as fp32 for fp32; may be NULL
+ *   z        : gets x W^T + b for the backward, as fp16 for both 16-bit types and as fp32
+ *              for fp32, in M rows of N rounded up to a multiple of 8 (16-byte aligned); may
+ *              be NULL
  *   y        : (M, N) contiguous
  *   workspace: wf_linear_workspace_bytes() bytes, 256-byte aligned (NULL if that is 0); its
  *              x_direct / w_direct (dy_direct in the backward) say whether that matrix

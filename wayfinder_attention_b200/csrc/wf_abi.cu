@@ -814,6 +814,7 @@ int wf_linear(const void* x, const void* w, const void* bias, const void* residu
                                             M, N, K, dtype, on_16_bytes(x, x_row_stride, dtype),
                                             on_16_bytes(w, w_row_stride, dtype)))))
     return rc;
+  if (reinterpret_cast<uintptr_t>(z) % 16) return fail(WF_ERR_INVALID_ARGUMENT, "z must be 16-byte aligned");
   wf::LinearParams p{};
   p.x = x; p.w = w; p.bias = bias; p.residual = residual; p.z = z; p.y = y;
   p.M = M; p.N = N; p.K = K;
@@ -843,6 +844,7 @@ int wf_linear_backward(const void* x, const void* w, const void* z, const void* 
                                   on_16_bytes(w, w_row_stride, dtype), on_16_bytes(dy, dy_row_stride, dtype)))))
       return rc;
   }
+  if (reinterpret_cast<uintptr_t>(z) % 16) return fail(WF_ERR_INVALID_ARGUMENT, "z must be 16-byte aligned");
   wf::LinearBwdParams p{};
   p.x = x; p.w = w; p.z = z; p.dy = dy; p.dx = dx; p.dw = dw; p.db = dbias;
   p.M = M; p.N = N; p.K = K;

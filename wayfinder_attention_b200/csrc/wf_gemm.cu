@@ -60,7 +60,7 @@ constexpr int kMaxSplits = 32;
 struct GemmParams {
   int M, N, tiles_n, units, splits, k_blocks;
   bool a_mn, b_mn;
-  bool store_tma, residual_tma;  // y and z, the residual start and step on 16 bytes
+  bool y_tma, residual_tma;  // y, the residual start and step on 16 bytes (z always does)
   bool bias_vec;                 // so does the bias
   GemmEpilogue out;
   int32_t* status;
@@ -138,26 +138,43 @@ __device__ __forceinline__ uint32_t staged(int r, int at) {
 }
 
 // Between a staging buffer and rows that start anywhere: 32 lanes take consecutive elements
-// of a row, or of two rows of 16.
+// of a row, or of two rows of 16.  For fp32 all sixteen accesses are under way at once; the
+// 16-bit types' usual way would pay for that in spilled registers (40 -> 45 us at 32768 x
+// 1024), so they have four.
 template <typename T>
 __device__ __forceinline__ void copy_rows_out(const unsigned char* buf, T* y, int64_t stride, int64_t m, int64_t M,
                                               int n, int N, int lane) {
-  constexpr int SC = kSliceBytes / (int)sizeof(T);
+  constexpr int SC = kSliceBytes / (int)sizeof(T), PER = 32 / SC;  // rows an access
+  constexpr int AT = sizeof(T) == 4 ? 16 : 4;
   const int c = lane % SC;
-#pragma unroll 4
-  for (int r = lane / SC; r < 32; r += 32 / SC)
+#pragma unroll(AT)
+  for (int r = lane / SC; r < 32; r += PER)
     if (m + r < M && n + c < N)
       y[(m + r) * stride + n + c] = *reinterpret_cast<const T*>(buf + staged(r, c * (int)sizeof(T)));
 }
 template <typename T>
 __device__ __forceinline__ void copy_rows_in(unsigned char* buf, const T* x, int64_t stride, int64_t m, int64_t M,
                                              int n, int N, int lane) {
-  constexpr int SC = kSliceBytes / (int)sizeof(T);
+  constexpr int SC = kSliceBytes / (int)sizeof(T), PER = 32 / SC;
   const int c = lane % SC;
+  if constexpr (sizeof(T) == 4) {
+    T v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = lane / SC + PER * i;
+      if (m + r < M && n + c < N) v[i] = x[(m + r) * stride + n + c];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = lane / SC + PER * i;
+      if (m + r < M && n + c < N) *reinterpret_cast<T*>(buf + staged(r, c * (int)sizeof(T))) = v[i];
+    }
+  } else {
 #pragma unroll 4
-  for (int r = lane / SC; r < 32; r += 32 / SC)
-    if (m + r < M && n + c < N)
-      *reinterpret_cast<T*>(buf + staged(r, c * (int)sizeof(T))) = x[(m + r) * stride + n + c];
+    for (int r = lane / SC; r < 32; r += PER)
+      if (m + r < M && n + c < N)
+        *reinterpret_cast<T*>(buf + staged(r, c * (int)sizeof(T))) = x[(m + r) * stride + n + c];
+  }
 }
 
 template <typename T>
@@ -399,9 +416,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       acc ^= 1;
       acc_phase ^= acc == 0;
     };
-    auto store = [&](const CUtensorMap* map, void* to, int64_t stride, int m, int n, int layer) {
+    auto store = [&](bool tma, const CUtensorMap* map, void* to, int64_t stride, int m, int n, int layer) {
       unsigned char* buf = buffer(turn++);
-      if (p.store_tma) {
+      if (tma) {
         fence_async_shared();
         __syncwarp();
         if (lane == 0) {
@@ -424,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < SC; ++j) kept[j] = kept_z(o.act, v[j]);
         stage_slice<typename Kept<T>::type>(smem_u32(buffer(turn)), lane, kept);
-        store(&zmap, o.z, o.z_stride, m, n, 0);
+        store(true, &zmap, nullptr, 0, m, n, 0);
       }
       if (lane == 0) bulk_wait_read<1>();
       __syncwarp();
@@ -450,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         add_staged_slice<T>(smem_u32(buffer(turn)), lane, v);
       }
       stage_slice<T>(smem_u32(buffer(turn)), lane, v);
-      store(&ymap, o.y, o.y_stride, m, n, layer);
+      store(p.y_tma, &ymap, o.y, o.y_stride, m, n, layer);
     };
     auto ready = [&] {
       if (!__all_sync(0xffffffffu, mbar_wait_asleep(&acc_full[acc], acc_phase, kWaitNs))) why = 32;
@@ -675,12 +692,11 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan,
   auto on16 = [](const void* q, int64_t stride) {
     return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
   };
-  p.store_tma = on16(out.y, out.y_stride) && on16(out.z, out.z_stride);
+  p.y_tma = on16(out.y, out.y_stride);
   // rows that overlap (a broadcast residual) are not a tensor map's
   p.residual_tma = out.residual && on16(out.residual, out.r_stride) && out.r_stride >= g.N;
-  if (p.store_tma && (!make_out_map<T>(&ymap, out.y, g.N, g.M, plan.splits, out.y_stride) ||
-                      (out.z && !make_out_map<T>(&zmap, out.z, g.N, g.M, 1, out.z_stride))))
-    return -1;
+  if (p.y_tma && !make_out_map<T>(&ymap, out.y, g.N, g.M, plan.splits, out.y_stride)) return -1;
+  if (out.z && !make_out_map<T>(&zmap, out.z, g.N, g.M, 1, out.z_stride)) return -1;
   if (p.residual_tma && !make_out_map<T>(&rmap, out.residual, g.N, g.M, 1, out.r_stride)) return -1;
   p.bias_vec = reinterpret_cast<uintptr_t>(out.bias) % 16 == 0;
   auto kern = gemm_kernel<T, BN, CG, PIECES>;

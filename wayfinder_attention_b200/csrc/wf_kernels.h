@@ -201,14 +201,15 @@ int launch_token_logprobs(const LogprobParams& p, int dtype, cudaStream_t stream
 int launch_token_logprobs_backward(const LogprobBwdParams& p, int dtype, cudaStream_t stream);
 
 // Linear layer with bias, activation and residual (wf_linear.cu).  x (M, K) and
-// w (N, K) are unit-strided on K; y, z and the gradients are contiguous.
+// w (N, K) are unit-strided on K; y and the gradients are contiguous.
 enum Activation : int { kActNone = 0, kActGelu = 1, kActRelu = 2, kActSilu = 3 };
 struct LinearParams {
   const void* x;
   const void* w;
   const void* bias;      // [N] or null
   const void* residual;  // (M, N) or null
-  void* z;               // (M, N) pre-activations for the backward (fp16, or fp32 for fp32), or null
+  // pre-activations for the backward (fp16, or fp32 for fp32), M rows of N rounded up to 8; or null
+  void* z;
   void* y;
   int64_t M, N, K, x_stride, w_stride, r_stride;
   int act;

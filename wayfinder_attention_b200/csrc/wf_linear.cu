@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * 8;
   float s[8] = {};
-  const bool z_vec = N % 8 == 0;
+  const int64_t z_pitch = (N + 7) / 8 * 8;
   constexpr int U = 2;  // rows asked for at once
   if (c < N)
     for (int64_t m0 = (int64_t)blockIdx.y * 8 + warp; m0 < M; m0 += (int64_t)gridDim.y * 8 * U) {
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, int64_t dy_
         const int64_t m = m0 + (int64_t)i * gridDim.y * 8;
         if (m < M) {
           rg[i].load(dy + m * dy_stride, c, N, dy_vec);
-          if constexpr (ACT != kActNone) rz[i].load(z + m * N, c, N, z_vec);
+          if constexpr (ACT != kActNone) rz[i].load(z + m * z_pitch, c, N, true);
         }
       }
 #pragma unroll
@@ -245,7 +245,7 @@ int launch_fwd(const LinearParams& p, int dtype, cudaStream_t stream) {
   GemmOperand o[2];
   if (int rc = operands<T>({{p.x, p.M, p.K, p.x_stride}, {p.w, p.N, p.K, p.w_stride}}, dtype, &ws, o, stream)) return rc;
   GemmProblem g = problem<T>(o[0], o[1], p.M, p.N, p.K, dtype, ws, p.status);
-  g.out = GemmEpilogue{p.bias, p.residual, p.z, p.y, p.r_stride, p.N, p.N, p.act};
+  g.out = GemmEpilogue{p.bias, p.residual, p.z, p.y, p.r_stride, round8(p.N), p.N, p.act};
   return launch_gemm(g, stream);
 }
 

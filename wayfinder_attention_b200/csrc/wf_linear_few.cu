@@ -30,7 +30,7 @@ template <typename T>
 __device__ __forceinline__ void put(const LinearParams& p, int64_t m, int64_t n, float v) {
   if (p.bias) v += to_f32(static_cast<const T*>(p.bias)[n]);
   using Z = typename Kept<T>::type;
-  if (p.z) static_cast<Z*>(p.z)[m * p.N + n] = from_f32<Z>(kept_z(p.act, v));
+  if (p.z) static_cast<Z*>(p.z)[m * ((p.N + 7) / 8 * 8) + n] = from_f32<Z>(kept_z(p.act, v));
   float a[2] = {v, 0.f};
   activate_all<T, 2>(p.act, a);
   if (p.residual) a[0] += to_f32(static_cast<const T*>(p.residual)[m * p.r_stride + n]);

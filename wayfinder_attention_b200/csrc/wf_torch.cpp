@@ -123,7 +123,7 @@ Tensor run_linear(const Tensor& x, const Tensor& w, const Tensor& b, const Tenso
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   const int code = dtype_code(x.scalar_type());
   Tensor y = at::empty(shape, x.options());
-  if (z) *z = at::empty({M, N}, code == WF_DTYPE_F32 ? x.options() : x.options().dtype(at::kHalf));
+  if (z) *z = at::empty({M, (N + 7) / 8 * 8}, code == WF_DTYPE_F32 ? x.options() : x.options().dtype(at::kHalf));
   const size_t n = wf.linear_workspace_bytes(M, N, K, code, on_16_bytes(x), on_16_bytes(w));
   const Tensor ws = bytes(n, x);
   check(wf.linear(x.data_ptr(), w.data_ptr(), ptr(b), ptr(r), code, M, N, K, x.stride(0), w.stride(0),
