@@ -13,38 +13,84 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// Phi(-|z|) for 16-bit results: Abramowitz and Stegun 7.1.26 (erfc(x) = (a1 t + .. + a5 t^5)
-// exp(-x^2), t = 1 / (1 + p x), off by at most 1.5e-7) at x = |z| / sqrt 2.  One reciprocal and
-// one exponential, where erff takes both of its branches in most warps.
-constexpr float kErfcP = 0.3275911f * 0.70710678118654752f;
-constexpr float kErfc0 = 0.5f * 0.254829592f, kErfc1 = 0.5f * -0.284496736f, kErfc2 = 0.5f * 1.421413741f,
-                kErfc3 = 0.5f * -1.453152027f, kErfc4 = 0.5f * 1.061405429f;
-constexpr float kGaussExp2 = -0.5f * 1.4426950408889634f;  // exp(-z^2 / 2) = 2^(this z^2)
 __device__ __forceinline__ float max_keep_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
 
-// gelu(z) = max(z, 0) - |z| Phi(-|z|), two at a time with the polynomial in paired
-// arithmetic.  Past 100 the tail is 0, and inf * 0 is kept out.  Paired instructions take
-// no immediates: the constants are made once, and hidden from the compiler so that it keeps
-// them in registers instead of moving them there again for each pair.
+// gelu for 16-bit results, two values at a time with the polynomials in paired arithmetic
+// (erff takes both of its branches in most warps).  Paired instructions take no immediates:
+// the constants are made once, and hidden from the compiler so that it keeps them in registers
+// instead of moving them there again for each pair.  B pairs go side by side: a pair alone is
+// a chain of some hundred cycles.
+__device__ __forceinline__ Pair kept_pair(float x) {
+  Pair q(x);
+  asm volatile("" : "+l"(q.v));
+  return q;
+}
+
+// gelu(z) = max(z, 0) - |z| Phi(-|z|) by Abramowitz and Stegun 7.1.28 (erfc(x) =
+// (1 + a1 x + .. + a6 x^6)^-16, off by at most 3e-7) at x = |z| / sqrt 2, the half in
+// Phi(-|z|) = erfc(x) / 2 taken into the polynomial as its sixteenth root.  One reciprocal a
+// value; 7.1.26 with a reciprocal and an exponential made a product of 32768 x 1024 take 41 us
+// instead of 38.  Past 100 the tail is 0, and inf * 0 is kept out.
 struct Gelu2 {
-  Pair p, g, c4, c3, c2, c1, c0, one;
-  __device__ __forceinline__ static Pair kept(float x) {
-    Pair q(x);
-    asm volatile("" : "+l"(q.v));
-    return q;
+  Pair c6, c5, c4, c3, c2, c1, c0;
+  __device__ static constexpr float factor(int k) {  // 2^(1/16) (-1 / sqrt 2)^k: the polynomial is in -|z|
+    float r = 1.0442737824274138f;
+    for (int i = 0; i < k; ++i) r *= -0.70710678118654752f;
+    return r;
   }
   __device__ __forceinline__ Gelu2()
-      : p(kept(kErfcP)), g(kept(kGaussExp2)), c4(kept(-kErfc4)), c3(kept(-kErfc3)), c2(kept(-kErfc2)),
-        c1(kept(-kErfc1)), c0(kept(-kErfc0)), one(kept(1.f)) {}
-  // -Phi(-|z|) and exp(-z^2 / 2) of B pairs side by side: a pair alone is a chain of some
-  // hundred cycles.
+      : c6(kept_pair(0.0000430638f * factor(6))), c5(kept_pair(0.0002765672f * factor(5))),
+        c4(kept_pair(0.0001520143f * factor(4))), c3(kept_pair(0.0092705272f * factor(3))),
+        c2(kept_pair(0.0422820123f * factor(2))), c1(kept_pair(0.0705230784f * factor(1))), c0(kept_pair(factor(0))) {}
   template <int B>
-  __device__ __forceinline__ void tail(const float* v, Pair (&az)[B], Pair (&q)[B], Pair (&e)[B]) const {
-    Pair t[B];
+  __device__ __forceinline__ void apply(float* v) const {
+    Pair z[B], q[B];  // z: -|z|
+#pragma unroll
+    for (int i = 0; i < B; ++i) z[i] = Pair(fmaxf(-fabsf(v[2 * i]), -100.f), fmaxf(-fabsf(v[2 * i + 1]), -100.f));
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], c6, c5);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c4);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c3);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c2);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c1);
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      float d0, d1;
+      fma2(z[i], q[i], c0).get(d0, d1);
+      q[i] = Pair(rcp_approx(d0), rcp_approx(d1));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < B; ++i) q[i] = mul2(q[i], q[i]);
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+      fma2(z[i], q[i], Pair(max_keep_nan(v[2 * i], 0.f), max_keep_nan(v[2 * i + 1], 0.f))).get(v[2 * i], v[2 * i + 1]);
+  }
+};
+
+// gelu'(z) = Phi(z) + z phi(z).  phi's exponential is needed here, and 7.1.26 of the same
+// book shares it: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by at most
+// 1.5e-7.
+struct GeluSlope2 {
+  static constexpr float kP = 0.3275911f * 0.70710678118654752f, k1 = 0.5f * 0.254829592f, k2 = 0.5f * -0.284496736f,
+                         k3 = 0.5f * 1.421413741f, k4 = 0.5f * -1.453152027f, k5 = 0.5f * 1.061405429f,
+                         kGauss = -0.5f * 1.4426950408889634f;  // exp(-z^2 / 2) = 2^(this z^2)
+  Pair p, g, c5, c4, c3, c2, c1, one;
+  __device__ __forceinline__ GeluSlope2()
+      : p(kept_pair(kP)), g(kept_pair(kGauss)), c5(kept_pair(-k5)), c4(kept_pair(-k4)), c3(kept_pair(-k3)),
+        c2(kept_pair(-k2)), c1(kept_pair(-k1)), one(kept_pair(1.f)) {}
+  template <int B>
+  __device__ __forceinline__ void apply(float* v) const {
+    Pair az[B], t[B], q[B], e[B];  // q: -Phi(-|z|), e: exp(-z^2 / 2)
 #pragma unroll
     for (int i = 0; i < B; ++i) {
       az[i] = Pair(fminf(fabsf(v[2 * i]), 100.f), fminf(fabsf(v[2 * i + 1]), 100.f));
@@ -59,32 +105,18 @@ struct Gelu2 {
       e[i] = Pair(exp2_approx(x0), exp2_approx(x1));
     }
 #pragma unroll
-    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], c4, c3);
+    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], c5, c4);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c3);
 #pragma unroll
     for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c2);
 #pragma unroll
     for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c1);
 #pragma unroll
-    for (int i = 0; i < B; ++i) q[i] = fma2(t[i], q[i], c0);
-#pragma unroll
     for (int i = 0; i < B; ++i) q[i] = mul2(mul2(q[i], t[i]), e[i]);
-  }
-  template <int B>
-  __device__ __forceinline__ void apply(float* v) const {
-    Pair az[B], q[B], e[B];
-    tail(v, az, q, e);
-#pragma unroll
-    for (int i = 0; i < B; ++i)
-      fma2(az[i], q[i], Pair(max_keep_nan(v[2 * i], 0.f), max_keep_nan(v[2 * i + 1], 0.f))).get(v[2 * i], v[2 * i + 1]);
-  }
-  // Phi(z) + z phi(z)
-  template <int B>
-  __device__ __forceinline__ void slope(float* v) const {
-    Pair az[B], q[B], e[B];
-    tail(v, az, q, e);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
-      float h0, h1, x0, x1, s0, s1;  // h: -Phi(-|z|);  x: |z| phi(z)
+      float h0, h1, x0, x1, s0, s1;  // x: |z| phi(z)
       q[i].get(h0, h1);
       mul2(mul2(az[i], e[i]), Pair(0.3989422804014327f)).get(x0, x1);
       s0 = v[2 * i] < 0.f ? -(h0 + x0) : 1.f + (h0 + x0);
@@ -115,7 +147,7 @@ template <int ACT, typename T>
 __device__ __forceinline__ float activation_slope(float z) {
   constexpr bool FAST = sizeof(T) == 2;
   if constexpr (ACT == kActGelu) {
-    static_assert(!FAST, "Gelu2 is the 16-bit form");
+    static_assert(!FAST, "GeluSlope2 is the 16-bit form");
     return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
   } else if constexpr (ACT == kActRelu) {
     return z > 0.f ? 1.f : 0.f;
@@ -144,8 +176,8 @@ __device__ __forceinline__ void times_slope(float* z, float* g) {
   if constexpr (ACT == kActNone) {
     return;
   } else if constexpr (ACT == kActGelu && sizeof(T) == 2) {
-    const Gelu2 gelu;
-    gelu.slope<N / 2>(z);
+    const GeluSlope2 gelu;
+    gelu.apply<N / 2>(z);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = activation_slope<ACT, T>(z[j]);
