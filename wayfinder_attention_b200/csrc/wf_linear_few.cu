@@ -70,24 +70,30 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_mma_kernel(LinearParam
   const bool live0 = n0 + r < p.N, live1 = n0 + r + 8 < p.N;
   float d[TILES][4] = {};
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  for (int64_t k0 = (int64_t)part * 32 * kAhead; k0 < p.K; k0 += (int64_t)parts * 32 * kAhead) {
-    uint4 a[kAhead][2], b[kAhead][TILES];
+  // kAhead steps of 32 of the depth are under way: a step's registers take the loads of the
+  // same step of the part's next piece as soon as the instructions have read them
+  uint4 a[kAhead][2], b[kAhead][TILES];
+  const int64_t stride = (int64_t)parts * 32 * kAhead;
+  auto load = [&](int i, int64_t k) {  // p.K is a multiple of 8: a piece is there or not
+    const bool there = k < p.K;
+    a[i][0] = there && live0 ? ldg16(w + k) : zero;
+    a[i][1] = there && live1 ? ldg16(w + 8 * p.w_stride + k) : zero;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) b[i][t] = there && r + 8 * t < M ? ldg16(x + 8 * t * p.x_stride + k) : zero;
+  };
+  int64_t k = (int64_t)part * 32 * kAhead + k_lane;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(i, k + 32 * i);
+  for (; k - k_lane < p.K; k += stride) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int64_t k = k0 + 32 * i + k_lane;  // p.K is a multiple of 8: a piece is there or not
-      const bool there = k < p.K;
-      a[i][0] = there && live0 ? ldg16(w + k) : zero;
-      a[i][1] = there && live1 ? ldg16(w + 8 * p.w_stride + k) : zero;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) b[i][t] = there && r + 8 * t < M ? ldg16(x + 8 * t * p.x_stride + k) : zero;
-    }
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
         mma_16x8x16<T>(d[t], a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b[i][t].x, b[i][t].y);
         mma_16x8x16<T>(d[t], a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b[i][t].z, b[i][t].w);
       }
+      load(i, k + stride + 32 * i);
+    }
   }
 #pragma unroll
   for (int t = 0; t < TILES; ++t)
@@ -240,7 +246,7 @@ int launch(const LinearParams& p, int dtype, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
     if (takes_mma(p, dtype)) {
       const int64_t groups = (p.N + kMmaCols - 1) / kMmaCols;
-      const int parts = parts_of(groups, p.K, 32 * kAhead);
+      const int parts = parts_of(groups, p.K, 128);
       const unsigned grid = (unsigned)((groups * parts + kWarps - 1) / kWarps);
       return (int)launch_pdl(p.M <= 8 ? linear_few_mma_kernel<T, 1> : linear_few_mma_kernel<T, 2>, dim3(grid),
                              dim3(32 * kWarps), 0, stream, p, parts);
