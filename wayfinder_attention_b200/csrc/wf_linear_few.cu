@@ -14,6 +14,11 @@
 // read shared memory; staging W there would add a pass over what is used once.)
 // Other rows, M <= 8: fused multiply-adds, 8 columns a warp (4 from three rows on); the sums
 // of a lane are halved lane by lane (62 exchanges for 64 sums, not 320).
+//
+// 8 x 4096 x 4096 takes 8.6 us in fp16 (33.5 MB at 3.9 TB/s; 8192 x 8192 4.9 TB/s) and 28 us
+// in fp32.  The next step's pieces of W are asked for before a step is computed (10.1 and 40 us
+// without), and two blocks fit an SM (fp32's 8 rows then spill some registers: 40 us at one
+// block, 62 us at three).
 #include "wf_activation.cuh"
 #include "wf_linear_few.h"
 #include "wf_rowio.cuh"
@@ -135,7 +140,7 @@ __device__ __forceinline__ void halve(float* v, int lane) {
 
 // VEC elements a lane and load; MB >= M rows; `parts` warps share a group of columns.
 template <typename T, int VEC, int MB, int kCols>
-__global__ void __launch_bounds__(32 * kWarps) linear_few_kernel(LinearParams p, int parts) {
+__global__ void __launch_bounds__(32 * kWarps, 2) linear_few_kernel(LinearParams p, int parts) {
   constexpr int SUMS = MB * kCols;
   __shared__ float sums[kWarps][SUMS];
   pdl_wait();
@@ -148,37 +153,39 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_kernel(LinearParams p,
   float acc[SUMS];
 #pragma unroll
   for (int i = 0; i < SUMS; ++i) acc[i] = 0.f;
-  // whole vectors of the depth first, then its end by elements
-  const int64_t whole = p.K / VEC * VEC;
-  auto multiply = [&](auto vec, int64_t k) {
-    constexpr int V = decltype(vec)::value;
-    RawVec<T, V> rw[kCols], rx[MB];
+  // W's vectors of a step of the depth; x's come from the caches
+  auto fetch = [&](auto& rw, int64_t k) {
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
       if (n0 + c < p.N) rw[c].load(w + (n0 + c) * p.w_stride + k);
       else rw[c].clear();
     }
+  };
+  auto multiply = [&](auto& rw, int64_t k, auto refill) {
+    constexpr int V = sizeof(rw[0]) / sizeof(T);
+    float fw[kCols][V];
+    RawVec<T, V> rx[MB];
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
       if (m < M) rx[m].load(x + m * p.x_stride + k);
       else rx[m].clear();
     }
-    float fx[MB][V];
 #pragma unroll
-    for (int m = 0; m < MB; ++m) rx[m].unpack(fx[m]);
+    for (int c = 0; c < kCols; ++c) rw[c].unpack(fw[c]);
+    refill();
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-      float fw[V];
-      rw[c].unpack(fw);
+    for (int m = 0; m < MB; ++m) {
+      float fx[V];
+      rx[m].unpack(fx);
 #pragma unroll
-      for (int m = 0; m < MB; ++m) {
+      for (int c = 0; c < kCols; ++c) {
         float& a = acc[m * kCols + c];
         if constexpr (V == 1) {
-          a = fmaf(fw[0], fx[m][0], a);
+          a = fmaf(fw[c][0], fx[0], a);
         } else {
           Pair q(a, 0.f);
 #pragma unroll
-          for (int j = 0; j < V; j += 2) q = fma2(Pair(fw[j], fw[j + 1]), Pair(fx[m][j], fx[m][j + 1]), q);
+          for (int j = 0; j < V; j += 2) q = fma2(Pair(fw[c][j], fw[c][j + 1]), Pair(fx[j], fx[j + 1]), q);
           float lo, hi;
           q.get(lo, hi);
           a = lo + hi;
@@ -186,10 +193,30 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_kernel(LinearParams p,
       }
     }
   };
+  // whole vectors of the depth first, kSteps of them on their way, then its end by elements
+  const int64_t whole = p.K / VEC * VEC, step = (int64_t)parts * 32 * VEC;
   if (n0 < p.N) {
-    for (int64_t k = (int64_t)(part * 32 + lane) * VEC; k < whole; k += (int64_t)parts * 32 * VEC)
-      multiply(std::integral_constant<int, VEC>{}, k);
-    if (part == parts - 1 && whole + lane < p.K) multiply(std::integral_constant<int, 1>{}, whole + lane);
+    constexpr int kSteps = MB == 4 ? 2 : 1;
+    RawVec<T, VEC> rw[kSteps][kCols];
+    int64_t k = (int64_t)(part * 32 + lane) * VEC;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      if (k + i * step < whole) fetch(rw[i], k + i * step);
+    while (k < whole) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i, k += step) {
+        if (k >= whole) break;
+        multiply(rw[i], k, [&] {
+          if (k + kSteps * step < whole) fetch(rw[i], k + kSteps * step);
+        });
+      }
+    }
+    const int64_t last = whole + lane;
+    if (part == parts - 1 && last < p.K) {
+      RawVec<T, 1> one[kCols];
+      fetch(one, last);
+      multiply(one, last, [] {});
+    }
   }
   halve<SUMS, 16>(acc, lane);
   if constexpr (SUMS >= 32) {
