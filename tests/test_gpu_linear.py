@@ -186,6 +186,24 @@ def test_empty_and_special_values(cuda_device):
                 assert torch.equal(fused_linear(-big, w1, activation=act), fused_linear(-big, w1))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("M,N,K", [(1, 257, 130), (5, 64, 512), (61, 96, 64), (300, 520, 200), (2047, 24, 72)])
+def test_small_gradients_are_rounded_once(M, N, K, act, dtype, cuda_device):
+    """dz keeps the bits that its type has no room for.  What is left beside the gradients' own
+    rounding is z's (an eleven-bit one: at most 0.4 of it after the slope's derivative, so
+    sqrt(1 + 0.16) = 1.08 for fp16); with dz rounded once more it would be sqrt 2."""
+    from wayfinder_attention_b200 import fused_linear
+
+    x, w, b, _, dy = _inputs(M, N, K, dtype, act, True, False, seed=3)
+    leaves = [t.to(cuda_device).requires_grad_() for t in (x, w)]
+    y = fused_linear(leaves[0], leaves[1], b.to(cuda_device), activation=act)
+    dz = dy.double() * _act(act, x.double() @ w.double().T + b.double())[1]
+    for got, want in zip(torch.autograd.grad(y, leaves, dy.to(cuda_device)), (dz @ w.double(), dz.T @ x.double())):
+        once = (want.to(dtype).double() - want).norm()
+        assert (got.cpu().double() - want).norm() <= 1.15 * once
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_gradients_against_differences(act, cuda_device):
     """Central differences of the operator itself along a random direction, fp32.

@@ -59,6 +59,7 @@ constexpr int kMaxSplits = 32;
 
 struct GemmParams {
   int M, N, tiles_n, units, splits, k_blocks;
+  int turn_blocks;  // of k_blocks: past them the depth is walked again, with a's second piece
   bool a_mn, b_mn;
   bool y_tma, residual_tma;  // y, the residual start and step on 16 bytes (z always does)
   bool bias_vec;                 // so does the bias
@@ -299,22 +300,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint64_t* bar = &full[r.stage];
             if (rank == 0) mbar_arrive_expect_tx(bar, CG * L::STAGE);
             const uint32_t on = CG == 2 ? map_peer(bar, 0) : 0;
-            auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
-              if constexpr (CG == 2) tma_load_3d_pair(dst, map, on, x, y, piece);
-              else tma_load_3d(dst, map, bar, x, y, piece);
+            auto load = [&](void* dst, const CUtensorMap* map, int x, int y, int layer) {
+              if constexpr (CG == 2) tma_load_3d_pair(dst, map, on, x, y, layer);
+              else tma_load_3d(dst, map, bar, x, y, layer);
             };
+            const int turn = !PIECES && kb >= p.turn_blocks ? 1 : 0, k = (kb - turn * p.turn_blocks) * kBK;
             if (p.a_mn) {
 #pragma unroll
-              for (int i = 0; i < kBM / 64; ++i) load(st + i * kBK * 128, &amap, am + 64 * i, kb * kBK);
+              for (int i = 0; i < kBM / 64; ++i) load(st + i * kBK * 128, &amap, am + 64 * i, k, piece + turn);
             } else {
-              load(st, &amap, kb * kBK, am);
+              load(st, &amap, k, am, piece + turn);
             }
             st += L::A_BYTES;
             if (p.b_mn) {
 #pragma unroll
-              for (int i = 0; i < BN / CG / 64; ++i) load(st + i * kBK * 128, &bmap, bn + 64 * i, kb * kBK);
+              for (int i = 0; i < BN / CG / 64; ++i) load(st + i * kBK * 128, &bmap, bn + 64 * i, k, piece);
             } else {
-              load(st, &bmap, kb * kBK, bn);
+              load(st, &bmap, k, bn, piece);
             }
             ++issued;
             r.next<L::STAGES>();
@@ -639,14 +641,14 @@ struct Plan {
   Shape shape;
   int tiles_n, tiles, splits, k_blocks;
 };
-Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces) {
+Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces, int turns) {
   Plan best{};
   double least = 0;
   for (const Shape& s : kShapes) {
     if (pieces > 1 && !s.cycles3) continue;
     Plan p{};
     p.shape = s;
-    p.k_blocks = (int)((K + kBK - 1) / kBK);
+    p.k_blocks = (int)((K + kBK - 1) / kBK) * turns;
     const int64_t tn = (N + s.bn - 1) / s.bn, tm = (M + kBM * s.cg - 1) / (kBM * s.cg);
     p.tiles_n = (int)tn;
     p.tiles = (int)(tn * tm);
@@ -673,7 +675,7 @@ template <typename T, int BN, int CG, bool PIECES>
 int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, cudaStream_t stream) {
   using L = Layout<T, BN, CG, PIECES>;
   CUtensorMap amap, bmap, ymap{}, zmap{}, rmap{};
-  if (!make_map(&amap, g.a, g.pieces, g.op_dtype, kBM) ||
+  if (!make_map(&amap, g.a, g.pieces * g.turns, g.op_dtype, kBM) ||
       !make_map(&bmap, g.b, g.pieces, g.op_dtype, BN / CG))
     return -1;
   GemmParams p{};
@@ -683,6 +685,7 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan,
   p.splits = plan.splits;
   p.units = plan.tiles * plan.splits;
   p.k_blocks = plan.k_blocks;
+  p.turn_blocks = plan.k_blocks / g.turns;
   p.a_mn = g.a.mn_major;
   p.b_mn = g.b.mn_major;
   p.out = out;
@@ -738,7 +741,7 @@ int launch_shape(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan
 template <typename T>
 int launch_type(const GemmProblem& g, cudaStream_t stream) {
   constexpr bool PIECES = std::is_same<T, float>::value;
-  const Plan plan = plan_of(g.M, g.N, g.K, g.pieces);
+  const Plan plan = plan_of(g.M, g.N, g.K, g.pieces, g.turns);
   if (plan.splits == 1) return launch_shape<T, PIECES>(g, g.out, plan, stream);
   GemmEpilogue parts{};
   parts.y = g.ws;
@@ -751,9 +754,9 @@ int launch_type(const GemmProblem& g, cudaStream_t stream) {
 
 }  // namespace
 
-size_t gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int pieces) {
+size_t gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int pieces, int turns) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan p = plan_of(M, N, K, pieces);
+  const Plan p = plan_of(M, N, K, pieces, turns);
   return p.splits > 1 ? (size_t)p.splits * M * round8(N) * sizeof(float) : 0;
 }
 

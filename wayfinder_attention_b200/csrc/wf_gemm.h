@@ -29,14 +29,15 @@ struct GemmProblem {
   GemmOperand a, b;
   int64_t M, N, K;
   int pieces;       // 1, or 3 for fp32
+  int turns;        // 2 where a 16-bit a is the sum of two pieces (then pieces is 1), else 1
   int op_dtype;     // kBF16 or kF16
   int out_dtype;
   GemmEpilogue out;
-  void* ws;         // gemm_workspace_bytes(M, N, K, pieces)
+  void* ws;         // gemm_workspace_bytes(M, N, K, pieces, turns)
   int32_t* status;
 };
 
-size_t gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int pieces);
+size_t gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int pieces, int turns = 1);
 int launch_gemm(const GemmProblem& p, cudaStream_t stream);
 
 }  // namespace wf

@@ -61,6 +61,15 @@ __device__ __forceinline__ void store_operand(void* out, int64_t at, int64_t pie
     }
   } else {
     store_vec<T, 8>(static_cast<T*>(out) + at, f);
+    if (piece) {  // what that rounding leaves, where the operand has a second piece
+      float left[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float r = to_f32(from_f32<T>(f[j]));
+        left[j] = isfinite(r) ? f[j] - r : 0.f;
+      }
+      store_vec<T, 8>(static_cast<T*>(out) + piece + at, left);
+    }
   }
 }
 
@@ -187,18 +196,18 @@ bool on_16_bytes(const void* p, int64_t stride) {
 }
 
 // A (rows, cols) matrix as the product reads it: itself, or laid out at *ws, which moves on.
-size_t operand_bytes(int64_t rows, int64_t cols, int dtype) {
-  return round256((size_t)rows * round8(cols) * 2 * (dtype == kF32 ? 3 : 1));
+size_t operand_bytes(int64_t rows, int64_t cols, int dtype, int turns = 1) {
+  return round256((size_t)rows * round8(cols) * 2 * (dtype == kF32 ? 3 : turns));
 }
 template <typename T>
-GemmOperand blank_operand(int64_t rows, int64_t cols, int dtype, unsigned char** ws) {
+GemmOperand blank_operand(int64_t rows, int64_t cols, int dtype, unsigned char** ws, int turns = 1) {
   GemmOperand o{};
   o.ptr = *ws;
   o.rows = rows;
   o.cols = cols;
   o.pitch = round8(cols);
-  o.piece_stride = rows * o.pitch;
-  *ws += operand_bytes(rows, cols, dtype);
+  o.piece_stride = dtype == kF32 || turns > 1 ? rows * o.pitch : 0;
+  *ws += operand_bytes(rows, cols, dtype, turns);
   return o;
 }
 // Two matrices as operands, either of which may be missing (no pointer); what has to be laid
@@ -236,6 +245,7 @@ GemmProblem problem(const GemmOperand& a, const GemmOperand& b, int64_t M, int64
   g.N = N;
   g.K = K;
   g.pieces = kPieces<T>;
+  g.turns = 1;
   g.op_dtype = dtype == kF16 ? kF16 : kBF16;
   g.out_dtype = dtype;
   g.ws = ws;
@@ -263,6 +273,17 @@ cudaError_t launch_dz(const LinearBwdParams& p, const GemmOperand& o, bool write
                     p.M, p.N, partials);
 }
 
+// Pieces of a 16-bit dz.  gelu's and silu's has more bits than its type, and rounding it
+// leaves dx and dW with 1.4 times the error of their own rounding (more by chance where they
+// have few elements).  Small products, whose passes wait for the host and for launches, take
+// what is left as a second piece and are exact but for their own rounding; from 2^30
+// multiplications on the second walk would cost time (8192 x 4096 x 1024: 218 us of kernels
+// with one piece, about 330 with two).
+int dz_turns(int64_t M, int64_t N, int64_t K, int dtype, int act) {
+  const bool rounded = dtype != kF32 && (act == kActGelu || act == kActSilu);
+  return rounded && (double)M * N * K <= (double)(1 << 30) ? 2 : 1;
+}
+
 template <typename T>
 int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
   if (p.M == 0) {  // sums over no rows
@@ -275,7 +296,8 @@ int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
   const bool products = p.dx || p.dw;
   const bool direct = p.act == kActNone && dtype != kF32 && on_16_bytes<T>(p.dy, p.dy_stride);
   GemmOperand dz{p.dy, p.M, p.N, p.dy_stride, 0, false};
-  if (products && !direct) dz = blank_operand<T>(p.M, p.N, dtype, &ws);
+  const int turns = dz_turns(p.M, p.N, p.K, dtype, p.act);
+  if (products && !direct) dz = blank_operand<T>(p.M, p.N, dtype, &ws, turns);
   float* partials = nullptr;
   if (p.db) {
     partials = reinterpret_cast<float*>(ws);
@@ -301,6 +323,7 @@ int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
   if (p.dx) {
     o[0].mn_major = true;  // its columns are dx's, its rows the depth
     GemmProblem g = problem<T>(dz, o[0], p.M, p.K, p.N, dtype, ws, p.status);
+    g.turns = turns;
     g.out.y = p.dx;
     g.out.y_stride = p.K;
     if (int rc = launch_gemm(g, stream)) return rc;
@@ -308,6 +331,7 @@ int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
   if (p.dw) {
     dz.mn_major = o[1].mn_major = true;  // the rows of both are the depth
     GemmProblem g = problem<T>(dz, o[1], p.N, p.K, p.M, dtype, ws, p.status);
+    g.turns = turns;
     g.out.y = p.dw;
     g.out.y_stride = p.K;
     if (int rc = launch_gemm(g, stream)) return rc;
@@ -326,11 +350,12 @@ size_t linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x
 size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int act, bool x_direct,
                                        bool w_direct, bool dy_direct) {
   const int pieces = dtype == kF32 ? 3 : 1;
-  const size_t dz = act == kActNone && pieces == 1 && dy_direct ? 0 : operand_bytes(M, N, dtype);
+  const int turns = dz_turns(M, N, K, dtype, act);
+  const size_t dz = act == kActNone && pieces == 1 && dy_direct ? 0 : operand_bytes(M, N, dtype, turns);
   const size_t sums = round256((size_t)row_shares(M, N) * N * sizeof(float));
   const size_t laid_out = (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) +
                           (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype));
-  const size_t dx = gemm_workspace_bytes(M, K, N, pieces), dw = gemm_workspace_bytes(N, K, M, pieces);
+  const size_t dx = gemm_workspace_bytes(M, K, N, pieces, turns), dw = gemm_workspace_bytes(N, K, M, pieces, turns);
   return dz + sums + laid_out + std::max(dx, dw);  // the products' parts, one after the other
 }
 
