@@ -5,8 +5,8 @@
 //
 // act: none, gelu (z Phi(z), Phi by erf), relu, silu (z sigmoid(z)).  Products and sums
 // are fp32; y is rounded once.  The backward reads z as the forward kept it (fp16 for both
-// 16-bit types), and rounds dz to the activations' type before the two products, as
-// operands of that type are what the products take; db sums the unrounded values.
+// 16-bit types), and takes dz in the activations' type to the two products, in one piece or
+// (small products, see dz_turns) two; db sums the unrounded values.
 //
 // The product reads 16-bit matrices whose rows start on 16 bytes.  Others are laid out in
 // the workspace first: 16-bit rows of any width or offset are copied to such rows, and an
