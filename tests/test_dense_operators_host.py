@@ -107,3 +107,24 @@ def test_abi_validates_before_launch():
     assert logprobs(rows=2 ** 31 - 1, vocab=1 << 20) == _lib.WF_ERR_UNSUPPORTED
     assert logprobs(rows=0) == _lib.WF_OK
     assert lib.wf_max_top_tokens() == 32
+
+
+def test_kept_pre_activations_start_on_16_bytes():
+    lib = _lib.load_library()
+    p, off = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
+    bf16 = 0
+    n = lib.wf_linear_backward_workspace_bytes(4, 8, 8, bf16, 1, 1, 1, 1)
+    assert lib.wf_linear(p, p, None, None, bf16, 4, 8, 8, 8, 8, 0, 1, off, p, None, 0, None, None) == \
+        _lib.WF_ERR_INVALID_ARGUMENT and b"z must be 16-byte aligned" in lib.wf_last_error()
+    assert lib.wf_linear_backward(p, p, off, p, bf16, 4, 8, 8, 8, 8, 8, 1, p, p, p, p, n, None, None) == \
+        _lib.WF_ERR_INVALID_ARGUMENT and b"z must be 16-byte aligned" in lib.wf_last_error()
+
+
+def test_small_rounded_gradients_take_two_pieces_of_workspace():
+    size = _lib.load_library().wf_linear_backward_workspace_bytes
+    bf16, none, gelu, relu = 0, 0, 1, 2
+    M, N, K = 1024, 1024, 1024  # 2^30 multiplications: the last size with two pieces
+    once = 2 * M * N
+    assert size(M, N, K, bf16, relu, 1, 1, 1) - size(M, N, K, bf16, none, 1, 1, 1) == once
+    assert size(M, N, K, bf16, gelu, 1, 1, 1) >= size(M, N, K, bf16, relu, 1, 1, 1) + once
+    assert size(M, N, 2 * K, bf16, gelu, 1, 1, 1) == size(M, N, 2 * K, bf16, relu, 1, 1, 1)
