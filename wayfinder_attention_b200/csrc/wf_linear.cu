@@ -277,8 +277,8 @@ cudaError_t launch_dz(const LinearBwdParams& p, const GemmOperand& o, bool write
 // leaves dx and dW with 1.4 times the error of their own rounding (more by chance where they
 // have few elements).  Small products, whose passes wait for the host and for launches, take
 // what is left as a second piece and are exact but for their own rounding; from 2^30
-// multiplications on the second walk would cost time (8192 x 4096 x 1024: 218 us of kernels
-// with one piece, about 330 with two).
+// multiplications on the second walk would cost time (8192 x 4096 x 1024: the two products
+// take 111 of 222 us with one piece, and would take twice that).
 int dz_turns(int64_t M, int64_t N, int64_t K, int dtype, int act) {
   const bool rounded = dtype != kF32 && (act == kActGelu || act == kActSilu);
   return rounded && (double)M * N * K <= (double)(1 << 30) ? 2 : 1;
