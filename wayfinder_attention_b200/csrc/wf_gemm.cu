@@ -434,10 +434,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     };
-    // z, activation, residual and y of one slice; the buffers take turns
+    // z, activation, residual and y of one slice; the buffers take turns.  A buffer may be
+    // written again once the copy engine has read what it held: where every use is a TMA store,
+    // that is the last but one group.  y's element stores make no group, so z's store of the
+    // slice before, from the same buffer, is then the newest one and has to be waited for.
     auto out = [&](float* v, int m, int n, int layer) {
       if (o.z) {
-        if (lane == 0) bulk_wait_read<1>();
+        if (lane == 0) {
+          if (p.y_tma) bulk_wait_read<1>();
+          else bulk_wait_read<0>();
+        }
         __syncwarp();
         float kept[SC];
 #pragma unroll
