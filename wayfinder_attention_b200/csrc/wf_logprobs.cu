@@ -398,6 +398,7 @@ __device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* keys, int c
 // Long rows: one row a cluster of 1 to 8 blocks.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams p) {
+  if (p.cluster > 1) cluster_arrive_started();
   pdl_wait();
   constexpr int V = Vec16<T>::N;
   __shared__ Sums warp_sums[kWarps];
@@ -486,6 +487,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams 
   }
   if (warp == 0) a = warp_join(lane < kWarps ? warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f});
   if (parts > 1) {
+    cluster_wait_started();  // the first block has started: its `sums` and `best` can be written
     if (warp == 0 && part > 0) {
       if (lane == 0) {
         const uint32_t d = map_peer(&sums[part], 0);
