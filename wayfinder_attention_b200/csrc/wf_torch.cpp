@@ -90,6 +90,10 @@ Tensor rows_of(const Tensor& t) {
   if ((r.stride(1) != 1 && r.size(1) > 1) || (r.stride(0) < r.size(1) && r.size(0) > 1)) r = r.contiguous();
   return r;
 }
+// What a node saves for rows_of(t): t itself where the rows are a view of it (a view made below the
+// AutoDispatchBelowADInplaceOrView guard has a version of its own, and a change of t before the
+// backward would go unnoticed), else the copy.  The backward takes the rows of it again.
+const Tensor& to_save(const Tensor& t, const Tensor& rows) { return rows.is_alias_of(t) ? t : rows; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool on_16_bytes(const Tensor& rows) {
   return reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 == 0 && rows.stride(0) * rows.element_size() % 16 == 0;
@@ -142,7 +146,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     Tensor z;
     Tensor y = run_linear(x2, w2, contiguous(b), r ? rows_of(*r) : Tensor(), (int)act, shape,
                           act ? &z : nullptr, reinterpret_cast<void*>(status));
-    ctx->save_for_backward({x2, w2, z});
+    ctx->save_for_backward({to_save(x, x2), to_save(w, w2), z});
     ctx->saved_data["bias"] = b.has_value();
     ctx->saved_data["residual"] = r.has_value();
     ctx->saved_data["act"] = act;
@@ -153,7 +157,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once_only();
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &z = saved[2], dy = grads[0];
+    const Tensor x = rows_of(saved[0]), w = rows_of(saved[1]), &z = saved[2], &dy = grads[0];
     const int64_t act = ctx->saved_data["act"].toInt();
     size_t edge = 2;
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
@@ -228,7 +232,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
     const Tensor x2 = rows_of(x), w2 = contiguous(w);
     Tensor stats;
     Tensor y = run_layer_norm(x2, w2, contiguous(b), (at::ScalarType)param, eps, x.sizes(), &stats);
-    ctx->save_for_backward({x2, w2, stats});
+    ctx->save_for_backward({to_save(x, x2), w2, stats});
     ctx->saved_data["weight"] = w.has_value();
     ctx->saved_data["bias"] = b.has_value();
     ctx->saved_data["param"] = param;
@@ -237,7 +241,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once_only();
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2], dy = grads[0];
+    const Tensor x = rows_of(saved[0]), &w = saved[1], &stats = saved[2], &dy = grads[0];
     const auto param = (at::ScalarType)ctx->saved_data["param"].toInt();
     size_t edge = 1;
     const bool need_x = ctx->needs_input_grad(0);
@@ -313,7 +317,7 @@ struct TokenLogprobsFunction : torch::autograd::Function<TokenLogprobsFunction> 
     const Tensor x = rows_of(logits);
     Tensor stats;
     Scored r = run_token_logprobs(x, tokens, top_n, ignore, lead, &stats, reinterpret_cast<void*>(status));
-    ctx->save_for_backward({x, tokens, stats, r.entropy});
+    ctx->save_for_backward({to_save(logits, x), tokens, stats, r.entropy});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["shape"] = logits.sizes().vec();
     ctx->mark_non_differentiable({r.top_logprobs, r.top_tokens});
@@ -325,7 +329,7 @@ struct TokenLogprobsFunction : torch::autograd::Function<TokenLogprobsFunction> 
     variable_list none(6);
     if (!grads[0].defined() && !grads[1].defined()) return none;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &tokens = saved[1], &stats = saved[2], &entropy = saved[3];
+    const Tensor x = rows_of(saved[0]), &tokens = saved[1], &stats = saved[2], &entropy = saved[3];
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor gl = grads[0].defined() ? grads[0].contiguous() : Tensor(),
                  gh = grads[1].defined() ? grads[1].contiguous() : Tensor();
