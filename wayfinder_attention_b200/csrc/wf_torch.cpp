@@ -88,6 +88,8 @@ void check_devices(const Tensor& first, std::initializer_list<const Tensor*> oth
 Tensor rows_of(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
   if ((r.stride(1) != 1 && r.size(1) > 1) || (r.stride(0) < r.size(1) && r.size(0) > 1)) r = r.contiguous();
+  // one row (a transposed column is (1, d) with strides (1, 1)) or none: its stride is never taken
+  if (r.size(0) <= 1 && r.stride(0) < r.size(1)) r = r.as_strided(r.sizes(), {r.size(1), 1});
   return r;
 }
 // What a node saves for rows_of(t): t itself where the rows are a view of it (a view made below the
