@@ -680,6 +680,11 @@ int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 template <typename T, int BN, int CG, bool PIECES>
 int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, cudaStream_t stream) {
   using L = Layout<T, BN, CG, PIECES>;
+  // encoding a tensor map is a driver call: it needs the device's context current in this thread,
+  // which the runtime sees to at a launch, and this may be a thread's first (a backward's)
+  int device = 0;
+  if (cudaError_t e = cudaGetDevice(&device)) return (int)e;
+  if (cudaError_t e = cudaSetDevice(device)) return (int)e;
   CUtensorMap amap, bmap, ymap{}, zmap{}, rmap{};
   if (!make_map(&amap, g.a, g.pieces * g.turns, g.op_dtype, kBM) ||
       !make_map(&bmap, g.b, g.pieces, g.op_dtype, BN / CG))
@@ -710,8 +715,6 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan,
   p.bias_vec = reinterpret_cast<uintptr_t>(out.bias) % 16 == 0;
   auto kern = gemm_kernel<T, BN, CG, PIECES>;
   static std::atomic<uint64_t> allowed{0};  // devices whose limit has been raised for this kernel
-  int device = 0;
-  if (cudaError_t e = cudaGetDevice(&device)) return (int)e;
   if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
     if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem))
       return (int)e;
