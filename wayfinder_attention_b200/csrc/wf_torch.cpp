@@ -104,7 +104,12 @@ Tensor bytes(size_t n, const Tensor& like) {
   return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
 }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+// Whether a node is needed.  A forward-mode dual has its tangent whatever it asks of the backward,
+// and these operators have no formula for it.
 bool wants_grad(std::initializer_list<const Tensor*> all) {
+  for (const Tensor* t : all)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw std::runtime_error("this operator has no forward-mode derivative; got an input with a tangent");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : all)
     if (t->defined() && t->requires_grad()) return true;
