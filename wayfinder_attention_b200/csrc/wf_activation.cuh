@@ -30,29 +30,33 @@ __device__ __forceinline__ Pair kept_pair(float x) {
   return q;
 }
 
-// gelu(z) = max(z, 0) - |z| Phi(-|z|) by Abramowitz and Stegun 7.1.28 (erfc(x) =
-// (1 + a1 x + .. + a6 x^6)^-16, off by at most 3e-7) at x = |z| / sqrt 2, the half in
-// Phi(-|z|) = erfc(x) / 2 taken into the polynomial as its sixteenth root.  One reciprocal a
-// value; 7.1.26 with a reciprocal and an exponential made a product of 32768 x 1024 take 41 us
-// instead of 38.  Past 100 the tail is 0, and inf * 0 is kept out.
+// gelu(z) = max(z, 0) - |z| Phi(-|z|) with log2 Phi(-a) as a polynomial in a: one exponential a
+// value and no reciprocal.  The logarithm is smooth where Phi itself falls by hundreds of
+// binades, so a small error of it is a small RELATIVE error of the tail, which is all of the
+// result where z < 0.  The coefficients are a weighted minimax fit (linear programming over 2300
+// points of [0, 13.4]): a Phi(-a) is off by at most 2^-20 (1 + a), by 2^-14 of itself down to
+// z = -5.8, where fp16 ends, and by 2^-10 beyond, where only bf16 is left.  Half of the
+// logarithm is what is computed, and the exponential taken twice: 2^-126 is passed at a = 13 and
+// bf16 ends at 13.6.  The bound on a keeps inf * 0 out.  (Abramowitz and Stegun 7.1.28, one
+// reciprocal and four squarings, takes as long, 36 us at 32768 x 1024; it is off by 3e-7
+// absolutely and so by 5% of the value at z = -5.  A ninth degree takes 1% longer.)
 struct Gelu2 {
-  Pair c6, c5, c4, c3, c2, c1, c0;
-  __device__ static constexpr float factor(int k) {  // 2^(1/16) (-1 / sqrt 2)^k: the polynomial is in -|z|
-    float r = 1.0442737824274138f;
-    for (int i = 0; i < k; ++i) r *= -0.70710678118654752f;
-    return r;
-  }
+  Pair c8, c7, c6, c5, c4, c3, c2, c1, c0;  // of log2(Phi(-a)) / 2 in -a
   __device__ __forceinline__ Gelu2()
-      : c6(kept_pair(0.0000430638f * factor(6))), c5(kept_pair(0.0002765672f * factor(5))),
-        c4(kept_pair(0.0001520143f * factor(4))), c3(kept_pair(0.0092705272f * factor(3))),
-        c2(kept_pair(0.0422820123f * factor(2))), c1(kept_pair(0.0705230784f * factor(1))), c0(kept_pair(factor(0))) {}
+      : c8(kept_pair(2.07575042e-08f)), c7(kept_pair(1.22331039e-06f)), c6(kept_pair(3.09177485e-05f)),
+        c5(kept_pair(0.000444811274f)), c4(kept_pair(0.00411469117f)), c3(kept_pair(0.0266025458f)),
+        c2(kept_pair(-0.229678065f)), c1(kept_pair(0.575416028f)), c0(kept_pair(-0.500026405f)) {}
   template <int B>
   __device__ __forceinline__ void apply(float* v) const {
     Pair z[B], q[B];  // z: -|z|
 #pragma unroll
-    for (int i = 0; i < B; ++i) z[i] = Pair(fmaxf(-fabsf(v[2 * i]), -100.f), fmaxf(-fabsf(v[2 * i + 1]), -100.f));
+    for (int i = 0; i < B; ++i) z[i] = Pair(fmaxf(-fabsf(v[2 * i]), -14.f), fmaxf(-fabsf(v[2 * i + 1]), -14.f));
 #pragma unroll
-    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], c6, c5);
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], c8, c7);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c6);
+#pragma unroll
+    for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c5);
 #pragma unroll
     for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c4);
 #pragma unroll
@@ -63,23 +67,20 @@ struct Gelu2 {
     for (int i = 0; i < B; ++i) q[i] = fma2(z[i], q[i], c1);
 #pragma unroll
     for (int i = 0; i < B; ++i) {
-      float d0, d1;
-      fma2(z[i], q[i], c0).get(d0, d1);
-      q[i] = Pair(rcp_approx(d0), rcp_approx(d1));
+      float l0, l1;
+      fma2(z[i], q[i], c0).get(l0, l1);
+      q[i] = Pair(exp2_approx(l0), exp2_approx(l1));
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int i = 0; i < B; ++i) q[i] = mul2(q[i], q[i]);
-#pragma unroll
     for (int i = 0; i < B; ++i)
-      fma2(z[i], q[i], Pair(max_keep_nan(v[2 * i], 0.f), max_keep_nan(v[2 * i + 1], 0.f))).get(v[2 * i], v[2 * i + 1]);
+      fma2(mul2(z[i], q[i]), q[i], Pair(max_keep_nan(v[2 * i], 0.f), max_keep_nan(v[2 * i + 1], 0.f)))
+          .get(v[2 * i], v[2 * i + 1]);
   }
 };
 
-// gelu'(z) = Phi(z) + z phi(z).  phi's exponential is needed here, and 7.1.26 of the same
-// book shares it: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by at most
-// 1.5e-7.
+// gelu'(z) = Phi(z) + z phi(z).  phi's exponential is needed here, and Abramowitz and Stegun
+// 7.1.26 shares it: erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), off by at most
+// 1.5e-7, and by 1e-4 of the slope down to z = -6 (z phi(z) is the larger part there).
 struct GeluSlope2 {
   static constexpr float kP = 0.3275911f * 0.70710678118654752f, k1 = 0.5f * 0.254829592f, k2 = 0.5f * -0.284496736f,
                          k3 = 0.5f * 1.421413741f, k4 = 0.5f * -1.453152027f, k5 = 0.5f * 1.061405429f,
@@ -127,13 +128,13 @@ struct GeluSlope2 {
   }
 };
 
-// T: the type of the result.  fp32 takes CUDA's erff and expf and a true division.
+// T: the type of the result.  fp32 takes CUDA's erfcf and expf and a true division.
 template <int ACT, typename T>
 __device__ __forceinline__ float activate(float z) {
   constexpr bool FAST = sizeof(T) == 2;
   if constexpr (ACT == kActGelu) {
     static_assert(!FAST, "Gelu2 is the 16-bit form");
-    return z * 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    return z * 0.5f * erfcf(z * -0.70710678118654752f);  // 1 + erff would cancel where z < 0
   } else if constexpr (ACT == kActRelu) {
     return z < 0.f ? 0.f : z;  // NaN stays
   } else if constexpr (ACT == kActSilu) {
@@ -148,7 +149,7 @@ __device__ __forceinline__ float activation_slope(float z) {
   constexpr bool FAST = sizeof(T) == 2;
   if constexpr (ACT == kActGelu) {
     static_assert(!FAST, "GeluSlope2 is the 16-bit form");
-    return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+    return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), 0.5f * erfcf(z * -0.70710678118654752f));
   } else if constexpr (ACT == kActRelu) {
     return z > 0.f ? 1.f : 0.f;
   } else if constexpr (ACT == kActSilu) {
