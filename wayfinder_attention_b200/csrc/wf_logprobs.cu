@@ -33,7 +33,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.92596299e-8f;  // log2 e and what that leaves of it
 constexpr unsigned kAll = 0xffffffffu;
 
 // NaN if either is
@@ -530,37 +530,88 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogprobParams 
     if (lane < p.top_n) write_top(p, row, lane, lists[0][lane], a, log_s);
 }
 
-// The gradient of a row's elements.
+// 2^(x log2 e - whole - part) 2^64 for two x, to fp32's bits: x log2 e is split into a whole number, which
+// goes into the exponent with `whole`, and the rest to twice fp32's precision (a rounded product
+// would carry 2^-24 of its whole part into the result).  |x| < 2^21; 0 below 2^-190.
+__device__ __forceinline__ Pair exp_up64(Pair x, int whole, float part) {
+  constexpr float kRound = 12582912.f;  // 1.5 2^23: a sum with it is rounded to a whole number
+  const Pair t = fma2(x, Pair(kLog2e), Pair(kRound));
+  const Pair rest = fma2(x, Pair(kLog2eLow), add2(fma2(x, Pair(kLog2e), fma2(t, Pair(-1.f), Pair(kRound))), Pair(-part)));
+  float t0, t1, r0, r1;
+  t.get(t0, t1);
+  rest.get(r0, r1);
+  const int bias = 64 + 127 - whole - (int)__float_as_uint(kRound);
+  auto up = [&](float n) {
+    const int e = (int)__float_as_uint(n) + bias;
+    return __int_as_float(e > 0 ? e << 23 : 0);
+  };
+  return mul2(Pair(exp2_approx(r0), exp2_approx(r1)), Pair(up(t0), up(t1)));
+}
+
+// The gradient of a row's elements, for logits of type T.
+template <typename T>
 struct RowGrad {
-  float m, log_s, gh, gl, base;
+  // 16-bit logits: p = exp((x - m) - log_s).  fp32: p = 2^(x' log2 e - whole - part) with x' = x - m; m is
+  // 0 then, so that x' is exact, and the row's log sum exp is in whole + part to fp32's precision of
+  // `part`; only rows with a maximum past 2^20 subtract it.
+  static constexpr bool kSplit = sizeof(T) == 4;
+  float m, log_s, gh, gl, base, lowest, part;
+  int whole;
   bool none;
   int64_t tok;
   __device__ __forceinline__ RowGrad(const LogprobBwdParams& p, int64_t row)
       : m(p.stats[row]), log_s(p.stats[p.rows + row]), gh(p.dentropy ? p.dentropy[row] : 0.f),
-        gl(p.dlogprob ? p.dlogprob[row] : 0.f), tok(p.tokens[row]) {
+        gl(p.dlogprob ? p.dlogprob[row] : 0.f), lowest(-200.f), tok(p.tokens[row]) {
     if (tok == p.ignore_index) gl = 0.f;
     else if (tok < 0 || tok >= p.vocab) gl = NAN;
     none = m == -INFINITY;
     base = fmaf(gh, p.entropy[row], gl);
+    if constexpr (kSplit) {
+      const bool far = !(fabsf(m) < 1048576.f);
+      const float a = far ? 0.f : m, l = a + log_s, b = l - a;
+      const float left = (a - (l - b)) + (log_s - b);  // a + log_s = l + left exactly
+      const float power = l * kLog2e;
+      whole = __float2int_rn(power);
+      part = (power - (float)whole) + (fmaf(l, kLog2e, -power) + fmaf(l, kLog2eLow, left * kLog2e));
+      lowest = far ? -200.f : m - 200.f;
+      m = far ? m : 0.f;
+      base = fmaf(gh, -l, base);
+    }
   }
   // f[j] is x[c + j] and becomes dx[c + j].  p is computed 2^64 times too large, so that its
   // last bits survive where a gradient multiplies them up again; it is 0 long before
-  // lp = -200, which keeps 0 * inf out.
+  // 200 below the maximum, which keeps 0 * inf out.  16-bit results take the exponential of a product
+  // rounded with the 64 in it (2^-18 of p); fp32 ones exp_up64.
   template <int N>
   __device__ __forceinline__ void apply(float* f, int64_t c) const {
     constexpr float kDown = 5.421010862427522e-20f;  // 2^-64
     if constexpr (N == 1) {
-      const float lp = max_nan(f[0] - m - log_s, -200.f);
-      f[0] = exp2_approx(fmaf(lp, kLog2e, 64.f)) * -fmaf(gh, lp, base) * kDown;
+      float lp, e, other;
+      if constexpr (kSplit) {
+        lp = max_nan(f[0] - m, lowest);
+        exp_up64(Pair(lp, 0.f), whole, part).get(e, other);
+      } else {
+        lp = max_nan(f[0] - m - log_s, lowest);
+        e = exp2_approx(fmaf(lp, kLog2e, 64.f));
+      }
+      f[0] = e * -fmaf(gh, lp, base) * kDown;
     } else {
 #pragma unroll
       for (int j = 0; j < N; j += 2) {
-        float l0, l1, y0, y1;
-        add2(add2(Pair(f[j], f[j + 1]), Pair(-m)), Pair(-log_s)).get(l0, l1);
-        const Pair lp(max_nan(l0, -200.f), max_nan(l1, -200.f));
-        fma2(lp, Pair(kLog2e), Pair(64.f)).get(y0, y1);
+        float l0, l1;
+        Pair d = add2(Pair(f[j], f[j + 1]), Pair(-m)), e;
+        if constexpr (!kSplit) d = add2(d, Pair(-log_s));
+        d.get(l0, l1);
+        const Pair lp(max_nan(l0, lowest), max_nan(l1, lowest));
+        if constexpr (kSplit) {
+          e = exp_up64(lp, whole, part);
+        } else {
+          float y0, y1;
+          fma2(lp, Pair(kLog2e), Pair(64.f)).get(y0, y1);
+          e = Pair(exp2_approx(y0), exp2_approx(y1));
+        }
         const Pair q = fma2(lp, Pair(-gh), Pair(-base));
-        mul2(mul2(Pair(exp2_approx(y0), exp2_approx(y1)), q), Pair(kDown)).get(f[j], f[j + 1]);
+        mul2(mul2(e, q), Pair(kDown)).get(f[j], f[j + 1]);
       }
     }
     if (none) {
@@ -590,7 +641,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_short_kernel
     const int c = (i * LANES + t) * V;
     if (c < p.vocab) raw[i].load(x + c);
   }
-  const RowGrad g(p, row);
+  const RowGrad<T> g(p, row);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * LANES + t) * V;
@@ -621,7 +672,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logpr
     lo = min(blockIdx.x % chunks * share, p.vocab);
     hi = min(lo + share, p.vocab);
   }
-  const RowGrad g(p, row);
+  const RowGrad<T> g(p, row);
   const Span<T> span(x, lo, hi);
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
   for (int64_t c0 = span.head + (int64_t)t * V; c0 < span.tail; c0 += (int64_t)G * V * kBwdVectors) {
