@@ -25,6 +25,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     pre-activations as kept in fp16 (fp32 for fp32) and gives every gradient in x's type.  fp32 inputs
     are multiplied to fp32 accuracy on the tensor cores, as three bf16 pieces each: an
     infinite or NaN input makes its outputs NaN or infinite, not always the same of the two.
+    relu's slope goes by the sign of the pre-activation as its sum came out: one within the
+    sum's own rounding of 0 (2^-22 of its terms' size) may fall on either side.
     """
     act = ACTIVATIONS.get(activation)
     if act is None:
