@@ -23,6 +23,8 @@ forward and backward; ``score`` gives the log probability of each next token wit
 
 from __future__ import annotations
 
+import functools
+import inspect
 from typing import Optional
 
 import torch
@@ -66,14 +68,24 @@ def _norm(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
     return layer_norm(x, ln.weight, ln.bias, ln.eps)
 
 
+@functools.lru_cache(maxsize=None)
+def _names_residual(forward) -> bool:
+    return "residual" in inspect.signature(forward).parameters
+
+
+def _adds_residual(attn: nn.Module) -> bool:
+    """Whether an attention module adds the block's residual itself: its forward names it (**kwargs would drop it)."""
+    return _names_residual(type(attn).forward)
+
+
 class TransformerBlock(nn.Module):
     def __init__(self, d_model: int, n_heads: int, d_ff: int, dropout: float, attention_module: nn.Module,
                  layer_idx: int = 0, fused_layers: bool = False):
         super().__init__()
         self.attn = attention_module
         self.fused_layers = fused_layers
-        if fused_layers:
-            self.attn.fused_linear = True
+        if fused_layers and hasattr(attention_module, "fused_linear"):
+            attention_module.fused_linear = True
         self.layer_idx = layer_idx
         self.ln1 = nn.LayerNorm(d_model)
         self.ln2 = nn.LayerNorm(d_model)
@@ -90,7 +102,11 @@ class TransformerBlock(nn.Module):
     def _forward_fused(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor]) -> torch.Tensor:
         """The same block on ``layer_norm`` and ``fused_linear``; dropout, where it acts, comes between them."""
         up, _, drop_hidden, down, drop_out = self.ff
-        x = self.attn(_norm(self.ln1, x), attn_mask=attn_mask, residual=x)
+        h = _norm(self.ln1, x)
+        if _adds_residual(self.attn):
+            x = self.attn(h, attn_mask=attn_mask, residual=x)
+        else:
+            x = x + self.attn(h, attn_mask=attn_mask)
         h = drop_hidden(project(up, _norm(self.ln2, x), True, activation="gelu"))
         if self.training and drop_out.p > 0.0:
             return x + drop_out(project(down, h, True))
