@@ -33,7 +33,7 @@ import torch.nn.functional as F
 
 from .attention import KeyVectorSparseAttention, LearnedAddressSparseAttention
 from .layer_norm import layer_norm
-from .linear import project
+from .linear import project, runs_as
 from .token_logprobs import TokenLogprobs, token_logprobs
 
 
@@ -64,8 +64,10 @@ class DenseSDPAAttention(nn.Module):
                        residual=residual)
 
 
-def _norm(ln: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
-    return layer_norm(x, ln.weight, ln.bias, ln.eps)
+def _norm(ln: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    if runs_as(ln, nn.LayerNorm) and len(ln.normalized_shape) == 1:
+        return layer_norm(x, ln.weight, ln.bias, ln.eps)
+    return ln(x)
 
 
 @functools.lru_cache(maxsize=None)
@@ -74,8 +76,11 @@ def _names_residual(forward) -> bool:
 
 
 def _adds_residual(attn: nn.Module) -> bool:
-    """Whether an attention module adds the block's residual itself: its forward names it (**kwargs would drop it)."""
-    return _names_residual(type(attn).forward)
+    """Whether an attention module adds the block's residual itself.
+
+    Its forward has to name it (**kwargs would drop it), and hooks have to see what they would see of it.
+    """
+    return _names_residual(type(attn).forward) and runs_as(attn, type(attn))
 
 
 class TransformerBlock(nn.Module):
@@ -100,17 +105,24 @@ class TransformerBlock(nn.Module):
         return x + self.ff(self.ln2(x))
 
     def _forward_fused(self, x: torch.Tensor, attn_mask: Optional[torch.Tensor]) -> torch.Tensor:
-        """The same block on ``layer_norm`` and ``fused_linear``; dropout, where it acts, comes between them."""
-        up, _, drop_hidden, down, drop_out = self.ff
+        """The same block on ``layer_norm`` and ``fused_linear``, where its modules are what they stand for."""
         h = _norm(self.ln1, x)
         if _adds_residual(self.attn):
             x = self.attn(h, attn_mask=attn_mask, residual=x)
         else:
             x = x + self.attn(h, attn_mask=attn_mask)
-        h = drop_hidden(project(up, _norm(self.ln2, x), True, activation="gelu"))
-        if self.training and drop_out.p > 0.0:
-            return x + drop_out(project(down, h, True))
-        return project(down, h, True, residual=x)
+        h = _norm(self.ln2, x)
+        if not (runs_as(self.ff, nn.Sequential) and len(self.ff) == 5):
+            return x + self.ff(h)
+        up, act, drop_hidden, down, drop_out = self.ff
+        if runs_as(act, nn.GELU) and act.approximate == "none":
+            h = project(up, h, True, activation="gelu")
+        else:
+            h = act(project(up, h, True))
+        h = drop_hidden(h)
+        if runs_as(drop_out, nn.Dropout) and not (drop_out.training and drop_out.p > 0.0):
+            return project(down, h, True, residual=x)
+        return x + drop_out(project(down, h, True))
 
 
 class TransformerLM(nn.Module):

@@ -39,10 +39,21 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     return y
 
 
-def project(layer: torch.nn.Linear, x: torch.Tensor, fused: bool, activation: str = "none",
+def runs_as(module: torch.nn.Module, kind: type) -> bool:
+    """Whether calling ``module`` is ``kind``'s own forward and nothing else: no subclass, hook or replaced forward."""
+    return type(module) is kind and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                                         or module._backward_pre_hooks or "forward" in module.__dict__)
+
+
+def project(layer: torch.nn.Module, x: torch.Tensor, fused: bool, activation: str = "none",
             residual: torch.Tensor | None = None) -> torch.Tensor:
-    """An ``nn.Linear`` of a model: through ``fused_linear``, or as PyTorch layers (no activation then)."""
-    if fused:
+    """A linear layer of a model with what follows it: through ``fused_linear``, or as PyTorch layers.
+
+    A layer that is not a plain ``nn.Linear`` (an adapter in its place, a hook on it) is called.
+    """
+    if fused and runs_as(layer, torch.nn.Linear):
         return fused_linear(x, layer.weight, layer.bias, activation=activation, residual=residual)
     y = layer(x)
+    if activation == "gelu":
+        y = torch.nn.functional.gelu(y)
     return y if residual is None else residual + y
