@@ -66,6 +66,9 @@ class DenseSDPAAttention(nn.Module):
 
 def _norm(ln: nn.Module, x: torch.Tensor) -> torch.Tensor:
     if runs_as(ln, nn.LayerNorm) and len(ln.normalized_shape) == 1:
+        if torch.is_autocast_enabled("cuda"):  # norms run in fp32 there
+            weight, bias = (None if p is None else p.float() for p in (ln.weight, ln.bias))
+            return layer_norm(x.float(), weight, bias, ln.eps)
         return layer_norm(x, ln.weight, ln.bias, ln.eps)
     return ln(x)
 

@@ -50,8 +50,15 @@ def project(layer: torch.nn.Module, x: torch.Tensor, fused: bool, activation: st
     """A linear layer of a model with what follows it: through ``fused_linear``, or as PyTorch layers.
 
     A layer that is not a plain ``nn.Linear`` (an adapter in its place, a hook on it) is called.
+    Under autocast the product is taken in its type, as ``nn.Linear``'s is, and the residual
+    is added in the wider of the two.
     """
     if fused and runs_as(layer, torch.nn.Linear):
+        if torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+            bias = None if layer.bias is None else layer.bias.to(dtype)
+            y = fused_linear(x.to(dtype), layer.weight.to(dtype), bias, activation=activation)
+            return y if residual is None else residual + y
         return fused_linear(x, layer.weight, layer.bias, activation=activation, residual=residual)
     y = layer(x)
     if activation == "gelu":
