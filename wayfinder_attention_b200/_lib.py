@@ -280,7 +280,7 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
 
 # ---------------------------------------------------------------- status word
 # Every kernel reports faults it can detect without stopping (an out-of-range
-# attention index: bit 0; a bounded wait that gave up: bit 1, plus a bit naming the
+# attention index or token: bit 0; a bounded wait that gave up: bit 1, plus a bit naming the
 # wait site from bit 4 up) by OR-ing bits into a caller-provided int32 status word.
 # A caller that passes none gets this per-device word.  Its value is copied
 # asynchronously into pinned host memory after a launch — after the first launch,
@@ -345,7 +345,8 @@ _status: dict[int, _DeviceStatus] = {}
 def describe_status(bits: int) -> str:
     parts = []
     if bits & STATUS_INDEX_OUT_OF_RANGE:
-        parts.append("an attention index was out of range (its output row is NaN)")
+        parts.append("an attention index, or a token to score, was out of range (its output row, or log probability, "
+                     "is NaN)")
     if bits & STATUS_WAIT_TIMEOUT:
         parts.append(f"a kernel's bounded wait timed out (wait-site bits 0x{bits >> 4:x}); its results are invalid")
     if not parts:
