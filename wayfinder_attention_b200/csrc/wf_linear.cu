@@ -343,6 +343,7 @@ int launch_bwd(const LinearBwdParams& p, int dtype, cudaStream_t stream) {
 }  // namespace
 
 size_t linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct, bool w_direct) {
+  if (M <= kFewRows) return 0;  // linear_few_takes them, whatever their type and alignment
   const int pieces = dtype == kF32 ? 3 : 1;
   return (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype)) +
          (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) + gemm_workspace_bytes(M, N, K, pieces);

@@ -294,7 +294,7 @@ int launch(const LinearParams& p, int dtype, cudaStream_t stream) {
 
 }  // namespace
 
-bool linear_few_takes(const LinearParams& p, int dtype) { return p.M <= (takes_mma(p, dtype) ? 16 : 8); }
+bool linear_few_takes(const LinearParams& p, int dtype) { return p.M <= (takes_mma(p, dtype) ? 16 : kFewRows); }
 
 int launch_linear_few(const LinearParams& p, int dtype, cudaStream_t stream) {
   if (dtype == kBF16) return launch<__nv_bfloat16>(p, dtype, stream);
