@@ -15,7 +15,7 @@
 // Other rows, M <= 8: fused multiply-adds, 8 columns a warp (4 from three rows on); the sums
 // of a lane are halved lane by lane (62 exchanges for 64 sums, not 320).
 //
-// 8 x 4096 x 4096 takes 8.6 us in fp16 (33.5 MB at 3.9 TB/s; 8192 x 8192 4.9 TB/s) and 28 us
+// 8 x 4096 x 4096 takes 8.3 us in fp16 (33.5 MB at 4.0 TB/s; 8192 x 8192 5.0 TB/s) and 29 us
 // in fp32.  The next step's pieces of W are asked for before a step is computed (10.1 and 40 us
 // without), and two blocks fit an SM (fp32's 8 rows then spill some registers: 40 us at one
 // block, 62 us at three).
