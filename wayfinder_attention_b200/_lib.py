@@ -300,8 +300,9 @@ READBACK_SECONDS = 0.05
 class _DeviceStatus:
     def __init__(self, dev: torch.device):
         self.dev = dev
-        self.word = torch.zeros(1, dtype=torch.int32, device=dev)
-        self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        with torch.inference_mode(False):  # written by every later call, whatever mode the first one runs in
+            self.word = torch.zeros(1, dtype=torch.int32, device=dev)
+            self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
         self.event = torch.cuda.Event()
         self.pending = False
         self.calls = 0
