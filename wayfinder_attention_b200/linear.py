@@ -21,14 +21,15 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     x: (..., d_in); weight: (d_out, d_in); bias: (d_out,) or None; residual: the output's
     shape (..., d_out) or None; all CUDA tensors of one type (bfloat16, float16 or
     float32).  activation: "none", "gelu" (the erf form), "relu" or "silu".
-    Differentiable in x, weight, bias and residual; the backward reads the
-    pre-activations as kept in fp16 (fp32 for fp32) and gives every gradient in x's type; from
-    2^30 multiplications on, the pre-activations' gradient of a 16-bit gelu or silu is rounded to
-    that type before the products, which leaves x's and the weight's gradients with 1.4 times the
-    error of their own rounding.  fp32 inputs are multiplied to fp32 accuracy on the tensor cores, as three bf16 pieces each: an
-    infinite or NaN input makes its outputs NaN or infinite, not always the same of the two.
+    Differentiable in x, weight, bias and residual, every gradient in x's type.  The backward
+    reads the pre-activations as kept in fp16 (fp32 for fp32), which adds 6% to the error of
+    gelu's and silu's fp16 gradients; from 2^30 multiplications on, their own gradient of a
+    16-bit gelu or silu is rounded to the type before the products, which leaves x's and the
+    weight's gradients with 1.4 times the error of their rounding.
     relu's slope goes by the sign of the pre-activation as its sum came out: one within the
     sum's own rounding of 0 (2^-22 of its terms' size) may fall on either side.
+    fp32 inputs are multiplied to fp32 accuracy on the tensor cores, as three bf16 pieces each: an
+    infinite or NaN input makes its outputs NaN or infinite, not always the same of the two.
     """
     act = ACTIVATIONS.get(activation)
     if act is None:
