@@ -465,6 +465,68 @@ WF_API int wf_token_logprobs_backward(const void* logits, int32_t dtype, int64_t
                                       const float* stats, const float* entropy, const float* dlogprob,
                                       const float* dentropy, void* dlogits, void* stream);
 
+/*
+ * The same from hidden rows and a head's weight, without the logits in memory: rows
+ * z = x W^T + bias of which only the running maximum and sums are kept.  fp32 throughout.
+ *
+ *   x        : (rows, d) rows x_row_stride apart;  w : (vocab, d) rows w_row_stride apart
+ *   bias     : (vocab) or NULL; -inf bans a token.  All three of dtype
+ *   tokens, ignore_index, logprob, entropy, stats, status : as wf_token_logprobs; status bit 1
+ *              is OR-ed in if a bounded wait timed out
+ *   workspace: wf_linear_token_logprobs_workspace_bytes() bytes, 256-byte aligned; x_direct /
+ *              w_direct as for wf_linear
+ * A NaN (or +inf) among a row's logits makes its logprob and entropy NaN.
+ */
+WF_API size_t wf_linear_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int32_t dtype,
+                                                       int32_t x_direct, int32_t w_direct);
+WF_API int wf_linear_token_logprobs(const void* x, const void* w, const void* bias, int32_t dtype, int64_t rows,
+                                    int64_t vocab, int64_t d, int64_t x_row_stride, int64_t w_row_stride,
+                                    const int64_t* tokens, int64_t ignore_index, float* logprob, float* entropy,
+                                    float* stats, void* workspace, size_t workspace_bytes, int32_t* status,
+                                    void* stream);
+/* Its backward, from the gradients of logprob and entropy (rows) fp32 (either may be NULL): dx
+ * (rows, d), dw (vocab, d) and dbias (vocab), contiguous, of dtype, each may be NULL.  The
+ * logits are made again, a piece of the vocabulary at a time.  The result does not depend
+ * on scheduling. */
+WF_API size_t wf_linear_token_logprobs_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int32_t dtype,
+                                                                int32_t x_direct, int32_t w_direct);
+WF_API int wf_linear_token_logprobs_backward(const void* x, const void* w, const void* bias, int32_t dtype,
+                                             int64_t rows, int64_t vocab, int64_t d, int64_t x_row_stride,
+                                             int64_t w_row_stride, const int64_t* tokens, int64_t ignore_index,
+                                             const float* stats, const float* entropy, const float* dlogprob,
+                                             const float* dentropy, void* dx, void* dw, void* dbias, void* workspace,
+                                             size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * Token embedding: y_i = scale * weight[tokens_i] + position_weight[p_i], rounded once.  No
+ * counterpart in the reference (two nn.Embedding and an add in models/transformer.py:76-312).
+ *
+ *   tokens          : (n) int64
+ *   weight          : (vocab, d) rows w_row_stride apart
+ *   position_weight : (places, d) rows p_row_stride apart, or NULL: nothing is added
+ *   positions       : (n) int64 p_i, or NULL: p_i = i % seq
+ *   y               : (n, d) contiguous, of dtype as the tables
+ *   status          : optional device int32; a token or position outside its table makes its row
+ *                     NaN and sets bit 0
+ */
+WF_API int wf_token_embedding(const int64_t* tokens, int64_t n, const void* weight, int32_t dtype, int64_t vocab,
+                              int64_t d, int64_t w_row_stride, float scale, const void* position_weight,
+                              int64_t places, int64_t p_row_stride, const int64_t* positions, int64_t seq, void* y,
+                              int32_t* status, void* stream);
+/* The gradient of one of its tables: dweight[v] = scale * the sum of dy's rows whose index is v,
+ * (rows, d) contiguous of dtype, summed in fp32 in a fixed order.
+ *
+ *   index         : (n) int64, or NULL: i % seq (n a multiple of seq)
+ *   dy            : (n, d) rows dy_row_stride apart
+ *   padding_index : the index whose row gets no gradient, or -1.  Nor do indices outside the table
+ *   workspace     : wf_token_embedding_backward_workspace_bytes() bytes, 256-byte aligned */
+WF_API size_t wf_token_embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t d, int32_t dtype,
+                                                          int32_t has_index);
+WF_API int wf_token_embedding_backward(const int64_t* index, int64_t n, int64_t seq, const void* dy, int32_t dtype,
+                                       int64_t rows, int64_t d, int64_t dy_row_stride, int64_t padding_index,
+                                       float scale, void* dweight, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,8 @@ Public API (names and arguments of the reference's ``routing_attention``):
 
 The decoder's other operators, each with its backward: fused_linear (bias,
 activation and residual in the product's epilogue), layer_norm and token_logprobs
-(log probability, entropy and top alternatives of given tokens).
+(log probability, entropy and top alternatives of given tokens); and its two ends,
+token_embedding and linear_token_logprobs (log probabilities without the logits).
 
 The compute runs in ``libwayfinder_sm100.so`` (C ABI: ``include/wayfinder.h``);
 there is no CPU path.  Kernel faults that do not stop a kernel (an out-of-range
@@ -30,7 +31,9 @@ from .causal_topk import causal_topk, causal_topk_available, promote_compute_dty
 from .decoder import DenseSDPAAttention, TransformerBlock, TransformerLM
 from .graphs import CapturedForward
 from .layer_norm import layer_norm
+from .embedding import token_embedding
 from .linear import fused_linear
+from .linear_logprobs import LinearLogprobs, linear_token_logprobs
 from .token_logprobs import TokenLogprobs, token_logprobs
 from .host_pipeline import HostFusedSparseAttention, host_fused_sparse_attention
 from .fused_sparse import (
@@ -57,6 +60,9 @@ __all__ = [
     "layer_norm",
     "token_logprobs",
     "TokenLogprobs",
+    "linear_token_logprobs",
+    "LinearLogprobs",
+    "token_embedding",
     "LearnedAddressModule",
     "LearnedAddressSparseAttention",
     "KeyVectorSparseAttention",

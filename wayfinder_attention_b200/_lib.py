@@ -69,6 +69,13 @@ EXPORTED_SYMBOLS = (
     "wf_max_top_tokens",
     "wf_token_logprobs",
     "wf_token_logprobs_backward",
+    "wf_linear_token_logprobs",
+    "wf_linear_token_logprobs_workspace_bytes",
+    "wf_linear_token_logprobs_backward",
+    "wf_linear_token_logprobs_backward_workspace_bytes",
+    "wf_token_embedding",
+    "wf_token_embedding_backward",
+    "wf_token_embedding_backward_workspace_bytes",
 )
 
 _DTYPE_CODES = {
@@ -188,6 +195,17 @@ def _declare(lib: ctypes.CDLL) -> None:
          [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
         ("wf_token_logprobs_backward", ctypes.c_int,
          [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+        ("wf_linear_token_logprobs_workspace_bytes", sz, [_i64] * 3 + [_i32] * 3),
+        ("wf_linear_token_logprobs", ctypes.c_int,
+         [_vp] * 3 + [_i32] + [_i64] * 5 + [_vp, _i64, _vp, _vp, _vp, _vp, sz, _vp, _vp]),
+        ("wf_linear_token_logprobs_backward_workspace_bytes", sz, [_i64] * 3 + [_i32] * 3),
+        ("wf_linear_token_logprobs_backward", ctypes.c_int,
+         [_vp] * 3 + [_i32] + [_i64] * 5 + [_vp, _i64] + [_vp] * 8 + [sz, _vp, _vp]),
+        ("wf_token_embedding", ctypes.c_int,
+         [_vp, _i64, _vp, _i32, _i64, _i64, _i64, _f32, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+        ("wf_token_embedding_backward_workspace_bytes", sz, [_i64] * 3 + [_i32] * 2),
+        ("wf_token_embedding_backward", ctypes.c_int,
+         [_vp, _i64, _i64, _vp, _i32] + [_i64] * 4 + [_f32, _vp, _vp, sz, _vp]),
     ):
         f = getattr(lib, name)
         f.restype, f.argtypes = restype, argtypes
@@ -347,7 +365,7 @@ def describe_status(bits: int) -> str:
     parts = []
     if bits & STATUS_INDEX_OUT_OF_RANGE:
         parts.append("an attention index, or a token to score, was out of range (its output row, or log probability, "
-                     "is NaN)")
+                     "is NaN), or a token or position to embed (its row is NaN)")
     if bits & STATUS_WAIT_TIMEOUT:
         parts.append(f"a kernel's bounded wait timed out (wait-site bits 0x{bits >> 4:x}); its results are invalid")
     if not parts:

@@ -162,6 +162,18 @@ int check_norm(int32_t dtype, int64_t rows, int64_t d, int32_t param_dtype, int6
   return WF_OK;
 }
 
+int check_embedding(const char* what, int32_t dtype, int64_t n, int64_t rows, int64_t d, int64_t stride) {
+  if (!valid_dtype(dtype)) return fail(WF_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (n < 0 || rows < 1 || d < 1)
+    return fail(WF_ERR_INVALID_ARGUMENT, "%s: bad sizes (n=%lld, rows=%lld, d=%lld)", what, (long long)n,
+                (long long)rows, (long long)d);
+  // indices and places are held in 32 bits, and a block takes 128 columns
+  if (n >= (1 << 30) || rows >= (1 << 30) || d >= (1 << 22))
+    return fail(WF_ERR_UNSUPPORTED, "%s: sizes too large (n, rows < 2^30, d < 2^22)", what);
+  if (stride < 0) return fail(WF_ERR_INVALID_ARGUMENT, "negative row stride");
+  return WF_OK;
+}
+
 int check_logits(int32_t dtype, int64_t rows, int64_t vocab, int64_t stride) {
   if (!valid_dtype(dtype)) return fail(WF_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
   if (rows < 0 || vocab < 1) return fail(WF_ERR_INVALID_ARGUMENT, "bad sizes (rows=%lld, vocab=%lld)", (long long)rows,
@@ -949,6 +961,124 @@ int wf_token_logprobs_backward(const void* logits, int32_t dtype, int64_t rows, 
   p.rows = rows; p.x_stride = row_stride; p.vocab = vocab; p.ignore_index = ignore_index;
   rc = wf::launch_token_logprobs_backward(p, dtype, static_cast<cudaStream_t>(stream));
   return rc ? cuda_fail(rc, "wf_token_logprobs_backward") : ok();
+}
+
+size_t wf_linear_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int32_t dtype,
+                                                int32_t x_direct, int32_t w_direct) {
+  if (rows <= 0 || vocab <= 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  return wf::linear_logprobs_workspace_bytes(rows, vocab, d, dtype, x_direct, w_direct);
+}
+
+size_t wf_linear_token_logprobs_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int32_t dtype,
+                                                         int32_t x_direct, int32_t w_direct) {
+  if (rows <= 0 || vocab <= 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  return wf::linear_logprobs_backward_workspace_bytes(rows, vocab, d, dtype, x_direct, w_direct);
+}
+
+int wf_linear_token_logprobs(const void* x, const void* w, const void* bias, int32_t dtype, int64_t rows, int64_t vocab,
+                             int64_t d, int64_t x_row_stride, int64_t w_row_stride, const int64_t* tokens,
+                             int64_t ignore_index, float* logprob, float* entropy, float* stats, void* workspace,
+                             size_t workspace_bytes, int32_t* status, void* stream) {
+  int rc = check_linear("wf_linear_token_logprobs", dtype, rows, vocab, d, x_row_stride, w_row_stride, WF_ACT_NONE);
+  if (rc) return rc;
+  if (vocab < 1) return fail(WF_ERR_INVALID_ARGUMENT, "wf_linear_token_logprobs: vocab must be >= 1");
+  if (rows == 0) return ok();
+  if (!x || !w || !tokens || !logprob || !entropy) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if ((rc = check_workspace("wf_linear_token_logprobs", workspace, workspace_bytes,
+                            wf::linear_logprobs_workspace_bytes(rows, vocab, d, dtype,
+                                                                on_16_bytes(x, x_row_stride, dtype),
+                                                                on_16_bytes(w, w_row_stride, dtype)))))
+    return rc;
+  wf::LinearLogprobsParams p{};
+  p.x = x; p.w = w; p.bias = bias; p.tokens = tokens; p.logprob = logprob; p.entropy = entropy; p.stats = stats;
+  p.rows = rows; p.vocab = vocab; p.d = d; p.x_stride = x_row_stride; p.w_stride = w_row_stride;
+  p.ignore_index = ignore_index;
+  p.ws = workspace;
+  p.status = status;
+  rc = wf::launch_linear_logprobs(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_linear_token_logprobs") : ok();
+}
+
+int wf_linear_token_logprobs_backward(const void* x, const void* w, const void* bias, int32_t dtype, int64_t rows,
+                                      int64_t vocab, int64_t d, int64_t x_row_stride, int64_t w_row_stride,
+                                      const int64_t* tokens, int64_t ignore_index, const float* stats,
+                                      const float* entropy, const float* dlogprob, const float* dentropy, void* dx,
+                                      void* dw, void* dbias, void* workspace, size_t workspace_bytes, int32_t* status,
+                                      void* stream) {
+  int rc = check_linear("wf_linear_token_logprobs_backward", dtype, rows, vocab, d, x_row_stride, w_row_stride,
+                        WF_ACT_NONE);
+  if (rc) return rc;
+  if (vocab < 1) return fail(WF_ERR_INVALID_ARGUMENT, "wf_linear_token_logprobs_backward: vocab must be >= 1");
+  if (!dx && !dw && !dbias) return ok();
+  if (rows > 0) {
+    if (!x || !w || !tokens || !stats || !entropy) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+    if ((rc = check_workspace("wf_linear_token_logprobs_backward", workspace, workspace_bytes,
+                              wf::linear_logprobs_backward_workspace_bytes(rows, vocab, d, dtype,
+                                                                           on_16_bytes(x, x_row_stride, dtype),
+                                                                           on_16_bytes(w, w_row_stride, dtype)))))
+      return rc;
+  }
+  wf::LinearLogprobsBwdParams p{};
+  p.x = x; p.w = w; p.bias = bias; p.tokens = tokens; p.stats = stats; p.entropy = entropy;
+  p.dlogprob = dlogprob; p.dentropy = dentropy; p.dx = dx; p.dw = dw; p.db = dbias;
+  p.rows = rows; p.vocab = vocab; p.d = d; p.x_stride = x_row_stride; p.w_stride = w_row_stride;
+  p.ignore_index = ignore_index;
+  p.ws = workspace;
+  p.status = status;
+  rc = wf::launch_linear_logprobs_backward(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_linear_token_logprobs_backward") : ok();
+}
+
+int wf_token_embedding(const int64_t* tokens, int64_t n, const void* weight, int32_t dtype, int64_t vocab, int64_t d,
+                       int64_t w_row_stride, float scale, const void* position_weight, int64_t places,
+                       int64_t p_row_stride, const int64_t* positions, int64_t seq, void* y, int32_t* status,
+                       void* stream) {
+  int rc = check_embedding("wf_token_embedding", dtype, n, vocab, d, w_row_stride);
+  if (rc) return rc;
+  if (position_weight) {
+    if ((rc = check_embedding("wf_token_embedding", dtype, n, places, d, p_row_stride))) return rc;
+    if (!positions && seq < 1) return fail(WF_ERR_INVALID_ARGUMENT, "seq must be >= 1 without positions");
+  }
+  if (n == 0) return ok();
+  if (!tokens || !weight || !y) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  wf::EmbeddingParams p{};
+  p.tokens = tokens; p.positions = positions; p.weight = weight; p.position_weight = position_weight; p.y = y;
+  p.n = n; p.seq = seq; p.vocab = vocab; p.places = places; p.d = d;
+  p.w_stride = w_row_stride; p.p_stride = p_row_stride;
+  p.scale = scale;
+  p.status = status;
+  rc = wf::launch_embedding(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_token_embedding") : ok();
+}
+
+size_t wf_token_embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t d, int32_t dtype,
+                                                   int32_t has_index) {
+  if (n <= 0 || rows <= 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  return wf::embedding_backward_workspace_bytes(n, rows, d, dtype, !has_index);
+}
+
+int wf_token_embedding_backward(const int64_t* index, int64_t n, int64_t seq, const void* dy, int32_t dtype,
+                                int64_t rows, int64_t d, int64_t dy_row_stride, int64_t padding_index, float scale,
+                                void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_embedding("wf_token_embedding_backward", dtype, n, rows, d, dy_row_stride);
+  if (rc) return rc;
+  if (!dweight) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (n > 0) {
+    if (!dy) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+    if (!index && (seq < 1 || n % seq))
+      return fail(WF_ERR_INVALID_ARGUMENT, "without an index n must be a multiple of seq (n=%lld, seq=%lld)",
+                  (long long)n, (long long)seq);
+    if ((rc = check_workspace("wf_token_embedding_backward", workspace, workspace_bytes,
+                              wf::embedding_backward_workspace_bytes(n, rows, d, dtype, !index))))
+      return rc;
+  }
+  wf::EmbeddingBwdParams p{};
+  p.index = index; p.dy = dy; p.dweight = dweight;
+  p.n = n; p.seq = seq; p.rows = rows; p.d = d; p.dy_stride = dy_row_stride; p.padding_index = padding_index;
+  p.scale = scale;
+  p.ws = workspace;
+  rc = wf::launch_embedding_backward(p, dtype, static_cast<cudaStream_t>(stream));
+  return rc ? cuda_fail(rc, "wf_token_embedding_backward") : ok();
 }
 
 }  // extern "C"

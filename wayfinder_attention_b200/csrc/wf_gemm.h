@@ -2,9 +2,13 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 namespace wf {
+
+inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // A row-major 16-bit matrix whose rows start on 16-byte boundaries.  K-major: rows are the
 // product's rows and columns its depth; MN-major: the other way round.  An fp32 matrix is
@@ -31,7 +35,7 @@ struct GemmProblem {
   int pieces;       // 1, or 3 for fp32
   int turns;        // 2 where a 16-bit a is the sum of two pieces (then pieces is 1), else 1
   int op_dtype;     // kBF16 or kF16
-  int out_dtype;
+  int out_dtype;    // of the epilogue's matrices (z apart): the operands' own, or fp32
   GemmEpilogue out;
   void* ws;         // gemm_workspace_bytes(M, N, K, pieces, turns)
   int32_t* status;

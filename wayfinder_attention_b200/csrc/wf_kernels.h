@@ -236,4 +236,63 @@ size_t linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtyp
 int launch_linear(const LinearParams& p, int dtype, cudaStream_t stream);
 int launch_linear_backward(const LinearBwdParams& p, int dtype, cudaStream_t stream);
 
+// Log probabilities of given tokens from the head's product (wf_linear_logprobs.cu).  x (rows, d)
+// and w (vocab, d) are unit-strided on d.
+struct LinearLogprobsParams {
+  const void* x;
+  const void* w;
+  const void* bias;  // [vocab] or null
+  const int64_t* tokens;
+  float* logprob;
+  float* entropy;
+  float* stats;  // [2][rows] for the backward, or null: the maximum m, and log sum exp(z - m)
+  int64_t rows, vocab, d, x_stride, w_stride, ignore_index;
+  void* ws;
+  int32_t* status;  // nullable
+};
+struct LinearLogprobsBwdParams {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const int64_t* tokens;
+  const float* stats;
+  const float* entropy;
+  const float* dlogprob;  // [rows] or null
+  const float* dentropy;  // [rows] or null
+  void* dx;               // each of the three may be null; contiguous
+  void* dw;
+  void* db;
+  int64_t rows, vocab, d, x_stride, w_stride, ignore_index;
+  void* ws;
+  int32_t* status;
+};
+size_t linear_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int dtype, bool x_direct, bool w_direct);
+size_t linear_logprobs_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int dtype, bool x_direct,
+                                                bool w_direct);
+int launch_linear_logprobs(const LinearLogprobsParams& p, int dtype, cudaStream_t stream);
+int launch_linear_logprobs_backward(const LinearLogprobsBwdParams& p, int dtype, cudaStream_t stream);
+
+// Token embedding (wf_embedding.cu): rows of tables, unit-strided on d.
+struct EmbeddingParams {
+  const int64_t* tokens;  // [n]
+  const int64_t* positions;  // [n], or null: i % seq
+  const void* weight;
+  const void* position_weight;  // or null
+  void* y;                      // [n][d]
+  int64_t n, seq, vocab, places, d, w_stride, p_stride;
+  float scale;
+  int32_t* status;  // nullable; bit 0 set on an index outside its table
+};
+struct EmbeddingBwdParams {
+  const int64_t* index;  // [n], or null: i % seq
+  const void* dy;        // (n, d) rows dy_stride apart
+  void* dweight;         // [rows][d]
+  int64_t n, seq, rows, d, dy_stride, padding_index;
+  float scale;
+  void* ws;
+};
+size_t embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t d, int dtype, bool sorted);
+int launch_embedding(const EmbeddingParams& p, int dtype, cudaStream_t stream);
+int launch_embedding_backward(const EmbeddingBwdParams& p, int dtype, cudaStream_t stream);
+
 }  // namespace wf

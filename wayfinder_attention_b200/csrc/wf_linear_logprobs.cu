@@ -1,0 +1,600 @@
+// Log probabilities of given tokens and entropies from hidden rows and the head's weight,
+// with their backward, in pieces of the vocabulary: the logits are never in memory.
+//
+//   z_j = x . w_j + b_j,  L = log sum_j exp z_j,  logprob = z_t - L,  H = L - sum_j p_j z_j
+//   dz_j = gl (1[j = t] - p_j) - gh p_j (z_j - L + H),   p_j = exp(z_j - L)
+//   dx = dz W,  dW = dz^T x,  db = sum_rows dz
+//
+// Forward: the tensor-core product (wf_gemm_kernel.cuh) whose epilogue keeps, for each row
+// of its run of tiles, the maximum m, s = sum exp(z - m) and u = sum exp(z - m) (z - m), and
+// picks the token's logit; a second kernel joins the runs' shares.
+//
+// Backward: for a piece of the vocabulary at a time the same product again, whose epilogue
+// makes dz of each logit and stores it in the operands' type; then dx += dz W over the piece
+// (in fp32) and the piece's rows of dW.  Four products where three would do if the logits
+// were kept: that is the price of not keeping them.
+#include "wf_columns.cuh"
+#include "wf_gemm_kernel.cuh"
+#include "wf_operand.cuh"
+#include "wf_pair.cuh"
+
+#include <cfloat>
+#include <climits>
+
+namespace wf {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// e^d and 2^d are 0 below this: the bound keeps 0 * inf out where a logit is -inf
+constexpr float kNothing = -200.f;
+constexpr int kShares = 4;  // epilogue warps that share a row of a tile, in every shape here
+
+// ------------------------------------------------------------------ forward
+// Running sums of a row over its run of tiles.  A NaN or +inf stays in the maximum (the
+// sums may lose it), and a row whose logits are all -inf has s = 0.
+struct ScoreStats {
+  static constexpr bool kRuns = true, kStores = false;
+  const int64_t* tokens;
+  float* parts;        // [3][ranges * kShares][M]: m, s, u
+  float* token_logit;  // [M]
+  int64_t part_rows;   // ranges * kShares * M
+  struct Row {
+    float m, s, u;
+    int token;
+    float* token_logit;
+  };
+  __device__ __forceinline__ void begin(Row& r, int row, int M, int N) const {
+    r.m = -FLT_MAX;
+    r.s = r.u = 0.f;
+    const int64_t t = row < M ? tokens[row] : -1;
+    r.token = t >= 0 && t < N ? (int)t : -1;
+    r.token_logit = token_logit + row;
+  }
+  template <int SC>
+  __device__ __forceinline__ void slice(Row& r, float* v, int n, int N) const {
+    if (n + SC > N) {
+#pragma unroll
+      for (int j = 0; j < SC; ++j)
+        if (n + j >= N) v[j] = -INFINITY;
+    }
+    if ((uint32_t)(r.token - n) < (uint32_t)SC) {
+      float z = v[0];
+#pragma unroll
+      for (int j = 1; j < SC; ++j)
+        if (n + j == r.token) z = v[j];
+      *r.token_logit = z;
+    }
+    float m = r.m;
+#pragma unroll
+    for (int j = 0; j < SC; ++j) m = max_keep_nan(m, v[j]);
+    const float d = fmaxf(r.m - m, kNothing), a = exp2_approx(d * kLog2e);
+    Pair s(0.f), u(0.f);
+#pragma unroll
+    for (int j = 0; j < SC; j += 2) {
+      float d0, d1;
+      add2(Pair(v[j], v[j + 1]), Pair(-m)).get(d0, d1);
+      const Pair t(fmaxf(d0, kNothing), fmaxf(d1, kNothing));
+      float t0, t1;
+      mul2(t, Pair(kLog2e)).get(t0, t1);
+      const Pair e(exp2_approx(t0), exp2_approx(t1));
+      s = add2(s, e);
+      u = fma2(e, t, u);
+    }
+    float s0, s1, u0, u1;
+    s.get(s0, s1);
+    u.get(u0, u1);
+    r.u = fmaf(a, fmaf(r.s, d, r.u), u0 + u1);
+    r.s = fmaf(a, r.s, s0 + s1);
+    r.m = m;
+  }
+  __device__ __forceinline__ void end(const Row& r, int row, int M, int part) const {
+    if (row >= M) return;
+    float* to = parts + (int64_t)part * M + row;
+    to[0] = r.m;
+    to[part_rows] = r.s;
+    to[2 * part_rows] = r.u;
+  }
+};
+
+// Joins the parts of 32 rows: 8 warps share the parts, a row a lane.
+__global__ void __launch_bounds__(256) linear_logprobs_join_kernel(const float* parts, int n_parts,
+                                                                   const float* token_logit, LinearLogprobsParams p) {
+  __shared__ float sm[8][32], ss[8][32], su[8][32];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 32 + lane, stride = (int64_t)n_parts * p.rows;
+  float m = -FLT_MAX, s = 0.f, u = 0.f;
+  auto join = [&](float m2, float s2, float u2) {
+    const float top = max_keep_nan(m, m2);
+    const float d = fmaxf(m - top, kNothing), d2 = fmaxf(m2 - top, kNothing);
+    const float a = exp2_approx(d * kLog2e), a2 = exp2_approx(d2 * kLog2e);
+    u = fmaf(a, fmaf(s, d, u), a2 * fmaf(s2, d2, u2));
+    s = fmaf(a, s, a2 * s2);
+    m = top;
+  };
+  if (row < p.rows)
+    for (int i = warp; i < n_parts; i += 8) {
+      const float* at = parts + (int64_t)i * p.rows + row;
+      join(at[0], at[stride], at[2 * stride]);
+    }
+  sm[warp][lane] = m;
+  ss[warp][lane] = s;
+  su[warp][lane] = u;
+  __syncthreads();
+  if (warp || row >= p.rows) return;
+  for (int i = 1; i < 8; ++i) join(sm[i][lane], ss[i][lane], su[i][lane]);
+  const bool none = s == 0.f && m == -FLT_MAX;
+  const bool bad = !(m < INFINITY);  // NaN or +inf
+  const float log_s = none ? -INFINITY : logf(s);
+  const int64_t tok = p.tokens[row];
+  float lp;
+  if (tok == p.ignore_index) {
+    lp = 0.f;
+  } else if (tok < 0 || tok >= p.vocab) {
+    lp = NAN;
+    if (p.status) atomicOr(p.status, 1);
+  } else {
+    lp = bad ? NAN : none ? -INFINITY : token_logit[row] - m - log_s;
+  }
+  p.logprob[row] = lp;
+  p.entropy[row] = bad ? NAN : none ? 0.f : log_s - u / s;
+  if (p.stats) {
+    p.stats[row] = none ? -INFINITY : m;
+    p.stats[p.rows + row] = log_s;
+  }
+}
+
+// ------------------------------------------------------------------ backward
+// What the backward's epilogue needs of a row: dz_j = p (a + b t) + g [j = token] with
+// t = (z - m) log2 e - l2s and p = 2^t.
+struct RowGrad {
+  float m, l2s, a, b;
+};
+struct RowToken {
+  float g;
+  int token;
+};
+
+// fp16 has no room for p of a gradient that is small itself (a mean over many rows): there a row's
+// gradient is multiplied by a power of two 2^e that brings |gl| + 32 |gh|, which bounds |dz|, to
+// 2^14 .. 2^15.  dx takes it off again by rows; for dW, x's rows are multiplied by 2^(least e - e)
+// and the product by 2^-least.
+constexpr int kNoRow = 1000;  // the exponent of a row without a gradient
+
+struct GradRows {
+  RowGrad* grad;
+  RowToken* token;
+  int* exponent;  // [rows], then the least of them; null: not scaled
+};
+
+__global__ void __launch_bounds__(256) linear_logprobs_rows_kernel(LinearLogprobsBwdParams p, GradRows out) {
+  pdl_wait();
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int e = kNoRow;
+  if (row < p.rows) {
+    float m = p.stats[row], log_s = p.stats[p.rows + row];
+    float gl = p.dlogprob ? p.dlogprob[row] : 0.f;
+    const float gh = p.dentropy ? p.dentropy[row] : 0.f;
+    const int64_t t = p.tokens[row];
+    int token = -1;
+    if (t == p.ignore_index) gl = 0.f;
+    else if (t < 0 || t >= p.vocab) gl = gl == 0.f ? 0.f : NAN;
+    else token = (int)t;
+    RowGrad r{m, log_s * kLog2e, -fmaf(gh, p.entropy[row], gl), -gh * kLn2};
+    float g = gl;
+    if (m == -INFINITY || (gl == 0.f && gh == 0.f)) {  // no distribution, or no gradient: p is 0
+      r = RowGrad{0.f, INFINITY, 0.f, 0.f};
+      g = 0.f;
+    } else {
+      if (!(m < INFINITY)) r = RowGrad{0.f, 0.f, NAN, 0.f};
+      if (out.exponent) {
+        const float size = fabsf(gl) + 32.f * fabsf(gh);
+        e = size > 0.f && size < INFINITY ? min(max(14 - ilogbf(size), -100), 100) : 0;
+        const float up = ldexpf(1.f, e);
+        r.a *= up;
+        r.b *= up;
+        g *= up;
+      }
+    }
+    out.grad[row] = r;
+    out.token[row] = RowToken{g, token};
+    if (out.exponent) out.exponent[row] = e;
+  }
+  if (out.exponent) {
+    const int least = __reduce_min_sync(0xffffffffu, e);
+    if ((threadIdx.x & 31) == 0 && least != kNoRow) atomicMin(out.exponent + p.rows, least);
+  }
+}
+// 2^(least - e), or 2^-least: no row has a gradient where there is no least exponent.
+__device__ __forceinline__ float down_by(int e, int least) { return least > 100 || e > 100 ? 0.f : ldexpf(1.f, least - e); }
+__device__ __forceinline__ float up_by(int least) { return least > 100 ? 0.f : ldexpf(1.f, -least); }
+
+struct ScoreGrad {
+  static constexpr bool kRuns = true, kStores = true;
+  int layers;
+  const RowGrad* grad;
+  const RowToken* token;
+  int first;  // of the vocabulary's piece
+  struct Row {
+    RowGrad r;
+    RowToken t;
+  };
+  __device__ __forceinline__ void begin(Row& r, int row, int M, int) const {
+    r.r = RowGrad{0.f, INFINITY, 0.f, 0.f};
+    r.t = RowToken{0.f, -1};
+    if (row < M) {
+      const float4 f = *reinterpret_cast<const float4*>(grad + row);
+      r.r = RowGrad{f.x, f.y, f.z, f.w};
+      r.t = token[row];
+      r.t.token -= first;
+    }
+  }
+  template <int SC>
+  __device__ __forceinline__ void slice(const Row& r, float* v, int n, int) const {
+#pragma unroll
+    for (int j = 0; j < SC; j += 2) {
+      float t0, t1;
+      fma2(add2(Pair(v[j], v[j + 1]), Pair(-r.r.m)), Pair(kLog2e), Pair(-r.r.l2s)).get(t0, t1);
+      t0 = fmaxf(t0, kNothing);
+      t1 = fmaxf(t1, kNothing);
+      const Pair e(exp2_approx(t0), exp2_approx(t1));
+      mul2(e, fma2(Pair(t0, t1), Pair(r.r.b), Pair(r.r.a))).get(v[j], v[j + 1]);
+    }
+    if ((uint32_t)(r.t.token - n) < (uint32_t)SC) {
+#pragma unroll
+      for (int j = 0; j < SC; ++j)
+        if (n + j == r.t.token) v[j] += r.t.g;
+    }
+  }
+  __device__ __forceinline__ void end(const Row&, int, int, int) const {}
+};
+
+// x's rows multiplied by 2^(least - e): the fp16 operand of dW.
+__global__ void __launch_bounds__(256) scale_rows_kernel(const __half* x, int64_t stride, bool vec, int64_t rows,
+                                                         int64_t cols, const int* exponent, __half* out) {
+  pdl_wait();
+  const int least = exponent[rows];
+  const int64_t pitch = (cols + 7) / 8 * 8, groups = pitch / 8, total = rows * groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups, c = i % groups * 8;
+    Raw8<__half> raw;
+    raw.load(x + r * stride, c, cols, vec);
+    float f[8];
+    raw.unpack(f);
+    const float s = down_by(exponent[r], least);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= s;
+    store_vec<__half, 8>(out + r * pitch + c, f);
+  }
+}
+
+// fp32 rows to their type, with the power of two taken off where there is one: by rows, or the
+// whole by the least exponent.
+template <typename T>
+__global__ void __launch_bounds__(256) round_rows_kernel(const float* x, int64_t pitch, int64_t rows, int64_t cols,
+                                                         const int* exponent, const int* least, T* out) {
+  pdl_wait();
+  const int64_t groups = (cols + 3) / 4, total = rows * groups;
+  const bool vec = cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const float all = least ? up_by(*least) : 1.f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / groups, c = i % groups * 4;
+    const float4 f = *reinterpret_cast<const float4*>(x + r * pitch + c);
+    const float s = exponent ? up_by(exponent[r]) : all;
+    const float v[4] = {f.x * s, f.y * s, f.z * s, f.w * s};
+    T* to = out + r * cols + c;
+    if (vec) {
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+      else *reinterpret_cast<uint2*>(to) = make_uint2(pack2(T(), v[0], v[1]), pack2(T(), v[2], v[3]));
+    } else {
+      for (int j = 0; j < 4 && c + j < cols; ++j) to[j] = from_f32<T>(v[j]);
+    }
+  }
+}
+
+// Partial column sums of dz: a block takes 256 columns (8 a lane) of a share of the rows.
+template <typename T>
+__global__ void __launch_bounds__(256) dz_columns_kernel(const T* dz, int64_t pitch, int layers, int64_t M, int64_t N,
+                                                         const int* exponent, float* partials) {
+  __shared__ float red[8][32][9];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * 8;
+  float s[8] = {};
+  if (c < N)
+    for (int64_t m = (int64_t)blockIdx.y * 8 + warp; m < M; m += (int64_t)gridDim.y * 8) {
+      const float up = exponent ? up_by(exponent[m]) : 1.f;
+      for (int layer = 0; layer < layers; ++layer) {
+        Raw8<T> raw;
+        raw.load(dz + (layer * M + m) * pitch, c, pitch, true);
+        float f[8];
+        raw.unpack(f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = fmaf(f[j], up, s[j]);
+      }
+    }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[warp][lane][j] = s[j];
+  __syncthreads();
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (col < N) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += red[i][threadIdx.x / 8][threadIdx.x % 8];
+    partials[(size_t)blockIdx.y * N + col] = v;
+  }
+}
+int column_shares(int64_t M, int64_t N) {
+  const int64_t by = (N + 255) / 256, want = (8 * kSms + by - 1) / by, most = (M + 15) / 16;
+  return (int)std::max<int64_t>(1, std::min(want, most));
+}
+
+// ------------------------------------------------------------------ plans
+// Tile shape, runs and their order for the logits' product: the least of an estimate, as for other
+// products (wf_gemm.cu), but a tile takes at least the 8 cycles a column that the exponentials of
+// 128 rows need.
+constexpr Shape kRunShapes[] = {{256, 2, 560, 0}, {128, 2, 400, 1700}, {128, 1, 540, 0}, {64, 1, 0, 1300}};
+constexpr int kMaxRanges = 1024;
+constexpr double kGroupBytes = 48e6;  // of A that a group's rows of tiles may have, to stay in L2
+Plan run_plan(int64_t M, int64_t N, int64_t K, int pieces) {
+  Plan best{};
+  double least = 0;
+  for (const Shape& s : kRunShapes) {
+    const int cycles = pieces > 1 ? s.cycles3 : s.cycles;
+    if (!cycles) continue;
+    Plan p{};
+    p.shape = s;
+    p.splits = p.layers = 1;
+    p.k_blocks = (int)((K + kBK - 1) / kBK);
+    const int64_t tn = (N + s.bn - 1) / s.bn, tm = (M + kBM * s.cg - 1) / (kBM * s.cg);
+    p.tiles_n = (int)tn;
+    p.tiles_m = (int)tm;
+    p.group = (int)std::max(1.0, std::min((double)tm, kGroupBytes / ((double)kBM * s.cg * K * 2 * pieces)));
+    const int slots = kSms / s.cg;
+    const double tile = std::max<double>((double)p.k_blocks * cycles, 8 * s.bn);
+    for (int64_t ranges = 1; ranges <= std::min<int64_t>(tn, kMaxRanges); ++ranges) {
+      const double waves = (double)((tm * ranges + slots - 1) / slots), length = (double)((tn + ranges - 1) / ranges);
+      // a wave ends with an epilogue that nothing covers; the parts are written and read once
+      const double t = waves * (length * tile + 8 * s.bn) + 24.0 * kShares * ranges * M / 2000;
+      if (best.ranges == 0 || t < least) {
+        least = t;
+        best = p;
+        best.ranges = (int)ranges;
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, class E>
+int launch_runs(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, const E& e, cudaStream_t stream) {
+  constexpr bool PIECES = std::is_same<T, float>::value;
+  const Shape& s = plan.shape;
+  if constexpr (PIECES) {
+    if (s.cg == 2) return launch_tile<T, 128, 2, true>(g, out, plan, e, stream);
+    return launch_tile<T, 64, 1, true>(g, out, plan, e, stream);
+  } else {
+    if (s.bn == 256) return launch_tile<T, 256, 2, false>(g, out, plan, e, stream);
+    if (s.cg == 2) return launch_tile<T, 128, 2, false>(g, out, plan, e, stream);
+    return launch_tile<T, 128, 1, false>(g, out, plan, e, stream);
+  }
+}
+
+size_t parts_bytes(const Plan& plan, int64_t M) {
+  return round256((size_t)3 * plan.ranges * kShares * M * sizeof(float)) + round256((size_t)M * sizeof(float));
+}
+
+template <typename T>
+int launch_fwd(const LinearLogprobsParams& p, int dtype, cudaStream_t stream) {
+  unsigned char* ws = static_cast<unsigned char*>(p.ws);
+  GemmOperand o[2];
+  if (int rc = operands<T>({{p.x, p.rows, p.d, p.x_stride}, {p.w, p.vocab, p.d, p.w_stride}}, dtype, &ws, o, stream))
+    return rc;
+  const Plan plan = run_plan(p.rows, p.vocab, p.d, kPieces<T>);
+  GemmProblem g = problem<T>(o[0], o[1], p.rows, p.vocab, p.d, dtype, nullptr, p.status);
+  GemmEpilogue out{};
+  out.bias = p.bias;
+  ScoreStats e;
+  e.tokens = p.tokens;
+  e.part_rows = (int64_t)plan.ranges * kShares * p.rows;
+  e.parts = reinterpret_cast<float*>(ws);
+  e.token_logit = reinterpret_cast<float*>(ws + round256((size_t)3 * e.part_rows * sizeof(float)));
+  if (int rc = launch_runs<T>(g, out, plan, e, stream)) return rc;
+  return (int)launch_pdl(linear_logprobs_join_kernel, dim3((unsigned)((p.rows + 31) / 32)), dim3(256), 0, stream,
+                         static_cast<const float*>(e.parts), plan.ranges * kShares,
+                         static_cast<const float*>(e.token_logit), p);
+}
+
+// Columns of the vocabulary that a piece has: as many as 256 MB of dz hold, but 2048 at least
+// (shorter ones leave the products' tiles idle) and all of them where they are few.
+constexpr int64_t kPieceBytes = 256ll << 20, kPieceLeast = 2048;
+int64_t piece_columns(int64_t M, int64_t N, int dtype, int layers) {
+  const int64_t fit = kPieceBytes / (M * (dtype == kF32 ? 10 : 2 * layers)) / 256 * 256;
+  const int64_t most = std::max(fit, kPieceLeast);
+  if (N <= most) return N;
+  const int64_t pieces = (N + most - 1) / most;  // of like size
+  return ((N + pieces - 1) / pieces + 255) / 256 * 256;
+}
+// Pieces of a 16-bit dz, as in wf_linear.cu: two where the products are small, so that rounding it
+// adds nothing to the gradients' own rounding.
+int dz_layers(int64_t M, int64_t N, int64_t K, int dtype) {
+  return dtype != kF32 && (double)M * N * K <= (double)(1 << 30) ? 2 : 1;
+}
+
+struct BwdPlan {
+  int64_t columns;
+  int layers, pieces;
+  bool scaled, dx_apart, dw_apart;
+  size_t rows, dz, dz_operand, dx, dw, sums, scaled_x, gemm;
+};
+BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+  BwdPlan b{};
+  b.layers = dz_layers(M, N, K, dtype);
+  b.columns = piece_columns(M, N, dtype, b.layers);
+  b.pieces = dtype == kF32 ? 3 : 1;
+  b.scaled = dtype == kF16;
+  b.dx_apart = dtype != kF32 && (b.scaled || b.columns < N);  // fp32 sums, rounded at the end
+  b.dw_apart = b.scaled;
+  b.rows = round256(M * sizeof(RowGrad)) + round256(M * sizeof(RowToken)) +
+           (b.scaled ? round256((M + 1) * sizeof(int)) : 0);
+  b.dz = round256((size_t)M * round8(b.columns) * (dtype == kF32 ? 4 : 2) * b.layers);
+  b.dz_operand = dtype == kF32 ? operand_bytes(M, b.columns, dtype) : 0;
+  b.dx = b.dx_apart ? round256((size_t)M * round8(K) * sizeof(float)) : 0;
+  b.dw = b.dw_apart ? round256((size_t)b.columns * round8(K) * sizeof(float)) : 0;
+  b.sums = round256((size_t)column_shares(M, b.columns) * b.columns * sizeof(float));
+  b.scaled_x = b.scaled ? operand_bytes(M, K, dtype) : 0;
+  const int64_t last = N - (N - 1) / b.columns * b.columns;
+  for (int64_t n : {b.columns, last})
+    b.gemm = std::max({b.gemm, gemm_workspace_bytes(M, K, n, b.pieces, b.layers),
+                       gemm_workspace_bytes(n, K, M, b.pieces, b.layers)});
+  return b;
+}
+
+template <typename T>
+int launch_bwd(const LinearLogprobsBwdParams& p, int dtype, cudaStream_t stream) {
+  const int64_t M = p.rows, N = p.vocab, K = p.d;
+  if (M == 0) {  // sums over no rows
+    for (auto [ptr, n] : {std::pair<void*, size_t>{p.dw, (size_t)N * K}, {p.db, (size_t)N}})
+      if (ptr)
+        if (cudaError_t e = cudaMemsetAsync(ptr, 0, n * sizeof(T), stream)) return (int)e;
+    return 0;
+  }
+  const BwdPlan b = bwd_plan(M, N, K, dtype);
+  unsigned char* ws = static_cast<unsigned char*>(p.ws);
+  auto take = [&](size_t bytes) {
+    unsigned char* at = ws;
+    ws += bytes;
+    return at;
+  };
+  GradRows rows{};
+  rows.grad = reinterpret_cast<RowGrad*>(take(round256(M * sizeof(RowGrad))));
+  rows.token = reinterpret_cast<RowToken*>(take(round256(M * sizeof(RowToken))));
+  const int *exponent = nullptr, *least = nullptr;
+  if (b.scaled) {
+    rows.exponent = reinterpret_cast<int*>(take(round256((M + 1) * sizeof(int))));
+    exponent = rows.exponent;
+    least = exponent + M;
+    // a least exponent above every row's
+    if (cudaError_t e = cudaMemsetAsync(rows.exponent + M, 0x7f, sizeof(int), stream)) return (int)e;
+  }
+  unsigned char* dz = take(b.dz);
+  unsigned char* dz_operand = take(b.dz_operand);
+  float* dx = reinterpret_cast<float*>(take(b.dx));
+  float* dw = reinterpret_cast<float*>(take(b.dw));
+  float* sums = reinterpret_cast<float*>(take(b.sums));
+  unsigned char* scaled_x = take(b.scaled_x);
+  unsigned char* gemm_ws = take(b.gemm);
+  GemmOperand o[2];
+  if (int rc = operands<T>({{p.x, M, K, p.x_stride}, {p.w, N, K, p.w_stride}}, dtype, &ws, o, stream)) return rc;
+  if (cudaError_t e = launch_pdl(linear_logprobs_rows_kernel, dim3((unsigned)((M + 255) / 256)), dim3(256), 0, stream,
+                                 p, rows))
+    return (int)e;
+  GemmOperand x_deep = o[0];  // of dW, whose depth are the rows
+  if constexpr (std::is_same<T, __half>::value) {
+    if (p.dw) {
+      x_deep = blank_operand<T>(M, K, dtype, &scaled_x);
+      const int64_t blocks = (M * (round8(K) / 8) + 255) / 256;
+      if (cudaError_t e = launch_pdl(scale_rows_kernel, dim3((unsigned)std::min<int64_t>(blocks, 16 * kSms)), dim3(256),
+                                     0, stream, static_cast<const __half*>(p.x), p.x_stride,
+                                     on_16_bytes<T>(p.x, p.x_stride), M, K, exponent,
+                                     static_cast<__half*>(const_cast<void*>(x_deep.ptr))))
+        return (int)e;
+    }
+  }
+  x_deep.mn_major = true;
+  auto round_rows = [&](const float* from, int64_t n, const int* by_row, const int* all, T* to) {
+    const int64_t blocks = (n * ((K + 3) / 4) + 255) / 256;
+    return launch_pdl(round_rows_kernel<T>, dim3((unsigned)std::min<int64_t>(blocks, 16 * kSms)), dim3(256), 0, stream,
+                      from, round8(K), n, K, by_row, all, to);
+  };
+  for (int64_t first = 0; first < N; first += b.columns) {
+    const int64_t n = std::min(b.columns, N - first), pitch = round8(n);
+    GemmOperand w = o[1];
+    w.ptr = static_cast<const unsigned char*>(w.ptr) + first * w.pitch * 2;
+    w.rows = n;
+    {
+      GemmProblem g = problem<T>(o[0], w, M, n, K, dtype, nullptr, p.status);
+      GemmEpilogue out{};
+      out.bias = p.bias ? static_cast<const T*>(p.bias) + first : nullptr;
+      out.y = dz;
+      out.y_stride = pitch;
+      Plan plan = run_plan(M, n, K, b.pieces);
+      plan.layers = b.layers;
+      if (int rc = launch_runs<T>(g, out, plan, ScoreGrad{b.layers, rows.grad, rows.token, (int)first}, stream)) return rc;
+    }
+    if (p.db) {
+      const int shares = column_shares(M, n);
+      if (cudaError_t e = launch_pdl(dz_columns_kernel<T>, dim3((unsigned)((n + 255) / 256), shares), dim3(256), 0,
+                                     stream, reinterpret_cast<const T*>(dz), pitch, b.layers, M, n, exponent, sums))
+        return (int)e;
+      if (cudaError_t e = join_columns<T>(sums, shares, n, n, static_cast<T*>(p.db) + first, nullptr, stream))
+        return (int)e;
+    }
+    GemmOperand d{dz, M, n, pitch, M * pitch, false};
+    if (dtype == kF32) {
+      GemmOperand laid[2];
+      unsigned char* at = dz_operand;
+      if (int rc = operands<T>({{dz, M, n, pitch}, {nullptr, 0, 0, 0}}, dtype, &at, laid, stream)) return rc;
+      d = laid[0];
+    }
+    if (p.dx) {
+      w.mn_major = true;  // its columns are dx's, its rows the depth
+      GemmProblem g = problem<T>(d, w, M, K, n, dtype, gemm_ws, p.status);
+      g.turns = b.layers;
+      const bool apart = b.dx_apart;
+      g.out.y = apart ? static_cast<void*>(dx) : p.dx;
+      g.out.y_stride = apart ? round8(K) : K;
+      if (apart) g.out_dtype = kF32;
+      if (first) {
+        g.out.residual = g.out.y;
+        g.out.r_stride = g.out.y_stride;
+      }
+      if (int rc = launch_gemm(g, stream)) return rc;
+    }
+    if (p.dw) {
+      d.mn_major = true;  // the rows of both are the depth
+      GemmProblem g = problem<T>(d, x_deep, n, K, M, dtype, gemm_ws, p.status);
+      g.turns = b.layers;
+      T* to = static_cast<T*>(p.dw) + first * K;
+      g.out.y = b.dw_apart ? static_cast<void*>(dw) : to;
+      g.out.y_stride = b.dw_apart ? round8(K) : K;
+      if (b.dw_apart) g.out_dtype = kF32;
+      if (int rc = launch_gemm(g, stream)) return rc;
+      if (b.dw_apart)
+        if (cudaError_t e = round_rows(dw, n, nullptr, least, to)) return (int)e;
+    }
+  }
+  if (p.dx && b.dx_apart)
+    if (cudaError_t e = round_rows(dx, M, exponent, nullptr, static_cast<T*>(p.dx))) return (int)e;
+  return 0;
+}
+
+}  // namespace
+
+size_t linear_logprobs_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct, bool w_direct) {
+  const int pieces = dtype == kF32 ? 3 : 1;
+  return (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype)) +
+         (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) + parts_bytes(run_plan(M, N, K, pieces), M);
+}
+
+size_t linear_logprobs_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct,
+                                                bool w_direct) {
+  const BwdPlan b = bwd_plan(M, N, K, dtype);
+  return b.rows + b.dz + b.dz_operand + b.dx + b.dw + b.sums + b.scaled_x + b.gemm +
+         (x_direct && b.pieces == 1 ? 0 : operand_bytes(M, K, dtype)) +
+         (w_direct && b.pieces == 1 ? 0 : operand_bytes(N, K, dtype));
+}
+
+int launch_linear_logprobs(const LinearLogprobsParams& p, int dtype, cudaStream_t stream) {
+  if (dtype == kBF16) return launch_fwd<__nv_bfloat16>(p, dtype, stream);
+  if (dtype == kF16) return launch_fwd<__half>(p, dtype, stream);
+  return launch_fwd<float>(p, dtype, stream);
+}
+
+int launch_linear_logprobs_backward(const LinearLogprobsBwdParams& p, int dtype, cudaStream_t stream) {
+  if (dtype == kBF16) return launch_bwd<__nv_bfloat16>(p, dtype, stream);
+  if (dtype == kF16) return launch_bwd<__half>(p, dtype, stream);
+  return launch_bwd<float>(p, dtype, stream);
+}
+
+}  // namespace wf

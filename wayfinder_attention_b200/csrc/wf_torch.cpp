@@ -1,4 +1,4 @@
-// fused_linear, layer_norm and token_logprobs as PyTorch calls: argument checks, outputs and
+// fused_linear, layer_norm, token_logprobs, linear_token_logprobs and token_embedding as PyTorch calls: argument checks, outputs and
 // autograd nodes around the C ABI (include/wayfinder.h), whose functions are looked up in the
 // library that the package loads.  A small training step is bound by the host: the same nodes
 // in Python took 118 us of host time for a layer norm's forward and backward, against 70 us
@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -39,6 +40,13 @@ struct Library {
   decltype(&wf_max_top_tokens) max_top_tokens;
   decltype(&wf_token_logprobs) token_logprobs;
   decltype(&wf_token_logprobs_backward) token_logprobs_backward;
+  decltype(&wf_linear_token_logprobs) linear_token_logprobs;
+  decltype(&wf_linear_token_logprobs_workspace_bytes) linear_token_logprobs_workspace_bytes;
+  decltype(&wf_linear_token_logprobs_backward) linear_token_logprobs_backward;
+  decltype(&wf_linear_token_logprobs_backward_workspace_bytes) linear_token_logprobs_backward_workspace_bytes;
+  decltype(&wf_token_embedding) token_embedding;
+  decltype(&wf_token_embedding_backward) token_embedding_backward;
+  decltype(&wf_token_embedding_backward_workspace_bytes) token_embedding_backward_workspace_bytes;
 };
 Library wf{};
 
@@ -374,6 +382,195 @@ variable_list token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t
   return {r.logprob, r.entropy, r.top_logprobs, r.top_tokens};
 }
 
+// ------------------------------------------------------------------ log probabilities without logits
+Tensor long_ids(const Tensor& t, const char* name) {
+  if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
+    throw BadValue(std::string(name) + " must be int64 or int32, got " + c10::toString(t.scalar_type()));
+  return t.to(at::kLong).contiguous();
+}
+
+std::pair<Tensor, Tensor> run_linear_logprobs(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& tokens,
+                                              int64_t ignore, at::IntArrayRef lead, Tensor* stats, void* status) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), d = x.size(1), vocab = w.size(0);
+  const int code = dtype_code(x.scalar_type());
+  const auto f32 = x.options().dtype(at::kFloat);
+  Tensor logprob = at::empty(lead, f32), entropy = at::empty(lead, f32);
+  if (stats) *stats = at::empty({2, rows}, f32);
+  const size_t n = wf.linear_token_logprobs_workspace_bytes(rows, vocab, d, code, on_16_bytes(x), on_16_bytes(w));
+  const Tensor ws = bytes(n, x);
+  check(wf.linear_token_logprobs(x.data_ptr(), w.data_ptr(), ptr(b), code, rows, vocab, d, x.stride(0), w.stride(0),
+                                 tokens.data_ptr<int64_t>(), ignore, logprob.data_ptr<float>(),
+                                 entropy.data_ptr<float>(), stats ? stats->data_ptr<float>() : nullptr, ptr(ws), n,
+                                 static_cast<int32_t*>(status), stream()));
+  return {logprob, entropy};
+}
+
+struct LinearLogprobsFunction : torch::autograd::Function<LinearLogprobsFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Optional& b,
+                               const Tensor& tokens, int64_t ignore, int64_t status) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor x2 = rows_of(x), w2 = rows_of(w), b2 = contiguous(b);
+    Tensor stats;
+    const auto lead = x.sizes().slice(0, x.dim() - 1);
+    auto [logprob, entropy] =
+        run_linear_logprobs(x2, w2, b2, tokens, ignore, lead, &stats, reinterpret_cast<void*>(status));
+    ctx->save_for_backward({to_save(x, x2), to_save(w, w2), b2, tokens, stats, entropy});
+    ctx->saved_data["bias"] = b.has_value();
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["status"] = status;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->set_materialize_grads(false);
+    return {logprob, entropy};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    once_only();
+    variable_list out(6);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor x = rows_of(saved[0]), w = rows_of(saved[1]), &b = saved[2], &tokens = saved[3], &stats = saved[4],
+                 &entropy = saved[5];
+    size_t edge = 2;
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    const bool need_b = needs_optional(ctx, "bias", edge);
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t rows = x.size(0), d = x.size(1), vocab = w.size(0);
+    const int code = dtype_code(x.scalar_type());
+    const Tensor gl = grads[0].defined() ? grads[0].contiguous() : Tensor(),
+                 gh = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    if (need_x) out[0] = at::empty(ctx->saved_data["shape"].toIntVector(), x.options());
+    if (need_w) out[1] = at::empty({vocab, d}, x.options());
+    if (need_b) out[2] = at::empty({vocab}, x.options());
+    const size_t n =
+        wf.linear_token_logprobs_backward_workspace_bytes(rows, vocab, d, code, on_16_bytes(x), on_16_bytes(w));
+    const Tensor ws = bytes(n, x);
+    check(wf.linear_token_logprobs_backward(
+        x.data_ptr(), w.data_ptr(), ptr(b), code, rows, vocab, d, x.stride(0), w.stride(0), tokens.data_ptr<int64_t>(),
+        ctx->saved_data["ignore"].toInt(), stats.data_ptr<float>(), entropy.data_ptr<float>(),
+        static_cast<const float*>(ptr(gl)), static_cast<const float*>(ptr(gh)), ptr(out[0]), ptr(out[1]), ptr(out[2]),
+        ptr(ws), n, reinterpret_cast<int32_t*>(ctx->saved_data["status"].toInt()), stream()));
+    return out;
+  }
+};
+
+variable_list linear_token_logprobs(const Tensor& x, const Tensor& w, const Tensor& tokens, const Tensor& b,
+                                    int64_t ignore, void* status, bool user_status) {
+  if (x.dim() < 1 || w.dim() != 2 || x.size(-1) != w.size(1) || w.numel() == 0)
+    throw BadValue("expected x (..., d) and weight (vocab, d) with sizes >= 1, got " + shape_of(x.sizes()) + " and " +
+                   shape_of(w.sizes()));
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  if (tokens.sizes() != lead)
+    throw BadValue("tokens " + shape_of(tokens.sizes()) + " do not match x " + shape_of(x.sizes()));
+  if (b.defined() && (b.dim() != 1 || b.size(0) != w.size(0)))
+    throw BadValue("bias " + shape_of(b.sizes()) + " does not match vocab=" + std::to_string(w.size(0)));
+  for (const Tensor* t : {&w, &b})
+    if (t->defined() && t->scalar_type() != x.scalar_type())
+      throw BadValue(std::string("x, weight and bias must have one type, got ") + c10::toString(x.scalar_type()) +
+                     " and " + c10::toString(t->scalar_type()));
+  check_devices(x, {&w, &tokens, &b});
+  dtype_code(x.scalar_type());
+  const Tensor flat = long_ids(tokens, "tokens");
+  if (wants_grad({&x, &w, &b})) {
+    if (user_status) throw BadValue("status is not supported on the differentiable path");
+    return LinearLogprobsFunction::apply(x, w, given(b), flat, ignore, reinterpret_cast<int64_t>(status));
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  auto [logprob, entropy] = run_linear_logprobs(rows_of(x), rows_of(w), b.defined() ? b.contiguous() : b, flat, ignore,
+                                                lead, nullptr, status);
+  return {logprob, entropy};
+}
+
+// ------------------------------------------------------------------ token embedding
+Tensor run_embedding(const Tensor& w, const Tensor& pw, const Tensor& tokens, const Tensor& positions, double scale,
+                     at::IntArrayRef lead, void* status) {
+  c10::cuda::CUDAGuard guard(w.device());
+  auto shape = lead.vec();
+  const int64_t seq = shape.empty() ? 1 : shape.back();
+  shape.push_back(w.size(1));
+  Tensor y = at::empty(shape, w.options());
+  check(wf.token_embedding(tokens.data_ptr<int64_t>(), tokens.numel(), w.data_ptr(), dtype_code(w.scalar_type()),
+                           w.size(0), w.size(1), w.stride(0), (float)scale, ptr(pw), pw.defined() ? pw.size(0) : 0,
+                           pw.defined() ? pw.stride(0) : 0,
+                           positions.defined() ? positions.data_ptr<int64_t>() : nullptr, std::max<int64_t>(seq, 1),
+                           y.data_ptr(), static_cast<int32_t*>(status), stream()));
+  return y;
+}
+
+struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& w, const Optional& pw, const Tensor& tokens,
+                        const Optional& positions, double scale, int64_t padding, const std::vector<int64_t>& lead,
+                        int64_t status) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor at = positions ? *positions : Tensor();
+    Tensor y = run_embedding(rows_of(w), pw ? rows_of(*pw) : Tensor(), tokens, at, scale, lead,
+                             reinterpret_cast<void*>(status));
+    ctx->save_for_backward({tokens, at});
+    ctx->saved_data["position_weight"] = pw.has_value();
+    ctx->saved_data["places"] = pw ? pw->size(0) : 0;
+    ctx->saved_data["vocab"] = w.size(0);
+    ctx->saved_data["seq"] = lead.empty() ? 1 : lead.back();
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    once_only();
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &tokens = saved[0], &positions = saved[1];
+    size_t edge = 1;
+    const bool need_w = ctx->needs_input_grad(0), need_p = needs_optional(ctx, "position_weight", edge);
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    const Tensor dy = rows_of(grads[0]);
+    const int64_t n = tokens.numel(), d = dy.size(1), seq = std::max<int64_t>(1, ctx->saved_data["seq"].toInt());
+    const int code = dtype_code(dy.scalar_type());
+    auto table = [&](int64_t rows, const Tensor& index, int64_t padding, double scale) {
+      Tensor dw = at::empty({rows, d}, dy.options());
+      const size_t bytes_n = wf.token_embedding_backward_workspace_bytes(n, rows, d, code, index.defined());
+      const Tensor ws = bytes(bytes_n, dy);
+      check(wf.token_embedding_backward(index.defined() ? index.data_ptr<int64_t>() : nullptr, n, seq, dy.data_ptr(),
+                                        code, rows, d, dy.stride(0), padding, (float)scale, dw.data_ptr(), ptr(ws),
+                                        bytes_n, stream()));
+      return dw;
+    };
+    variable_list out(8);
+    if (need_w)
+      out[0] = table(ctx->saved_data["vocab"].toInt(), tokens, ctx->saved_data["padding"].toInt(),
+                     ctx->saved_data["scale"].toDouble());
+    if (need_p) out[1] = table(ctx->saved_data["places"].toInt(), positions, -1, 1.0);
+    return out;
+  }
+};
+
+Tensor token_embedding(const Tensor& tokens, const Tensor& w, double scale, const Tensor& pw, const Tensor& positions,
+                       int64_t padding, void* status, bool user_status) {
+  if (w.dim() != 2 || w.numel() == 0)
+    throw BadValue("expected weight (vocab, d) with sizes >= 1, got " + shape_of(w.sizes()));
+  if (pw.defined() && (pw.dim() != 2 || pw.numel() == 0 || pw.size(1) != w.size(1)))
+    throw BadValue("position_weight " + shape_of(pw.sizes()) + " does not match weight " + shape_of(w.sizes()));
+  if (pw.defined() && pw.scalar_type() != w.scalar_type())
+    throw BadValue(std::string("weight and position_weight must have one type, got ") + c10::toString(w.scalar_type()) +
+                   " and " + c10::toString(pw.scalar_type()));
+  if (positions.defined() && !pw.defined()) throw BadValue("positions need a position_weight");
+  const auto lead = tokens.sizes();
+  if (positions.defined() && positions.sizes() != lead &&
+      (positions.dim() != 1 || lead.empty() || positions.size(0) != lead.back()))
+    throw BadValue("positions " + shape_of(positions.sizes()) + " are neither of the tokens' shape " + shape_of(lead) +
+                   " nor of its last axis");
+  if (padding >= w.size(0)) throw BadValue("padding_index must be below vocab=" + std::to_string(w.size(0)));
+  if (!std::isfinite(scale)) throw BadValue("scale must be finite");
+  check_devices(w, {&tokens, &pw, &positions});
+  dtype_code(w.scalar_type());
+  const Tensor flat = long_ids(tokens, "tokens"),
+               at = positions.defined() ? long_ids(positions.expand(lead), "positions") : Tensor();
+  if (wants_grad({&w, &pw})) {
+    if (user_status) throw BadValue("status is not supported on the differentiable path");
+    return EmbeddingFunction::apply(w, given(pw), flat, given(at), scale, padding, lead.vec(),
+                                    reinterpret_cast<int64_t>(status));
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return run_embedding(rows_of(w), pw.defined() ? rows_of(pw) : pw, flat, at, scale, lead, status);
+}
+
 // ------------------------------------------------------------------ Python
 template <typename F>
 PyObject* guarded(F f) {
@@ -428,6 +625,13 @@ PyObject* py_bind(PyObject*, PyObject* path) {
     find(wf.max_top_tokens, "wf_max_top_tokens");
     find(wf.token_logprobs, "wf_token_logprobs");
     find(wf.token_logprobs_backward, "wf_token_logprobs_backward");
+    find(wf.linear_token_logprobs, "wf_linear_token_logprobs");
+    find(wf.linear_token_logprobs_workspace_bytes, "wf_linear_token_logprobs_workspace_bytes");
+    find(wf.linear_token_logprobs_backward, "wf_linear_token_logprobs_backward");
+    find(wf.linear_token_logprobs_backward_workspace_bytes, "wf_linear_token_logprobs_backward_workspace_bytes");
+    find(wf.token_embedding, "wf_token_embedding");
+    find(wf.token_embedding_backward, "wf_token_embedding_backward");
+    find(wf.token_embedding_backward_workspace_bytes, "wf_token_embedding_backward_workspace_bytes");
     Py_RETURN_NONE;
   });
 }
@@ -484,11 +688,55 @@ PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// linear_token_logprobs(x, weight, tokens, bias, ignore_index, status pointer, the status is the user's)
+PyObject* py_linear_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 7);
+    const Tensor x = tensor_arg(a[0], "x"), w = tensor_arg(a[1], "weight"), tokens = tensor_arg(a[2], "tokens"),
+                 b = tensor_arg(a[3], "bias", true);
+    const int64_t ignore = int_arg(a[4]), status = int_arg(a[5]);
+    const bool user = a[6] == Py_True;
+    variable_list r;
+    {
+      Unlocked unlocked;
+      r = linear_token_logprobs(x, w, tokens, b, ignore, reinterpret_cast<void*>(status), user);
+    }
+    PyObject* out = PyTuple_New(2);
+    if (!out) return nullptr;
+    for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(out, i, THPVariable_Wrap(std::move(r[i])));
+    return out;
+  });
+}
+
+// token_embedding(tokens, weight, scale, position_weight, positions, padding_index or -1, status pointer,
+// the status is the user's)
+PyObject* py_token_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    count(n, 8);
+    const Tensor tokens = tensor_arg(a[0], "tokens"), w = tensor_arg(a[1], "weight"),
+                 pw = tensor_arg(a[3], "position_weight", true), positions = tensor_arg(a[4], "positions", true);
+    const double scale = PyFloat_AsDouble(a[2]);
+    if (PyErr_Occurred()) throw std::runtime_error("number expected");
+    const int64_t padding = int_arg(a[5]), status = int_arg(a[6]);
+    const bool user = a[7] == Py_True;
+    Tensor y;
+    {
+      Unlocked unlocked;
+      y = token_embedding(tokens, w, scale, pw, positions, padding, reinterpret_cast<void*>(status), user);
+    }
+    return THPVariable_Wrap(std::move(y));
+  });
+}
+
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_O, "Look the C ABI up in the library at this path."},
     {"fused_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_fused_linear)), METH_FASTCALL, nullptr},
     {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_layer_norm)), METH_FASTCALL, nullptr},
     {"token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_token_logprobs)), METH_FASTCALL,
+     nullptr},
+    {"linear_token_logprobs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_token_logprobs)),
+     METH_FASTCALL, nullptr},
+    {"token_embedding", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_token_embedding)), METH_FASTCALL,
      nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_wf_torch", "PyTorch calls over the wayfinder C ABI.", -1, methods,
