@@ -513,19 +513,22 @@ WF_API int wf_token_embedding(const int64_t* tokens, int64_t n, const void* weig
                               int64_t d, int64_t w_row_stride, float scale, const void* position_weight,
                               int64_t places, int64_t p_row_stride, const int64_t* positions, int64_t seq, void* y,
                               int32_t* status, void* stream);
-/* The gradient of one of its tables: dweight[v] = scale * the sum of dy's rows whose index is v,
- * (rows, d) contiguous of dtype, summed in fp32 in a fixed order.
+/* The gradients of its tables: dweight[v] = scale * the sum of dy's rows whose token is v, and
+ * dposition_weight[q] = the sum of those whose position is q; contiguous, 16-byte aligned, of dtype,
+ * each may be NULL; summed in fp32 in a fixed order.
  *
- *   index         : (n) int64, or NULL: i % seq (n a multiple of seq)
  *   dy            : (n, d) rows dy_row_stride apart
- *   padding_index : the index whose row gets no gradient, or -1.  Nor do indices outside the table
- *   workspace     : wf_token_embedding_backward_workspace_bytes() bytes, 256-byte aligned */
-WF_API size_t wf_token_embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t d, int32_t dtype,
-                                                          int32_t has_index);
-WF_API int wf_token_embedding_backward(const int64_t* index, int64_t n, int64_t seq, const void* dy, int32_t dtype,
-                                       int64_t rows, int64_t d, int64_t dy_row_stride, int64_t padding_index,
-                                       float scale, void* dweight, void* workspace, size_t workspace_bytes,
-                                       void* stream);
+ *   positions     : (n) int64, or NULL: i % seq (n a multiple of seq)
+ *   padding_index : the token whose row gets no gradient, or -1.  Nor do tokens and positions
+ *                   outside their table
+ *   workspace     : wf_token_embedding_backward_workspace_bytes() bytes, 256-byte aligned; vocab or
+ *                   places is 0 there where that gradient is not wanted */
+WF_API size_t wf_token_embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int64_t places, int64_t d,
+                                                          int32_t dtype, int32_t has_positions);
+WF_API int wf_token_embedding_backward(const int64_t* tokens, const int64_t* positions, int64_t n, int64_t seq,
+                                       const void* dy, int32_t dtype, int64_t d, int64_t dy_row_stride, int64_t vocab,
+                                       float scale, int64_t padding_index, void* dweight, int64_t places,
+                                       void* dposition_weight, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -67,15 +67,21 @@ def test_abi_validates_before_launch():
     assert embed(w=None) == bad and b"null" in lib.wf_last_error()
     assert embed(n=0, w=None) == _lib.WF_OK
 
-    def embed_bwd(index=p, n=100, seq=10, rows=50, d=64, out=p, ws=p, short=1):
-        size = lib.wf_token_embedding_backward_workspace_bytes(n, rows, d, 0, index is not None)
-        return lib.wf_token_embedding_backward(index, n, seq, p, 0, rows, d, d, -1, 1.0, out, ws, size - short, None)
+    def embed_bwd(tokens=p, positions=None, n=100, seq=10, d=64, out=p, places=20, dpos=p, ws=p, short=1, dtype=0):
+        size = lib.wf_token_embedding_backward_workspace_bytes(n, 50 if out else 0, places if dpos else 0, d, 0,
+                                                               positions is not None)
+        return lib.wf_token_embedding_backward(tokens, positions, n, seq, p, dtype, d, d, 50, 1.0, -1, out, places, dpos, ws,
+                                               size - short, None)
 
     assert embed_bwd() == bad and b"workspace" in lib.wf_last_error()
-    assert embed_bwd(index=None) == bad and b"workspace" in lib.wf_last_error()
-    assert embed_bwd(index=None, seq=7) == bad and b"multiple of seq" in lib.wf_last_error()
-    assert embed_bwd(out=None) == bad and b"null" in lib.wf_last_error()
-    assert lib.wf_token_embedding_backward_workspace_bytes(0, 50, 64, 0, 1) == 0
+    assert embed_bwd(dpos=None) == bad and b"workspace" in lib.wf_last_error()
+    assert embed_bwd(positions=p, out=None) == bad and b"workspace" in lib.wf_last_error()
+    assert embed_bwd(seq=7) == bad and b"multiple of seq" in lib.wf_last_error()
+    assert embed_bwd(tokens=None) == bad and b"null" in lib.wf_last_error()
+    assert embed_bwd(places=0) == bad and embed_bwd(dtype=9) == bad
+    assert embed_bwd(out=ctypes.c_void_p(4104)) == bad and b"aligned" in lib.wf_last_error()
+    assert embed_bwd(out=None, dpos=None) == _lib.WF_OK  # nothing is asked for
+    assert lib.wf_token_embedding_backward_workspace_bytes(0, 50, 0, 64, 0, 1) == 0
 
     def head(dtype=0, rows=4, V=8, d=8, xs=8, ws=8, tokens=p, n=0):
         return lib.wf_linear_token_logprobs(p, p, None, dtype, rows, V, d, xs, ws, tokens, -100, p, p, None, p, n, None, None)

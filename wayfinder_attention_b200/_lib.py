@@ -203,9 +203,9 @@ def _declare(lib: ctypes.CDLL) -> None:
          [_vp] * 3 + [_i32] + [_i64] * 5 + [_vp, _i64] + [_vp] * 8 + [sz, _vp, _vp]),
         ("wf_token_embedding", ctypes.c_int,
          [_vp, _i64, _vp, _i32, _i64, _i64, _i64, _f32, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
-        ("wf_token_embedding_backward_workspace_bytes", sz, [_i64] * 3 + [_i32] * 2),
+        ("wf_token_embedding_backward_workspace_bytes", sz, [_i64] * 4 + [_i32] * 2),
         ("wf_token_embedding_backward", ctypes.c_int,
-         [_vp, _i64, _i64, _vp, _i32] + [_i64] * 4 + [_f32, _vp, _vp, sz, _vp]),
+         [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _i64, _i64, _f32, _i64, _vp, _i64, _vp, _vp, sz, _vp]),
     ):
         f = getattr(lib, name)
         f.restype, f.argtypes = restype, argtypes

@@ -1051,30 +1051,37 @@ int wf_token_embedding(const int64_t* tokens, int64_t n, const void* weight, int
   return rc ? cuda_fail(rc, "wf_token_embedding") : ok();
 }
 
-size_t wf_token_embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t d, int32_t dtype,
-                                                   int32_t has_index) {
-  if (n <= 0 || rows <= 0 || d <= 0 || !valid_dtype(dtype)) return 0;
-  return wf::embedding_backward_workspace_bytes(n, rows, d, dtype, !has_index);
+size_t wf_token_embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int64_t places, int64_t d, int32_t dtype,
+                                                   int32_t has_positions) {
+  if (n <= 0 || vocab < 0 || places < 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  return wf::embedding_backward_workspace_bytes(n, vocab, places, d, dtype, has_positions);
 }
 
-int wf_token_embedding_backward(const int64_t* index, int64_t n, int64_t seq, const void* dy, int32_t dtype,
-                                int64_t rows, int64_t d, int64_t dy_row_stride, int64_t padding_index, float scale,
-                                void* dweight, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_embedding("wf_token_embedding_backward", dtype, n, rows, d, dy_row_stride);
+int wf_token_embedding_backward(const int64_t* tokens, const int64_t* positions, int64_t n, int64_t seq, const void* dy,
+                                int32_t dtype, int64_t d, int64_t dy_row_stride, int64_t vocab, float scale,
+                                int64_t padding_index, void* dweight, int64_t places, void* dposition_weight,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = WF_OK;
+  if (dweight) rc = check_embedding("wf_token_embedding_backward", dtype, n, vocab, d, dy_row_stride);
+  if (!rc && dposition_weight) rc = check_embedding("wf_token_embedding_backward", dtype, n, places, d, dy_row_stride);
   if (rc) return rc;
-  if (!dweight) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (!dweight && !dposition_weight) return ok();
+  if ((reinterpret_cast<uintptr_t>(dweight) | reinterpret_cast<uintptr_t>(dposition_weight)) % 16)
+    return fail(WF_ERR_INVALID_ARGUMENT, "wf_token_embedding_backward: gradients must be 16-byte aligned");
   if (n > 0) {
-    if (!dy) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
-    if (!index && (seq < 1 || n % seq))
-      return fail(WF_ERR_INVALID_ARGUMENT, "without an index n must be a multiple of seq (n=%lld, seq=%lld)",
+    if (!dy || (dweight && !tokens)) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
+    if (dposition_weight && !positions && (seq < 1 || n % seq))
+      return fail(WF_ERR_INVALID_ARGUMENT, "without positions n must be a multiple of seq (n=%lld, seq=%lld)",
                   (long long)n, (long long)seq);
     if ((rc = check_workspace("wf_token_embedding_backward", workspace, workspace_bytes,
-                              wf::embedding_backward_workspace_bytes(n, rows, d, dtype, !index))))
+                              wf::embedding_backward_workspace_bytes(n, dweight ? vocab : 0, dposition_weight ? places : 0,
+                                                                     d, dtype, positions != nullptr))))
       return rc;
   }
   wf::EmbeddingBwdParams p{};
-  p.index = index; p.dy = dy; p.dweight = dweight;
-  p.n = n; p.seq = seq; p.rows = rows; p.d = d; p.dy_stride = dy_row_stride; p.padding_index = padding_index;
+  p.tokens = tokens; p.positions = positions; p.dy = dy; p.dweight = dweight; p.dposition_weight = dposition_weight;
+  p.n = n; p.seq = seq; p.vocab = vocab; p.places = places; p.d = d; p.dy_stride = dy_row_stride;
+  p.padding_index = padding_index;
   p.scale = scale;
   p.ws = workspace;
   rc = wf::launch_embedding_backward(p, dtype, static_cast<cudaStream_t>(stream));

@@ -19,6 +19,12 @@ __device__ __forceinline__ float max_keep_nan(float a, float b) {
   return y;
 }
 
+__device__ __forceinline__ float max_keep_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 // gelu for 16-bit results, two values at a time with the polynomials in paired arithmetic
 // (erff takes both of its branches in most warps).  Paired instructions take no immediates:
 // the constants are made once, and hidden from the compiler so that it keeps them in registers

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(EmbeddingParams p, 
     const int64_t row = row0 + r;
     token[r] = row < p.n ? p.tokens[row] : 0;
     place[r] = 0;
-    if (p.position_weight && row < p.n) place[r] = p.positions ? p.positions[row] : row % p.seq;
+    if (p.position_weight && row < p.n) place[r] = p.positions ? p.positions[row] : (uint32_t)row % (uint32_t)p.seq;
     bad[r] = (uint64_t)token[r] >= (uint64_t)p.vocab || (p.position_weight && (uint64_t)place[r] >= (uint64_t)p.places);
     if (bad[r]) {
       token[r] = place[r] = 0;
@@ -77,59 +77,102 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(EmbeddingParams p, 
 }
 
 // ------------------------------------------------------------------ sort
-// Stable radix sort of (index, position) pairs.  A block takes kTile of them: a warp ranks 32 at
-// a time by a match over its lanes, on top of its own count of each digit so far.
-constexpr int kTile = 4096, kSortThreads = 512, kSortWarps = kSortThreads / 32, kPerWarp = kTile / kSortWarps;
-constexpr int kMaxDigits = 512;
-constexpr int kScanBlocks = 64;
-
-struct SortParams {
-  const int64_t* index;  // the first pass reads these; later ones `from`
-  const uint64_t* from;  // index above, position below
-  uint64_t* to;
+// The gradients of up to two tables are made side by side, a table's blocks in each launch.
+struct Table {
+  const int64_t* index;  // [n]; null: i % seq
+  uint64_t* entries[2];  // sorted lists, by turns: index above, position below
   int* counts;           // [blocks][digits]; null where one block has all
   int* totals;           // [digits] where sort_scan_kernel has made the counts places within their digit, or null
-  int64_t n;
+  void* out;             // [rows][d]
+  float* partials;       // [chunks][2][pitch]: a chunk's first row where it began before, its last where it goes on
   int64_t rows, skip;    // indices outside [0, rows), and `skip`, sort behind all others (as `rows`)
-  int shift, bits;
+  int64_t fill0, fill1;  // bytes of out to be zeroed
+  int passes, bits;
+  float scale;
 };
-__device__ __forceinline__ uint64_t sort_entry(const SortParams& p, int64_t i) {
-  if (p.from) return p.from[i];
-  const int64_t t = p.index[i];
-  const bool in = t >= 0 && t < p.rows && t != p.skip;
-  return (uint64_t)(in ? t : p.rows) << 32 | (uint32_t)i;
-}
-__device__ __forceinline__ int digit_of(const SortParams& p, uint64_t e) {
-  return (int)(e >> (32 + p.shift)) & ((1 << p.bits) - 1);
+struct Tables {
+  Table t[2];
+  int64_t n, seq;
+};
+
+// Zeroes a share of a table: the sort's launches leave most of the GPU idle, and each does a part.
+__device__ __forceinline__ void fill_share(const Table& t, int share, int shares, int64_t thread, int64_t threads) {
+  const int64_t bytes = t.fill1 - t.fill0;
+  unsigned char* out = static_cast<unsigned char*>(t.out);
+  int64_t a = t.fill0 + bytes * share / shares, b = t.fill0 + bytes * (share + 1) / shares;
+  const int64_t a16 = min((a + 15) / 16 * 16, b), b16 = max(b / 16 * 16, a16);
+  if (thread < a16 - a) out[a + thread] = 0;
+  if (thread < b - b16) out[b16 + thread] = 0;
+  for (int64_t i = a16 + 16 * thread; i < b16; i += 16 * threads) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortParams p) {
+// Stable radix sort of (index, position) pairs, 8 or 9 bits a pass.  A block's warps take kRounds
+// times 32 of them each, and rank them 32 at a time, by ballots of the digit's bits, on top of
+// their own count of each digit so far.  (A match instruction in place of the ballots: twice the
+// time.)
+constexpr int kRounds = 8, kMaxDigits = 512, kScanBlocks = 256;
+constexpr int kSortWarps = 4, kAloneWarps = 16;  // of many blocks, and of one that has all
+constexpr int kTile = 32 * kRounds * kSortWarps, kAlone = 32 * kRounds * kAloneWarps;
+
+__device__ __forceinline__ uint64_t sort_entry(const Tables& p, const Table& t, int pass, int64_t i) {
+  if (pass) return t.entries[(pass - 1) & 1][i];
+  const int64_t v = t.index[i];
+  const bool in = v >= 0 && v < t.rows && v != t.skip;
+  return (uint64_t)(in ? v : t.rows) << 32 | (uint32_t)i;
+}
+__device__ __forceinline__ int digit_of(uint64_t e, int pass, int bits) {
+  return (int)(e >> (32 + pass * bits)) & ((1 << bits) - 1);
+}
+// The lanes that hold this lane's digit (in-range lanes only).
+__device__ __forceinline__ unsigned lanes_of(int digit, int bits, bool in) {
+  unsigned same = __ballot_sync(0xffffffffu, in);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned ones = __ballot_sync(0xffffffffu, digit >> b & 1);
+    same &= digit >> b & 1 ? ones : ~ones;
+  }
+  return same;
+}
+
+__global__ void __launch_bounds__(32 * kSortWarps) sort_count_kernel(Tables p, int pass, int blocks, int share,
+                                                                     int shares) {
+  constexpr int THREADS = 32 * kSortWarps;
   __shared__ int count[kMaxDigits];
   pdl_wait();
-  const int digits = 1 << p.bits;
-  for (int d = threadIdx.x; d < digits; d += kSortThreads) count[d] = 0;
+  const Table& t = p.t[blockIdx.y];
+  if ((int)blockIdx.x >= blocks) {
+    fill_share(t, share, shares, (int64_t)(blockIdx.x - blocks) * THREADS + threadIdx.x, (int64_t)(gridDim.x - blocks) * THREADS);
+    return;
+  }
+  if (pass >= t.passes) return;
+  const int digits = 1 << t.bits;
+  for (int d = threadIdx.x; d < digits; d += THREADS) count[d] = 0;
   __syncthreads();
-  const int64_t i0 = (int64_t)blockIdx.x * kTile;
+  const int64_t i0 = (int64_t)blockIdx.x * kTile + threadIdx.x;
+  uint64_t entry[kRounds];
 #pragma unroll
-  for (int k = 0; k < kTile / kSortThreads; ++k) {
-    const int64_t i = i0 + k * kSortThreads + threadIdx.x;
-    const int d = i < p.n ? digit_of(p, sort_entry(p, i)) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, d);
-    if (d >= 0 && (same & lanemask_lt()) == 0) atomicAdd(&count[d], __popc(same));
+  for (int k = 0; k < kRounds; ++k) entry[k] = i0 + k * THREADS < p.n ? sort_entry(p, t, pass, i0 + k * THREADS) : 0;
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) {
+    const bool in = i0 + k * THREADS < p.n;
+    const int d = digit_of(entry[k], pass, t.bits);
+    const unsigned same = lanes_of(d, t.bits, in);
+    if (in && (same & lanemask_lt()) == 0) atomicAdd(&count[d], __popc(same));
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += kSortThreads) p.counts[(int64_t)blockIdx.x * digits + d] = count[d];
+  for (int d = threadIdx.x; d < digits; d += THREADS) t.counts[(int64_t)blockIdx.x * digits + d] = count[d];
 }
 
 // Many blocks: their counts of a digit become each block's first place within it.  A block a digit.
-__global__ void __launch_bounds__(kThreads) sort_scan_kernel(SortParams p, int blocks) {
+__global__ void __launch_bounds__(kThreads) sort_scan_kernel(Tables p, int pass, int blocks) {
   __shared__ int warp_total[kThreads / 32];
   pdl_wait();
-  const int digits = 1 << p.bits, d = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Table& t = p.t[blockIdx.y];
+  const int digits = 1 << t.bits, d = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (pass >= t.passes || d >= digits) return;
   int so_far = 0;
   for (int b0 = 0; b0 < blocks; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    const int c = b < blocks ? p.counts[(int64_t)b * digits + d] : 0;
+    const int c = b < blocks ? t.counts[(int64_t)b * digits + d] : 0;
     int scan = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -143,55 +186,70 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(SortParams p, int b
       if (w < warp) place += warp_total[w];
       so_far += warp_total[w];
     }
-    if (b < blocks) p.counts[(int64_t)b * digits + d] = place;
+    if (b < blocks) t.counts[(int64_t)b * digits + d] = place;
     __syncthreads();
   }
-  if (threadIdx.x == 0) p.totals[d] = so_far;
+  if (threadIdx.x == 0) t.totals[d] = so_far;
 }
 
 // Without counts the block's own are all there are.
-__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortParams p) {
-  __shared__ int at[kSortWarps][kMaxDigits];  // counts, then places
-  __shared__ int warp_total[kSortWarps];
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) sort_place_kernel(Tables p, int pass, int blocks, int share, int shares) {
+  constexpr int THREADS = 32 * WARPS, EACH = kMaxDigits / THREADS > 1 ? kMaxDigits / THREADS : 1;
+  __shared__ int at[WARPS][kMaxDigits];  // counts, then places
+  __shared__ int warp_total[WARPS];
   pdl_wait();
-  const int digits = 1 << p.bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Table& t = p.t[blockIdx.y];
+  if ((int)blockIdx.x >= blocks) {
+    fill_share(t, share, shares, (int64_t)(blockIdx.x - blocks) * THREADS + threadIdx.x, (int64_t)(gridDim.x - blocks) * THREADS);
+    return;
+  }
+  if (pass >= t.passes) return;
+  const int digits = 1 << t.bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int d = lane; d < digits; d += 32) at[warp][d] = 0;
   __syncwarp();
-  const int64_t i0 = (int64_t)blockIdx.x * kTile + warp * kPerWarp + lane;
-  constexpr int kRounds = kPerWarp / 32;
+  const int64_t i0 = ((int64_t)blockIdx.x * WARPS + warp) * 32 * kRounds + lane;
   uint64_t entry[kRounds];
   int rank[kRounds];
 #pragma unroll
-  for (int k = 0; k < kRounds; ++k) entry[k] = i0 + 32 * k < p.n ? sort_entry(p, i0 + 32 * k) : 0;
+  for (int k = 0; k < kRounds; ++k) entry[k] = i0 + 32 * k < p.n ? sort_entry(p, t, pass, i0 + 32 * k) : 0;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
-    const int d = i0 + 32 * k < p.n ? digit_of(p, entry[k]) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, d), before = same & lanemask_lt();
-    const int so_far = d >= 0 ? at[warp][d] : 0;
+    const bool in = i0 + 32 * k < p.n;
+    const int d = digit_of(entry[k], pass, t.bits);
+    const unsigned same = lanes_of(d, t.bits, in), before = same & lanemask_lt();
+    const int so_far = at[warp][d];
     __syncwarp();
-    if (d >= 0 && !before) at[warp][d] = so_far + __popc(same);
+    if (in && !before) at[warp][d] = so_far + __popc(same);
     __syncwarp();
     rank[k] = so_far + __popc(before);
   }
   __syncthreads();
-  // each digit's place: all of the smaller ones, and this one's in the blocks before
-  int total = 0, before = 0;
-  const int d = threadIdx.x;
-  if (d < digits) {
-    if (p.totals) {
-      total = p.totals[d];
-      before = p.counts[(int64_t)blockIdx.x * digits + d];
-    } else if (p.counts) {
-      for (int b = 0; b < (int)gridDim.x; ++b) {
-        const int c = p.counts[(int64_t)b * digits + d];
-        total += c;
-        if (b < (int)blockIdx.x) before += c;
+  // each digit's place: all of the smaller ones, and this one's in the blocks before.  A thread
+  // takes EACH neighbours.
+  int total[EACH], before[EACH], sum = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int d = threadIdx.x * EACH + e;
+    total[e] = before[e] = 0;
+    if (d < digits) {
+      if (t.totals) {
+        total[e] = t.totals[d];
+        before[e] = t.counts[(int64_t)blockIdx.x * digits + d];
+      } else if (t.counts) {
+#pragma unroll 8
+        for (int b = 0; b < blocks; ++b) {
+          const int c = t.counts[(int64_t)b * digits + d];
+          total[e] += c;
+          if (b < (int)blockIdx.x) before[e] += c;
+        }
+      } else {
+        for (int w = 0; w < WARPS; ++w) total[e] += at[w][d];
       }
-    } else {
-      for (int w = 0; w < kSortWarps; ++w) total += at[w][d];
     }
+    sum += total[e];
   }
-  int scan = total;
+  int scan = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, scan, o);
@@ -199,34 +257,48 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortParams p) 
   }
   if (lane == 31) warp_total[warp] = scan;
   __syncthreads();
-  if (d < digits) {
-    int place = scan - total + before;
-    for (int w = 0; w < warp; ++w) place += warp_total[w];
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = at[w][d];
-      at[w][d] = place;
-      place += c;
+  int first = scan - sum;
+  for (int w = 0; w < warp; ++w) first += warp_total[w];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int d = threadIdx.x * EACH + e;
+    if (d < digits) {
+      int place = first + before[e];
+      for (int w = 0; w < WARPS; ++w) {
+        const int c = at[w][d];
+        at[w][d] = place;
+        place += c;
+      }
     }
+    first += total[e];
   }
   __syncthreads();
+  uint64_t* to = t.entries[pass & 1];
 #pragma unroll
   for (int k = 0; k < kRounds; ++k)
-    if (i0 + 32 * k < p.n) p.to[at[warp][digit_of(p, entry[k])] + rank[k]] = entry[k];
+    if (i0 + 32 * k < p.n) to[at[warp][digit_of(entry[k], pass, t.bits)] + rank[k]] = entry[k];
+}
+
+__global__ void __launch_bounds__(kThreads) fill_kernel(Tables p) {
+  pdl_wait();
+  fill_share(p.t[blockIdx.y], 0, 1, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
 }
 
 // ------------------------------------------------------------------ sums
-// The sorted list: as sorted, or that of the positions 0 .. seq - 1 of n / seq sequences.
-struct Sorted {
+// A table's sorted list: as sorted, or that of the positions 0 .. seq - 1 of n / seq sequences.
+struct List {
   const uint64_t* entries;
-  int64_t n, seq, batch;
+  int64_t seq, batch;
+  __device__ __forceinline__ List(const Tables& p, const Table& t)
+      : entries(t.index ? t.entries[(t.passes - 1) & 1] : nullptr), seq(p.seq), batch(t.index ? 0 : p.n / p.seq) {}
   __device__ __forceinline__ void get(int64_t i, int& row, int& from) const {
     if (entries) {
       const uint64_t e = entries[i];
       row = (int)(e >> 32);
       from = (int)(uint32_t)e;
     } else {
-      row = (int)(i / batch);
-      from = (int)(i - row * batch) * (int)seq + row;
+      row = (int)((uint32_t)i / (uint32_t)batch);
+      from = ((int)i - row * (int)batch) * (int)seq + row;
     }
   }
   __device__ __forceinline__ int row(int64_t i) const {
@@ -235,71 +307,80 @@ struct Sorted {
     return r;
   }
 };
-struct SumParams {
-  Sorted list;
+struct Sum {
   const void* dy;
-  void* out;        // [rows][d]
-  float* partials;  // [chunks][2][pitch]: a chunk's first row where it began before, its last where it goes on
-  int64_t stride, d, pitch, rows;
-  int chunk;
-  float scale;
+  int64_t stride, d, pitch;
+  int chunk;  // 32 at most: a warp has a chunk's list in its lanes
 };
 constexpr int kAhead = 8;  // rows of dy on their way at once
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams p, int log_g) {
+__global__ void __launch_bounds__(kThreads) embedding_sum_kernel(Tables tables, Sum p, int log_g) {
   pdl_wait();
-  const int g = 1 << log_g;
+  const Table& t = tables.t[blockIdx.z];
+  const List list(tables, t);
+  const int g = 1 << log_g, lane = threadIdx.x & 31;  // g is a warp at least
   const int64_t chunk = (int64_t)blockIdx.x * (kThreads >> log_g) + (threadIdx.x >> log_g);
-  const int64_t c = ((int64_t)blockIdx.y * g + (threadIdx.x & (g - 1))) * VEC;
-  const int64_t i0 = chunk * p.chunk;
-  if (i0 >= p.list.n || c >= p.d) return;
-  const int64_t i1 = min(i0 + p.chunk, p.list.n);
+  const int64_t c = ((int64_t)blockIdx.y * g + (threadIdx.x & (g - 1))) * VEC, i0 = chunk * p.chunk;
+  const bool on = c < p.d;
+  if (i0 >= tables.n) return;
+  const int64_t i1 = min(i0 + p.chunk, tables.n);
+  int my_row = (int)t.rows, my_from = 0;
+  if (i0 + lane < i1) list.get(i0 + lane, my_row, my_from);
+  const int outside = lane == 0 ? (i0 ? list.row(i0 - 1) : -1) : lane == 1 ? (i1 < tables.n ? list.row(i1) : -1) : 0;
+  const int n = __popc(__ballot_sync(0xffffffffu, my_row < t.rows));  // those that count come first
+  if (n == 0) return;
+  const int before = __shfl_sync(0xffffffffu, outside, 0), after = __shfl_sync(0xffffffffu, outside, 1);
   const T* dy = static_cast<const T*>(p.dy) + c;
   float sum[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
-  const int before = i0 ? p.list.row(i0 - 1) : -1, after = i1 < p.list.n ? p.list.row(i1) : -1;
-  int row = p.list.row(i0);
+  int row = __shfl_sync(0xffffffffu, my_row, 0);
   bool open = row == before;  // the row began in an earlier chunk
-  if (row >= p.rows) return;
   auto flush = [&](bool goes_on) {
+    if (!on) return;
     if (open || goes_on) {
-      float* to = p.partials + (2 * chunk + (open ? 0 : 1)) * p.pitch + c;
+      float* to = t.partials + (2 * chunk + (open ? 0 : 1)) * p.pitch + c;
+      if constexpr (VEC == 1) {
+        *to = sum[0];
+      } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) to[j] = sum[j];
+        for (int j = 0; j < VEC; j += 4)
+          *reinterpret_cast<float4*>(to + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+      }
     } else {
       float f[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = sum[j] * p.scale;
-      store_vec<T, VEC>(static_cast<T*>(p.out) + row * p.d + c, f);
+      for (int j = 0; j < VEC; ++j) f[j] = sum[j] * t.scale;
+      store_vec<T, VEC>(static_cast<T*>(t.out) + row * p.d + c, f);
     }
   };
-  for (int64_t i = i0; i < i1; i += kAhead) {
-    int rows[kAhead], from[kAhead];
-    RawVec<T, VEC> v[kAhead];
+  RawVec<T, VEC> v[kAhead];
+  auto load = [&](int k, int i) {
+    const int from = __shfl_sync(0xffffffffu, my_from, i & 31);
+    if (i < n && on) v[k].load(dy + from * p.stride);
+  };
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) load(k, k);
+  for (int i = 0; i < n; i += kAhead) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      rows[k] = (int)p.rows;
-      if (i + k < i1) p.list.get(i + k, rows[k], from[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (rows[k] < p.rows) v[k].load(dy + from[k] * p.stride);
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (rows[k] >= p.rows) break;  // the end of the chunk, or of the indices that count
-      if (rows[k] != row) {
+      if (i + k >= n) break;
+      const int next = __shfl_sync(0xffffffffu, my_row, i + k);
+      if (next != row) {
         flush(false);
-        row = rows[k];
+        row = next;
         open = false;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) sum[j] = 0.f;
       }
       float f[VEC];
       v[k].unpack(f);
+      load(k, i + k + kAhead);
+      if (on) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[j] += f[j];
+        for (int j = 0; j < VEC; ++j) sum[j] += f[j];
+      }
     }
   }
   flush(row == after);
@@ -309,21 +390,23 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(SumParams p, in
 // the first that the row does not fill.  A block takes 128 columns; its warps share the parts.
 constexpr int kJoinWarps = 4;
 template <typename T>
-__global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(SumParams p, int chunks) {
+__global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(Tables tables, Sum p, int chunks) {
   __shared__ float4 part[kJoinWarps][32];
   pdl_wait();
+  const Table& t = tables.t[blockIdx.z];
+  const List list(tables, t);
   const int chunk = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t i0 = (int64_t)chunk * p.chunk, i1 = i0 + p.chunk;
-  if (i1 >= p.list.n) return;
-  const int row = p.list.row(i1 - 1);
-  if (row >= p.rows || p.list.row(i1) != row) return;                            // ends here
-  if (p.list.row(i0) == row && i0 && p.list.row(i0 - 1) == row) return;          // began before
+  if (i1 >= tables.n) return;
+  const int row = list.row(i1 - 1), next = list.row(i1), first = list.row(i0), before = i0 ? list.row(i0 - 1) : -1;
+  if (row >= t.rows || next != row) return;    // ends here
+  if (first == row && before == row) return;   // began before
   int more = 0;  // chunks that the row fills
   for (int k = chunk + 1;;) {
     const int mine = k + threadIdx.x;
     const int64_t end = (int64_t)(mine + 1) * p.chunk;
     // filled, and going on in the next
-    const bool filled = mine < chunks && end < p.list.n && p.list.row(end) == row;
+    const bool filled = mine < chunks && end < tables.n && list.row(end) == row;
     const int n = __syncthreads_count(filled);
     more += n;
     k += n;
@@ -336,7 +419,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(SumPara
 #pragma unroll 4
     for (int k = warp; k < parts; k += kJoinWarps) {
       const float4 f =
-          *reinterpret_cast<const float4*>(p.partials + (2 * (int64_t)(chunk + k) + (k ? 0 : 1)) * p.pitch + c);
+          *reinterpret_cast<const float4*>(t.partials + (2 * (int64_t)(chunk + k) + (k ? 0 : 1)) * p.pitch + c);
       s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w;
     }
   part[warp][lane] = s;
@@ -346,8 +429,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(SumPara
     const float4 f = part[w][lane];
     s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w;
   }
-  const float v[4] = {s.x * p.scale, s.y * p.scale, s.z * p.scale, s.w * p.scale};
-  T* to = static_cast<T*>(p.out) + row * p.d + c;
+  const float v[4] = {s.x * t.scale, s.y * t.scale, s.z * t.scale, s.w * t.scale};
+  T* to = static_cast<T*>(t.out) + row * p.d + c;
   for (int j = 0; j < 4 && c + j < p.d; ++j) to[j] = from_f32<T>(v[j]);
 }
 
@@ -357,31 +440,38 @@ int bits_of(int64_t most) {  // of the numbers 0 .. most
   while (most >> b) ++b;
   return b;
 }
-struct SumPlan {
-  int passes, bits, blocks, chunk, log_g, columns;  // columns: blocks over a row
-  int64_t chunks;
+struct TablePlan {
+  int passes, bits;
   size_t entries, counts, partials;
   size_t bytes() const { return 2 * entries + counts + partials; }
 };
-SumPlan sum_plan(int64_t n, int64_t rows, int64_t d, bool sorted, int vec) {
+struct SumPlan {
+  int blocks, chunk, log_g, columns;  // of the sort; of a list; threads a row; blocks over a row
+  int64_t chunks;
+};
+SumPlan sum_plan(int64_t n, int64_t d, int vec) {
   SumPlan s{};
-  if (!sorted) {
-    const int bits = bits_of(rows);
-    s.passes = (bits + 8) / 9;
-    s.bits = (bits + s.passes - 1) / s.passes;
-    s.blocks = (int)((n + kTile - 1) / kTile);
-    s.entries = round256((size_t)n * sizeof(uint64_t));
-    s.counts = s.blocks > 1 ? round256((size_t)(s.blocks + 1) * (1 << s.bits) * sizeof(int)) : 0;
-  }
+  s.blocks = n <= kAlone ? 1 : (int)((n + kTile - 1) / kTile);
   const int64_t vectors = (d + vec - 1) / vec;
-  const int g = group_of(vectors);
+  const int g = std::max(32, group_of(vectors));
   s.log_g = bits_of(g) - 1;
   s.columns = (int)((vectors + g - 1) / g);
   s.chunk = 32;
   while (s.chunk > 8 && (n + s.chunk - 1) / s.chunk * vectors < 512 * kSms) s.chunk /= 2;
   s.chunks = (n + s.chunk - 1) / s.chunk;
-  s.partials = round256((size_t)s.chunks * 2 * ((d + 7) / 8 * 8) * sizeof(float));
   return s;
+}
+TablePlan table_plan(const SumPlan& s, int64_t n, int64_t rows, int64_t d, bool sorted) {
+  TablePlan t{};
+  if (!sorted) {
+    const int bits = bits_of(rows);
+    t.passes = (bits + 8) / 9;
+    t.bits = (bits + t.passes - 1) / t.passes;
+    t.entries = round256((size_t)n * sizeof(uint64_t));
+    t.counts = s.blocks > 1 ? round256((size_t)(s.blocks + 1) * (1 << t.bits) * sizeof(int)) : 0;
+  }
+  t.partials = round256((size_t)s.chunks * 2 * round8(d) * sizeof(float));
+  return t;
 }
 int vec_of(int dtype, const void* a, int64_t stride_a, const void* b, int64_t stride_b, int64_t d) {
   const int64_t size = dtype == kF32 ? 4 : 2;
@@ -410,68 +500,120 @@ int launch_fwd_type(const EmbeddingParams& p, int dtype, cudaStream_t stream) {
 }
 
 template <typename T, int VEC>
-int launch_sum(const SumPlan& s, const SumParams& q, cudaStream_t stream) {
+int launch_sums(const SumPlan& s, const Tables& tables, int count, const Sum& q, cudaStream_t stream) {
   const int per_block = kThreads >> s.log_g;
   if (cudaError_t e = launch_pdl(embedding_sum_kernel<T, VEC>,
-                                 dim3((unsigned)((s.chunks + per_block - 1) / per_block), s.columns), dim3(kThreads), 0,
-                                 stream, q, s.log_g))
+                                 dim3((unsigned)((s.chunks + per_block - 1) / per_block), s.columns, count),
+                                 dim3(kThreads), 0, stream, tables, q, s.log_g))
     return (int)e;
   if (s.chunks == 1) return 0;
-  return (int)launch_pdl(embedding_join_kernel<T>, dim3((unsigned)s.chunks, (unsigned)((q.d + 127) / 128)),
-                         dim3(32 * kJoinWarps), 0, stream, q, (int)s.chunks);
+  return (int)launch_pdl(embedding_join_kernel<T>, dim3((unsigned)s.chunks, (unsigned)((q.d + 127) / 128), count),
+                         dim3(32 * kJoinWarps), 0, stream, tables, q, (int)s.chunks);
+}
+
+int launch_sort(const SumPlan& s, const Tables& tables, int count, cudaStream_t stream) {
+  int passes = 0, digits = 0;
+  int64_t fill = 0;
+  bool scan = false;
+  for (int i = 0; i < count; ++i) {
+    const Table& t = tables.t[i];
+    passes = std::max(passes, t.passes);
+    digits = std::max(digits, t.passes ? 1 << t.bits : 0);
+    fill = std::max(fill, t.fill1 - t.fill0);
+    scan |= t.totals != nullptr;
+  }
+  // enough blocks to fill at full rate, 16 KB a block and launch at least
+  const int shares = std::max(1, passes * (s.blocks > 1 ? 2 : 1));
+  const int fillers = (int)std::min<int64_t>(((fill + shares - 1) / shares + 16383) / 16384, 8 * kSms);
+  if (!passes) {
+    if (!fill) return 0;
+    return (int)launch_pdl(fill_kernel, dim3(fillers, count), dim3(kThreads), 0, stream, tables);
+  }
+  int share = 0;
+  for (int pass = 0; pass < passes; ++pass) {
+    cudaError_t e = cudaSuccess;
+    if (s.blocks == 1) {
+      e = launch_pdl(sort_place_kernel<kAloneWarps>, dim3(1 + fillers, count), dim3(32 * kAloneWarps), 0, stream, tables,
+                     pass, 1, share++, shares);
+    } else {
+      e = launch_pdl(sort_count_kernel, dim3(s.blocks + fillers, count), dim3(32 * kSortWarps), 0, stream, tables, pass,
+                     s.blocks, share++, shares);
+      if (!e && scan) e = launch_pdl(sort_scan_kernel, dim3(digits, count), dim3(kThreads), 0, stream, tables, pass, s.blocks);
+      if (!e)
+        e = launch_pdl(sort_place_kernel<kSortWarps>, dim3(s.blocks + fillers, count), dim3(32 * kSortWarps), 0, stream,
+                       tables, pass, s.blocks, share++, shares);
+    }
+    if (e) return (int)e;
+  }
+  return 0;
 }
 
 template <typename T>
 int launch_bwd(const EmbeddingBwdParams& p, int dtype, cudaStream_t stream) {
-  if (cudaError_t e = cudaMemsetAsync(p.dweight, 0, (size_t)p.rows * p.d * sizeof(T), stream)) return (int)e;
-  if (p.n == 0) return 0;
   constexpr int V = Vec16<T>::N;
-  const int vec = vec_of(dtype, p.dy, p.dy_stride, p.dweight, 0, p.d);
-  const SumPlan s = sum_plan(p.n, p.rows, p.d, !p.index, vec);
-  unsigned char* ws = static_cast<unsigned char*>(p.ws);
-  uint64_t* entries[2] = {reinterpret_cast<uint64_t*>(ws), reinterpret_cast<uint64_t*>(ws + s.entries)};
-  SumParams q{};
-  q.list = Sorted{nullptr, p.n, p.seq, p.index ? 0 : p.n / p.seq};
-  if (p.index) {
-    SortParams t{};
-    t.index = p.index;
-    t.counts = s.counts ? reinterpret_cast<int*>(ws + 2 * s.entries) : nullptr;
-    // every block adding up all blocks' counts is one launch less (a pass of 32 blocks), but grows with their square
-    if (s.blocks > kScanBlocks) t.totals = t.counts + ((size_t)s.blocks << s.bits);
-    t.n = p.n;
-    t.rows = p.rows;
-    t.skip = p.padding_index;
-    t.bits = s.bits;
-    for (int pass = 0; pass < s.passes; ++pass) {
-      t.shift = pass * s.bits;
-      t.to = entries[pass & 1];
-      if (t.counts)
-        if (cudaError_t e = launch_pdl(sort_count_kernel, dim3(s.blocks), dim3(kSortThreads), 0, stream, t)) return (int)e;
-      if (t.totals)
-        if (cudaError_t e = launch_pdl(sort_scan_kernel, dim3(1 << s.bits), dim3(kThreads), 0, stream, t, s.blocks))
-          return (int)e;
-      if (cudaError_t e = launch_pdl(sort_place_kernel, dim3(s.blocks), dim3(kSortThreads), 0, stream, t)) return (int)e;
-      t.from = t.to;
-    }
-    q.list.entries = t.from;
+  struct Asked {
+    void* out;
+    const int64_t* index;
+    int64_t rows, skip;
+    float scale;
+  } asked[2] = {{p.dweight, p.tokens, p.vocab, p.padding_index, p.scale}, {p.dposition_weight, p.positions, p.places, -1, 1.f}};
+  if (p.n == 0) {
+    for (const Asked& a : asked)
+      if (a.out)
+        if (cudaError_t e = cudaMemsetAsync(a.out, 0, (size_t)a.rows * p.d * sizeof(T), stream)) return (int)e;
+    return 0;
   }
-  q.dy = p.dy;
-  q.out = p.dweight;
-  q.partials = reinterpret_cast<float*>(ws + 2 * s.entries + s.counts);
-  q.stride = p.dy_stride;
-  q.d = p.d;
-  q.pitch = (p.d + 7) / 8 * 8;
-  q.rows = p.rows;
-  q.chunk = s.chunk;
-  q.scale = p.scale;
-  return vec == V ? launch_sum<T, V>(s, q, stream) : launch_sum<T, 1>(s, q, stream);
+  int vec = vec_of(dtype, p.dy, p.dy_stride, nullptr, 0, p.d);
+  for (const Asked& a : asked)
+    if (a.out) vec = std::min(vec, vec_of(dtype, a.out, 0, nullptr, 0, p.d));
+  const SumPlan s = sum_plan(p.n, p.d, vec);
+  unsigned char* ws = static_cast<unsigned char*>(p.ws);
+  Tables tables{};
+  tables.n = p.n;
+  tables.seq = p.seq;
+  int count = 0;
+  for (const Asked& a : asked) {
+    if (!a.out) continue;
+    const TablePlan q = table_plan(s, p.n, a.rows, p.d, !a.index);
+    Table& t = tables.t[count++];
+    t.index = a.index;
+    t.out = a.out;
+    t.rows = a.rows;
+    t.skip = a.skip;
+    t.scale = a.scale;
+    t.passes = q.passes;
+    t.bits = q.bits;
+    // positions in order write the first seq rows themselves
+    t.fill0 = a.index ? 0 : std::min(p.seq, a.rows) * p.d * (int64_t)sizeof(T);
+    t.fill1 = a.rows * p.d * (int64_t)sizeof(T);
+    t.entries[0] = reinterpret_cast<uint64_t*>(ws);
+    t.entries[1] = reinterpret_cast<uint64_t*>(ws + q.entries);
+    if (q.counts) {
+      t.counts = reinterpret_cast<int*>(ws + 2 * q.entries);
+      // every block adding up all blocks' counts is one launch less, but grows with their square
+      if (s.blocks > kScanBlocks) t.totals = t.counts + ((size_t)s.blocks << q.bits);
+    }
+    t.partials = reinterpret_cast<float*>(ws + 2 * q.entries + q.counts);
+    ws += q.bytes();
+  }
+  if (!count) return 0;
+  if (int rc = launch_sort(s, tables, count, stream)) return rc;
+  const Sum q{p.dy, p.dy_stride, p.d, round8(p.d), s.chunk};
+  return vec == V ? launch_sums<T, V>(s, tables, count, q, stream) : launch_sums<T, 1>(s, tables, count, q, stream);
 }
 
 }  // namespace
 
-size_t embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t d, int dtype, bool sorted) {
-  const int wide = dtype == kF32 ? 4 : 8;  // the plan goes by the alignment of dy: the larger of both
-  return std::max(sum_plan(n, rows, d, sorted, 1).bytes(), sum_plan(n, rows, d, sorted, wide).bytes());
+size_t embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int64_t places, int64_t d, int dtype, bool positions) {
+  size_t most = 0;
+  for (int vec : {1, dtype == kF32 ? 4 : 8}) {  // the plan goes by the alignment of dy: the larger of both
+    const SumPlan s = sum_plan(n, d, vec);
+    size_t bytes = 0;
+    if (vocab) bytes += table_plan(s, n, vocab, d, false).bytes();
+    if (places) bytes += table_plan(s, n, places, d, !positions).bytes();
+    most = std::max(most, bytes);
+  }
+  return most;
 }
 
 int launch_embedding(const EmbeddingParams& p, int dtype, cudaStream_t stream) {

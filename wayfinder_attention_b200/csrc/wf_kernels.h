@@ -284,14 +284,17 @@ struct EmbeddingParams {
   int32_t* status;  // nullable; bit 0 set on an index outside its table
 };
 struct EmbeddingBwdParams {
-  const int64_t* index;  // [n], or null: i % seq
-  const void* dy;        // (n, d) rows dy_stride apart
-  void* dweight;         // [rows][d]
-  int64_t n, seq, rows, d, dy_stride, padding_index;
+  const int64_t* tokens;     // [n]
+  const int64_t* positions;  // [n], or null: i % seq
+  const void* dy;            // (n, d) rows dy_stride apart
+  void* dweight;             // [vocab][d], 16-byte aligned, or null
+  void* dposition_weight;    // [places][d], 16-byte aligned, or null
+  int64_t n, seq, vocab, places, d, dy_stride, padding_index;
   float scale;
   void* ws;
 };
-size_t embedding_backward_workspace_bytes(int64_t n, int64_t rows, int64_t d, int dtype, bool sorted);
+// places 0: no position_weight's gradient; vocab 0: no weight's
+size_t embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int64_t places, int64_t d, int dtype, bool positions);
 int launch_embedding(const EmbeddingParams& p, int dtype, cudaStream_t stream);
 int launch_embedding_backward(const EmbeddingBwdParams& p, int dtype, cudaStream_t stream);
 

@@ -30,8 +30,8 @@ constexpr float kNothing = -200.f;
 constexpr int kShares = 4;  // epilogue warps that share a row of a tile, in every shape here
 
 // ------------------------------------------------------------------ forward
-// Running sums of a row over its run of tiles.  A NaN or +inf stays in the maximum (the
-// sums may lose it), and a row whose logits are all -inf has s = 0.
+// Running sums of a row over its run of tiles.  A NaN or +inf stays in the maximum (the sums may
+// lose it), and a row whose logits are all -inf has s = 0.
 struct ScoreStats {
   static constexpr bool kRuns = true, kStores = false;
   const int64_t* tokens;
@@ -41,17 +41,15 @@ struct ScoreStats {
   struct Row {
     float m, s, u;
     int token;
-    float* token_logit;
   };
   __device__ __forceinline__ void begin(Row& r, int row, int M, int N) const {
     r.m = -FLT_MAX;
     r.s = r.u = 0.f;
     const int64_t t = row < M ? tokens[row] : -1;
     r.token = t >= 0 && t < N ? (int)t : -1;
-    r.token_logit = token_logit + row;
   }
   template <int SC>
-  __device__ __forceinline__ void slice(Row& r, float* v, int n, int N) const {
+  __device__ __forceinline__ void slice(Row& r, float* v, int row, int n, int N) const {
     if (n + SC > N) {
 #pragma unroll
       for (int j = 0; j < SC; ++j)
@@ -62,21 +60,24 @@ struct ScoreStats {
 #pragma unroll
       for (int j = 1; j < SC; ++j)
         if (n + j == r.token) z = v[j];
-      *r.token_logit = z;
+      token_logit[row] = z;
     }
-    float m = r.m;
+    float m = r.m, m2 = max_keep_nan(v[0], v[1]);
 #pragma unroll
-    for (int j = 0; j < SC; ++j) m = max_keep_nan(m, v[j]);
+    for (int j = 2; j < SC; j += 2) {  // two chains
+      if (j % 4) m = max_keep_nan(m, v[j], v[j + 1]);
+      else m2 = max_keep_nan(m2, v[j], v[j + 1]);
+    }
+    m = max_keep_nan(m, m2);
     const float d = fmaxf(r.m - m, kNothing), a = exp2_approx(d * kLog2e);
     Pair s(0.f), u(0.f);
 #pragma unroll
     for (int j = 0; j < SC; j += 2) {
-      float d0, d1;
-      add2(Pair(v[j], v[j + 1]), Pair(-m)).get(d0, d1);
-      const Pair t(fmaxf(d0, kNothing), fmaxf(d1, kNothing));
-      float t0, t1;
-      mul2(t, Pair(kLog2e)).get(t0, t1);
-      const Pair e(exp2_approx(t0), exp2_approx(t1));
+      float t0, t1, p0, p1;
+      add2(Pair(v[j], v[j + 1]), Pair(-m)).get(t0, t1);
+      const Pair t(fmaxf(t0, kNothing), fmaxf(t1, kNothing));
+      mul2(t, Pair(kLog2e)).get(p0, p1);
+      const Pair e(exp2_approx(p0), exp2_approx(p1));
       s = add2(s, e);
       u = fma2(e, t, u);
     }
@@ -96,13 +97,15 @@ struct ScoreStats {
   }
 };
 
-// Joins the parts of 32 rows: 8 warps share the parts, a row a lane.
-__global__ void __launch_bounds__(256) linear_logprobs_join_kernel(const float* parts, int n_parts,
-                                                                   const float* token_logit, LinearLogprobsParams p) {
-  __shared__ float sm[8][32], ss[8][32], su[8][32];
+// Joins the parts of R rows a block: its threads share the parts, R neighbours a row each.
+constexpr int kJoinThreads = 256;
+template <int R>
+__global__ void __launch_bounds__(kJoinThreads) linear_logprobs_join_kernel(const float* parts, int n_parts,
+                                                                            const float* token_logit,
+                                                                            LinearLogprobsParams p) {
+  __shared__ float sm[kJoinThreads], ss[kJoinThreads], su[kJoinThreads];
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * 32 + lane, stride = (int64_t)n_parts * p.rows;
+  const int64_t row = (int64_t)blockIdx.x * R + threadIdx.x % R, stride = (int64_t)n_parts * p.rows;
   float m = -FLT_MAX, s = 0.f, u = 0.f;
   auto join = [&](float m2, float s2, float u2) {
     const float top = max_keep_nan(m, m2);
@@ -113,16 +116,20 @@ __global__ void __launch_bounds__(256) linear_logprobs_join_kernel(const float* 
     m = top;
   };
   if (row < p.rows)
-    for (int i = warp; i < n_parts; i += 8) {
+#pragma unroll 4
+    for (int i = threadIdx.x / R; i < n_parts; i += kJoinThreads / R) {
       const float* at = parts + (int64_t)i * p.rows + row;
       join(at[0], at[stride], at[2 * stride]);
     }
-  sm[warp][lane] = m;
-  ss[warp][lane] = s;
-  su[warp][lane] = u;
-  __syncthreads();
-  if (warp || row >= p.rows) return;
-  for (int i = 1; i < 8; ++i) join(sm[i][lane], ss[i][lane], su[i][lane]);
+  for (int half = kJoinThreads / 2; half >= R; half /= 2) {
+    sm[threadIdx.x] = m;
+    ss[threadIdx.x] = s;
+    su[threadIdx.x] = u;
+    __syncthreads();
+    if ((int)threadIdx.x < half) join(sm[threadIdx.x + half], ss[threadIdx.x + half], su[threadIdx.x + half]);
+    __syncthreads();
+  }
+  if (threadIdx.x >= R || row >= p.rows) return;
   const bool none = s == 0.f && m == -FLT_MAX;
   const bool bad = !(m < INFINITY);  // NaN or +inf
   const float log_s = none ? -INFINITY : logf(s);
@@ -230,7 +237,7 @@ struct ScoreGrad {
     }
   }
   template <int SC>
-  __device__ __forceinline__ void slice(const Row& r, float* v, int n, int) const {
+  __device__ __forceinline__ void slice(const Row& r, float* v, int, int n, int) const {
 #pragma unroll
     for (int j = 0; j < SC; j += 2) {
       float t0, t1;
@@ -400,9 +407,15 @@ int launch_fwd(const LinearLogprobsParams& p, int dtype, cudaStream_t stream) {
   e.parts = reinterpret_cast<float*>(ws);
   e.token_logit = reinterpret_cast<float*>(ws + round256((size_t)3 * e.part_rows * sizeof(float)));
   if (int rc = launch_runs<T>(g, out, plan, e, stream)) return rc;
-  return (int)launch_pdl(linear_logprobs_join_kernel, dim3((unsigned)((p.rows + 31) / 32)), dim3(256), 0, stream,
-                         static_cast<const float*>(e.parts), plan.ranges * kShares,
-                         static_cast<const float*>(e.token_logit), p);
+  auto join = [&](auto rows_a_block) {
+    constexpr int R = decltype(rows_a_block)::value;
+    return (int)launch_pdl(linear_logprobs_join_kernel<R>, dim3((unsigned)((p.rows + R - 1) / R)), dim3(kJoinThreads),
+                           0, stream, static_cast<const float*>(e.parts), plan.ranges * kShares,
+                           static_cast<const float*>(e.token_logit), p);
+  };
+  // a sector's rows, or one row a block where they are few and their parts many
+  if (p.rows <= kSms) return join(std::integral_constant<int, 1>());
+  return p.rows <= 32 * kSms ? join(std::integral_constant<int, 8>()) : join(std::integral_constant<int, 32>());
 }
 
 // Columns of the vocabulary that a piece has: as many as 256 MB of dz hold, but 2048 at least

@@ -523,20 +523,18 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     const Tensor dy = rows_of(grads[0]);
     const int64_t n = tokens.numel(), d = dy.size(1), seq = std::max<int64_t>(1, ctx->saved_data["seq"].toInt());
     const int code = dtype_code(dy.scalar_type());
-    auto table = [&](int64_t rows, const Tensor& index, int64_t padding, double scale) {
-      Tensor dw = at::empty({rows, d}, dy.options());
-      const size_t bytes_n = wf.token_embedding_backward_workspace_bytes(n, rows, d, code, index.defined());
-      const Tensor ws = bytes(bytes_n, dy);
-      check(wf.token_embedding_backward(index.defined() ? index.data_ptr<int64_t>() : nullptr, n, seq, dy.data_ptr(),
-                                        code, rows, d, dy.stride(0), padding, (float)scale, dw.data_ptr(), ptr(ws),
-                                        bytes_n, stream()));
-      return dw;
-    };
+    const int64_t vocab = ctx->saved_data["vocab"].toInt(), places = ctx->saved_data["places"].toInt();
     variable_list out(8);
-    if (need_w)
-      out[0] = table(ctx->saved_data["vocab"].toInt(), tokens, ctx->saved_data["padding"].toInt(),
-                     ctx->saved_data["scale"].toDouble());
-    if (need_p) out[1] = table(ctx->saved_data["places"].toInt(), positions, -1, 1.0);
+    if (need_w) out[0] = at::empty({vocab, d}, dy.options());
+    if (need_p) out[1] = at::empty({places, d}, dy.options());
+    const size_t size = wf.token_embedding_backward_workspace_bytes(n, need_w ? vocab : 0, need_p ? places : 0, d, code,
+                                                                    positions.defined());
+    const Tensor ws = bytes(size, dy);
+    check(wf.token_embedding_backward(tokens.data_ptr<int64_t>(),
+                                      positions.defined() ? positions.data_ptr<int64_t>() : nullptr, n, seq,
+                                      dy.data_ptr(), code, d, dy.stride(0), vocab,
+                                      (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(),
+                                      ptr(out[0]), places, ptr(out[1]), ptr(ws), size, stream()));
     return out;
   }
 };
