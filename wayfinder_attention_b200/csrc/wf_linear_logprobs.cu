@@ -359,7 +359,10 @@ Plan run_plan(int64_t M, int64_t N, int64_t K, int pieces) {
     p.group = (int)std::max(1.0, std::min((double)tm, kGroupBytes / ((double)kBM * s.cg * K * 2 * pieces)));
     const int slots = kSms / s.cg;
     const double tile = std::max<double>((double)p.k_blocks * cycles, 8 * s.bn);
-    for (int64_t ranges = 1; ranges <= std::min<int64_t>(tn, kMaxRanges); ++ranges) {
+    // for each number of waves as many ranges as it holds, and one for each tile of columns
+    const int64_t most = std::min<int64_t>(tn, kMaxRanges);
+    for (int64_t n = 1, ranges = 0; ranges < most; ++n) {
+      ranges = n > 64 ? most : std::min(most, std::max<int64_t>(ranges + 1, n * slots / tm));
       const double waves = (double)((tm * ranges + slots - 1) / slots), length = (double)((tn + ranges - 1) / ranges);
       // a wave ends with an epilogue that nothing covers; the parts are written and read once
       const double t = waves * (length * tile + 8 * s.bn) + 24.0 * kShares * ranges * M / 2000;
