@@ -2,12 +2,13 @@
 //
 //   y_i = s W[t_i] + P[p_i], rounded once;   dW[v] = s sum of dy_i over t_i = v,  dP likewise
 //
-// The gradient sums rows of dy in a fixed order, with no atomics: the indices are sorted (stable
-// radix sort, 8 or 9 bits a pass), and the sorted list is cut into chunks of equal length,
+// The gradient sums rows of dy in a fixed order, with no atomics on sums: the indices are sorted
+// (stable radix sort, 8 or 9 bits a pass), and the sorted list is cut into chunks of equal length,
 // whatever their rows: a group of threads walks a chunk with its columns' sum in registers
 // and writes a table's row when the list moves on to the next.  A row whose list crosses the
-// edge of a chunk leaves partial sums in fp32, which a second kernel adds.  Positions 0, 1, ...
-// of each sequence need no sort: their sorted list is known.
+// edge of a chunk leaves partial sums in fp32, which are added within the block, and across blocks
+// by a second kernel.  The table is zeroed beside the sort, which leaves most of the GPU idle.
+// Positions 0, 1, ... of each sequence need no sort: their sorted list is known.
 //
 // Bound by bytes: the forward reads and writes each row once; the backward reads dy once and
 // writes the table, most of whose rows are zeros where the vocabulary is large.
@@ -19,6 +20,7 @@
 #include "wf_sm100.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace wf {
 namespace {
@@ -74,8 +76,8 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(EmbeddingParams p, 
 
 // Many rows: a warp walks up to 32 neighbours with its share of the columns, the next AHEAD rows on their
 // way into its threads' own slots of shared memory.  Loads are then under way while others are
-// stored, at no cost in registers: four rows loaded and then stored by each thread took 92 us where this
-// takes FIGURE (65536 rows of 2048, fp16).
+// stored, at no cost in registers: 60 us for 65536 rows of 2048 in fp16 (347 MB that have to move: 5.8 TB/s),
+// where four rows loaded and then stored by each thread took 92.
 template <typename T, bool POSITIONS>
 __global__ void __launch_bounds__(kThreads) embedding_rows_kernel(EmbeddingParams p, int log_g, int chunk) {
   constexpr int VEC = Vec16<T>::N, AHEAD = POSITIONS ? 5 : 8;
@@ -125,13 +127,13 @@ __global__ void __launch_bounds__(kThreads) embedding_rows_kernel(EmbeddingParam
 // The gradients of up to two tables are made side by side, a table's blocks in each launch.
 struct Table {
   const int64_t* index;  // [n]; null: i % seq
-  uint64_t* entries[2];  // sorted lists, by turns: index above, position below
+  uint64_t* entries[2];  // the sorted list, index above and position below, and what passes before the last leave
   int* counts;           // [blocks][digits], then each block's first place within the digit
   int* totals;           // [digits]
   void* out;             // [rows][d]
-  float* partials;       // [chunks][2][pitch]: a chunk's first row where it began before, its last where it goes on
-  int* crossings;        // how many rows begin in a chunk and go on in the next
-  int2* crossing;        // those chunks and rows, in any order
+  float* partials;       // [blocks][2][pitch]: a block's first row where it began before, its last where it goes on
+  int* crossings;        // how many rows begin in a block of chunks and go on in the next
+  int2* crossing;        // those blocks and rows, in any order
   int64_t rows, skip;    // indices outside [0, rows), and `skip`, sort behind all others (as `rows`)
   int64_t fill0, fill1;  // bytes of out to be zeroed
   int passes, bits;
@@ -158,7 +160,7 @@ __device__ __forceinline__ void fill_share(const Table& t, int share, int shares
   for (int i = threadIdx.x; i < bytes / 16; i += blockDim.x) static_cast<uint4*>(zeros)[i] = make_uint4(0, 0, 0, 0);
   sm100::fence_async_shared();
   __syncthreads();
-  if (threadIdx.x) return;
+  if (threadIdx.x) return;  // nothing follows that all threads would have to reach
   for (int64_t i = a16 + (int64_t)block * bytes; i < b16; i += (int64_t)blocks * bytes) {
     const int n = (int)min((int64_t)bytes, b16 - i);
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(out + i),
@@ -173,18 +175,20 @@ __device__ __forceinline__ void fill_share(const Table& t, int share, int shares
 // and ranks them by ballots of the digit's bits, on top of its own count of each digit so far.
 // (A match instruction in place of the ballots took twice the time.)  Up to kAlone pairs are
 // sorted by one cluster of blocks in one launch, which share their counts over distributed shared
-// memory; more by three launches a pass.  The rest of the GPU zeroes the table meanwhile.
+// memory; more by three launches a pass.  The SMs without a part in it zero the table meanwhile.
 constexpr int kMaxDigits = 512;
 constexpr int kClusterWarps = 16, kMaxCluster = 8;
-constexpr int cluster_tile(int rounds) { return 32 * kClusterWarps * rounds; }  // of a block
+__host__ __device__ constexpr int cluster_tile(int rounds) { return 32 * kClusterWarps * rounds; }  // of a block
 constexpr int kAlone = kMaxCluster * cluster_tile(16);
 constexpr int kSortWarps = 8, kRounds = 8, kTile = 32 * kRounds * kSortWarps;
 
-__device__ __forceinline__ uint64_t sort_entry(const Tables& p, const Table& t, int pass, int64_t i) {
-  if (pass) return t.entries[(pass - 1) & 1][i];
+__device__ __forceinline__ uint64_t first_entry(const Table& t, int64_t i) {
   const int64_t v = t.index[i];
   const bool in = v >= 0 && v < t.rows && v != t.skip;
   return (uint64_t)(in ? v : t.rows) << 32 | (uint32_t)i;
+}
+__device__ __forceinline__ uint64_t sort_entry(const Table& t, int pass, int64_t i) {
+  return pass ? t.entries[(t.passes - pass) & 1][i] : first_entry(t, i);  // the last pass ends in the first of the two
 }
 __device__ __forceinline__ int digit_of(uint64_t e, int pass, int bits) {
   return (int)(e >> (32 + pass * bits)) & ((1 << bits) - 1);
@@ -200,12 +204,10 @@ __device__ __forceinline__ unsigned lanes_of(int digit, bool in) {
   return same;
 }
 
-// Ranks a warp's pairs i0 + 32 k (i0 has the lane in it): at[digit] counts them.
+// Ranks a warp's pairs, which are i0 + 32 k of the list (i0 has the lane in it): at[digit] counts them.
 template <int ROUNDS>
 __device__ __forceinline__ void rank_pairs(const Tables& p, const Table& t, int pass, int64_t i0, int* at,
-                                           uint64_t (&entry)[ROUNDS], int (&rank)[ROUNDS]) {
-#pragma unroll
-  for (int k = 0; k < ROUNDS; ++k) entry[k] = i0 + 32 * k < p.n ? sort_entry(p, t, pass, i0 + 32 * k) : 0;
+                                           const uint64_t (&entry)[ROUNDS], int (&rank)[ROUNDS]) {
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k) rank[k] = (int)lanes_of(digit_of(entry[k], pass, t.bits), i0 + 32 * k < p.n);
 #pragma unroll
@@ -237,36 +239,49 @@ __device__ __forceinline__ int block_scan(int v, int* warp_total) {
   return before;
 }
 
-// One cluster sorts a table's list; the clusters behind it fill.
+// One cluster sorts a table's list, and the clusters behind those that sort (first, so that none waits for an SM)
+// fill.  Between passes the list lies in the blocks' shared memory, a tile each.
 template <int ROUNDS>
-__global__ void __launch_bounds__(32 * kClusterWarps) sort_cluster_kernel(Tables p, int cluster) {
-  constexpr int THREADS = 32 * kClusterWarps;
+__global__ void __launch_bounds__(32 * kClusterWarps) sort_cluster_kernel(Tables p, int cluster, int count) {
+  constexpr int THREADS = 32 * kClusterWarps, TILE = cluster_tile(ROUNDS);
   static_assert(THREADS == kMaxDigits, "a digit a thread");
-  __shared__ __align__(16) int at[kClusterWarps][kMaxDigits];  // counts, then places
-  __shared__ int mine[kMaxDigits];               // this block's counts, which the others read
+  extern __shared__ __align__(16) unsigned char sort_smem[];
+  uint64_t* list = reinterpret_cast<uint64_t*>(sort_smem);                            // [TILE]
+  int* at = reinterpret_cast<int*>(list + TILE);                                      // [warps][digits]: counts, then places
+  __shared__ int mine[kMaxDigits];  // this block's counts, which the others read
   __shared__ int warp_total[kClusterWarps];
   pdl_wait();
-  const Table& t = p.t[blockIdx.y];
-  if ((int)blockIdx.x >= cluster) {
-    fill_share(t, 0, 1, blockIdx.x - cluster, gridDim.x - cluster, at, sizeof(at));
+  const int behind = (int)blockIdx.x - cluster * count, block = blockIdx.x % cluster;
+  if (behind >= 0) {
+    for (int i = 0; i < count; ++i)
+      fill_share(p.t[i], 0, 1, behind, gridDim.x - cluster * count, sort_smem, TILE * sizeof(uint64_t));
     return;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *t.crossings = 0;
+  const Table& t = p.t[blockIdx.x / cluster];
+  if (block == 0 && threadIdx.x == 0) *t.crossings = 0;
   const int digits = 1 << t.bits, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = threadIdx.x;
+  const int in_tile = warp * 32 * ROUNDS + lane;
+  const int64_t i0 = (int64_t)block * TILE + in_tile;
+  uint64_t entry[ROUNDS];
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) entry[k] = t.passes && i0 + 32 * k < p.n ? first_entry(t, i0 + 32 * k) : 0;
   for (int pass = 0; pass < t.passes; ++pass) {
-    for (int i = lane; i < digits; i += 32) at[warp][i] = 0;
+    if (pass)
+#pragma unroll
+      for (int k = 0; k < ROUNDS; ++k) entry[k] = list[in_tile + 32 * k];
+    int* counts = at + warp * kMaxDigits;
+    for (int i = lane; i < digits; i += 32) counts[i] = 0;
     __syncwarp();
-    const int64_t i0 = ((int64_t)blockIdx.x * kClusterWarps + warp) * 32 * ROUNDS + lane;
-    uint64_t entry[ROUNDS];
     int rank[ROUNDS];
-    rank_pairs(p, t, pass, i0, at[warp], entry, rank);
+    rank_pairs(p, t, pass, i0, counts, entry, rank);
     __syncthreads();
     if (d < digits) {
       int sum = 0;
-      for (int w = 0; w < kClusterWarps; ++w) sum += at[w][d];
+#pragma unroll
+      for (int w = 0; w < kClusterWarps; ++w) sum += at[w * kMaxDigits + d];
       mine[d] = sum;
     }
-    sm100::cluster_sync();
+    sm100::cluster_sync();  // and all have their part of the list in registers
     int total = 0, before = 0, theirs[kMaxCluster];
     if (d < digits) {
 #pragma unroll
@@ -275,21 +290,29 @@ __global__ void __launch_bounds__(32 * kClusterWarps) sort_cluster_kernel(Tables
 #pragma unroll
       for (int b = 0; b < kMaxCluster; ++b) {
         total += theirs[b];
-        if (b < (int)blockIdx.x) before += theirs[b];
+        if (b < block) before += theirs[b];
       }
     }
     int place = block_scan<kClusterWarps>(total, warp_total) + before;
-    if (d < digits)
-      for (int w = 0; w < kClusterWarps; ++w) {
-        const int c = at[w][d];
-        at[w][d] = place;
-        place += c;
-      }
-    __syncthreads();
-    uint64_t* to = t.entries[pass & 1];
+    if (d < digits) {
+      int count[kClusterWarps];
 #pragma unroll
-    for (int k = 0; k < ROUNDS; ++k)
-      if (i0 + 32 * k < p.n) to[at[warp][digit_of(entry[k], pass, t.bits)] + rank[k]] = entry[k];
+      for (int w = 0; w < kClusterWarps; ++w) count[w] = at[w * kMaxDigits + d];
+#pragma unroll
+      for (int w = 0; w < kClusterWarps; ++w) {
+        at[w * kMaxDigits + d] = place;
+        place += count[w];
+      }
+    }
+    __syncthreads();
+    const bool last = pass + 1 == t.passes;
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+      if (i0 + 32 * k >= p.n) continue;
+      const int to = counts[digit_of(entry[k], pass, t.bits)] + rank[k];
+      if (last) t.entries[0][to] = entry[k];
+      else sm100::st_peer_u64(sm100::map_peer(&list[to % TILE], to / TILE), entry[k]);
+    }
     // the list is whole, and all have read this block's counts
     sm100::cluster_sync();
   }
@@ -313,7 +336,7 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_count_kernel(Tables p, i
   const int64_t i0 = (int64_t)blockIdx.x * kTile + threadIdx.x;
   uint64_t entry[kRounds];
 #pragma unroll
-  for (int k = 0; k < kRounds; ++k) entry[k] = i0 + k * THREADS < p.n ? sort_entry(p, t, pass, i0 + k * THREADS) : 0;
+  for (int k = 0; k < kRounds; ++k) entry[k] = i0 + k * THREADS < p.n ? sort_entry(t, pass, i0 + k * THREADS) : 0;
 #pragma unroll
   for (int k = 0; k < kRounds; ++k) {
     const bool in = i0 + k * THREADS < p.n;
@@ -361,6 +384,8 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_place_kernel(Tables p, i
   const int64_t i0 = ((int64_t)blockIdx.x * kSortWarps + warp) * 32 * kRounds + lane;
   uint64_t entry[kRounds];
   int rank[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; ++k) entry[k] = i0 + 32 * k < p.n ? sort_entry(t, pass, i0 + 32 * k) : 0;
   rank_pairs(p, t, pass, i0, at[warp], entry, rank);
   __syncthreads();
   // each digit's place: all of the smaller ones, and this one's in the blocks before.  A thread
@@ -387,14 +412,15 @@ __global__ void __launch_bounds__(32 * kSortWarps) sort_place_kernel(Tables p, i
     first += total[e];
   }
   __syncthreads();
-  uint64_t* to = t.entries[pass & 1];
+  uint64_t* to = t.entries[(t.passes - 1 - pass) & 1];
 #pragma unroll
   for (int k = 0; k < kRounds; ++k)
     if (i0 + 32 * k < p.n) to[at[warp][digit_of(entry[k], pass, t.bits)] + rank[k]] = entry[k];
 }
 
+// A table whose list is known needs no sort.
 __global__ void __launch_bounds__(kThreads) fill_kernel(Tables p) {
-  __shared__ uint4 zeros[512];
+  __shared__ uint4 zeros[1024];
   pdl_wait();
   const Table& t = p.t[blockIdx.y];
   if (blockIdx.x == 0 && threadIdx.x == 0) *t.crossings = 0;
@@ -407,7 +433,7 @@ struct List {
   const uint64_t* entries;
   int64_t seq, batch;
   __device__ __forceinline__ List(const Tables& p, const Table& t)
-      : entries(t.index ? t.entries[(t.passes - 1) & 1] : nullptr), seq(p.seq), batch(t.index ? 0 : p.n / p.seq) {}
+      : entries(t.index ? t.entries[0] : nullptr), seq(p.seq), batch(t.index ? 0 : p.n / p.seq) {}
   __device__ __forceinline__ void get(int64_t i, int& row, int& from) const {
     if (entries) {
       const uint64_t e = entries[i];
@@ -429,26 +455,31 @@ struct Sum {
   int64_t stride, d, pitch;
   int chunk;  // 32 at most: a warp has a chunk's list in its lanes
 };
-constexpr int kAhead = 6;  // rows of dy on their way at once
+
 
 // VEC elements a vector (16 bytes, or one where rows do not start on them), W vectors a thread, 32 lanes apart.
 template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(kThreads) embedding_sum_kernel(Tables tables, Sum p, int log_g) {
-  constexpr int N = VEC * W;
+__global__ void __launch_bounds__(kThreads, 4) embedding_sum_kernel(Tables tables, Sum p, int log_g) {
+  constexpr int N = VEC * W, kAhead = W > 1 ? 4 : 8;
+  __shared__ uint4 ring[VEC > 1 ? kAhead * W * kThreads : 1];
+  __shared__ float heads[(kThreads - 32) * N];  // of the block's chunks but the first: what belongs to a row that began before
+  __shared__ bool fills[kThreads / 32];         // whether that is all of the chunk, and the row goes on
   pdl_wait();
   const Table& t = tables.t[blockIdx.z];
   const List list(tables, t);
   const int g = 1 << log_g, lane = threadIdx.x & 31;  // g is a warp at least
-  const int64_t chunk = (int64_t)blockIdx.x * (kThreads >> log_g) + (threadIdx.x >> log_g);
+  const int group = threadIdx.x >> log_g, groups = kThreads >> log_g;
+  const int64_t chunk = (int64_t)blockIdx.x * groups + group;
   // a warp's columns are next to each other: its w-th vectors start 32 VEC further each
   const int64_t c = (((int64_t)blockIdx.y * g + (threadIdx.x & (g - 32))) * W + lane) * VEC, i0 = chunk * p.chunk;
-  if (i0 >= tables.n) return;
   const int64_t i1 = min(i0 + p.chunk, tables.n);
-  int my_row = (int)t.rows, my_from = 0;
-  if (i0 + lane < i1) list.get(i0 + lane, my_row, my_from);
-  const int outside = lane == 0 ? (i0 ? list.row(i0 - 1) : -1) : lane == 1 ? (i1 < tables.n ? list.row(i1) : -1) : 0;
+  int my_row = (int)t.rows, my_from = 0, outside = -1;
+  if (i0 < tables.n) {
+    if (i0 + lane < i1) list.get(i0 + lane, my_row, my_from);
+    if (lane == 0 && i0) outside = list.row(i0 - 1);
+    if (lane == 1 && i1 < tables.n) outside = list.row(i1);
+  }
   const int n = __popc(__ballot_sync(0xffffffffu, my_row < t.rows));  // those that count come first
-  if (n == 0) return;
   const int before = __shfl_sync(0xffffffffu, outside, 0), after = __shfl_sync(0xffffffffu, outside, 1);
   const T* dy = static_cast<const T*>(p.dy) + c;
   const int64_t my_start = my_from * p.stride;  // of this lane's row in dy
@@ -459,32 +490,45 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(Tables tables, 
 #pragma unroll
   for (int j = 0; j < N; ++j) sum[j] = 0.f;
   int row = __shfl_sync(0xffffffffu, my_row, 0);
-  bool open = row == before;  // the row began in an earlier chunk
-  auto flush = [&](bool goes_on) {
-    const bool part = open || goes_on;
-    float* to = t.partials + (2 * chunk + (open ? 0 : 1)) * p.pitch + c;
+  bool open = n && row == before;  // the row began in an earlier chunk
+  auto write = [&](float* f) {
     T* out = static_cast<T*>(t.out) + row * p.d + c;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       if (!on[w]) continue;
-      float* f = sum + w * VEC;
-      if (part) {
-        if constexpr (VEC == 1) {
-          to[32 * w] = f[0];
-        } else {
 #pragma unroll
-          for (int j = 0; j < VEC; j += 4)
-            *reinterpret_cast<float4*>(to + 32 * VEC * w + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-        }
+      for (int j = 0; j < VEC; ++j) f[w * VEC + j] *= t.scale;
+      store_vec<T, VEC>(out + 32 * VEC * w, f + w * VEC);
+    }
+  };
+  auto leave = [&](const float* f, int which) {
+    float* to = t.partials + (2 * (int64_t)blockIdx.x + which) * p.pitch + c;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (!on[w]) continue;
+      if constexpr (VEC == 1) {
+        *to = f[0];
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] *= t.scale;
-        store_vec<T, VEC>(out + 32 * VEC * w, f);
+        for (int j = 0; j < VEC; j += 4)
+          *reinterpret_cast<float4*>(to + 32 * VEC * w + j) =
+              make_float4(f[w * VEC + j], f[w * VEC + j + 1], f[w * VEC + j + 2], f[w * VEC + j + 3]);
       }
     }
   };
+  auto head = [&](int of, int j) -> float& { return heads[((of - 1) * N + j) * g + (threadIdx.x & (g - 1))]; };
+  auto finish = [&] {  // of a row that ends in this chunk
+    if (!open) {
+      write(sum);
+    } else if (group) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) head(group, j) = sum[j];
+    } else {
+      leave(sum, 0);
+    }
+  };
   auto start = [&](int next) {
-    flush(false);
+    finish();
     row = next;
     open = false;
 #pragma unroll
@@ -497,8 +541,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(Tables tables, 
   // the next rows are on their way while one is added: in this thread's slots of shared memory, or
   // in registers where rows do not start on 16 bytes
   if constexpr (VEC > 1) {
-    __shared__ uint4 ring[kAhead][W][kThreads];
-    const uint32_t slot = sm100::smem_u32(&ring[0][0][threadIdx.x]);
+    const uint32_t slot = sm100::smem_u32(&ring[threadIdx.x]);
     uint32_t asked = slot, read = slot;  // slots by turns
     constexpr uint32_t kTurn = W * kThreads * 16;
     auto turn = [&](uint32_t& at) { at = at == slot + (kAhead - 1) * kTurn ? slot : at + kTurn; };
@@ -547,39 +590,61 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(Tables tables, 
       }
     }
   }
-  // a row that begins here and goes on in the next chunk is joined from here
-  if (!open && row == after && blockIdx.y == 0 && (threadIdx.x & (g - 1)) == 0)
-    t.crossing[atomicAdd(t.crossings, 1)] = make_int2((int)chunk, row);
-  flush(row == after);
+  const bool goes_on = n && row == after, fills_chunk = open && goes_on;
+  if (n && !goes_on) finish();
+  if (fills_chunk && group) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) head(group, j) = sum[j];
+  }
+  if ((threadIdx.x & (g - 1)) == 0) fills[group] = fills_chunk;
+  __syncthreads();
+  if (!goes_on || (open && group)) return;
+  // this chunk's last row, or for the first chunk one that fills it, goes on in the next ones
+  bool ends = false;
+  for (int k = group + 1; k < groups && !ends; ++k) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] += head(k, j);
+    ends = !fills[k];
+  }
+  if (open) {
+    leave(sum, 0);
+  } else if (ends) {
+    write(sum);
+  } else {  // and on in the next block: joined from here
+    leave(sum, 1);
+    if (blockIdx.y == 0 && (threadIdx.x & (g - 1)) == 0)
+      t.crossing[atomicAdd(t.crossings, 1)] = make_int2((int)blockIdx.x, row);
+  }
 }
 
-// Rows that cross chunks: the parts of the chunk where one begins and of the chunks up to the first
-// that the row does not fill are added.  A block takes 512 columns of such a row; its warps share the
-// parts.
+// Rows that cross blocks of chunks: the parts of the block where one begins and of the blocks up to the
+// first that the row does not fill are added.  A thread block takes 512 columns of such a row; its warps
+// share the parts.
 constexpr int kJoinWarps = 4;
 template <typename T>
-__global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(Tables tables, Sum p, int chunks) {
+__global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(Tables tables, Sum p, int blocks, int64_t length) {
   __shared__ float4 part[kJoinWarps][128];
   pdl_wait();
   const Table& t = tables.t[blockIdx.z];
   const List list(tables, t);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rows = *t.crossings;
-  int2 at = t.crossing[blockIdx.x];  // chunk and row; nothing yet where there are fewer rows
+  int2 at = make_int2(0, 0);  // block and row
+  if ((int)blockIdx.x < blocks) at = t.crossing[blockIdx.x];  // asked for before it is known whether there are as many
   for (int r = blockIdx.x; r < rows; r += gridDim.x) {
     if (r != (int)blockIdx.x) at = t.crossing[r];
-    const int chunk = at.x, row = at.y;
-    int more = 0;  // chunks that the row fills
-    for (int k = chunk + 1;;) {
+    const int block = at.x, row = at.y;
+    int more = 0;  // blocks that the row fills
+    for (int k = block + 1;;) {
       const int mine = k + threadIdx.x;
-      const int64_t end = (int64_t)(mine + 1) * p.chunk;
+      const int64_t end = (mine + 1) * length;
       // filled, and going on in the next
-      const bool filled = mine < chunks && end < tables.n && list.row(end) == row;
+      const bool filled = mine < blocks && end < tables.n && list.row(end) == row;
       const int n = __syncthreads_count(filled);
       more += n;
       k += n;
       if (n < 32 * kJoinWarps) break;
     }
-    const int parts = more + 2;  // this chunk's, the filled ones', the last one's
+    const int parts = more + 2;  // this block's, the filled ones', the last one's
     const int64_t c0 = (int64_t)blockIdx.y * 512;
     auto add = [&](float4& s, float4 f) { s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w; };
     float4 sum[4];
@@ -587,7 +652,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) embedding_join_kernel(Tables 
     for (int i = 0; i < 4; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
     for (int k = warp; k < parts; k += kJoinWarps) {
-      const float* from = t.partials + (2 * (int64_t)(chunk + k) + (k ? 0 : 1)) * p.pitch;
+      const float* from = t.partials + (2 * (int64_t)(block + k) + (k ? 0 : 1)) * p.pitch;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int64_t c = c0 + 128 * i + 4 * lane;
@@ -618,6 +683,7 @@ int bits_of(int64_t most) {  // of the numbers 0 .. most
 struct Walk {
   int chunk, wide, log_g, columns;
   int64_t chunks;
+  int64_t sum_blocks() const { return (chunks + (kThreads >> log_g) - 1) / (kThreads >> log_g); }
 };
 Walk walk_of(int64_t n, int64_t d, int vec, int most_wide) {
   Walk s{};
@@ -655,8 +721,8 @@ TablePlan table_plan(const SumPlan& s, int64_t n, int64_t rows, int64_t d, bool 
     t.entries = round256((size_t)n * sizeof(uint64_t));
     t.counts = s.cluster ? 0 : round256((size_t)(s.blocks + 1) * (1 << t.bits) * sizeof(int));
   }
-  t.partials = round256((size_t)s.chunks * 2 * round8(d) * sizeof(float));
-  t.crossing = round256(sizeof(int)) + round256((size_t)s.chunks * sizeof(int2));
+  t.partials = round256((size_t)s.sum_blocks() * 2 * round8(d) * sizeof(float));
+  t.crossing = round256(sizeof(int)) + round256((size_t)s.sum_blocks() * sizeof(int2));
   return t;
 }
 int vec_of(int dtype, const void* a, int64_t stride_a, const void* b, int64_t stride_b, int64_t d) {
@@ -688,14 +754,41 @@ int launch_fwd(const EmbeddingParams& p, int dtype, cudaStream_t stream) {
 
 template <typename T, int VEC, int W>
 int launch_sums(const SumPlan& s, const Tables& tables, int count, const Sum& q, cudaStream_t stream) {
-  const int per_block = kThreads >> s.log_g;
-  if (cudaError_t e = launch_pdl(embedding_sum_kernel<T, VEC, W>,
-                                 dim3((unsigned)((s.chunks + per_block - 1) / per_block), s.columns, count),
-                                 dim3(kThreads), 0, stream, tables, q, s.log_g))
+  const int blocks = (int)s.sum_blocks();
+  if (cudaError_t e = launch_pdl(embedding_sum_kernel<T, VEC, W>, dim3(blocks, s.columns, count), dim3(kThreads), 0,
+                                 stream, tables, q, s.log_g))
     return (int)e;
-  if (s.chunks == 1) return 0;
-  return (int)launch_pdl(embedding_join_kernel<T>, dim3((unsigned)std::min<int64_t>(s.chunks, 8 * kSms), (unsigned)((q.d + 511) / 512), count),
-                         dim3(32 * kJoinWarps), 0, stream, tables, q, (int)s.chunks);
+  if (blocks == 1) return 0;
+  return (int)launch_pdl(embedding_join_kernel<T>,
+                         dim3((unsigned)std::min(blocks, 8 * kSms), (unsigned)((q.d + 511) / 512), count),
+                         dim3(32 * kJoinWarps), 0, stream, tables, q, blocks, (int64_t)q.chunk * (kThreads >> s.log_g));
+}
+
+template <int ROUNDS>
+int launch_cluster_sort(const Tables& tables, int cluster, int count, int fillers, cudaStream_t stream) {
+  constexpr size_t smem = cluster_tile(ROUNDS) * sizeof(uint64_t) + kClusterWarps * kMaxDigits * sizeof(int);
+  int device = 0;
+  if (cudaError_t e = cudaGetDevice(&device)) return (int)e;
+  static std::atomic<uint64_t> allowed{0};  // devices whose limit has been raised for this kernel
+  if (device >= 64 || !(allowed.load(std::memory_order_relaxed) >> device & 1)) {
+    if (cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<ROUNDS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
+      return (int)e;
+    if (device < 64) allowed.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster * count + (fillers + cluster - 1) / cluster * cluster);
+  cfg.blockDim = dim3(32 * kClusterWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&cfg, sort_cluster_kernel<ROUNDS>, tables, cluster, count);
 }
 
 int launch_sort(const SumPlan& s, const Tables& tables, int count, cudaStream_t stream) {
@@ -713,21 +806,9 @@ int launch_sort(const SumPlan& s, const Tables& tables, int count, cudaStream_t 
   };
   if (!passes) return (int)launch_pdl(fill_kernel, dim3(std::max(1, fillers(1)), count), dim3(kThreads), 0, stream, tables);
   if (s.cluster) {
-    cudaLaunchConfig_t cfg = {};
-    const int blocks = s.cluster + fillers(1);
-    cfg.gridDim = dim3((blocks + s.cluster - 1) / s.cluster * s.cluster, count);
-    cfg.blockDim = dim3(32 * kClusterWarps);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = s.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    if (s.cluster * cluster_tile(8) >= tables.n) return (int)cudaLaunchKernelEx(&cfg, sort_cluster_kernel<8>, tables, s.cluster);
-    return (int)cudaLaunchKernelEx(&cfg, sort_cluster_kernel<16>, tables, s.cluster);
+    return s.cluster * cluster_tile(8) >= tables.n
+               ? launch_cluster_sort<8>(tables, s.cluster, count, fillers(1), stream)
+               : launch_cluster_sort<16>(tables, s.cluster, count, fillers(1), stream);
   }
   const int shares = 2 * passes, more = fillers(shares);
   int share = 0;

@@ -295,6 +295,9 @@ __device__ __forceinline__ uint32_t map_peer(const void* p, uint32_t rank) {
 __device__ __forceinline__ void st_peer_u32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+__device__ __forceinline__ void st_peer_u64(uint32_t addr, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
 // Asynchronous remote stores into a peer CTA's shared memory: each completes its
 // bytes on the peer's mbarrier (whose owner posted expect_tx), so the receiver
 // needs no per-sender arrive and the sender no cluster-scope fence.
