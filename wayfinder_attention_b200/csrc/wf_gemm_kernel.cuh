@@ -56,6 +56,11 @@ constexpr int kChunk = 4;               // stages between additions to fp32 regi
 // by 2^-24 of the sum each on average, which at a depth of 4096 had log probabilities off by 4e-6
 // of their size, and has them by 3e-7 in chunks of 512.
 constexpr int kDeepChunk = 8;
+// A run of up to so many stages of depth keeps its rows of A in shared memory and streams B alone.  The
+// products of a 256-wide pair read 64 bytes a cycle of an SM's shared memory and their loads
+// write 64, which is all it can do: where the loads are halved, 32768 x 256 -> 50001 goes from 725 to
+// FIGURE us.
+constexpr int kResident = 4;
 constexpr int kEpilogueWarps = 16;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kSliceBytes = 64;         // of a row of output
@@ -66,6 +71,7 @@ constexpr int kMaxSplits = 32;
 struct GemmParams {
   int M, N, tiles_n, units, splits, k_blocks;
   int tiles_m, group, ranges;  // of runs (see Unit)
+  bool resident;               // A stays for a run (see kResident)
   int turn_blocks;  // of k_blocks: past them the depth is walked again, with a's second piece
   bool a_mn, b_mn;
   bool y_tma, residual_tma;  // y, the residual start and step on 16 bytes (z always does)
@@ -81,9 +87,13 @@ struct Layout {
   static constexpr uint32_t STAGING = kEpilogueWarps * 2 * kBuffer;
   static constexpr int FIT = (227 * 1024 - 2048 - (int)STAGING) / (int)STAGE;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
+  // a run's A where it stays (see kResident), and the stages of B alone that this leaves room for
+  static constexpr int B_FIT = (STAGES * (int)STAGE - kResident * (int)A_BYTES) / (int)B_BYTES;
+  static constexpr int B_STAGES = B_FIT < 8 ? B_FIT : 8;
+  static constexpr int RING = STAGES > B_STAGES ? STAGES : B_STAGES;
   static constexpr size_t off_staging = (size_t)STAGES * STAGE;
   static constexpr size_t off_bar = off_staging + STAGING;
-  static constexpr size_t off_misc = off_bar + 8 * (2 * STAGES + 5 + 2 * kEpilogueWarps);
+  static constexpr size_t off_misc = off_bar + 8 * (2 * RING + 5 + 2 * kEpilogueWarps + 2 * kResident);
   static constexpr size_t smem = off_misc + 16 + 1024;
   static constexpr int ACC = PIECES ? 2 * BN : BN;  // TMEM columns of an accumulator (main and small products)
   static constexpr uint32_t TMEM_COLS = 2 * ACC;
@@ -269,11 +279,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(base + L::off_bar);
-  uint64_t* empty = full + L::STAGES;
-  uint64_t* acc_full = empty + L::STAGES;  // [2]
+  uint64_t* empty = full + L::RING;
+  uint64_t* acc_full = empty + L::RING;    // [2]
   uint64_t* acc_empty = acc_full + 2;      // [2]
   uint64_t* drained = acc_empty + 2;
   uint64_t* res_full = drained + 1;        // [kEpilogueWarps][2]
+  uint64_t* a_full = res_full + 2 * kEpilogueWarps;  // [kResident]
+  uint64_t* a_empty = a_full + kResident;            // [kResident]
   uint32_t* tmem_s = reinterpret_cast<uint32_t*>(base + L::off_misc);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
@@ -283,9 +295,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Pair: `full` and `acc_empty` are the leader's alone; the leader's products arrive on
   // `empty`, `acc_full` and `drained` of both.
   if (threadIdx.x == 0) {
-    for (int s = 0; s < L::STAGES; ++s) {
+    for (int s = 0; s < L::RING; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < kResident; ++s) {
+      mbar_init(&a_full[s], 1);
+      mbar_init(&a_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
@@ -323,6 +339,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       prefetch_tmap(&bmap);
       Ring r;
       uint32_t issued = 0;
+      if constexpr (E::kRuns && !PIECES) {
+        if (p.resident) {
+          auto load = [&](uint64_t* bar, void* dst, const CUtensorMap* map, int x, int y, uint32_t bytes) {
+            if (rank == 0) mbar_arrive_expect_tx(bar, CG * bytes);
+            if constexpr (CG == 2) tma_load_3d_pair(dst, map, map_peer(bar, 0), x, y, 0);
+            else tma_load_3d(dst, map, bar, x, y, 0);
+          };
+          uint32_t runs = 0, a_issued = 0;  // a_issued: of this run
+          for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step, ++runs) {
+            const Work w(p, u, BM, BN);
+            a_issued = 0;
+            for (int t = 0; t < w.tiles() && !why; ++t)
+              for (int kb = 0; kb < p.k_blocks && !why; ++kb) {
+                if (t == 0) {
+                  if (!mbar_wait_asleep(&a_empty[kb], (runs & 1) ^ 1, kWaitNs)) { why = 4; break; }
+                  load(&a_full[kb], base + (size_t)kb * L::A_BYTES, &amap, kb * kBK, w.m0 + (int)rank * kBM, L::A_BYTES);
+                  ++a_issued;
+                }
+                if (!mbar_wait_asleep(&empty[r.stage], r.phase ^ 1, kWaitNs)) { why = 4; break; }
+                load(&full[r.stage], base + (size_t)kResident * L::A_BYTES + (size_t)r.stage * L::B_BYTES, &bmap, kb * kBK,
+                     w.n0 + t * BN + (int)rank * (BN / CG), L::B_BYTES);
+                ++issued;
+                r.next<L::B_STAGES>();
+              }
+          }
+          // as below: what is in flight lands before the block ends
+          if (why && rank == 0) {
+            for (uint32_t s = 0; s < (uint32_t)L::B_STAGES && s < issued; ++s)
+              mbar_wait_asleep(&full[s], (issued - 1 - s) / L::B_STAGES & 1, kWaitNs);
+            for (uint32_t s = 0; s < a_issued; ++s) mbar_wait_asleep(&a_full[s], runs - 1 & 1, kWaitNs);
+          }
+        }
+      }
+      if (!(E::kRuns && !PIECES && p.resident))
       for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step) {
         const Work w(p, u, BM, BN);
         const int am = w.m0 + (int)rank * kBM;
@@ -359,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // after a wait that gave up, loads may be in flight that no product will wait for
-      if (why && rank == 0)
+      if (why && rank == 0 && !(E::kRuns && !PIECES && p.resident))
         for (uint32_t s = 0; s < (uint32_t)L::STAGES && s < issued; ++s) {
           const uint32_t last = (issued - 1 - s) / L::STAGES;  // round of the newest load of stage s
           mbar_wait_asleep(&full[s], last & 1, kWaitNs);
@@ -375,6 +425,42 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (CG == 2) mma_commit_pair(bar);
         else mma_commit(bar);
       };
+      if constexpr (E::kRuns && !PIECES) {
+        if (p.resident) {
+          uint32_t runs = 0;
+          auto wait = [&](uint64_t* bar, uint32_t phase, uint32_t site) {
+            if (mbar_wait_asleep(bar, phase, kWaitNs)) return true;
+            why = site;
+            return false;
+          };
+          for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step, ++runs) {
+            const Work w(p, u, BM, BN);
+            for (int t = 0; t < w.tiles() && !why; ++t) {
+              if (!wait(&acc_empty[acc], acc_phase ^ 1, 8)) break;
+              tc_fence_after();
+              for (int kb = 0; kb < p.k_blocks; ++kb) {
+                if ((t == 0 && !wait(&a_full[kb], runs & 1, 16)) || !wait(&full[r.stage], r.phase, 16)) break;
+                tc_fence_after();
+                const uint32_t as = smem_u32(base + (size_t)kb * L::A_BYTES);
+                const uint32_t bs = smem_u32(base + (size_t)kResident * L::A_BYTES + (size_t)r.stage * L::B_BYTES);
+#pragma unroll
+                for (int k = 0; k < kBK / 16; ++k) {
+                  const uint64_t da = smem_desc_kmajor(as + k * 32, 128), db = smem_desc_kmajor(bs + k * 32, 128);
+                  if constexpr (CG == 2) mma_f16_pair(tmem + acc * L::ACC, da, db, p.idesc, kb > 0 || k > 0);
+                  else mma_f16(tmem + acc * L::ACC, da, db, p.idesc, kb > 0 || k > 0);
+                }
+                commit(&empty[r.stage]);
+                if (t + 1 == w.tiles()) commit(&a_empty[kb]);
+                r.next<L::B_STAGES>();
+              }
+              commit(&acc_full[acc]);
+              acc ^= 1;
+              acc_phase ^= acc == 0;
+            }
+          }
+        }
+      }
+      if (!(E::kRuns && !PIECES && p.resident))
       for (uint32_t u = first; u < (uint32_t)p.units && !why; u += step) {
         const Work w(p, u, BM, BN);
         for (int t = 0; t < w.tiles() && !why; ++t)
@@ -743,6 +829,7 @@ int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan,
   p.tiles_m = plan.tiles_m;
   p.group = plan.group;
   p.ranges = plan.ranges;
+  p.resident = E::kRuns && !PIECES && !g.a.mn_major && !g.b.mn_major && g.turns == 1 && plan.k_blocks <= kResident;
   p.k_blocks = plan.k_blocks;
   p.turn_blocks = plan.k_blocks / g.turns;
   p.a_mn = g.a.mn_major;

@@ -6,8 +6,9 @@
 //   dx = dz W,  dW = dz^T x,  db = sum_rows dz
 //
 // Forward: the tensor-core product (wf_gemm_kernel.cuh) whose epilogue keeps, for each row
-// of its run of tiles, the maximum m, s = sum exp(z - m) and u = sum exp(z - m) (z - m), and
-// picks the token's logit; a second kernel joins the runs' shares.
+// of its run of tiles, a base m, s = sum exp(z - m) and u = sum exp(z - m) (z - m), and
+// picks the token's logit; a second kernel joins the runs' shares, and L = m + log s,
+// H = log s - u / s.
 //
 // Backward: for a piece of the vocabulary at a time the same product again, whose epilogue
 // makes dz of each logit and stores it in the operands' type; then dx += dz W over the piece
@@ -30,8 +31,11 @@ constexpr float kNothing = -200.f;
 constexpr int kShares = 4;  // epilogue warps that share a row of a tile, in every shape here
 
 // ------------------------------------------------------------------ forward
-// Running sums of a row over its run of tiles.  A NaN or +inf stays in the maximum (the sums may
-// lose it), and a row whose logits are all -inf has s = 0.
+// Running sums of a row over its run of tiles: s and u to a base m that is a logit of the row, though not
+// always the largest.  A slice is taken with the base there is: three instructions and one exponential
+// a logit.  Where that overflows (2^64 above it), or meets an infinity or NaN, and for the first slice,
+// the base becomes the largest so far and the slice is done again.  -inf counts as nothing; a NaN or
+// +inf stays in m (the sums may lose it); m is -inf while nothing has counted.
 struct ScoreStats {
   static constexpr bool kRuns = true, kStores = false;
   const int64_t* tokens;
@@ -43,7 +47,7 @@ struct ScoreStats {
     int token;
   };
   __device__ __forceinline__ void begin(Row& r, int row, int M, int N) const {
-    r.m = -FLT_MAX;
+    r.m = -INFINITY;
     r.s = r.u = 0.f;
     const int64_t t = row < M ? tokens[row] : -1;
     r.token = t >= 0 && t < N ? (int)t : -1;
@@ -62,31 +66,39 @@ struct ScoreStats {
         if (n + j == r.token) z = v[j];
       token_logit[row] = z;
     }
-    float m = r.m, m2 = max_keep_nan(v[0], v[1]);
-#pragma unroll
-    for (int j = 2; j < SC; j += 2) {  // two chains
-      if (j % 4) m = max_keep_nan(m, v[j], v[j + 1]);
-      else m2 = max_keep_nan(m2, v[j], v[j + 1]);
-    }
-    m = max_keep_nan(m, m2);
-    const float d = fmaxf(r.m - m, kNothing), a = exp2_approx(d * kLog2e);
-    Pair s(0.f), u(0.f);
-#pragma unroll
-    for (int j = 0; j < SC; j += 2) {
-      float t0, t1, p0, p1;
-      add2(Pair(v[j], v[j + 1]), Pair(-m)).get(t0, t1);
-      const Pair t(fmaxf(t0, kNothing), fmaxf(t1, kNothing));
-      mul2(t, Pair(kLog2e)).get(p0, p1);
-      const Pair e(exp2_approx(p0), exp2_approx(p1));
-      s = add2(s, e);
-      u = fma2(e, t, u);
-    }
     float s0, s1, u0, u1;
-    s.get(s0, s1);
-    u.get(u0, u1);
-    r.u = fmaf(a, fmaf(r.s, d, r.u), u0 + u1);
-    r.s = fmaf(a, r.s, s0 + s1);
-    r.m = m;
+    bool none = false;
+#pragma unroll 1
+    for (int again = 0;; ++again) {
+      Pair s[2] = {Pair(0.f), Pair(0.f)}, u[2] = {Pair(0.f), Pair(0.f)};
+      const Pair m(-r.m), log2e(kLog2e);
+#pragma unroll
+      for (int j = 0; j < SC; j += 2) {
+        const Pair t = add2(Pair(v[j], v[j + 1]), m);
+        float p0, p1;
+        mul2(t, log2e).get(p0, p1);
+        const Pair e(exp2_approx(p0), exp2_approx(p1));
+        s[j / 2 % 2] = add2(s[j / 2 % 2], e);
+        u[j / 2 % 2] = fma2(e, t, u[j / 2 % 2]);
+      }
+      add2(s[0], s[1]).get(s0, s1);
+      add2(u[0], u[1]).get(u0, u1);
+      s0 += s1;
+      u0 += u1;
+      if (again || __all_sync(0xffffffffu, s0 < 1.8e19f && u0 == u0)) break;
+      float top = r.m;
+#pragma unroll
+      for (int j = 0; j < SC; j += 2) top = max_keep_nan(top, v[j], v[j + 1]);
+#pragma unroll
+      for (int j = 0; j < SC; ++j) v[j] = fmaxf(v[j], -FLT_MAX);
+      const float d = fmaxf(r.m - top, kNothing), a = exp2_approx(d * kLog2e);
+      r.u = a * fmaf(r.s, d, r.u);
+      r.s *= a;
+      r.m = top;
+      none = top == -INFINITY;
+    }
+    r.s += none ? 0.f : s0;
+    r.u += none ? 0.f : u0;
   }
   __device__ __forceinline__ void end(const Row& r, int row, int M, int part) const {
     if (row >= M) return;
@@ -106,7 +118,7 @@ __global__ void __launch_bounds__(kJoinThreads) linear_logprobs_join_kernel(cons
   __shared__ float sm[kJoinThreads], ss[kJoinThreads], su[kJoinThreads];
   pdl_wait();
   const int64_t row = (int64_t)blockIdx.x * R + threadIdx.x % R, stride = (int64_t)n_parts * p.rows;
-  float m = -FLT_MAX, s = 0.f, u = 0.f;
+  float m = -INFINITY, s = 0.f, u = 0.f;
   auto join = [&](float m2, float s2, float u2) {
     const float top = max_keep_nan(m, m2);
     const float d = fmaxf(m - top, kNothing), d2 = fmaxf(m2 - top, kNothing);
@@ -130,7 +142,7 @@ __global__ void __launch_bounds__(kJoinThreads) linear_logprobs_join_kernel(cons
     __syncthreads();
   }
   if (threadIdx.x >= R || row >= p.rows) return;
-  const bool none = s == 0.f && m == -FLT_MAX;
+  const bool none = m == -INFINITY;
   const bool bad = !(m < INFINITY);  // NaN or +inf
   const float log_s = none ? -INFINITY : logf(s);
   const int64_t tok = p.tokens[row];
@@ -146,7 +158,7 @@ __global__ void __launch_bounds__(kJoinThreads) linear_logprobs_join_kernel(cons
   p.logprob[row] = lp;
   p.entropy[row] = bad ? NAN : none ? 0.f : log_s - u / s;
   if (p.stats) {
-    p.stats[row] = none ? -INFINITY : m;
+    p.stats[row] = m;
     p.stats[p.rows + row] = log_s;
   }
 }
