@@ -164,14 +164,23 @@ __global__ void __launch_bounds__(kJoinThreads) linear_logprobs_join_kernel(cons
 }
 
 // ------------------------------------------------------------------ backward
-// What the backward's epilogue needs of a row: dz_j = p (a + b t) + g [j = token] with
-// t = (z - m) log2 e - l2s and p = 2^t.
-struct RowGrad {
-  float m, l2s, a, b;
-};
-struct RowToken {
-  float g;
-  int token;
+// A row's gradients, of its token's log probability (0 where that is not asked for) and its entropy.
+struct RowInputs {
+  const int64_t* tokens;
+  const float* stats;  // [2][rows]
+  const float* entropy;
+  const float* dlogprob;  // or null
+  const float* dentropy;  // or null
+  int64_t rows, vocab, ignore_index;
+  // The token in the vocabulary, or -1.  One outside of it that a gradient is asked for makes that NaN.
+  __device__ __forceinline__ int gradients(int64_t row, float& gl, float& gh) const {
+    gl = dlogprob ? dlogprob[row] : 0.f;
+    gh = dentropy ? dentropy[row] : 0.f;
+    const int64_t t = tokens[row];
+    if (t != ignore_index && t >= 0 && t < vocab) return (int)t;
+    gl = t == ignore_index || gl == 0.f ? 0.f : NAN;
+    return -1;
+  }
 };
 
 // fp16 has no room for p of a gradient that is small itself (a mean over many rows): there a row's
@@ -179,73 +188,59 @@ struct RowToken {
 // 2^14 .. 2^15.  dx takes it off again by rows; for dW, x's rows are multiplied by 2^(least e - e)
 // and the product by 2^-least.
 constexpr int kNoRow = 1000;  // the exponent of a row without a gradient
-
-struct GradRows {
-  RowGrad* grad;
-  RowToken* token;
-  int* exponent;  // [rows], then the least of them; null: not scaled
-};
-
-__global__ void __launch_bounds__(256) linear_logprobs_rows_kernel(LinearLogprobsBwdParams p, GradRows out) {
+__global__ void __launch_bounds__(256) linear_logprobs_exponents_kernel(RowInputs in, int* exponent) {
   pdl_wait();
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   int e = kNoRow;
-  if (row < p.rows) {
-    float m = p.stats[row], log_s = p.stats[p.rows + row];
-    float gl = p.dlogprob ? p.dlogprob[row] : 0.f;
-    const float gh = p.dentropy ? p.dentropy[row] : 0.f;
-    const int64_t t = p.tokens[row];
-    int token = -1;
-    if (t == p.ignore_index) gl = 0.f;
-    else if (t < 0 || t >= p.vocab) gl = gl == 0.f ? 0.f : NAN;
-    else token = (int)t;
-    RowGrad r{m, log_s * kLog2e, -fmaf(gh, p.entropy[row], gl), -gh * kLn2};
-    float g = gl;
-    if (m == -INFINITY || (gl == 0.f && gh == 0.f)) {  // no distribution, or no gradient: p is 0
-      r = RowGrad{0.f, INFINITY, 0.f, 0.f};
-      g = 0.f;
-    } else {
-      if (!(m < INFINITY)) r = RowGrad{0.f, 0.f, NAN, 0.f};
-      if (out.exponent) {
-        const float size = fabsf(gl) + 32.f * fabsf(gh);
-        e = size > 0.f && size < INFINITY ? min(max(14 - ilogbf(size), -100), 100) : 0;
-        const float up = ldexpf(1.f, e);
-        r.a *= up;
-        r.b *= up;
-        g *= up;
-      }
-    }
-    out.grad[row] = r;
-    out.token[row] = RowToken{g, token};
-    if (out.exponent) out.exponent[row] = e;
+  if (row < in.rows) {
+    float gl, gh;
+    in.gradients(row, gl, gh);
+    const float size = fabsf(gl) + 32.f * fabsf(gh);
+    if (in.stats[row] != -INFINITY && !(size == 0.f))
+      e = size < INFINITY ? min(max(14 - ilogbf(size), -100), 100) : 0;
+    exponent[row] = e;
   }
-  if (out.exponent) {
-    const int least = __reduce_min_sync(0xffffffffu, e);
-    if ((threadIdx.x & 31) == 0 && least != kNoRow) atomicMin(out.exponent + p.rows, least);
-  }
+  const int least = __reduce_min_sync(0xffffffffu, e);
+  if ((threadIdx.x & 31) == 0 && least != kNoRow) atomicMin(exponent + in.rows, least);
 }
 // 2^(least - e), or 2^-least: no row has a gradient where there is no least exponent.
 __device__ __forceinline__ float down_by(int e, int least) { return least > 100 || e > 100 ? 0.f : ldexpf(1.f, least - e); }
 __device__ __forceinline__ float up_by(int least) { return least > 100 ? 0.f : ldexpf(1.f, -least); }
 
+// dz_j = p (a + b t) + g [j = token] with t = (z - m) log2 e - l2s and p = 2^t.
 struct ScoreGrad {
   static constexpr bool kRuns = true, kStores = true;
   int layers;
-  const RowGrad* grad;
-  const RowToken* token;
   int first;  // of the vocabulary's piece
+  RowInputs in;
+  const int* exponent;  // or null
   struct Row {
-    RowGrad r;
-    RowToken t;
+    float m, l2s, a, b, g;
+    int token;
   };
   __device__ __forceinline__ void begin(Row& r, int row, int M, int) const {
-    r.r = RowGrad{0.f, INFINITY, 0.f, 0.f};
-    r.t = RowToken{0.f, -1};
-    if (row < M) {
-      const float4 f = *reinterpret_cast<const float4*>(grad + row);
-      r.r = RowGrad{f.x, f.y, f.z, f.w};
-      r.t = token[row];
-      r.t.token -= first;
+    r = Row{0.f, INFINITY, 0.f, 0.f, 0.f, -1};  // no row, no distribution or no gradient: p is 0
+    if (row >= M) return;
+    float gl, gh;
+    const int token = in.gradients(row, gl, gh);
+    const float m = in.stats[row];
+    if (m == -INFINITY || (gl == 0.f && gh == 0.f)) return;
+    r.token = token - first;
+    r.g = gl;
+    if (!(m < INFINITY)) {  // a NaN or +inf among the row's logits
+      r.l2s = 0.f;
+      r.a = NAN;
+      return;
+    }
+    r.m = m;
+    r.l2s = in.stats[in.rows + row] * kLog2e;
+    r.a = -fmaf(gh, in.entropy[row], gl);
+    r.b = -gh * kLn2;
+    if (exponent) {
+      const float up = ldexpf(1.f, exponent[row]);
+      r.a *= up;
+      r.b *= up;
+      r.g *= up;
     }
   }
   template <int SC>
@@ -253,16 +248,16 @@ struct ScoreGrad {
 #pragma unroll
     for (int j = 0; j < SC; j += 2) {
       float t0, t1;
-      fma2(add2(Pair(v[j], v[j + 1]), Pair(-r.r.m)), Pair(kLog2e), Pair(-r.r.l2s)).get(t0, t1);
+      fma2(add2(Pair(v[j], v[j + 1]), Pair(-r.m)), Pair(kLog2e), Pair(-r.l2s)).get(t0, t1);
       t0 = fmaxf(t0, kNothing);
       t1 = fmaxf(t1, kNothing);
       const Pair e(exp2_approx(t0), exp2_approx(t1));
-      mul2(e, fma2(Pair(t0, t1), Pair(r.r.b), Pair(r.r.a))).get(v[j], v[j + 1]);
+      mul2(e, fma2(Pair(t0, t1), Pair(r.b), Pair(r.a))).get(v[j], v[j + 1]);
     }
-    if ((uint32_t)(r.t.token - n) < (uint32_t)SC) {
+    if ((uint32_t)(r.token - n) < (uint32_t)SC) {
 #pragma unroll
       for (int j = 0; j < SC; ++j)
-        if (n + j == r.t.token) v[j] += r.t.g;
+        if (n + j == r.token) v[j] += r.g;
     }
   }
   __device__ __forceinline__ void end(const Row&, int, int, int) const {}
@@ -433,15 +428,35 @@ int launch_fwd(const LinearLogprobsParams& p, int dtype, cudaStream_t stream) {
   return p.rows <= 32 * kSms ? join(std::integral_constant<int, 8>()) : join(std::integral_constant<int, 32>());
 }
 
-// Columns of the vocabulary that a piece has: as many as 256 MB of dz hold, but 2048 at least
-// (shorter ones leave the products' tiles idle) and all of them where they are few.
-constexpr int64_t kPieceBytes = 256ll << 20, kPieceLeast = 2048;
-int64_t piece_columns(int64_t M, int64_t N, int dtype, int layers) {
+// Columns of the vocabulary that a piece has: as many as 512 MB of dz hold, but 2048 at least
+// (shorter ones leave the products' tiles idle) and all of them where they are few.  More are cut into pieces of
+// like size, in the least number or one of the next few, whichever leaves the pairs of blocks idle
+// least: each product of a piece takes whole waves of tiles.  (Training at 8192 x 1024 -> 50001: 256 MB
+// 2.68 ms, 512 MB 2.61; pieces of 64 MB, which L2 would hold, 2.87.)
+constexpr int64_t kPieceBytes = 512ll << 20, kPieceLeast = 2048;
+int64_t piece_columns(int64_t M, int64_t N, int64_t K, int dtype, int layers) {
   const int64_t fit = kPieceBytes / (M * (dtype == kF32 ? 10 : 2 * layers)) / 256 * 256;
   const int64_t most = std::max(fit, kPieceLeast);
   if (N <= most) return N;
-  const int64_t pieces = (N + most - 1) / most;  // of like size
-  return ((N + pieces - 1) / pieces + 255) / 256 * 256;
+  auto waves = [](int64_t tiles) { return (tiles + kSms / 2 - 1) / (kSms / 2); };
+  const int64_t tm = (M + 255) / 256, tk = (K + 255) / 256;
+  auto stages = [&](int64_t n) {  // of a piece's three products
+    const int64_t tn = (n + 255) / 256;
+    return waves(tm * tn) * ((K + 63) / 64) + waves(tm * tk) * ((n + 63) / 64) + waves(tn * tk) * ((M + 63) / 64) + 12;
+  };
+  int64_t best = 0, least = 0;
+  const int64_t fewest = (N + most - 1) / most;
+  for (int64_t pieces = fewest; pieces < fewest + 6; ++pieces) {
+    const int64_t columns = ((N + pieces - 1) / pieces + 255) / 256 * 256;
+    if (columns > most || (pieces > fewest && columns < kPieceLeast)) continue;
+    const int64_t whole = N / columns, rest = N % columns;
+    const int64_t cost = whole * stages(columns) + (rest ? stages(rest) : 0);
+    if (!best || cost < least) {
+      least = cost;
+      best = columns;
+    }
+  }
+  return best ? best : most;
 }
 // Pieces of a 16-bit dz, as in wf_linear.cu: two where the products are small, so that rounding it
 // adds nothing to the gradients' own rounding.
@@ -453,18 +468,17 @@ struct BwdPlan {
   int64_t columns;
   int layers, pieces;
   bool scaled, dx_apart, dw_apart;
-  size_t rows, dz, dz_operand, dx, dw, sums, scaled_x, gemm;
+  size_t exponents, dz, dz_operand, dx, dw, sums, scaled_x, gemm;
 };
 BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int dtype) {
   BwdPlan b{};
   b.layers = dz_layers(M, N, K, dtype);
-  b.columns = piece_columns(M, N, dtype, b.layers);
+  b.columns = piece_columns(M, N, K, dtype, b.layers);
   b.pieces = dtype == kF32 ? 3 : 1;
   b.scaled = dtype == kF16;
   b.dx_apart = dtype != kF32 && (b.scaled || b.columns < N);  // fp32 sums, rounded at the end
   b.dw_apart = b.scaled;
-  b.rows = round256(M * sizeof(RowGrad)) + round256(M * sizeof(RowToken)) +
-           (b.scaled ? round256((M + 1) * sizeof(int)) : 0);
+  b.exponents = b.scaled ? round256((M + 1) * sizeof(int)) : 0;
   b.dz = round256((size_t)M * round8(b.columns) * (dtype == kF32 ? 4 : 2) * b.layers);
   b.dz_operand = dtype == kF32 ? operand_bytes(M, b.columns, dtype) : 0;
   b.dx = b.dx_apart ? round256((size_t)M * round8(K) * sizeof(float)) : 0;
@@ -494,17 +508,8 @@ int launch_bwd(const LinearLogprobsBwdParams& p, int dtype, cudaStream_t stream)
     ws += bytes;
     return at;
   };
-  GradRows rows{};
-  rows.grad = reinterpret_cast<RowGrad*>(take(round256(M * sizeof(RowGrad))));
-  rows.token = reinterpret_cast<RowToken*>(take(round256(M * sizeof(RowToken))));
-  const int *exponent = nullptr, *least = nullptr;
-  if (b.scaled) {
-    rows.exponent = reinterpret_cast<int*>(take(round256((M + 1) * sizeof(int))));
-    exponent = rows.exponent;
-    least = exponent + M;
-    // a least exponent above every row's
-    if (cudaError_t e = cudaMemsetAsync(rows.exponent + M, 0x7f, sizeof(int), stream)) return (int)e;
-  }
+  int* exponents = reinterpret_cast<int*>(take(b.exponents));
+  const int *exponent = b.scaled ? exponents : nullptr, *least = b.scaled ? exponents + M : nullptr;
   unsigned char* dz = take(b.dz);
   unsigned char* dz_operand = take(b.dz_operand);
   float* dx = reinterpret_cast<float*>(take(b.dx));
@@ -514,9 +519,14 @@ int launch_bwd(const LinearLogprobsBwdParams& p, int dtype, cudaStream_t stream)
   unsigned char* gemm_ws = take(b.gemm);
   GemmOperand o[2];
   if (int rc = operands<T>({{p.x, M, K, p.x_stride}, {p.w, N, K, p.w_stride}}, dtype, &ws, o, stream)) return rc;
-  if (cudaError_t e = launch_pdl(linear_logprobs_rows_kernel, dim3((unsigned)((M + 255) / 256)), dim3(256), 0, stream,
-                                 p, rows))
-    return (int)e;
+  const RowInputs in{p.tokens, p.stats, p.entropy, p.dlogprob, p.dentropy, M, N, p.ignore_index};
+  if (b.scaled) {
+    // a least exponent above every row's
+    if (cudaError_t e = cudaMemsetAsync(exponents + M, 0x7f, sizeof(int), stream)) return (int)e;
+    if (cudaError_t e = launch_pdl(linear_logprobs_exponents_kernel, dim3((unsigned)((M + 255) / 256)), dim3(256), 0,
+                                   stream, in, exponents))
+      return (int)e;
+  }
   GemmOperand x_deep = o[0];  // of dW, whose depth are the rows
   if constexpr (std::is_same<T, __half>::value) {
     if (p.dw) {
@@ -548,7 +558,7 @@ int launch_bwd(const LinearLogprobsBwdParams& p, int dtype, cudaStream_t stream)
       out.y_stride = pitch;
       Plan plan = run_plan(M, n, K, b.pieces);
       plan.layers = b.layers;
-      if (int rc = launch_runs<T>(g, out, plan, ScoreGrad{b.layers, rows.grad, rows.token, (int)first}, stream)) return rc;
+      if (int rc = launch_runs<T>(g, out, plan, ScoreGrad{b.layers, (int)first, in, exponent}, stream)) return rc;
     }
     if (p.db) {
       const int shares = column_shares(M, n);
@@ -608,7 +618,7 @@ size_t linear_logprobs_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtyp
 size_t linear_logprobs_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct,
                                                 bool w_direct) {
   const BwdPlan b = bwd_plan(M, N, K, dtype);
-  return b.rows + b.dz + b.dz_operand + b.dx + b.dw + b.sums + b.scaled_x + b.gemm +
+  return b.exponents + b.dz + b.dz_operand + b.dx + b.dw + b.sums + b.scaled_x + b.gemm +
          (x_direct && b.pieces == 1 ? 0 : operand_bytes(M, K, dtype)) +
          (w_direct && b.pieces == 1 ? 0 : operand_bytes(N, K, dtype));
 }
