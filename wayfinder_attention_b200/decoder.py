@@ -19,6 +19,13 @@ forward and backward; ``score`` gives the log probability of each next token wit
     r = lm.score(input_ids, top_n=5)          # .logprob, .entropy, .top_logprobs, .top_tokens
     loss = -r.logprob.sum() / (input_ids[:, 1:] != lm.pad_token_id).sum()
     loss.backward()
+
+``fused_ends=True`` runs the model's two ends, which share a weight, on ``token_embedding`` and
+``linear_token_logprobs``: ``loss`` and ``score`` (without alternatives) then hold no logits,
+whatever the vocabulary, and the tied weight's gradient is the sum of the two operators':
+
+    lm = TransformerLM(vocab, fused_layers=True, fused_ends=True, dropout=0.0).to("cuda", torch.bfloat16)
+    lm.loss(input_ids).backward()
 """
 
 from __future__ import annotations
@@ -32,8 +39,10 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .attention import KeyVectorSparseAttention, LearnedAddressSparseAttention
+from .embedding import token_embedding
 from .layer_norm import layer_norm
 from .linear import project, runs_as
+from .linear_logprobs import linear_token_logprobs
 from .token_logprobs import TokenLogprobs, token_logprobs
 
 
@@ -71,6 +80,12 @@ def _norm(ln: nn.Module, x: torch.Tensor) -> torch.Tensor:
             return layer_norm(x.float(), weight, bias, ln.eps)
         return layer_norm(x, ln.weight, ln.bias, ln.eps)
     return ln(x)
+
+
+def _plain_embedding(emb: nn.Module) -> bool:
+    """Whether a module is an ``nn.Embedding`` whose forward and gradient are ``token_embedding``'s."""
+    return (runs_as(emb, nn.Embedding) and emb.padding_idx is None and emb.max_norm is None
+            and not emb.scale_grad_by_freq and not emb.sparse)
 
 
 @functools.lru_cache(maxsize=None)
@@ -144,6 +159,7 @@ class TransformerLM(nn.Module):
         retrieval_config: Optional[dict] = None,
         pad_token_id: int = 0,
         fused_layers: bool = False,
+        fused_ends: bool = False,
     ):
         super().__init__()
         if attention_type not in ("learned_address", "key_vector", "dense_flash", "dense"):
@@ -152,6 +168,7 @@ class TransformerLM(nn.Module):
         self.max_seq_len = max_seq_len
         self.pad_token_id = pad_token_id
         self.fused_layers = fused_layers
+        self.fused_ends = fused_ends
         self.token_emb = nn.Embedding(vocab_size, d_model)
         self.pos_emb = nn.Embedding(max_seq_len, d_model)
         self.dropout = nn.Dropout(dropout)
@@ -173,26 +190,49 @@ class TransformerLM(nn.Module):
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)
         self.lm_head.weight = self.token_emb.weight
 
-    def forward(self, input_ids: torch.Tensor, attn_mask: Optional[torch.Tensor] = None) -> dict:
-        B, T = input_ids.shape
+    def _embed(self, input_ids: torch.Tensor) -> torch.Tensor:
+        if (self.fused_ends and _plain_embedding(self.token_emb) and _plain_embedding(self.pos_emb)
+                and self.token_emb.weight.dtype == self.pos_emb.weight.dtype):
+            return token_embedding(input_ids, self.token_emb.weight, position_weight=self.pos_emb.weight)
+        pos = torch.arange(input_ids.shape[1], device=input_ids.device).unsqueeze(0)
+        return self.token_emb(input_ids) + self.pos_emb(pos)
+
+    def _hidden(self, input_ids: torch.Tensor, attn_mask: Optional[torch.Tensor]) -> torch.Tensor:
+        """What the head takes: the last norm's rows."""
         if attn_mask is None:
             attn_mask = input_ids != self.pad_token_id
-        pos = torch.arange(T, device=input_ids.device).unsqueeze(0)
-        x = self.dropout(self.token_emb(input_ids) + self.pos_emb(pos))
+        x = self.dropout(self._embed(input_ids))
         for block in self.blocks:
             x = block(x, attn_mask=attn_mask)
-        if self.fused_layers:
-            return {"logits": project(self.lm_head, _norm(self.ln_f, x), True)}
-        return {"logits": self.lm_head(self.ln_f(x))}
+        return _norm(self.ln_f, x) if self.fused_layers else self.ln_f(x)
+
+    def forward(self, input_ids: torch.Tensor, attn_mask: Optional[torch.Tensor] = None) -> dict:
+        h = self._hidden(input_ids, attn_mask)
+        return {"logits": project(self.lm_head, h, True) if self.fused_layers else self.lm_head(h)}
 
     def score(self, input_ids: torch.Tensor, attn_mask: Optional[torch.Tensor] = None, top_n: int = 0) -> TokenLogprobs:
         """How likely each next token is: ``TokenLogprobs`` of shape (B, T - 1) for ``input_ids`` (B, T).
 
         Entry t is about token t + 1 given the tokens up to t.  Padding (``pad_token_id``) gets
-        log probability 0 and no gradient.
+        log probability 0 and no gradient.  With ``fused_ends`` and no alternatives the logits are
+        not rounded to the model's type, nor held.
         """
-        logits = self(input_ids, attn_mask)["logits"]
         # the last position has no next token; a whole row of logits a token keeps them uncopied
         following = torch.cat([input_ids[:, 1:], input_ids.new_full((input_ids.shape[0], 1), self.pad_token_id)], 1)
-        r = token_logprobs(logits, following, top_n=top_n, ignore_index=self.pad_token_id)
+        if self.fused_ends and top_n == 0 and runs_as(self.lm_head, nn.Linear):
+            h, weight, bias = self._hidden(input_ids, attn_mask), self.lm_head.weight, self.lm_head.bias
+            if torch.is_autocast_enabled("cuda"):  # the product in its type, as nn.Linear's is
+                dtype = torch.get_autocast_dtype("cuda")
+                h, weight, bias = (None if t is None else t.to(dtype) for t in (h, weight, bias))
+            r = linear_token_logprobs(h, weight, following, bias=bias, ignore_index=self.pad_token_id)
+            none = r.logprob.new_empty((*following.shape, 0))
+            r = TokenLogprobs(r.logprob, r.entropy, none, none.long())
+        else:
+            logits = self(input_ids, attn_mask)["logits"]
+            r = token_logprobs(logits, following, top_n=top_n, ignore_index=self.pad_token_id)
         return TokenLogprobs(*(t[:, :-1] for t in r))
+
+    def loss(self, input_ids: torch.Tensor, attn_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Mean cross entropy of the next tokens, padding left out (0 where there is nothing else), in float32."""
+        count = (input_ids[:, 1:] != self.pad_token_id).sum()
+        return -self.score(input_ids, attn_mask).logprob.sum() / count.clamp_min(1)
