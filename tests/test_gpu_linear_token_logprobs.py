@@ -185,6 +185,30 @@ def test_banned_tokens(V, dtype, cuda_device):
         within(dw, *want["dw"], "dw")
 
 
+@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_near_the_ends_of_fp32(dtype, rows, cuda_device):
+    """Logits of 8e32, and of -1e38 and 8e32 more, beside banned ones: the largest has all the weight, and nothing becomes NaN."""
+    from wayfinder_attention_b200 import linear_token_logprobs
+
+    x = torch.tensor([1e16, -1e16, 1.0, 0.0], device=cuda_device).repeat(rows // 4)[:, None].to(dtype)
+    w = (torch.arange(700, device=cuda_device).remainder(50) * 1e14)[:, None].to(dtype)
+    w[400], w[200] = 8e16, -8e16
+    best = torch.tensor([400, 200, 400, 5], device=cuda_device).repeat(rows // 4)
+    for base in (0.0, -1e38):
+        b = torch.full((700,), base, device=cuda_device, dtype=dtype)
+        b[::3] = -math.inf
+        b[[200, 400, 5]] = base
+        leaf = x.clone().requires_grad_()
+        r = linear_token_logprobs(leaf, w, best, bias=b)
+        assert torch.isfinite(r.entropy).all() and torch.isfinite(r.logprob).all()
+        sure = torch.arange(rows, device=cuda_device) % 4 < 2
+        assert (r.logprob[sure].abs() <= 1e-6).all() and (r.entropy[sure].abs() <= 1e-6).all()
+        assert (r.entropy[3::4] - math.log(int(torch.isfinite(b).sum()))).abs().max() <= 1e-4  # equal logits
+        dx, = torch.autograd.grad(r.logprob.sum() + r.entropy.sum(), [leaf])
+        assert torch.isfinite(dx).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_large_and_special_rows(dtype, cuda_device):
     """A NaN row and rows with infinite logits stay by themselves; logits of several hundred."""

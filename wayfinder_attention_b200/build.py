@@ -27,7 +27,8 @@ SOURCES = ["wf_abi.cu", "wf_topk.cu", "wf_topk_tc.cu", "wf_attn.cu", "wf_attn_bf
            "wf_attn_f32.cu", "wf_addr_proj.cu",
            "wf_attn_bwd.cu", "wf_keymask.cu", "wf_bench.cu",
            "wf_gemm.cu", "wf_linear.cu", "wf_linear_few.cu",
-           "wf_layer_norm.cu", "wf_logprobs.cu", "wf_linear_logprobs.cu", "wf_embedding.cu"]
+           "wf_layer_norm.cu", "wf_logprobs.cu", "wf_linear_logprobs.cu", "wf_linear_logprobs_few.cu",
+           "wf_embedding.cu"]
 TORCH_SOURCE = "wf_torch.cpp"
 TORCH_LIB_PATH = PKG_DIR / "_wf_torch.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

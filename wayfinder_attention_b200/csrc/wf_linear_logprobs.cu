@@ -16,18 +16,15 @@
 // were kept: that is the price of not keeping them.
 #include "wf_columns.cuh"
 #include "wf_gemm_kernel.cuh"
+#include "wf_linear_logprobs.cuh"
 #include "wf_operand.cuh"
 #include "wf_pair.cuh"
 
 #include <cfloat>
-#include <climits>
 
 namespace wf {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// e^d and 2^d are 0 below this: the bound keeps 0 * inf out where a logit is -inf
-constexpr float kNothing = -200.f;
 constexpr int kShares = 4;  // epilogue warps that share a row of a tile, in every shape here
 
 // ------------------------------------------------------------------ forward
@@ -89,8 +86,10 @@ struct ScoreStats {
       float top = r.m;
 #pragma unroll
       for (int j = 0; j < SC; j += 2) top = max_keep_nan(top, v[j], v[j + 1]);
+      // far enough below the largest to have no weight, and near enough for the difference to be finite
+      const float low = fmaxf(top - 0.5f * fabsf(top) - 1e5f, -FLT_MAX);
 #pragma unroll
-      for (int j = 0; j < SC; ++j) v[j] = fmaxf(v[j], -FLT_MAX);
+      for (int j = 0; j < SC; ++j) v[j] = fmaxf(v[j], low);
       const float d = fmaxf(r.m - top, kNothing), a = exp2_approx(d * kLog2e);
       r.u = a * fmaf(r.s, d, r.u);
       r.s *= a;
@@ -119,26 +118,19 @@ __global__ void __launch_bounds__(kJoinThreads) linear_logprobs_join_kernel(cons
   pdl_wait();
   const int64_t row = (int64_t)blockIdx.x * R + threadIdx.x % R, stride = (int64_t)n_parts * p.rows;
   float m = -INFINITY, s = 0.f, u = 0.f;
-  auto join = [&](float m2, float s2, float u2) {
-    const float top = max_keep_nan(m, m2);
-    const float d = fmaxf(m - top, kNothing), d2 = fmaxf(m2 - top, kNothing);
-    const float a = exp2_approx(d * kLog2e), a2 = exp2_approx(d2 * kLog2e);
-    u = fmaf(a, fmaf(s, d, u), a2 * fmaf(s2, d2, u2));
-    s = fmaf(a, s, a2 * s2);
-    m = top;
-  };
   if (row < p.rows)
 #pragma unroll 4
     for (int i = threadIdx.x / R; i < n_parts; i += kJoinThreads / R) {
       const float* at = parts + (int64_t)i * p.rows + row;
-      join(at[0], at[stride], at[2 * stride]);
+      join_sums(m, s, u, at[0], at[stride], at[2 * stride]);
     }
   for (int half = kJoinThreads / 2; half >= R; half /= 2) {
     sm[threadIdx.x] = m;
     ss[threadIdx.x] = s;
     su[threadIdx.x] = u;
     __syncthreads();
-    if ((int)threadIdx.x < half) join(sm[threadIdx.x + half], ss[threadIdx.x + half], su[threadIdx.x + half]);
+    if ((int)threadIdx.x < half)
+      join_sums(m, s, u, sm[threadIdx.x + half], ss[threadIdx.x + half], su[threadIdx.x + half]);
     __syncthreads();
   }
   if (threadIdx.x >= R || row >= p.rows) return;
@@ -397,8 +389,9 @@ int launch_runs(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan,
   }
 }
 
-size_t parts_bytes(const Plan& plan, int64_t M) {
-  return round256((size_t)3 * plan.ranges * kShares * M * sizeof(float)) + round256((size_t)M * sizeof(float));
+bool few_rows(int64_t M, int dtype) { return M <= kFewLogprobRows && dtype != kF32; }
+size_t parts_bytes(int parts, int64_t M) {
+  return round256((size_t)3 * parts * M * sizeof(float)) + round256((size_t)M * sizeof(float));
 }
 
 template <typename T>
@@ -407,21 +400,23 @@ int launch_fwd(const LinearLogprobsParams& p, int dtype, cudaStream_t stream) {
   GemmOperand o[2];
   if (int rc = operands<T>({{p.x, p.rows, p.d, p.x_stride}, {p.w, p.vocab, p.d, p.w_stride}}, dtype, &ws, o, stream))
     return rc;
-  const Plan plan = run_plan(p.rows, p.vocab, p.d, kPieces<T>);
-  GemmProblem g = problem<T>(o[0], o[1], p.rows, p.vocab, p.d, dtype, nullptr, p.status);
-  GemmEpilogue out{};
-  out.bias = p.bias;
-  ScoreStats e;
-  e.tokens = p.tokens;
-  e.part_rows = (int64_t)plan.ranges * kShares * p.rows;
-  e.parts = reinterpret_cast<float*>(ws);
-  e.token_logit = reinterpret_cast<float*>(ws + round256((size_t)3 * e.part_rows * sizeof(float)));
-  if (int rc = launch_runs<T>(g, out, plan, e, stream)) return rc;
+  const bool few = few_rows(p.rows, dtype);
+  const Plan plan = few ? Plan{} : run_plan(p.rows, p.vocab, p.d, kPieces<T>);
+  const int n_parts = few ? linear_logprobs_few_parts(p.vocab) : plan.ranges * kShares;
+  float* parts = reinterpret_cast<float*>(ws);
+  float* token_logit = reinterpret_cast<float*>(ws + round256((size_t)3 * n_parts * p.rows * sizeof(float)));
+  if (few) {
+    if (int rc = launch_linear_logprobs_few(o[0], o[1], p, parts, token_logit, dtype, stream)) return rc;
+  } else {
+    GemmProblem g = problem<T>(o[0], o[1], p.rows, p.vocab, p.d, dtype, nullptr, p.status);
+    GemmEpilogue out{};
+    out.bias = p.bias;
+    if (int rc = launch_runs<T>(g, out, plan, ScoreStats{p.tokens, parts, token_logit, n_parts * p.rows}, stream)) return rc;
+  }
   auto join = [&](auto rows_a_block) {
     constexpr int R = decltype(rows_a_block)::value;
     return (int)launch_pdl(linear_logprobs_join_kernel<R>, dim3((unsigned)((p.rows + R - 1) / R)), dim3(kJoinThreads),
-                           0, stream, static_cast<const float*>(e.parts), plan.ranges * kShares,
-                           static_cast<const float*>(e.token_logit), p);
+                           0, stream, static_cast<const float*>(parts), n_parts, static_cast<const float*>(token_logit), p);
   };
   // a sector's rows, or one row a block where they are few and their parts many
   if (p.rows <= kSms) return join(std::integral_constant<int, 1>());
@@ -470,7 +465,7 @@ struct BwdPlan {
   bool scaled, dx_apart, dw_apart;
   size_t exponents, dz, dz_operand, dx, dw, sums, scaled_x, gemm;
 };
-BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+BwdPlan make_bwd_plan(int64_t M, int64_t N, int64_t K, int dtype) {
   BwdPlan b{};
   b.layers = dz_layers(M, N, K, dtype);
   b.columns = piece_columns(M, N, K, dtype, b.layers);
@@ -490,6 +485,19 @@ BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int dtype) {
     b.gemm = std::max({b.gemm, gemm_workspace_bytes(M, K, n, b.pieces, b.layers),
                        gemm_workspace_bytes(n, K, M, b.pieces, b.layers)});
   return b;
+}
+
+// A call asks for its workspace's size and is then launched: 4 us of a plan's making, once.
+BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+  struct Last {
+    int64_t M, N, K;
+    int dtype;
+    BwdPlan plan;
+  };
+  thread_local Last last{};
+  if (last.M != M || last.N != N || last.K != K || last.dtype != dtype)
+    last = Last{M, N, K, dtype, make_bwd_plan(M, N, K, dtype)};
+  return last.plan;
 }
 
 template <typename T>
@@ -612,7 +620,7 @@ int launch_bwd(const LinearLogprobsBwdParams& p, int dtype, cudaStream_t stream)
 size_t linear_logprobs_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct, bool w_direct) {
   const int pieces = dtype == kF32 ? 3 : 1;
   return (x_direct && pieces == 1 ? 0 : operand_bytes(M, K, dtype)) +
-         (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) + parts_bytes(run_plan(M, N, K, pieces), M);
+         (w_direct && pieces == 1 ? 0 : operand_bytes(N, K, dtype)) + parts_bytes(few_rows(M, dtype) ? linear_logprobs_few_parts(N) : run_plan(M, N, K, pieces).ranges * kShares, M);
 }
 
 size_t linear_logprobs_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, bool x_direct,
