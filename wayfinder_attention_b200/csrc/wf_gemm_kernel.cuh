@@ -80,10 +80,11 @@ struct GemmParams {
   uint32_t idesc;
 };
 
-template <typename T, int BN, int CG, bool PIECES>
+// BUFFERS: of staging, an epilogue warp (the stages take what they leave).
+template <typename T, int BN, int CG, bool PIECES, int BUFFERS>
 struct Layout {
   static constexpr uint32_t A_BYTES = kBM * 128, B_BYTES = BN / CG * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr uint32_t STAGING = kEpilogueWarps * 2 * kBuffer;
+  static constexpr uint32_t STAGING = kEpilogueWarps * BUFFERS * kBuffer;
   static constexpr int FIT = (227 * 1024 - 2048 - (int)STAGING) / (int)STAGE;
   static constexpr int STAGES = FIT < 8 ? FIT : 8;
   // a run's A where it stays (see kResident), and the stages of B alone that this leaves room for
@@ -263,6 +264,7 @@ __device__ __forceinline__ void add_bias(const GemmParams& p, int n, float* v) {
 // `layers` pieces.
 struct Finish {
   static constexpr bool kRuns = false, kStores = false;
+  static constexpr int kBuffers = 2;
 };
 
 template <typename T, int BN, int CG, bool PIECES, class E>
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                 const __grid_constant__ CUtensorMap ymap, const __grid_constant__ CUtensorMap zmap,
                 const __grid_constant__ CUtensorMap rmap, const GemmParams p, const E e) {
-  using L = Layout<T, BN, CG, PIECES>;
+  using L = Layout<T, BN, CG, PIECES, E::kBuffers>;
   using Work = Unit<E::kRuns>;
   // stages between additions to fp32 registers in runs
   constexpr int kRunChunk = PIECES ? kChunk : kDeepChunk;
@@ -525,10 +527,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // warp w reads TMEM lanes 32 (w % 4) .. + 31 (a row a lane) and share w / 4 of the columns
     constexpr int COLS = L::COLS, SC = L::SC;
     const uint32_t lbase = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (warp >> 2) * COLS;
-    unsigned char* bufs = base + L::off_staging + (size_t)warp * 2 * kBuffer;
+    constexpr int kBuffers = E::kBuffers;
+    unsigned char* bufs = base + L::off_staging + (size_t)warp * kBuffers * kBuffer;
     const GemmEpilogue& o = p.out;
     uint32_t acc = 0, acc_phase = 0, turn = 0, res_phase = 0;
-    auto buffer = [&](uint32_t i) { return bufs + (i & 1) * kBuffer; };
+    auto buffer = [&](uint32_t i) { return bufs + (kBuffers > 1 ? i & 1 : 0) * kBuffer; };
     auto release = [&] {
       tc_fence_before();
       __syncwarp();
@@ -611,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         e.template slice<SC>(row, v, m + lane, n, p.N);
         if constexpr (E::kStores) {
           for (int layer = 0;; ++layer) {
-            if (lane == 0) bulk_wait_read<1>();
+            if (lane == 0) bulk_wait_read<kBuffers - 1>();
             __syncwarp();
             stage_slice<T>(smem_u32(buffer(turn)), lane, v);
             store(true, &ymap, nullptr, 0, m, n, layer);
@@ -809,7 +812,7 @@ struct Plan {
 
 template <typename T, int BN, int CG, bool PIECES, class E>
 int launch_tile(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, const E& e, cudaStream_t stream) {
-  using L = Layout<T, BN, CG, PIECES>;
+  using L = Layout<T, BN, CG, PIECES, E::kBuffers>;
   // encoding a tensor map is a driver call: it needs the device's context current in this thread,
   // which the runtime sees to at a launch, and this may be a thread's first (a backward's)
   int device = 0;

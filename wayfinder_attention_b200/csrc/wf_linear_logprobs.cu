@@ -35,6 +35,7 @@ constexpr int kShares = 4;  // epilogue warps that share a row of a tile, in eve
 // +inf stays in m (the sums may lose it); m is -inf while nothing has counted.
 struct ScoreStats {
   static constexpr bool kRuns = true, kStores = false;
+  static constexpr int kBuffers = 0;
   const int64_t* tokens;
   float* parts;        // [3][ranges * kShares][M]: m, s, u
   float* token_logit;  // [M]
@@ -202,6 +203,7 @@ __device__ __forceinline__ float up_by(int least) { return least > 100 ? 0.f : l
 // dz_j = p (a + b t) + g [j = token] with t = (z - m) log2 e - l2s and p = 2^t.
 struct ScoreGrad {
   static constexpr bool kRuns = true, kStores = true;
+  static constexpr int kBuffers = 1;
   int layers;
   int first;  // of the vocabulary's piece
   RowInputs in;
