@@ -106,3 +106,15 @@ def test_the_backward_holds_pieces_of_the_vocabulary():
     for rows, V, d in ((8192, 50001, 1024), (32768, 131072, 256), (65536, 131072, 512)):
         rest = rows * d * 4 + (1 << 26)  # dx in fp32, sums
         assert size(rows, V, d, 0, 1, 1) <= max(1 << 29, 2048 * 2 * rows) + rest
+
+
+def test_workspaces_of_sizes_that_no_call_takes():
+    lib = _lib.load_library()
+    huge = (1 << 30, 1 << 31, 1 << 61, 1 << 62, (1 << 63) - 1)
+    for size in (lib.wf_linear_token_logprobs_workspace_bytes, lib.wf_linear_token_logprobs_backward_workspace_bytes):
+        for n in huge:
+            for dtype in range(3):
+                assert size(n, 8, 8, dtype, 1, 1) == size(8, n, 8, dtype, 1, 1) == size(8, 8, n, dtype, 1, 1) == 0
+    size = lib.wf_token_embedding_backward_workspace_bytes
+    for n in huge:
+        assert size(n, 8, 8, 8, 0, 1) == size(8, n, 8, 8, 0, 1) == size(8, 8, n, 8, 0, 1) == size(8, 8, 8, n, 0, 1) == 0

@@ -3,6 +3,7 @@
 #include "../../include/wayfinder.h"
 #include "wf_kernels.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -172,6 +173,11 @@ int check_embedding(const char* what, int32_t dtype, int64_t n, int64_t rows, in
     return fail(WF_ERR_UNSUPPORTED, "%s: sizes too large (n, rows < 2^30, d < 2^22)", what);
   if (stride < 0) return fail(WF_ERR_INVALID_ARGUMENT, "negative row stride");
   return WF_OK;
+}
+
+// Sizes that wf_linear_token_logprobs takes: a plan is only made for those.
+bool head_sizes(int64_t rows, int64_t vocab, int64_t d) {
+  return std::min({rows, vocab, d}) > 0 && std::max({rows, vocab, d}) < (1 << 30);
 }
 
 int check_logits(int32_t dtype, int64_t rows, int64_t vocab, int64_t stride) {
@@ -965,13 +971,13 @@ int wf_token_logprobs_backward(const void* logits, int32_t dtype, int64_t rows, 
 
 size_t wf_linear_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int32_t dtype,
                                                 int32_t x_direct, int32_t w_direct) {
-  if (rows <= 0 || vocab <= 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  if (!head_sizes(rows, vocab, d) || !valid_dtype(dtype)) return 0;
   return wf::linear_logprobs_workspace_bytes(rows, vocab, d, dtype, x_direct, w_direct);
 }
 
 size_t wf_linear_token_logprobs_backward_workspace_bytes(int64_t rows, int64_t vocab, int64_t d, int32_t dtype,
                                                          int32_t x_direct, int32_t w_direct) {
-  if (rows <= 0 || vocab <= 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  if (!head_sizes(rows, vocab, d) || !valid_dtype(dtype)) return 0;
   return wf::linear_logprobs_backward_workspace_bytes(rows, vocab, d, dtype, x_direct, w_direct);
 }
 
@@ -1054,6 +1060,7 @@ int wf_token_embedding(const int64_t* tokens, int64_t n, const void* weight, int
 size_t wf_token_embedding_backward_workspace_bytes(int64_t n, int64_t vocab, int64_t places, int64_t d, int32_t dtype,
                                                    int32_t has_positions) {
   if (n <= 0 || vocab < 0 || places < 0 || d <= 0 || !valid_dtype(dtype)) return 0;
+  if (n >= (1 << 30) || vocab >= (1 << 30) || places >= (1 << 30) || d >= (1 << 22)) return 0;
   return wf::embedding_backward_workspace_bytes(n, vocab, places, d, dtype, has_positions);
 }
 
