@@ -118,3 +118,11 @@ def test_workspaces_of_sizes_that_no_call_takes():
     size = lib.wf_token_embedding_backward_workspace_bytes
     for n in huge:
         assert size(n, 8, 8, 8, 0, 1) == size(8, n, 8, 8, 0, 1) == size(8, 8, n, 8, 0, 1) == size(8, 8, 8, n, 0, 1) == 0
+
+
+def test_the_fp16_backward_holds_pieces_of_the_weights_gradient():
+    """It is summed in fp32 before its power of two comes off: a piece's rows of it have 512 MB at most."""
+    size = _lib.load_library().wf_linear_token_logprobs_backward_workspace_bytes
+    for rows, V, d in ((1, 262144, 4096), (16, 131072, 4096), (512, 131072, 8192), (8192, 50001, 1024)):
+        rest = rows * d * 8 + (1 << 27)  # dx in fp32, x's copy, sums, shares of products
+        assert size(rows, V, d, _lib.WF_DTYPE_F16, 1, 1) <= (2 << 29) + rest, (rows, V, d)

@@ -432,7 +432,8 @@ int launch_fwd(const LinearLogprobsParams& p, int dtype, cudaStream_t stream) {
 // 2.68 ms, 512 MB 2.61; pieces of 64 MB, which L2 would hold, 2.87.)
 constexpr int64_t kPieceBytes = 512ll << 20, kPieceLeast = 2048;
 int64_t piece_columns(int64_t M, int64_t N, int64_t K, int dtype, int layers) {
-  const int64_t fit = kPieceBytes / (M * (dtype == kF32 ? 10 : 2 * layers)) / 256 * 256;
+  int64_t fit = kPieceBytes / (M * (dtype == kF32 ? 10 : 2 * layers)) / 256 * 256;
+  if (dtype == kF16) fit = std::min(fit, kPieceBytes / (4 * round8(K)) / 256 * 256);  // the piece's rows of dW in fp32
   const int64_t most = std::max(fit, kPieceLeast);
   if (N <= most) return N;
   auto waves = [](int64_t tiles) { return (tiles + kSms / 2 - 1) / (kSms / 2); };
