@@ -248,6 +248,23 @@ def test_another_stream_a_graph_and_another_thread(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_one_sequence_longer_than_the_tokens(cuda_device):
+    """Through the C ABI, whose seq is any number: positions 0, 1, ... n - 1."""
+    import ctypes
+
+    from wayfinder_attention_b200 import _lib
+
+    w, pw = _tables(30, 50, 16, torch.float32, cuda_device)
+    tokens = torch.arange(20, device=cuda_device)
+    for seq in (20, 21, 1 << 31, 1 << 32, (1 << 40) + 3):
+        y = torch.full((20, 16), math.nan, device=cuda_device)
+        at = [ctypes.c_void_p(t.data_ptr()) for t in (tokens, w, pw, y)]
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        rc = _lib.load_library().wf_token_embedding(at[0], 20, at[1], _lib.WF_DTYPE_F32, 30, 16, 16, 1.0, at[2], 50, 16,
+                                                    None, seq, at[3], None, stream)
+        assert rc == _lib.WF_OK and torch.equal(y, w[:20] + pw[:20]), seq
+
+
 def test_refusals_on_the_gpu(cuda_device):
     from wayfinder_attention_b200 import token_embedding
 

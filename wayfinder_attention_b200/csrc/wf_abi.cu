@@ -1049,7 +1049,8 @@ int wf_token_embedding(const int64_t* tokens, int64_t n, const void* weight, int
   if (!tokens || !weight || !y) return fail(WF_ERR_INVALID_ARGUMENT, "null pointer argument");
   wf::EmbeddingParams p{};
   p.tokens = tokens; p.positions = positions; p.weight = weight; p.position_weight = position_weight; p.y = y;
-  p.n = n; p.seq = seq; p.vocab = vocab; p.places = places; p.d = d;
+  p.n = n; p.vocab = vocab; p.places = places; p.d = d;
+  p.seq = std::min(seq, n);  // a longer one counts the same, and the kernels divide in 32 bits
   p.w_stride = w_row_stride; p.p_stride = p_row_stride;
   p.scale = scale;
   p.status = status;
