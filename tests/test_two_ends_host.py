@@ -27,7 +27,7 @@ def test_token_embedding_refuses():
     for padding in (-1, 6):
         with pytest.raises(ValueError, match="padding_index"):
             token_embedding(t, w, padding_index=padding)
-    for scale in (float("inf"), float("nan")):
+    for scale in (float("inf"), float("nan"), 1e39, -1e300):
         with pytest.raises(ValueError, match="scale"):
             token_embedding(t, w, scale=scale)
     with pytest.raises(RuntimeError, match="no CPU fallback"):

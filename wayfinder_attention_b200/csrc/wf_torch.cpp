@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -555,7 +556,7 @@ Tensor token_embedding(const Tensor& tokens, const Tensor& w, double scale, cons
     throw BadValue("positions " + shape_of(positions.sizes()) + " are neither of the tokens' shape " + shape_of(lead) +
                    " nor of its last axis");
   if (padding >= w.size(0)) throw BadValue("padding_index must be below vocab=" + std::to_string(w.size(0)));
-  if (!std::isfinite(scale)) throw BadValue("scale must be finite");
+  if (!(std::abs(scale) <= std::numeric_limits<float>::max())) throw BadValue("scale must be finite in float32");
   check_devices(w, {&tokens, &pw, &positions});
   dtype_code(w.scalar_type());
   const Tensor flat = long_ids(tokens, "tokens"),
