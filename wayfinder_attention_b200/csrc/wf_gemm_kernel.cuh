@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
           }
           // as below: what is in flight lands before the block ends
-          if (why && rank == 0) {
+          if (rank == 0) {
             for (uint32_t s = 0; s < (uint32_t)L::B_STAGES && s < issued; ++s)
               mbar_wait_asleep(&full[s], (issued - 1 - s) / L::B_STAGES & 1, kWaitNs);
             for (uint32_t s = 0; s < a_issued; ++s) mbar_wait_asleep(&a_full[s], runs - 1 & 1, kWaitNs);
@@ -409,8 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // after a wait that gave up, loads may be in flight that no product will wait for
-      if (why && rank == 0 && !(E::kRuns && !PIECES && p.resident))
+      // where a wait gave up, here or in the products, loads may be in flight that no product will wait for
+      if (rank == 0 && !(E::kRuns && !PIECES && p.resident))
         for (uint32_t s = 0; s < (uint32_t)L::STAGES && s < issued; ++s) {
           const uint32_t last = (issued - 1 - s) / L::STAGES;  // round of the newest load of stage s
           mbar_wait_asleep(&full[s], last & 1, kWaitNs);

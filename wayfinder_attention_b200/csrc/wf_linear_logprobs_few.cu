@@ -94,10 +94,9 @@ __global__ void __launch_bounds__(FewLayout<NT>::THREADS, 1)
           ++issued;
           r.next<L::STAGES>();
         }
-      // after a wait that gave up, loads may be in flight that no product will wait for
-      if (why)
-        for (uint32_t s = 0; s < (uint32_t)L::STAGES && s < issued; ++s)
-          mbar_wait_asleep(&full[s], (issued - 1 - s) / L::STAGES & 1, kWaitNs);
+      // where a wait gave up, here or in the products, loads may be in flight that no product will wait for
+      for (uint32_t s = 0; s < (uint32_t)L::STAGES && s < issued; ++s)
+        mbar_wait_asleep(&full[s], (issued - 1 - s) / L::STAGES & 1, kWaitNs);
     }
   } else if (warp == 1) {
     if (lane == 0) {
