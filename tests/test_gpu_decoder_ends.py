@@ -141,3 +141,44 @@ def test_no_logits_in_memory(cuda_device):
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - before < 1.2e9
     assert torch.isfinite(x.grad).all() and torch.isfinite(w.grad).all()
+
+
+@pytest.mark.parametrize("which", ["embedding", "head"])
+def test_a_captured_backward_beside_a_live_graph(which, cuda_device):
+    """Refused while a graph of the same leaf, made on the default stream, lives; captured and replayed once that is gone."""
+    from wayfinder_attention_b200 import linear_token_logprobs, token_embedding
+
+    w = torch.randn(300, 64, device=cuda_device).requires_grad_()
+    x, tokens = torch.randn(70, 64, device=cuda_device), torch.randint(0, 300, (70,), device=cuda_device)
+
+    def loss():
+        if which == "embedding":
+            return (token_embedding(tokens, w) * x).sum()
+        return linear_token_logprobs(x, w, tokens).logprob.sum()
+
+    def step():
+        w.grad = None
+        loss().backward()
+
+    step()
+    want = w.grad.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    alive = loss()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="same leaves"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    got = w.grad
+    got.zero_()
+    graph.replay()
+    assert torch.equal(got, want)
+    step()  # and eager passes go on
+    assert torch.equal(w.grad, want)

@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -134,6 +135,20 @@ bool needs_optional(AutogradContext* ctx, const char* has, size_t& edge) {
 }
 void once_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "this operator's backward is not differentiable (create_graph=True)");
+}
+// A gradient goes on on the stream of the node that takes it.  A leaf's node that a graph made outside of a capture keeps
+// alive has the default stream, which cannot wait for a capture: the engine's attempt breaks the capture, so
+// it is refused before.
+void check_capture() {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    const auto to = edge.function ? edge.function->stream() : std::nullopt;
+    TORCH_CHECK(!to || *to != c10::cuda::getDefaultCUDAStream(to->device_index()).unwrap(),
+                "a backward is captured into a CUDA graph while an autograd graph of the same leaves, made on the "
+                "default stream, is alive: delete that first");
+  }
 }
 
 // ------------------------------------------------------------------ linear
@@ -426,6 +441,7 @@ struct LinearLogprobsFunction : torch::autograd::Function<LinearLogprobsFunction
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once_only();
+    check_capture();
     variable_list out(6);
     if (!grads[0].defined() && !grads[1].defined()) return out;
     const auto saved = ctx->get_saved_variables();
@@ -516,6 +532,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once_only();
+    check_capture();
     const auto saved = ctx->get_saved_variables();
     const Tensor &tokens = saved[0], &positions = saved[1];
     size_t edge = 1;
