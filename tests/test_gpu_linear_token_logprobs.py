@@ -159,6 +159,40 @@ def test_rows_of_very_different_gradients(dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_rows_of_one_gradient_are_not_all_off_to_one_side(dtype, cuda_device):
+    """A mean's gradients are alike, here half a step of the type above a power of two: rounding dz must not scale them all.
+
+    1024 x 128 -> 16384, past the sizes whose dz is in two pieces.  Off by the token's probability at
+    most (6.2e-5 for logits within +-0.6 or so), which rounding 1 - p may lose: t = 2^-13 covers
+    it; half a step would be 2^-8 in bf16 and 2^-11 in fp16.  The results' own rounding does not average
+    out (dw's rows are x's times 1 + 2^-8, so 8 bits and half a step), but is monotone: a value within
+    t of the exact one becomes something between what (1 - t) and (1 + t) times that become.
+    """
+    from wayfinder_attention_b200 import linear_token_logprobs
+
+    rows, V, d = 1024, 16384, 128
+    g = torch.Generator(device=cuda_device).manual_seed(6)
+    x = torch.randn(rows, d, generator=g, device=cuda_device).to(dtype).requires_grad_()
+    w = (torch.randn(V, d, generator=g, device=cuda_device) * 0.1 * d ** -0.5).to(dtype).requires_grad_()
+    b = torch.zeros(V, device=cuda_device, dtype=dtype, requires_grad=True)
+    tokens = torch.randint(0, V, (rows,), generator=g, device=cuda_device)
+    for size in (1.0, 1e-3):
+        gl = torch.full((rows,), -size * (1 + ROUNDOFF[dtype]), device=cuda_device)
+        gl[::9] = 0.0
+        r = linear_token_logprobs(x, w, tokens, bias=b)
+        grads = torch.autograd.grad(r.logprob, [x, w, b], gl)
+        X, W = x.detach().double(), w.detach().double()
+        dz = -torch.softmax(X @ W.T, 1)
+        dz[torch.arange(rows, device=cuda_device), tokens] += 1
+        dz *= gl.double()[:, None]
+        for name, got, want in zip(("dx", "dw", "db"), grads, (dz @ W, dz.T @ X, dz.sum(0))):
+            t = 2.0 ** -13
+            low, along, high = (((v.double() * want).sum() / (want * want).sum()).item()
+                                for v in ((want * (1 - t)).to(dtype), got, (want * (1 + t)).to(dtype)))
+            assert low - t <= along <= high + t, (name, size, low, along, high)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [50, 1000, 7001])
 def test_banned_tokens(V, dtype, cuda_device):
     """A bias of -inf: for a share of the tokens, the given one among them, all but one, all."""

@@ -19,6 +19,8 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const float* partial, in
       const float4 f = *reinterpret_cast<const float4*>(partial + ((int64_t)s * M + m) * pitch + n);
       v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
     }
+    if (o.factor)
+      for (int j = 0; j < 4; ++j) v[j] *= *o.factor;
     if (o.bias)
       for (int j = 0; j < live; ++j) v[j] += to_f32(static_cast<const T*>(o.bias)[n + j]);
     if (o.z)
@@ -65,21 +67,25 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int pieces, int turns) {
   return best;
 }
 
-template <typename T, bool PIECES>
+template <typename T, bool PIECES, class E = Finish>
 int launch_shape(const GemmProblem& g, const GemmEpilogue& out, const Plan& plan, cudaStream_t stream) {
   const Shape& s = plan.shape;
   if constexpr (!PIECES) {
-    if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, plan, Finish{}, stream);
-    if (s.bn == 128 && s.cg == 1) return launch_tile<T, 128, 1, PIECES>(g, out, plan, Finish{}, stream);
+    if (s.bn == 256) return launch_tile<T, 256, 2, PIECES>(g, out, plan, E{}, stream);
+    if (s.bn == 128 && s.cg == 1) return launch_tile<T, 128, 1, PIECES>(g, out, plan, E{}, stream);
   }
-  if (s.cg == 2) return launch_tile<T, 128, 2, PIECES>(g, out, plan, Finish{}, stream);
-  return launch_tile<T, 64, 1, PIECES>(g, out, plan, Finish{}, stream);
+  if (s.cg == 2) return launch_tile<T, 128, 2, PIECES>(g, out, plan, E{}, stream);
+  return launch_tile<T, 64, 1, PIECES>(g, out, plan, E{}, stream);
 }
 
 template <typename T, bool PIECES>
 int launch_type(const GemmProblem& g, cudaStream_t stream) {
   const Plan plan = plan_of(g.M, g.N, g.K, g.pieces, g.turns);
-  if (plan.splits == 1) return launch_shape<T, PIECES>(g, g.out, plan, stream);
+  if (plan.splits == 1) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      if (g.out.factor) return launch_shape<T, PIECES, FinishByFactor>(g, g.out, plan, stream);
+    return launch_shape<T, PIECES>(g, g.out, plan, stream);
+  }
   GemmEpilogue parts{};
   parts.y = g.ws;
   parts.y_stride = round8(g.N);
@@ -99,6 +105,7 @@ size_t gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int pieces, int tur
 
 int launch_gemm(const GemmProblem& g, cudaStream_t stream) {
   if (g.M == 0 || g.N == 0) return 0;
+  if (g.out.factor && g.out_dtype != kBF16) return -1;  // nothing asks for it
   if (g.out_dtype == kBF16) return launch_type<__nv_bfloat16, false>(g, stream);
   if (g.out_dtype == kF16) return launch_type<__half, false>(g, stream);
   return g.pieces == 1 ? launch_type<float, false>(g, stream) : launch_type<float, true>(g, stream);

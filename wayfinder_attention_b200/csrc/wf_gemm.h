@@ -19,7 +19,7 @@ struct GemmOperand {
   bool mn_major;
 };
 
-// C = act(A B^T + bias) + residual, or its parts.  Rows of bias/residual/z/y are unit-strided.
+// C = act(factor A B^T + bias) + residual, or its parts.  Rows of bias/residual/z/y are unit-strided.
 struct GemmEpilogue {
   const void* bias;
   const void* residual;
@@ -27,6 +27,7 @@ struct GemmEpilogue {
   void* y;
   int64_t r_stride, z_stride, y_stride;
   int act;
+  const float* factor;  // one, on the device; null: 1.  Of a bf16 C only
 };
 
 struct GemmProblem {

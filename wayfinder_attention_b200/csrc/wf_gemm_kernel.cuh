@@ -263,8 +263,11 @@ __device__ __forceinline__ void add_bias(const GemmParams& p, int n, float* v) {
 // slice() by slice of it, and end(); where STORES is set, what a slice became goes to ymap, in
 // `layers` pieces.
 struct Finish {
-  static constexpr bool kRuns = false, kStores = false;
+  static constexpr bool kRuns = false, kStores = false, kFactor = false;
   static constexpr int kBuffers = 2;
+};
+struct FinishByFactor : Finish {  // with a factor: apart, since its registers spill 16 bytes more
+  static constexpr bool kFactor = true;
 };
 
 template <typename T, int BN, int CG, bool PIECES, class E>
@@ -720,6 +723,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < SC; ++j) v[j] = __uint_as_float(r[j]);
+          if constexpr (E::kFactor) {
+            const float factor = __ldg(o.factor);
+#pragma unroll
+            for (int j = 0; j < SC; j += 2) mul2(Pair(v[j], v[j + 1]), Pair(factor)).get(v[j], v[j + 1]);
+          }
           add_bias<T>(p, n0 + c, v);
           if (c + SC < COLS) {
             tmem_ld(lbase + acc * L::ACC + c + SC, r);

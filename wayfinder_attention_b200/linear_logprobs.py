@@ -32,8 +32,8 @@ def linear_token_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.T
     entropy 0 and no gradient.  A NaN or +inf among its logits makes a row NaN.
     Differentiable in x, weight and bias through logprob and entropy.  The backward makes the
     logits again.  Their gradients are taken to x's type before the two products (two pieces of
-    it up to 2^30 multiplications, one above, which leaves x's and weight's gradients with 1.4
-    times the error of their rounding; float32 in three bf16 pieces).  Its workspace holds them
+    it up to 64 rows or 2^30 multiplications, one above, which leaves x's and weight's gradients
+    with 1.4 times the error of their rounding; float32 in three bf16 pieces).  Its workspace holds them
     for a piece of the vocabulary: at most 512 MB, or 2048 columns; in float16 as much again for
     the piece's rows of weight's gradient.
     """
