@@ -268,6 +268,30 @@ def test_large_and_special_rows(dtype, cuda_device):
     assert torch.isfinite(dx[others]).all() and not dx[17].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_near_the_ends_of_fp32(dtype, cuda_device):
+    """Gradients of 2^127 and of 2^-100 to a row's log probability, past the sizes whose dz is in two pieces.
+
+    x is 2^-20 and the weight 0, so that every distribution is even and nothing else overflows.
+    """
+    from wayfinder_attention_b200 import linear_token_logprobs
+
+    rows, V, d = 1024, 16384, 80
+    x = torch.full((rows, d), 2.0 ** -20, device=cuda_device, dtype=dtype).requires_grad_()
+    w = torch.zeros(V, d, device=cuda_device, dtype=dtype).requires_grad_()
+    tokens = torch.arange(rows, device=cuda_device)
+    for size in (2.0 ** 127, 1.9 * 2.0 ** 126, 2.0 ** -100):
+        gl = torch.full((rows,), size, device=cuda_device)
+        r = linear_token_logprobs(x, w, tokens)
+        dx, dw = torch.autograd.grad(r.logprob, [x, w], gl)
+        assert not dx.any()
+        # row t of dw: x (1 - 1 / V) of its own row, less x / V of the others
+        want = size * 2.0 ** -20 * (1 - rows / V)
+        u = ROUNDOFF[dtype]
+        assert (dw[:rows].double() / want - 1).abs().max() <= 3 * u + 2.0 ** -13, size
+        assert (dw[rows:].double() / (-size * 2.0 ** -20 * rows / V) - 1).abs().max() <= 3 * u + 2.0 ** -13, size
+
+
 def test_strides_leading_axes_and_empty(cuda_device):
     from wayfinder_attention_b200 import linear_token_logprobs
 

@@ -203,8 +203,8 @@ __device__ __forceinline__ float up_by(int least) { return least > 100 ? 0.f : l
 // Rounding dz to one piece of its type costs most where |dz| is large: at the row's token, where it is
 // |gl| or a little less.  A value just above a power of two is rounded twice as coarsely for its size as one
 // just below the next, and where all |gl| are alike (the mean of a loss) each row is off to the same
-// side, by up to half a step of the type.  So dz is multiplied by 1.625 / m, m in [1, 2) the
-// mean |gl|'s mantissa, and the products by its reciprocal in fp32: equal |gl| then have no
+// side, by up to half a step of the type.  So dz is multiplied by 0.8125 / m (below 1: nothing overflows by it),
+// m in [1, 2) the mean |gl|'s mantissa, which puts that mean at 1.625 of its binade, and the products by its reciprocal in fp32: equal |gl| then have no
 // rounding of their own, and others are in the finer part of their binade: with |gl| of 1 +- 0.2 the
 // gradients' error, of which their own rounding is 1, is 1.37 (1.26 to 1.43 over 96 to 1024 rows)
 // where it was 1.45 (to 1.53).  3 us more a backward, and nothing in the products.
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kFactorThreads) linear_logprobs_factor_kernel(
   count = over_warp(counts[threadIdx.x]);
   if (threadIdx.x) return;
   const float mean = sum / count;  // NaN where there are none
-  const float c = mean > 0.f ? 1.625f / scalbnf(mean, -ilogbf(mean)) : 1.f;
+  const float c = mean > 0.f ? 0.8125f / scalbnf(mean, -ilogbf(mean)) : 1.f;
   factor[0] = c;
   factor[1] = 1.f / c;
 }
