@@ -126,3 +126,11 @@ def test_the_fp16_backward_holds_pieces_of_the_weights_gradient():
     for rows, V, d in ((1, 262144, 4096), (16, 131072, 4096), (512, 131072, 8192), (8192, 50001, 1024)):
         rest = rows * d * 8 + (1 << 27)  # dx in fp32, x's copy, sums, shares of products
         assert size(rows, V, d, _lib.WF_DTYPE_F16, 1, 1) <= (2 << 29) + rest, (rows, V, d)
+
+
+def test_indices_that_are_not_whole_numbers_are_refused():
+    t, w = torch.zeros(2, 3, dtype=torch.int64), torch.zeros(6, 8)
+    with pytest.raises(TypeError):
+        token_embedding(t, w, padding_index=1.5)
+    with pytest.raises((TypeError, RuntimeError)):
+        linear_token_logprobs(w[:2], w, t[0, :2], ignore_index=1.5)

@@ -7,6 +7,8 @@ over the sorted tokens, the same bits each time.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _lib
@@ -25,7 +27,7 @@ def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1
     position outside its table makes its row NaN, adds nothing to a gradient of the table it is
     outside of, and sets the status word's bit 0.
     """
-    padding = -1 if padding_index is None else int(padding_index)
+    padding = -1 if padding_index is None else operator.index(padding_index)
     if padding_index is not None and padding < 0:
         raise ValueError(f"padding_index must be >= 0, got {padding_index}")
     if not weight.is_cuda:  # refused, after the checks that come before
