@@ -4,7 +4,7 @@
 // The tiled product pads the rows to 128 and multiplies them with 128 of the vocabulary: at 16 rows
 // seven eighths of that is padding, which costs no bytes but power, and under a sustained load the
 // power cap takes it out of the memory's rate (16 rows, 4096 -> 131072 in fp16, one pass after the
-// other: 216 us there, 176 here, 164 at the rate of a copy; a pass by itself 182 and 172).  Here 128 rows of W are A, the given rows
+// other: 216 us there, 170 here, 164 at the rate of a copy; a pass by itself 182 and 172).  Here 128 rows of W are A, the given rows
 // (padded to 16, 32 or 64) are B, and an accumulator's lanes are tokens of the vocabulary, its columns
 // the rows.  A thread keeps the running maximum m, s = sum exp(z - m) and u = sum exp(z - m) (z - m) of
 // its lane's tokens for each row, over all tiles of the block; lanes are joined once, at the end.
