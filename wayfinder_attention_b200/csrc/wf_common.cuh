@@ -11,6 +11,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "wf_kernels.h"
+
 namespace wf {
 
 // Programmatic dependent launch: a kernel launched with launch_pdl may start while
@@ -34,10 +36,6 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
-
-
-// Matches the WF_DTYPE_* constants of include/wayfinder.h.
-enum Dtype : int { kBF16 = 0, kF16 = 1, kF32 = 2 };
 
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "wf_kernels.h"
+
 namespace wf {
 
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -18,6 +20,11 @@ struct GemmOperand {
   int64_t rows, cols, pitch, piece_stride;
   bool mn_major;
 };
+
+// Bytes of a matrix laid out as an operand (wf_operand.cuh).
+inline size_t operand_bytes(int64_t rows, int64_t cols, int dtype, int turns = 1) {
+  return round256((size_t)rows * round8(cols) * 2 * (dtype == kF32 ? 3 : turns));
+}
 
 // C = act(factor A B^T + bias) + residual, or its parts.  Rows of bias/residual/z/y are unit-strided.
 struct GemmEpilogue {

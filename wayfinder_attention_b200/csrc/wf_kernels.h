@@ -9,6 +9,9 @@ namespace wf {
 
 constexpr int kSms = 148;  // of a B200
 
+// Matches the WF_DTYPE_* constants of include/wayfinder.h.
+enum Dtype : int { kBF16 = 0, kF16 = 1, kF32 = 2 };
+
 // Causal top-K over address vectors.
 //   query rows:  q[b, l, :]  for local row l in [0, Tq); its sequence position
 //                g(l) = ((l / rt) * rs + r0) * rt + l % rt   (identity when rs=1, r0=0, rt>=Tq)

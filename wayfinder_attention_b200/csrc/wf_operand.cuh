@@ -118,9 +118,6 @@ bool on_16_bytes(const void* p, int64_t stride) {
 }
 
 // A (rows, cols) matrix as the product reads it: itself, or laid out at *ws, which moves on.
-size_t operand_bytes(int64_t rows, int64_t cols, int dtype, int turns = 1) {
-  return round256((size_t)rows * round8(cols) * 2 * (dtype == kF32 ? 3 : turns));
-}
 template <typename T>
 GemmOperand blank_operand(int64_t rows, int64_t cols, int dtype, unsigned char** ws, int turns = 1) {
   GemmOperand o{};
