@@ -467,12 +467,14 @@ WF_API int wf_token_logprobs_backward(const void* logits, int32_t dtype, int64_t
 
 /*
  * The same from hidden rows and a head's weight, without the logits in memory: rows
- * z = x W^T + bias of which only the running maximum and sums are kept.  fp32 throughout.
+ * z = x W^T + bias of which only running sums to a base are kept.  fp32 throughout.
  *
  *   x        : (rows, d) rows x_row_stride apart;  w : (vocab, d) rows w_row_stride apart
  *   bias     : (vocab) or NULL; -inf bans a token.  All three of dtype
- *   tokens, ignore_index, logprob, entropy, stats, status : as wf_token_logprobs; status bit 1
- *              is OR-ed in if a bounded wait timed out
+ *   tokens, ignore_index, logprob, entropy, status : as wf_token_logprobs; status bit 1 is
+ *              OR-ed in if a bounded wait timed out
+ *   stats    : (2, rows) fp32 for the backward, or NULL: a base m of each row (one of its logits, not
+ *              always the largest) and log sum exp(z - m); only their sum is the row's own
  *   workspace: wf_linear_token_logprobs_workspace_bytes() bytes, 256-byte aligned; x_direct /
  *              w_direct as for wf_linear
  * A NaN (or +inf) among a row's logits makes its logprob and entropy NaN.

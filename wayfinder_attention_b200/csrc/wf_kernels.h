@@ -248,7 +248,7 @@ struct LinearLogprobsParams {
   const int64_t* tokens;
   float* logprob;
   float* entropy;
-  float* stats;  // [2][rows] for the backward, or null: the maximum m, and log sum exp(z - m)
+  float* stats;  // [2][rows] for the backward, or null: a base m, near the maximum or it, and log sum exp(z - m)
   int64_t rows, vocab, d, x_stride, w_stride, ignore_index;
   void* ws;
   int32_t* status;  // nullable
