@@ -100,13 +100,17 @@ struct ScoreStats {
       for (int j = 0; j < SC; j += 2) top = max_keep_nan(top, v[j], v[j + 1]);
       // far enough below the largest to have no weight, and near enough for the difference to be finite
       const float low = fmaxf(top - 0.5f * fabsf(top) - 1e5f, -FLT_MAX);
-#pragma unroll
-      for (int j = 0; j < SC; ++j) v[j] = fmaxf(v[j], low);
       const float d = fmaxf(r.m - top, kNothing), a = exp2_approx(d * kLog2e);
       r.u = a * fmaf(r.s, d, r.u);
       r.s *= a;
       r.m = top;
       none = top == -INFINITY;
+      if (top == -FLT_MAX) {  // nothing finite is below it: a -inf will add its weight of 1, which comes off here
+#pragma unroll
+        for (int j = 0; j < SC; ++j) r.s -= v[j] == -INFINITY ? 1.f : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < SC; ++j) v[j] = fmaxf(v[j], low);
     }
     r.s += none ? 0.f : s0;
     r.u += none ? 0.f : u0;
