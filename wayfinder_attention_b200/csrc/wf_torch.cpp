@@ -138,13 +138,14 @@ void once_only() {
 }
 // A gradient goes on on the stream of the node that takes it.  A leaf's node that a graph made outside of a capture keeps
 // alive has the default stream, which cannot wait for a capture: the engine's attempt breaks the capture, so
-// it is refused before.
+// it is refused before.  A leaf that this pass wants nothing of (autograd.grad for others) is not gone to.
 void check_capture() {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
-  for (const auto& edge : node->next_edges()) {
-    const auto to = edge.function ? edge.function->stream() : std::nullopt;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    if (!node->task_should_compute_output(i)) continue;
+    const auto to = node->next_edge(i).function->stream();
     TORCH_CHECK(!to || *to != c10::cuda::getDefaultCUDAStream(to->device_index()).unwrap(),
                 "a backward is captured into a CUDA graph while an autograd graph of the same leaves, made on the "
                 "default stream, is alive: delete that first");
