@@ -192,10 +192,17 @@ struct RowInputs {
 };
 
 // fp16 has no room for p of a gradient that is small itself (a mean over many rows): there a row's
-// gradient is multiplied by a power of two 2^e that brings |gl| + 32 |gh|, which bounds |dz|, to
-// 2^14 .. 2^15.  dx takes it off again by rows; for dW, x's rows are multiplied by 2^(least e - e)
-// and the product by 2^-least.
+// gradient is multiplied by a power of two 2^h.  dx takes it off again by rows; for dW, x's rows are multiplied by
+// 2^(least - h) and the product by 2^-least.
+//
+// e brings |gl| + 32 |gh|, which bounds |dz|, to 2^14 .. 2^15, and least is the smallest e, that of the largest
+// gradient.  x's rows are normal fp16 numbers down to 2^-14 only, so h is not e but up to kSpare less: rows up to
+// 2^10 below the largest leave x as it is, and those up to 2^24 below it still cost x no more than half its
+// last bit at |x| = 1 (2^14 with h = e).  dz's smallest steps are then 2^-28 of the row's gradient instead of 2^-38: over
+// 131072 tokens what they can lose is 2^-12 of the distribution.
+constexpr int kSpare = 10;
 constexpr int kNoRow = 1000;  // the exponent of a row without a gradient
+__device__ __forceinline__ int held(int e, int least) { return max(e - kSpare, least); }
 __global__ void __launch_bounds__(256) linear_logprobs_exponents_kernel(RowInputs in, int* exponent) {
   pdl_wait();
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -211,8 +218,11 @@ __global__ void __launch_bounds__(256) linear_logprobs_exponents_kernel(RowInput
   const int least = __reduce_min_sync(0xffffffffu, e);
   if ((threadIdx.x & 31) == 0 && least != kNoRow) atomicMin(exponent + in.rows, least);
 }
-// 2^(least - e), or 2^-least: no row has a gradient where there is no least exponent.
-__device__ __forceinline__ float down_by(int e, int least) { return least > 100 || e > 100 ? 0.f : ldexpf(1.f, least - e); }
+// 2^(least - h) and 2^-h of a row, and 2^-least: no row has a gradient where there is no least exponent.
+__device__ __forceinline__ float down_by(int e, int least) {
+  return least > 100 || e > 100 ? 0.f : ldexpf(1.f, least - held(e, least));
+}
+__device__ __forceinline__ float up_by(int e, int least) { return least > 100 || e > 100 ? 0.f : ldexpf(1.f, -held(e, least)); }
 __device__ __forceinline__ float up_by(int least) { return least > 100 ? 0.f : ldexpf(1.f, -least); }
 
 // Rounding dz to one piece of its type costs most where |dz| is large: at the row's token, where it is
@@ -267,7 +277,7 @@ struct ScoreGrad {
   int layers;
   int first;  // of the vocabulary's piece
   RowInputs in;
-  const int* exponent;  // or null
+  const int* exponent;  // [rows], then the least; or null
   const float* factor;  // or null
   struct Row {
     float m, l2s, a, b, g;
@@ -292,7 +302,7 @@ struct ScoreGrad {
     r.a = -fmaf(gh, in.entropy[row], gl);
     r.b = -gh * kLn2;
     if (exponent || factor) {
-      const float up = (exponent ? ldexpf(1.f, exponent[row]) : 1.f) * (factor ? *factor : 1.f);
+      const float up = (exponent ? ldexpf(1.f, held(exponent[row], exponent[in.rows])) : 1.f) * (factor ? *factor : 1.f);
       r.a *= up;
       r.b *= up;
       r.g *= up;
@@ -318,7 +328,7 @@ struct ScoreGrad {
   __device__ __forceinline__ void end(const Row&, int, int, int) const {}
 };
 
-// x's rows multiplied by 2^(least - e): the fp16 operand of dW.
+// x's rows multiplied by 2^(least - h): the fp16 operand of dW.
 __global__ void __launch_bounds__(256) scale_rows_kernel(const __half* x, int64_t stride, bool vec, int64_t rows,
                                                          int64_t cols, const int* exponent, __half* out) {
   pdl_wait();
@@ -350,7 +360,7 @@ __global__ void __launch_bounds__(256) round_rows_kernel(const float* x, int64_t
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / groups, c = i % groups * 4;
     const float4 f = *reinterpret_cast<const float4*>(x + r * pitch + c);
-    const float s = exponent ? up_by(exponent[r]) * down : all;
+    const float s = exponent ? up_by(exponent[r], exponent[rows]) * down : all;
     const float v[4] = {f.x * s, f.y * s, f.z * s, f.w * s};
     T* to = out + r * cols + c;
     if (vec) {
@@ -373,7 +383,7 @@ __global__ void __launch_bounds__(256) dz_columns_kernel(const T* dz, int64_t pi
   float s[8] = {};
   if (c < N)
     for (int64_t m = (int64_t)blockIdx.y * 8 + warp; m < M; m += (int64_t)gridDim.y * 8) {
-      const float up = exponent ? up_by(exponent[m]) : 1.f;
+      const float up = exponent ? up_by(exponent[m], exponent[M]) : 1.f;
       for (int layer = 0; layer < layers; ++layer) {
         Raw8<T> raw;
         raw.load(dz + (layer * M + m) * pitch, c, pitch, true);

@@ -33,7 +33,8 @@ def linear_token_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.T
     Differentiable in x, weight and bias through logprob and entropy.  The backward makes the
     logits again.  Their gradients are taken to x's type before the two products (two pieces of
     it up to 64 rows or 2^30 multiplications, one above, which leaves x's and weight's gradients
-    with 1.4 times the error of their rounding; float32 in three bf16 pieces).  Its workspace holds them
+    with 1.4 times the error of their rounding; float32 in three bf16 pieces).  In float16 a row whose
+    gradient is 2^-24 of the largest row's, or less, loses digits of x in weight's gradient.  The workspace holds them
     for a piece of the vocabulary: at most 512 MB, or 2048 columns; in float16 as much again for
     the piece's rows of weight's gradient.
     """
