@@ -219,7 +219,9 @@ class TransformerLM(nn.Module):
         """
         # the last position has no next token; a whole row of logits a token keeps them uncopied
         following = torch.cat([input_ids[:, 1:], input_ids.new_full((input_ids.shape[0], 1), self.pad_token_id)], 1)
-        if self.fused_ends and top_n == 0 and runs_as(self.lm_head, nn.Linear):
+        # a hook on the model, or a subclass's forward, is about the logits
+        plain = runs_as(self, type(self)) and type(self).forward is TransformerLM.forward
+        if self.fused_ends and top_n == 0 and plain and runs_as(self.lm_head, nn.Linear):
             h, weight, bias = self._hidden(input_ids, attn_mask), self.lm_head.weight, self.lm_head.bias
             if torch.is_autocast_enabled("cuda"):  # the product in its type, as nn.Linear's is
                 dtype = torch.get_autocast_dtype("cuda")
