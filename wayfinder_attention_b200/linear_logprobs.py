@@ -36,7 +36,9 @@ def linear_token_logprobs(x: torch.Tensor, weight: torch.Tensor, tokens: torch.T
     with 1.4 times the error of their rounding; float32 in three bf16 pieces).  In float16 a row whose
     gradient is 2^-24 of the largest row's, or less, loses digits of x in weight's gradient.  The workspace holds them
     for a piece of the vocabulary: at most 512 MB, or 2048 columns; in float16 as much again for
-    the piece's rows of weight's gradient.
+    the piece's rows of weight's gradient.  What the tensor cores cannot read as it lies is laid out in
+    the workspace besides, forward and backward: float32 x and weight whole, in 6 bytes an element (3.2 GB for
+    a weight of (131072, 4096)), and 16-bit ones whose rows do not start on 16 bytes, in 2.
     """
     if not x.is_cuda:  # refused, after the checks that come before
         return LinearLogprobs(*_lib.torch_ops().linear_token_logprobs(x, weight, tokens, bias, ignore_index, 0,
