@@ -3,8 +3,10 @@
 //
 // The tiled product pads the rows to 128 and multiplies them with 128 of the vocabulary: at 16 rows
 // seven eighths of that is padding, which costs no bytes but power, and under a sustained load the
-// power cap takes it out of the memory's rate (16 rows, 4096 -> 131072 in fp16, one pass after the
-// other: 216 us there, 170 here, 164 at the rate of a copy; a pass by itself 182 and 172).  Here 128 rows of W are A, the given rows
+// power cap takes it out of the memory's rate.  4096 -> 131072 in fp16 without a bias, one pass after the other, there and
+// here: 257 and 164 us for 1 row, 178 and 165 for 16, 199 and 182 for 64, where a copy's rate gives 164 (a warmer GPU
+// takes up to 193 for 16 rows; with a bias of which a quarter is banned 179).  A weight that L2 holds most of: 1024 -> 50001 in bf16
+// 42 and 33 us for 16 rows, but 35 and 41 for 64.  Here 128 rows of W are A, the given rows
 // (padded to 16, 32 or 64) are B, and an accumulator's lanes are tokens of the vocabulary, its columns
 // the rows.  A thread keeps the running maximum m, s = sum exp(z - m) and u = sum exp(z - m) (z - m) of
 // its lane's tokens for each row, over all tiles of the block; lanes are joined once, at the end.
@@ -20,8 +22,8 @@ namespace {
 
 constexpr int kFewTile = 128;  // tokens of the vocabulary
 // Stages of depth between additions to fp32 registers, half of kDeepChunk: log probabilities off by 1.5e-7
-// of their size instead of 3e-7, in the time that the weight needs (16 rows, 4096 -> 131072 198 / 194 us,
-// 64 rows, 1024 -> 50001 44 / 44; with 2 stages 204 and 48).
+// of their size instead of 3e-7, in the time that the weight needs (16 rows, 4096 -> 131072 with 8, 4 and 2 stages:
+// 174, 165 and 180 us; 64 rows 178, 182 and 203; 64 rows, 1024 -> 50001 40, 41 and 42).
 constexpr int kFewChunk = 4;
 template <int NT>
 struct FewLayout {

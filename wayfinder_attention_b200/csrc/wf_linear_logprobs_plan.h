@@ -54,7 +54,7 @@ inline int64_t piece_columns(int64_t M, int64_t N, int64_t K, int dtype, int lay
 // Pieces of a 16-bit dz, as in wf_linear.cu: two where the products are small, so that rounding it
 // adds nothing to the gradients' own rounding.  And up to 64 rows, where a row of dW is a row or
 // two of x and one rounding makes much of its error: the products are bound by the weight's bytes
-// there and pay a quarter for it (64 rows, 1024 -> 50001: 88 -> 106 us; at 512 rows it would be 161 -> 246).
+// there and pay a sixth for it (64 rows, 1024 -> 50001: 86 -> 100 us; at 512 rows it would be 162 -> 251).
 inline int dz_layers(int64_t M, int64_t N, int64_t K, int dtype) {
   return dtype != kF32 && ((double)M * N * K <= (double)(1 << 30) || M <= 64) ? 2 : 1;
 }
